@@ -118,6 +118,44 @@ int tcc_pack_features_int8x16(const int8_t* q, int8_t* packed, uint32_t sources,
 int tcc_quantize_pack_features_int8(const float* x, int8_t* packed, float* scale, uint32_t sources,
                                     uint32_t features, void* stream);
 
+/* ---- dense layers in 8-bit blocks (HIP; include/blocks.h, no reference counterpart) ----
+ * Dense matrices are row-major with a row stride in elements and a type: 0 float32, 1 bfloat16, 2 float16.
+ * Blocks are codes (0 E4M3, 1 INT8) and exponents, laid out as include/blocks.h says. kind: 0 silu,
+ * 1 gelu, 2 gelu by tanh. Zero rows return TCC_OK without a launch. */
+int tcc_quantize_blocks(const void* x, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                        uint32_t codeType, uint32_t rows, uint32_t columns, void* stream);
+int tcc_dequantize_blocks(const uint8_t* codes, const uint8_t* exponents, uint32_t codeType, void* out,
+                          uint64_t stride, uint32_t type, uint32_t rows, uint32_t columns, void* stream);
+/* The transposed copy is made if codesT and exponentsT are given. */
+int tcc_quantize_weight_blocks(const void* w, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                               uint8_t* codesT, uint8_t* exponentsT, uint32_t outer, uint32_t inner,
+                               void* stream);
+/* Workspace queries write the bytes that the call with the same arguments needs at least. */
+int tcc_matmul_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, size_t* bytes);
+int tcc_matmul_blocks(const uint8_t* xCodes, const uint8_t* xExponents, const uint8_t* wCodes,
+                      const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type,
+                      uint32_t rows, uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes,
+                      void* stream);
+int tcc_linear_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, int keep,
+                                size_t* bytes);
+/* keepCodes and keepExponents may be null: x's blocks are not kept then. */
+int tcc_linear_blocks(const void* x, uint64_t stride, uint32_t type, const uint8_t* wCodes,
+                      const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride,
+                      uint8_t* keepCodes, uint8_t* keepExponents, uint32_t rows, uint32_t inner, uint32_t outer,
+                      void* workspace, size_t workspaceBytes, void* stream);
+int tcc_weight_grad_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type,
+                                     size_t* bytes);
+/* db may be null. */
+int tcc_weight_grad_blocks(const void* dy, uint64_t stride, uint32_t type, const uint8_t* xCodes,
+                           const uint8_t* xExponents, float* dw, float* db, uint32_t rows, uint32_t inner,
+                           uint32_t outer, void* workspace, size_t workspaceBytes, void* stream);
+int tcc_activation_blocks(const void* x, uint64_t stride, uint32_t type, uint32_t kind, int gated, void* y,
+                          uint64_t yStride, uint8_t* keepCodes, uint8_t* keepExponents, uint32_t codeType,
+                          uint32_t rows, uint32_t width, void* stream);
+int tcc_activation_blocks_backward(const void* dy, uint64_t stride, uint32_t type, const uint8_t* codes,
+                                   const uint8_t* exponents, uint32_t codeType, uint32_t kind, int gated, void* dx,
+                                   uint64_t dxStride, uint32_t rows, uint32_t width, void* stream);
+
 /* DeviceMatrix — reference src/device_matrix.cuh:8-37: uploads every array of a bucketed format,
  * allocates partials (partialCount*8*features floats) and counters (nSW*(features/128) uint32,
  * zeroed) when partialCount > 0, and hands out the view and the workspace. */

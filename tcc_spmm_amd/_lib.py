@@ -81,6 +81,33 @@ SIGNATURES = {
                                             C.c_void_p]),
     "tcc_quantize_pack_features_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32,
                                                   C.c_uint32, C.c_void_p]),
+    "tcc_quantize_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
+                                      C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "tcc_dequantize_blocks": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64,
+                                        C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "tcc_quantize_weight_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "tcc_matmul_blocks_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                              C.POINTER(C.c_size_t)]),
+    "tcc_matmul_blocks": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p,
+                                    C.c_size_t, C.c_void_p]),
+    "tcc_linear_blocks_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+                                              C.POINTER(C.c_size_t)]),
+    "tcc_linear_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
+                                    C.c_uint32, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tcc_weight_grad_blocks_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                                   C.POINTER(C.c_size_t)]),
+    "tcc_weight_grad_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
+                                         C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tcc_activation_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p,
+                                        C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
+                                        C.c_uint32, C.c_void_p]),
+    "tcc_activation_blocks_backward": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
+                                                 C.c_uint32, C.c_uint32, C.c_int, C.c_void_p, C.c_uint64,
+                                                 C.c_uint32, C.c_uint32, C.c_void_p]),
     "tcc_device_matrix_create": (C.c_int, [C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p)]),
     "tcc_device_matrix_view": (C.c_int, [C.c_void_p, C.POINTER(DeviceView),
                                          C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),

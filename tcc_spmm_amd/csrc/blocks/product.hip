@@ -1,0 +1,478 @@
+// The product of 8-bit blocks, y = x w^T + bias (include/blocks.h), and the linear layer on dense x.
+#include "device_blocks.h"
+#include "hip_support.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+using namespace blocks;
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+struct Product {
+    const std::uint8_t *x, *xe; // null x: dense input
+    const std::uint8_t *w, *we;
+    const float* bias;
+    void* y;
+    std::uint64_t yStride;
+    unsigned rows, outer, count, expPitch; // count: blocks of a row; code rows are 128 * count bytes
+    unsigned inner, tilesM;
+    const void* dense;
+    std::uint64_t denseStride;
+    std::uint8_t *keep, *keepExp;
+};
+
+__device__ __forceinline__ i32x8 join(u32x4 p, u32x4 q) {
+    return i32x8{int(p.x), int(p.y), int(p.z), int(p.w), int(q.x), int(q.y), int(q.z), int(q.w)};
+}
+
+// The values of 8 E4M3 codes as bf16, exact: the conversion multiplies by the scale's power of two.
+__device__ __forceinline__ bf16x8 values8(unsigned lo, unsigned hi, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// 16 bytes a lane from `rsrc`, at `lane + uniform`, to LDS at `to` + 16 * lane, past the registers.
+__device__ __forceinline__ void loadToLds(__amdgpu_buffer_rsrc_t rsrc, std::uint8_t* to, unsigned lane, unsigned uniform) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)to, 16, lane, uniform, 0, 0);
+}
+
+// Waits until at most N of this wave's memory loads are outstanding and its LDS reads are done, then
+// for the workgroup. One asm block with a memory clobber, so that no access moves across it.
+template <unsigned N> __device__ __forceinline__ void waitBarrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------
+// 16-bit outputs: the scaled 8-bit MFMA on tiles of BM x BN.
+//
+// A block of 128 along the inner axis is one step: 128 bytes of each of the tile's rows, loaded to LDS
+// without passing registers, Stages deep. The 16-byte chunks of a row are stored in an order that
+// depends on the row (its key), so that the rows an MFMA operand takes at once lie in different banks.
+// The order of the inner axis inside a block is free, since both operands share it and each has one
+// scale there: a lane takes chunks g and g + 4 of its row.
+// The weight is the MFMA's first operand, whose rows become consecutive values of one lane: rows are
+// dealt to pairs of MFMAs so that a lane ends with 8 consecutive outputs of one row of y.
+template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages>
+__global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
+    constexpr unsigned Waves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+    constexpr unsigned XL = BM / 8 / Waves, WL = BN / 8 / Waves;
+    static_assert(Stages == 2 || Stages == 4, "the stage is a constant of the unrolled step");
+    static_assert(BN / WN <= 128 && NT % 2 == 0, "a wave's columns share a weight tile");
+    extern __shared__ __align__(1024) std::uint8_t lds[];
+    const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned tm = blockIdx.x % a.tilesM * BM, tn = blockIdx.x / a.tilesM * BN;
+    const unsigned pitch = a.count * kBlock;
+    const auto xr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<std::uint8_t*>(a.x) + std::uint64_t(tm) * pitch, 0, 0x7FFFFFFF, 0x00020000);
+    const auto wr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<std::uint8_t*>(a.w) + std::uint64_t(tn) * pitch, 0, 0x7FFFFFFF, 0x00020000);
+    // Rows past the end read the last row; their results are not stored.
+    unsigned xo[XL], wo[WL];
+#pragma unroll
+    for (unsigned j = 0; j < XL; ++j) {
+        const unsigned r = (j * Waves + wave) * 8 + lane / 8;
+        xo[j] = min(r, a.rows - 1 - tm) * pitch + ((lane % 8) ^ (r & 7)) * 16;
+    }
+#pragma unroll
+    for (unsigned j = 0; j < WL; ++j) {
+        const unsigned r = (j * Waves + wave) * 8 + lane / 8;
+        wo[j] = min(r, a.outer - 1 - tn) * pitch + ((lane % 8) ^ ((r & 3) | ((r >> 1) & 4))) * 16;
+    }
+    // Step k's bytes into stage s; past the last step the last one again, so that every wave has the
+    // same number of loads outstanding.
+    auto load = [&](unsigned k, unsigned s) {
+        std::uint8_t* to = lds + s * (BM + BN) * kBlock + wave * 1024;
+        const unsigned from = min(k, a.count - 1) * kBlock;
+#pragma unroll
+        for (unsigned j = 0; j < XL; ++j)
+            loadToLds(xr, to + j * Waves * 1024, xo[j], from);
+#pragma unroll
+        for (unsigned j = 0; j < WL; ++j)
+            loadToLds(wr, to + BM * kBlock + j * Waves * 1024, wo[j], from);
+    };
+    const unsigned wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    const unsigned l16 = lane % 16, g = lane / 16;
+    // Four steps' exponents a dword: of this lane's row of each X operand, and of the wave's weight tile.
+    const std::uint8_t* we = a.we + std::uint64_t(min((tn + wn) / kBlock, (a.outer - 1) / kBlock)) * a.expPitch;
+    const std::uint8_t* xe[MT];
+    unsigned xs[MT], ws, xsNext[MT], wsNext;
+#pragma unroll
+    for (unsigned m = 0; m < MT; ++m)
+        xe[m] = a.xe + std::uint64_t(min(tm + wm + m * 16 + l16, a.rows - 1)) * a.expPitch;
+    auto loadExponents = [&](unsigned k4) {
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) xsNext[m] = *reinterpret_cast<const unsigned*>(xe[m] + k4);
+        wsNext = *reinterpret_cast<const unsigned*>(we + k4);
+    };
+    f32x4 acc[NT][MT] = {};
+    loadExponents(0);
+#pragma unroll
+    for (unsigned s = 0; s + 1 < Stages; ++s) load(s, s);
+    const unsigned xKey = l16 & 7, wKey = (l16 & 3) | (l16 & 4);
+    const std::uint8_t* xRead = lds + (wm + l16) * kBlock;
+    const std::uint8_t* wRead = lds + BM * kBlock + (wn + l16 / 4 * 8 + l16 % 4) * kBlock;
+    auto step = [&](unsigned k, auto sel) {
+        constexpr unsigned S = decltype(sel)::value, at = S % Stages * (BM + BN) * kBlock;
+        waitBarrier<(Stages - 2) * (XL + WL)>();
+        load(k + Stages - 1, (S + Stages - 1) % Stages);
+        i32x8 xf[MT];
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m)
+            xf[m] = join(*reinterpret_cast<const u32x4*>(xRead + at + m * 16 * kBlock + ((g ^ xKey) * 16)),
+                         *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * kBlock + (((g + 4) ^ xKey) * 16)));
+#pragma unroll
+        for (unsigned n = 0; n < NT; ++n) {
+            const unsigned r = (n / 2 * 32 + n % 2 * 4) * kBlock;
+            const i32x8 wf = join(*reinterpret_cast<const u32x4*>(wRead + at + r + ((g ^ wKey) * 16)),
+                                  *reinterpret_cast<const u32x4*>(wRead + at + r + (((g + 4) ^ wKey) * 16)));
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m)
+                acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[m], acc[n][m], 0, 0, S, int(ws), S,
+                                                                             int(xs[m]));
+        }
+    };
+    auto nextExponents = [&](unsigned k4) {
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) xs[m] = xsNext[m];
+        ws = wsNext;
+        loadExponents(min(k4 + 4, (a.count - 1) / 4 * 4));
+    };
+    unsigned k = 0;
+    for (; k + 4 <= a.count; k += 4) {
+        nextExponents(k);
+        step(k, std::integral_constant<unsigned, 0>{});
+        step(k + 1, std::integral_constant<unsigned, 1>{});
+        step(k + 2, std::integral_constant<unsigned, 2>{});
+        step(k + 3, std::integral_constant<unsigned, 3>{});
+    }
+    if (k < a.count) {
+        nextExponents(k);
+        step(k, std::integral_constant<unsigned, 0>{});
+        if (k + 1 < a.count) step(k + 1, std::integral_constant<unsigned, 1>{});
+        if (k + 2 < a.count) step(k + 2, std::integral_constant<unsigned, 2>{});
+    }
+    // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+#pragma unroll
+    for (unsigned n = 0; n < NT; n += 2) {
+        const unsigned column = tn + wn + n * 16 + g * 8;
+        if (column >= a.outer) continue;
+        float b[8];
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) b[i] = a.bias ? a.bias[min(column + i, a.outer - 1)] : 0.0f;
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) {
+            const unsigned row = tm + wm + m * 16 + l16;
+            if (row >= a.rows) continue;
+            float v[8];
+#pragma unroll
+            for (unsigned i = 0; i < 8; ++i) v[i] = acc[n + i / 4][m][i % 4] + b[i];
+            store8<T>(y + row * a.yStride, column, a.outer, v);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// FP32 outputs: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
+// 128 x 128, steps of half a block: a row's 64 values are 128 bytes of LDS, stored in the chunk order of
+// the 8-bit kernel. Codes pass through registers to be converted.
+__global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
+    constexpr unsigned B = 128;
+    __shared__ __align__(1024) std::uint8_t lds[2][2][B * 128];
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave;
+    const unsigned tm = blockIdx.x % a.tilesM * B, tn = blockIdx.x / a.tilesM * B;
+    const unsigned pitch = a.count * kBlock;
+    const unsigned r = t / 4, part = t % 4; // 16 codes of rows r and r + 64 of each operand
+    const std::uint8_t *xp[2], *wp[2], *xep[2];
+#pragma unroll
+    for (unsigned h = 0; h < 2; ++h) {
+        const std::uint64_t xrow = min(tm + r + 64 * h, a.rows - 1);
+        xp[h] = a.x + xrow * pitch + part * 16;
+        xep[h] = a.xe + xrow * a.expPitch;
+        wp[h] = a.w + std::uint64_t(min(tn + r + 64 * h, a.outer - 1)) * pitch + part * 16;
+    }
+    const std::uint8_t* wep = a.we + std::uint64_t(tn / kBlock) * a.expPitch;
+    u32x4 xq[2], wq[2];
+    unsigned xb[2], wb;
+    auto fetch = [&](unsigned k) {
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            xq[h] = *reinterpret_cast<const u32x4*>(xp[h] + k * 64);
+            wq[h] = *reinterpret_cast<const u32x4*>(wp[h] + k * 64);
+            xb[h] = xep[h][k / 2];
+        }
+        wb = wep[k / 2];
+    };
+    auto put = [&](std::uint8_t* to, unsigned row, u32x4 q, float scale) {
+        *reinterpret_cast<bf16x8*>(to + row * 128 + ((2 * part) ^ (row & 7)) * 16) = values8(q.x, q.y, scale);
+        *reinterpret_cast<bf16x8*>(to + row * 128 + ((2 * part + 1) ^ (row & 7)) * 16) = values8(q.z, q.w, scale);
+    };
+    auto stash = [&](unsigned s) {
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            put(lds[s][0], r + 64 * h, xq[h], scaleOf(xb[h]));
+            put(lds[s][1], r + 64 * h, wq[h], scaleOf(wb));
+        }
+    };
+    const unsigned wm = wave % 2 * 64, wn = wave / 2 * 64, l16 = lane % 16, g = lane / 16;
+    f32x4 acc[4][4] = {};
+    const unsigned steps = 2 * a.count;
+    fetch(0);
+    stash(0);
+    __syncthreads();
+    for (unsigned k = 0; k < steps; ++k) {
+        if (k + 1 < steps) fetch(k + 1);
+        const std::uint8_t *bx = lds[k % 2][0], *bw = lds[k % 2][1];
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            bf16x8 xf[4];
+#pragma unroll
+            for (unsigned m = 0; m < 4; ++m) {
+                const unsigned row = wm + m * 16 + l16;
+                xf[m] = *reinterpret_cast<const bf16x8*>(bx + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
+            }
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) {
+                const unsigned row = wn + n * 16 + l16;
+                const bf16x8 wf = *reinterpret_cast<const bf16x8*>(bw + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
+#pragma unroll
+                for (unsigned m = 0; m < 4; ++m)
+                    acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[m], acc[n][m], 0, 0, 0);
+            }
+        }
+        if (k + 1 < steps) {
+            stash((k + 1) % 2);
+            __syncthreads();
+        }
+    }
+    float* y = static_cast<float*>(a.y);
+#pragma unroll
+    for (unsigned n = 0; n < 4; ++n) {
+        const unsigned column = tn + wn + n * 16 + g * 4;
+#pragma unroll
+        for (unsigned m = 0; m < 4; ++m) {
+            const unsigned row = tm + wm + m * 16 + l16;
+            if (row >= a.rows) continue;
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i)
+                if (column + i < a.outer)
+                    y[row * a.yStride + column + i] = acc[n][m][i] + (a.bias ? a.bias[column + i] : 0.0f);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few rows (single tokens, small batches): a workgroup takes 16 columns of y for all rows; its eight waves
+// share the blocks of the inner axis and add their sums through LDS in the waves' order. The weight's
+// codes go from memory to the MFMA's registers, each byte read once on the chip; a lane takes 32
+// consecutive codes of its row. Dense x is quantized by every workgroup for itself, in the operand's
+// layout: a row's block lies in lanes 16 apart.
+constexpr unsigned kTokenWaves = 8;
+
+template <typename T, unsigned MT, bool Dense>
+__global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) {
+    constexpr bool Exact = std::is_same<T, F32>::value;
+    __shared__ f32x4 sums[kTokenWaves][MT][kWave];
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave, l16 = lane % 16, g = lane / 16;
+    const unsigned n0 = blockIdx.x * 16;
+    const std::uint64_t pitch = std::uint64_t(a.count) * kBlock;
+    const std::uint8_t* wp = a.w + min(n0 + l16, a.outer - 1) * pitch + g * 32;
+    const std::uint8_t* wep = a.we + std::uint64_t(n0 / kBlock) * a.expPitch;
+    f32x4 acc[MT] = {};
+    for (unsigned k = wave; k < a.count; k += kTokenWaves) {
+        const u32x4 w0 = *reinterpret_cast<const u32x4*>(wp + k * kBlock);
+        const u32x4 w1 = *reinterpret_cast<const u32x4*>(wp + k * kBlock + 16);
+        const unsigned we = wep[k];
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) {
+            const unsigned row = m * 16 + l16;
+            u32x4 x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+            unsigned xe = 127;
+            if constexpr (Dense) {
+                float v[4][8];
+                unsigned peak = 0;
+                const auto* xp = static_cast<const typename T::Raw*>(a.dense) + min(row, a.rows - 1) * a.denseStride;
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) {
+                    load8<T>(xp, k * kBlock + g * 32 + i * 8, a.inner, v[i]);
+                    peak = max(peak, peakBits(v[i]));
+                }
+                peak = max(peak, unsigned(__shfl_xor(int(peak), 16)));
+                peak = max(peak, unsigned(__shfl_xor(int(peak), 32)));
+                xe = exponentOf<BlockCodes::e4m3>(peak);
+                const u32x2 q0 = encode8<BlockCodes::e4m3>(v[0], xe), q1 = encode8<BlockCodes::e4m3>(v[1], xe);
+                const u32x2 q2 = encode8<BlockCodes::e4m3>(v[2], xe), q3 = encode8<BlockCodes::e4m3>(v[3], xe);
+                x0 = u32x4{q0.x, q0.y, q1.x, q1.y};
+                x1 = u32x4{q2.x, q2.y, q3.x, q3.y};
+                if (a.keep && blockIdx.x == 0 && row < a.rows) {
+                    u32x4* to = reinterpret_cast<u32x4*>(a.keep + row * pitch + k * kBlock + g * 32);
+                    to[0] = x0;
+                    to[1] = x1;
+                    if (k + g < (k + 1 == a.count ? a.expPitch : k + 1))
+                        a.keepExp[std::uint64_t(row) * a.expPitch + k + g] = std::uint8_t(g ? 127u : xe);
+                }
+            } else {
+                const std::uint64_t at = min(row, a.rows - 1);
+                x0 = *reinterpret_cast<const u32x4*>(a.x + at * pitch + k * kBlock + g * 32);
+                x1 = *reinterpret_cast<const u32x4*>(a.x + at * pitch + k * kBlock + g * 32 + 16);
+                xe = a.xe[at * a.expPitch + k];
+            }
+            if constexpr (Exact) {
+                const float xs = scaleOf(xe), ws = scaleOf(we);
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) {
+                    const u32x4 wq = i < 2 ? w0 : w1, xq = i < 2 ? x0 : x1;
+                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values8(wq[i % 2 * 2], wq[i % 2 * 2 + 1], ws),
+                                                                     values8(xq[i % 2 * 2], xq[i % 2 * 2 + 1], xs),
+                                                                     acc[m], 0, 0, 0);
+                }
+            } else {
+                acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w0, w1), join(x0, x1), acc[m], 0, 0, 0,
+                                                                          int(we), 0, int(xe));
+            }
+        }
+    }
+#pragma unroll
+    for (unsigned m = 0; m < MT; ++m) sums[wave][m][lane] = acc[m];
+    __syncthreads();
+    // Output i of 256 * MT: column fastest.
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    for (unsigned i = t; i < 256 * MT; i += kWave * kTokenWaves) {
+        const unsigned column = i % 16, row = i / 16;
+        if (n0 + column >= a.outer || row >= a.rows) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][row / 16][row % 16 + column / 4 * 16][column % 4];
+        if (a.bias) s += a.bias[n0 + column];
+        y[row * a.yStride + n0 + column] = T::put(s);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+
+constexpr unsigned kTokenRows = 64;
+
+template <typename T, bool Dense> void launchTokens(const Product& p, hipStream_t stream) {
+    const dim3 grid((p.outer + 15) / 16), threads(kWave * kTokenWaves);
+    if (p.rows <= 16)
+        hipLaunchKernelGGL((multiplyTokens<T, 1, Dense>), grid, threads, 0, stream, p);
+    else if (p.rows <= 32)
+        hipLaunchKernelGGL((multiplyTokens<T, 2, Dense>), grid, threads, 0, stream, p);
+    else
+        hipLaunchKernelGGL((multiplyTokens<T, 4, Dense>), grid, threads, 0, stream, p);
+    checkHip(hipGetLastError());
+}
+
+template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages>
+void launchTiles(Product p, hipStream_t stream) {
+    p.tilesM = (p.rows + BM - 1) / BM;
+    const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + BN - 1) / BN);
+    const std::size_t lds = Stages * (BM + BN) * kBlock;
+    if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+    hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages>), dim3(unsigned(tiles)), dim3(64 * WM * WN), lds,
+                       stream, p);
+    checkHip(hipGetLastError());
+}
+
+template <typename T> void launchProduct(Product p, hipStream_t stream) {
+    if (p.rows <= kTokenRows) return launchTokens<T, false>(p, stream);
+    if constexpr (std::is_same<T, F32>::value) {
+        p.tilesM = (p.rows + 127) / 128;
+        const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + 127) / 128);
+        if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+        hipLaunchKernelGGL(multiplyTilesExact, dim3(unsigned(tiles)), dim3(256), 0, stream, p);
+        checkHip(hipGetLastError());
+    } else {
+        launchTiles<T, 128, 128, 2, 2, 2>(p, stream);
+    }
+}
+
+void checkWeight(const char* where, const BlockWeightView& w, const float* bias) {
+    checkCodes(where, w.codes, w.exponents);
+    if (reinterpret_cast<std::uintptr_t>(bias) % 4) reject(where, "bias not float-aligned");
+}
+
+} // namespace
+
+std::size_t matmulBlocksWorkspace(std::uint32_t, std::uint32_t, std::uint32_t, DenseType) { return 0; }
+
+void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, DenseType type, std::uint64_t stride,
+                  std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, void*, std::size_t,
+                  hipStream_t stream) {
+    const char* where = "matmul blocks";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkRows(where, rows);
+    if (x.type != BlockCodes::e4m3) reject(where, "x must have E4M3 codes");
+    checkType(where, type);
+    if (!rows) return;
+    checkCodes(where, x.codes, x.exponents);
+    checkWeight(where, w, bias);
+    checkDense(where, y, stride, type, outer);
+    Product p = {};
+    p.x = x.codes, p.xe = x.exponents, p.w = w.codes, p.we = w.exponents, p.bias = bias;
+    p.y = y, p.yStride = stride, p.rows = rows, p.outer = outer, p.inner = inner;
+    p.count = (inner + kBlock - 1) / kBlock;
+    p.expPitch = unsigned(blockExponentPitch(inner));
+    withType(type, [&](auto tag) { launchProduct<decltype(tag)>(p, stream); });
+}
+
+namespace {
+bool fusedTokens(std::uint32_t rows) { return rows <= kTokenRows; }
+
+std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
+} // namespace
+
+std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
+                                  bool keep) {
+    std::size_t bytes = matmulBlocksWorkspace(rows, inner, outer, type);
+    if (!keep && !fusedTokens(rows))
+        bytes += rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
+    return bytes;
+}
+
+void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, std::uint64_t yStride, BlockRows keep,
+                  std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, void* workspace,
+                  std::size_t workspaceBytes, hipStream_t stream) {
+    const char* where = "linear blocks";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkRows(where, rows);
+    checkType(where, x.type);
+    if (!keep.codes != !keep.exponents) reject(where, "kept codes and exponents come together");
+    if (keep.codes && keep.type != BlockCodes::e4m3) reject(where, "kept blocks must have E4M3 codes");
+    if (!rows) return;
+    checkDense(where, x.data, x.stride, x.type, inner);
+    checkDense(where, y, yStride, x.type, outer);
+    checkWeight(where, w, bias);
+    if (keep.codes) checkCodes(where, keep.codes, keep.exponents);
+    const std::size_t need = linearBlocksWorkspace(rows, inner, outer, x.type, keep.codes);
+    if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
+    if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
+    if (fusedTokens(rows)) {
+        Product p = {};
+        p.w = w.codes, p.we = w.exponents, p.bias = bias, p.y = y, p.yStride = yStride;
+        p.rows = rows, p.outer = outer, p.inner = inner;
+        p.count = (inner + kBlock - 1) / kBlock;
+        p.expPitch = unsigned(blockExponentPitch(inner));
+        p.dense = x.data, p.denseStride = x.stride, p.keep = keep.codes, p.keepExp = keep.exponents;
+        withType(x.type, [&](auto tag) { launchTokens<decltype(tag), true>(p, stream); });
+        return;
+    }
+    auto* spare = static_cast<std::uint8_t*>(workspace);
+    if (!keep.codes) {
+        keep = {spare, spare + rounded(rows * blockCodePitch(inner)), BlockCodes::e4m3};
+        const std::size_t used = rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
+        spare += used, workspaceBytes -= used;
+    }
+    quantizeBlocks(x, keep, rows, inner, stream);
+    matmulBlocks(keep, w, bias, y, x.type, yStride, rows, inner, outer, spare, workspaceBytes, stream);
+}

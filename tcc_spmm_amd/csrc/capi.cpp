@@ -3,6 +3,7 @@
 // class into a status code, keeping the message for tcc_last_error().
 #include "tcc_spmm_c.h"
 
+#include "blocks.h"
 #include "device_matrix.h"
 #include "format/csr.h"
 #include "format/int8_features.h"
@@ -59,6 +60,9 @@ template <typename Body> int guarded(Body body) {
 void need(const void* p, const char* what) {
     if (!p) throw std::invalid_argument(std::string("null ") + what);
 }
+
+// The library's functions only read through the pointers of an input's blocks.
+std::uint8_t* input(const uint8_t* p) { return const_cast<std::uint8_t*>(p); }
 
 Sw32DeviceView toView(const tcc_device_view* v) {
     Sw32DeviceView out;
@@ -247,6 +251,105 @@ int tcc_quantize_pack_features_int8(const float* x, int8_t* packed, float* scale
                                     uint32_t features, void* stream) {
     return guarded([&] {
         quantizePackFeaturesInt8(x, packed, scale, sources, features,
+                                 static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_quantize_blocks(const void* x, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                        uint32_t codeType, uint32_t rows, uint32_t columns, void* stream) {
+    return guarded([&] {
+        quantizeBlocks({x, stride, DenseType(type)}, {codes, exponents, BlockCodes(codeType)}, rows, columns,
+                       static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_dequantize_blocks(const uint8_t* codes, const uint8_t* exponents, uint32_t codeType, void* out,
+                          uint64_t stride, uint32_t type, uint32_t rows, uint32_t columns, void* stream) {
+    return guarded([&] {
+        dequantizeBlocks({input(codes), input(exponents), BlockCodes(codeType)}, out, DenseType(type), stride, rows,
+                         columns, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_quantize_weight_blocks(const void* w, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                               uint8_t* codesT, uint8_t* exponentsT, uint32_t outer, uint32_t inner,
+                               void* stream) {
+    return guarded([&] {
+        quantizeWeightBlocks({w, stride, DenseType(type)}, {codes, exponents, codesT, exponentsT}, outer, inner,
+                             static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_matmul_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = matmulBlocksWorkspace(rows, inner, outer, DenseType(type));
+    });
+}
+
+int tcc_matmul_blocks(const uint8_t* xCodes, const uint8_t* xExponents, const uint8_t* wCodes,
+                      const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type,
+                      uint32_t rows, uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes,
+                      void* stream) {
+    return guarded([&] {
+        matmulBlocks({input(xCodes), input(xExponents), BlockCodes::e4m3},
+                     {input(wCodes), input(wExponents), nullptr, nullptr}, bias, y, DenseType(type), stride, rows,
+                     inner, outer, workspace, workspaceBytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_linear_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, int keep,
+                                size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = linearBlocksWorkspace(rows, inner, outer, DenseType(type), keep != 0);
+    });
+}
+
+int tcc_linear_blocks(const void* x, uint64_t stride, uint32_t type, const uint8_t* wCodes,
+                      const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride,
+                      uint8_t* keepCodes, uint8_t* keepExponents, uint32_t rows, uint32_t inner, uint32_t outer,
+                      void* workspace, size_t workspaceBytes, void* stream) {
+    return guarded([&] {
+        linearBlocks({x, stride, DenseType(type)}, {input(wCodes), input(wExponents), nullptr, nullptr}, bias, y,
+                     yStride, {keepCodes, keepExponents, BlockCodes::e4m3}, rows, inner, outer, workspace,
+                     workspaceBytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_weight_grad_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type,
+                                     size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = weightGradBlocksWorkspace(rows, inner, outer, DenseType(type));
+    });
+}
+
+int tcc_weight_grad_blocks(const void* dy, uint64_t stride, uint32_t type, const uint8_t* xCodes,
+                           const uint8_t* xExponents, float* dw, float* db, uint32_t rows, uint32_t inner,
+                           uint32_t outer, void* workspace, size_t workspaceBytes, void* stream) {
+    return guarded([&] {
+        weightGradBlocks({dy, stride, DenseType(type)}, {input(xCodes), input(xExponents), BlockCodes::e4m3}, dw, db,
+                         rows, inner, outer, workspace, workspaceBytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_activation_blocks(const void* x, uint64_t stride, uint32_t type, uint32_t kind, int gated, void* y,
+                          uint64_t yStride, uint8_t* keepCodes, uint8_t* keepExponents, uint32_t codeType,
+                          uint32_t rows, uint32_t width, void* stream) {
+    return guarded([&] {
+        activationBlocks({x, stride, DenseType(type)}, BlockActivation(kind), gated != 0, y, yStride,
+                         {keepCodes, keepExponents, BlockCodes(codeType)}, rows, width,
+                         static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_activation_blocks_backward(const void* dy, uint64_t stride, uint32_t type, const uint8_t* codes,
+                                   const uint8_t* exponents, uint32_t codeType, uint32_t kind, int gated, void* dx,
+                                   uint64_t dxStride, uint32_t rows, uint32_t width, void* stream) {
+    return guarded([&] {
+        activationBlocksBackward({dy, stride, DenseType(type)}, {input(codes), input(exponents), BlockCodes(codeType)},
+                                 BlockActivation(kind), gated != 0, dx, dxStride, rows, width,
                                  static_cast<hipStream_t>(stream));
     });
 }
