@@ -180,11 +180,12 @@ def _ring_waits(instrs, labels, asm_blocks, rows):
     return found
 
 
-def check(asm_text: str) -> list:
-    """Problems in every kernel of a gfx950 assembly listing (hipcc --cuda-device-only -S)."""
+def check(asm_text: str, kernels: str = "Kernel") -> list:
+    """Problems in every kernel of a gfx950 assembly listing (hipcc --cuda-device-only -S) whose name
+    contains `kernels`; spills are looked for in all of them."""
     lines = asm_text.split("\n")
     problems = []
-    starts = [k for k, l in enumerate(lines) if re.match(r"^_Z\S+:", l) and "Kernel" in l]
+    starts = [k for k, l in enumerate(lines) if re.match(r"^_Z\S+:", l) and kernels in l]
     for k in starts:
         name = lines[k].split(":")[0]
         end = next((j for j in range(k, len(lines)) if lines[j].startswith(".Lfunc_end")), len(lines))

@@ -68,13 +68,28 @@ def check_kernel_asm(src: pathlib.Path = CSRC / "kernel" / "spmm.hip") -> None:
         raise RuntimeError("SpMM kernel assembly check failed:\n  " + "\n  ".join(problems))
 
 
+def check_product_asm(src: pathlib.Path = CSRC / "blocks" / "product.hip") -> None:
+    """The same for the product of 8-bit blocks: multiplyWide's MFMAs are inline assembly, whose latency
+    the compiler does not know."""
+    from . import asm_check
+    out = BUILD / "product-gfx950.s"
+    cmd = [str(ROCM / "bin" / "hipcc"), *HIP_FLAGS, "--cuda-device-only", "-S", str(src), "-o", str(out)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"assembly listing failed: {shlex.join(cmd)}\n{res.stderr}")
+    problems = asm_check.check(out.read_text(), "multiplyWide")
+    if problems:
+        raise RuntimeError("Block product assembly check failed:\n  " + "\n  ".join(problems))
+
+
 def build(verbose: bool = False) -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
-        asm = pool.submit(check_kernel_asm)
+        checks = [pool.submit(check_kernel_asm), pool.submit(check_product_asm)]
         objs = list(pool.map(_compile, srcs))
-        asm.result()
+        for check in checks:
+            check.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [str(ROCM / "bin" / "hipcc"), "-shared", f"--offload-arch={ARCH}", "-fPIC", "-o", str(tmp),
            *map(str, objs), "-lpthread"]

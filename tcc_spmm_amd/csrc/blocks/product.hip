@@ -18,7 +18,7 @@ struct Product {
     void* y;
     std::uint64_t yStride;
     unsigned rows, outer, count, expPitch; // count: blocks of a row; code rows are 128 * count bytes
-    unsigned inner, tilesM;
+    unsigned inner, tilesM, tilesN;
     const void* dense;
     std::uint64_t denseStride;
     std::uint8_t *keep, *keepExp;
@@ -42,10 +42,60 @@ __device__ __forceinline__ void loadToLds(__amdgpu_buffer_rsrc_t rsrc, std::uint
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)to, 16, lane, uniform, 0, 0);
 }
 
+// Eight consecutive outputs, columns [at, at + 8) of a row of n, with the bias added. Plain stores: the
+// L2 puts the lines together that several stores of a wave fill.
+template <typename T, bool Whole>
+__device__ __forceinline__ void put8(typename T::Raw* row, unsigned at, unsigned n, const float (&v)[8], const float (&b)[8]) {
+    typename Group<T>::Vec g;
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) g[i] = T::put(v[i] + b[i]);
+    if (Whole || at + 8 <= n) {
+        *reinterpret_cast<typename Group<T>::Loose*>(row + at) = g;
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i)
+            if (at + i < n) row[at + i] = g[i];
+    }
+}
+
+// bias[at .. at + 8), or zeros without one or past its end.
+template <bool Whole> __device__ __forceinline__ void bias8(const float* bias, unsigned at, unsigned n, float (&b)[8]) {
+    typedef f32x4 Loose4 __attribute__((aligned(4)));
+    if (!bias) {
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) b[i] = 0.0f;
+    } else if (Whole || at + 8 <= n) {
+        const f32x4 lo = *reinterpret_cast<const Loose4*>(bias + at), hi = *reinterpret_cast<const Loose4*>(bias + at + 4);
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i) b[i] = lo[i], b[4 + i] = hi[i];
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) b[i] = at + i < n ? bias[at + i] : 0.0f;
+    }
+}
+
 // Waits until at most N of this wave's memory loads are outstanding and its LDS reads are done, then
 // for the workgroup. One asm block with a memory clobber, so that no access moves across it.
 template <unsigned N> __device__ __forceinline__ void waitBarrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Rows from `first` on of a matrix of `rows` rows of `pitch` bytes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rowsAt(const std::uint8_t* p, unsigned pitch, unsigned first, unsigned rows) {
+    const std::uint64_t bytes = std::uint64_t(rows - first) * pitch;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p) + std::uint64_t(first) * pitch, 0,
+                                             unsigned(min(bytes, std::uint64_t(0x7FFFFFFF))), 0x00020000);
+}
+
+// The tile of a workgroup, as (row tile) + tilesM * (column tile). Workgroups go round the eight XCDs, each
+// with an L2 of its own: an XCD gets a run of tiles that walks bands of eight row tiles, so that the tiles
+// it works on at once share rows of both operands.
+__device__ __forceinline__ unsigned tileOf(unsigned id, unsigned total, unsigned tilesM, unsigned tilesN) {
+    const unsigned xcd = id % 8, each = total / 8, more = total % 8;
+    const unsigned i = xcd * each + min(xcd, more) + id / 8;
+    const unsigned band = i / (8 * tilesN), in = i - band * 8 * tilesN;
+    const unsigned high = min(8u, tilesM - 8 * band);
+    return 8 * band + in % high + tilesM * (in / high);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -66,24 +116,17 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
     static_assert(BN / WN <= 128 && NT % 2 == 0, "a wave's columns share a weight tile");
     extern __shared__ __align__(1024) std::uint8_t lds[];
     const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const unsigned tm = blockIdx.x % a.tilesM * BM, tn = blockIdx.x / a.tilesM * BN;
+    const unsigned tile = tileOf(blockIdx.x, gridDim.x, a.tilesM, a.tilesN);
+    const unsigned tm = tile % a.tilesM * BM, tn = tile / a.tilesM * BN;
     const unsigned pitch = a.count * kBlock;
-    const auto xr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<std::uint8_t*>(a.x) + std::uint64_t(tm) * pitch, 0, 0x7FFFFFFF, 0x00020000);
-    const auto wr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<std::uint8_t*>(a.w) + std::uint64_t(tn) * pitch, 0, 0x7FFFFFFF, 0x00020000);
-    // Rows past the end read the last row; their results are not stored.
-    unsigned xo[XL], wo[WL];
-#pragma unroll
-    for (unsigned j = 0; j < XL; ++j) {
-        const unsigned r = (j * Waves + wave) * 8 + lane / 8;
-        xo[j] = min(r, a.rows - 1 - tm) * pitch + ((lane % 8) ^ (r & 7)) * 16;
-    }
-#pragma unroll
-    for (unsigned j = 0; j < WL; ++j) {
-        const unsigned r = (j * Waves + wave) * 8 + lane / 8;
-        wo[j] = min(r, a.outer - 1 - tn) * pitch + ((lane % 8) ^ ((r & 3) | ((r >> 1) & 4))) * 16;
-    }
+    // Rows past the end are past the buffer and read as zeros; their results are not stored.
+    const auto xr = rowsAt(a.x, pitch, tm, a.rows), wr = rowsAt(a.w, pitch, tn, a.outer);
+    // A load fills 8 rows of LDS in order, 16 bytes a lane, so a lane fetches the chunk that belongs in its
+    // place; a wave's loads are 8 * Waves rows apart, which leaves the rows' keys the same.
+    static_assert(Waves % 2 == 0, "the weight's key takes bit 3 of the row");
+    const unsigned r = wave * 8 + lane / 8;
+    const unsigned xo = r * pitch + ((lane % 8) ^ (r & 7)) * 16;
+    const unsigned wo = r * pitch + ((lane % 8) ^ ((r & 3) | ((r >> 1) & 4))) * 16;
     // Step k's bytes into stage s; past the last step the last one again, so that every wave has the
     // same number of loads outstanding.
     auto load = [&](unsigned k, unsigned s) {
@@ -91,10 +134,10 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
         const unsigned from = min(k, a.count - 1) * kBlock;
 #pragma unroll
         for (unsigned j = 0; j < XL; ++j)
-            loadToLds(xr, to + j * Waves * 1024, xo[j], from);
+            loadToLds(xr, to + j * Waves * 1024, xo, from + j * Waves * 8 * pitch);
 #pragma unroll
         for (unsigned j = 0; j < WL; ++j)
-            loadToLds(wr, to + BM * kBlock + j * Waves * 1024, wo[j], from);
+            loadToLds(wr, to + BM * kBlock + j * Waves * 1024, wo, from + j * Waves * 8 * pitch);
     };
     const unsigned wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
     const unsigned l16 = lane % 16, g = lane / 16;
@@ -160,23 +203,200 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
     // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    auto store = [&](auto whole) {
+        constexpr bool Whole = decltype(whole)::value;
 #pragma unroll
-    for (unsigned n = 0; n < NT; n += 2) {
-        const unsigned column = tn + wn + n * 16 + g * 8;
-        if (column >= a.outer) continue;
-        float b[8];
+        for (unsigned n = 0; n < NT; n += 2) {
+            const unsigned column = tn + wn + n * 16 + g * 8;
+            float b[8];
+            bias8<Whole>(a.bias, column, a.outer, b);
 #pragma unroll
-        for (unsigned i = 0; i < 8; ++i) b[i] = a.bias ? a.bias[min(column + i, a.outer - 1)] : 0.0f;
+            for (unsigned m = 0; m < MT; ++m) {
+                const unsigned row = tm + wm + m * 16 + l16;
+                float v[8];
 #pragma unroll
-        for (unsigned m = 0; m < MT; ++m) {
-            const unsigned row = tm + wm + m * 16 + l16;
-            if (row >= a.rows) continue;
-            float v[8];
-#pragma unroll
-            for (unsigned i = 0; i < 8; ++i) v[i] = acc[n + i / 4][m][i % 4] + b[i];
-            store8<T>(y + row * a.yStride, column, a.outer, v);
+                for (unsigned i = 0; i < 8; ++i) v[i] = acc[n + i / 4][m][i % 4];
+                if (Whole || row < a.rows) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
+            }
         }
+    };
+    if (tm + BM <= a.rows && tn + BN <= a.outer)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
+}
+
+// acc += a b with the operands' scales in byte S of `as` and `bs`, in the accumulation registers. Where
+// accumulators fill them, the compiler moves them about between MFMAs; asm with one operand for both the
+// sum and the result does not let it. The compiler does not know this instruction's latency: whoever
+// reads acc has to let the last one finish.
+template <unsigned S>
+__device__ __forceinline__ void multiplyInPlace(f32x4& acc, i32x8 a, i32x8 b, unsigned as, unsigned bs) {
+    static_assert(S < 2, "the bytes that the two forms below select");
+    if constexpr (S == 0)
+        asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+            : "+a"(acc) : "v"(a), "v"(b), "v"(as), "v"(bs));
+    else
+        asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+            : "+a"(acc) : "v"(a), "v"(b), "v"(as), "v"(bs));
+}
+
+// The same on tiles of 256 x 256, for products with enough of them: a CU can then multiply twice as long on
+// every byte it loads (a tile of 128 x 128 needs 64 bytes a clock, all that a CU can load).
+// Four waves, one a SIMD, of 128 x 128 each, whose accumulators fill the accumulation registers. LDS holds two
+// stages of a block. A block is multiplied in four quarters, a pair of the weight's operands with all of
+// x's in each: in a quarter the next pair is read from LDS, and in the last one also, as each operand of
+// x is used for the last time, its place is filled with the next block's. So no MFMA waits for LDS. The
+// loads into LDS are spread over the quarters, each into a place that was read for the last time a
+// quarter or more before, and each has at least a block's time to arrive:
+//   quarter 0: pairs 2 and 3 of block k + 1;  1 and 2: x of block k + 2;  3: pairs 0 and 1 of block k + 2
+// with a barrier before quarters 1 and 3.
+// The 16 x 16 MFMA is the one to feed: on random codes the card's power holds the scaled 32 x 32 x 64 to 3.2
+// PFLOP/s and the scaled 16 x 16 x 128 to 3.8 (on zeros both reach 4.7).
+template <typename T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void multiplyWide(Product a) {
+    constexpr unsigned B = 256, Stage = 2 * B * kBlock, Tiles = 8;
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages: 256 rows of x, 256 of w
+    const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned tile = tileOf(blockIdx.x, gridDim.x, a.tilesM, a.tilesN);
+    const unsigned tm = tile % a.tilesM * B, tn = tile / a.tilesM * B;
+    const unsigned pitch = a.count * kBlock;
+    const auto xr = rowsAt(a.x, pitch, tm, a.rows), wr = rowsAt(a.w, pitch, tn, a.outer);
+    // Chunks and rows are dealt as in multiplyTiles.
+    auto keyX = [](unsigned r) { return r & 7; };
+    auto keyW = [](unsigned r) { return (r & 3) | (r >> 1 & 4); };
+    const unsigned fill = wave * 8 + lane / 8; // a wave's loads are 32 rows apart, with the same keys
+    const unsigned xo = fill * pitch + ((lane % 8) ^ keyX(fill)) * 16;
+    const unsigned wo = fill * pitch + ((lane % 8) ^ keyW(fill)) * 16;
+    // An eighth of block k's rows of x or w into stage s; past the last block zeros, from beyond the buffer.
+    auto from = [&](unsigned k) { return k < a.count ? k * kBlock : 0x7FFFFFFFu; };
+    auto loadX = [&](unsigned k, unsigned s, unsigned part) {
+        loadToLds(xr, lds + s * Stage + wave * 1024 + part * 4096, xo, from(k) + part * 32 * pitch);
+    };
+    auto loadW = [&](unsigned k, unsigned s, unsigned part) {
+        loadToLds(wr, lds + s * Stage + B * kBlock + wave * 1024 + part * 4096, wo, from(k) + part * 32 * pitch);
+    };
+    const unsigned wm = wave % 2 * 128, wn = wave / 2 * 128, l16 = lane % 16, g = lane / 16;
+    const unsigned wRow = l16 / 4 * 8 + l16 % 4;
+    // A lane's two chunks of its row in either stage: bytes of LDS, which the loads' offsets reach a stage of.
+    unsigned xRead[2][2], wRead[2][2];
+#pragma unroll
+    for (unsigned s = 0; s < 2; ++s)
+#pragma unroll
+        for (unsigned c = 0; c < 2; ++c) {
+            xRead[s][c] = s * Stage + (wm + l16) * kBlock + ((g + 4 * c) ^ keyX(l16)) * 16;
+            wRead[s][c] = s * Stage + (B + wn + wRow) * kBlock + ((g + 4 * c) ^ keyW(wRow)) * 16;
+            asm("" : "+v"(xRead[s][c]), "+v"(wRead[s][c])); // kept, not computed again for every load
+        }
+    i32x8 xf[Tiles], wf[2][2];
+    auto readX = [&](unsigned s, unsigned m) {
+        const std::uint8_t* at = lds + m * 16 * kBlock;
+        xf[m] = join(*reinterpret_cast<const u32x4*>(at + xRead[s][0]), *reinterpret_cast<const u32x4*>(at + xRead[s][1]));
+    };
+    auto readW = [&](unsigned s, unsigned n) {
+        const std::uint8_t* at = lds + (n / 2 * 32 + n % 2 * 4) * kBlock;
+        wf[n / 2 % 2][n % 2] =
+            join(*reinterpret_cast<const u32x4*>(at + wRead[s][0]), *reinterpret_cast<const u32x4*>(at + wRead[s][1]));
+    };
+    const auto er = rowsAt(a.xe, a.expPitch, tm, a.rows);
+    const std::uint8_t* we = a.we + std::uint64_t(min((tn + wn) / kBlock, (a.outer - 1) / kBlock)) * a.expPitch;
+    // Two blocks' exponents at a time, a byte each.
+    unsigned xs[Tiles], ws, xsNext[Tiles], wsNext;
+    auto loadExponents = [&](unsigned block) {
+        block = min(block, (a.count - 1) / 2 * 2);
+#pragma unroll
+        for (unsigned m = 0; m < Tiles; ++m)
+            xsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(er, (wm + l16) * a.expPitch, m * 16 * a.expPitch + block, 0);
+        wsNext = *reinterpret_cast<const unsigned short*>(we + block);
+    };
+    f32x4 acc[Tiles][Tiles] = {};
+    loadExponents(0);
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) loadX(0, 0, i), loadW(0, 0, i);
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) loadX(1, 1, i);
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) loadW(1, 1, i / 2 + i % 2 * 4);
+    waitBarrier<12>();
+#pragma unroll
+    for (unsigned i = 0; i < 2; ++i) readW(0, i);
+#pragma unroll
+    for (unsigned i = 0; i < Tiles; ++i) readX(0, i);
+    // Block S of the pair that the exponents are for. The fences keep the compiler from moving the reads and
+    // loads between the MFMAs down to where their results are needed, which is where they would be
+    // waited for.
+    auto blockStep = [&](unsigned k, auto block) {
+        constexpr unsigned S = decltype(block)::value;
+        auto multiply = [&](unsigned m, unsigned n0) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (unsigned n = n0; n < n0 + 2; ++n)
+                multiplyInPlace<S>(acc[n][m], wf[n / 2 % 2][n % 2], xf[m], ws, xs[m]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // Pair p of the weight's operands lies in eighths p and p + 4: waves start at row 0 or 128.
+#pragma unroll
+        for (unsigned q = 0; q < 4; ++q) {
+            // Before quarter 1 pairs 2 and 3 of this block have to be there, before 3 x and pair 0 of the next. What
+            // was loaded since stays outstanding, and in a pair's first block the exponents.
+            if (q == 1) waitBarrier<S == 0 ? 25 : 16>();
+            if (q == 3) waitBarrier<S == 0 ? 21 : 12>();
+#pragma unroll
+            for (unsigned m = 0; m < Tiles; ++m) {
+                if (m % 4 == 0) {
+                    if (q < 3)
+                        readW(S, 2 * q + 2 + m / 4);
+                    else
+                        readW(1 - S, m / 4);
+                }
+                if (m % 2 == 1) {
+                    const unsigned i = m / 2, eighth = i / 2 + i % 2 * 4;
+                    if (q == 0) loadW(k + S + 1, 1 - S, 2 + eighth);
+                    if (q == 1) loadX(k + S + 2, S, i);
+                    if (q == 2) loadX(k + S + 2, S, 4 + i);
+                    if (q == 3) loadW(k + S + 2, S, eighth);
+                }
+                multiply(m, 2 * q);
+                if (q == 3) readX(1 - S, m);
+            }
+        }
+        // Where the loop ends the compiler copies the sums, without knowing that they come from an MFMA: the last
+        // ones, of 8 passes, have to be done by then.
+        if (S == 1)
+            asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[6][6]), "+a"(acc[7][6]), "+a"(acc[6][7]), "+a"(acc[7][7]));
+    };
+    for (unsigned k = 0; k < a.count; k += 2) {
+#pragma unroll
+        for (unsigned m = 0; m < Tiles; ++m) xs[m] = xsNext[m];
+        ws = wsNext;
+        loadExponents(k + 2);
+        blockStep(k, std::integral_constant<unsigned, 0>{});
+        blockStep(k, std::integral_constant<unsigned, 1>{});
     }
+    // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    auto store = [&](auto whole) {
+        constexpr bool Whole = decltype(whole)::value;
+#pragma unroll
+        for (unsigned n = 0; n < Tiles; n += 2) {
+            const unsigned column = tn + wn + n * 16 + g * 8;
+            float b[8];
+            bias8<Whole>(a.bias, column, a.outer, b);
+#pragma unroll
+            for (unsigned m = 0; m < Tiles; ++m) {
+                const unsigned row = tm + wm + m * 16 + l16;
+                float v[8];
+#pragma unroll
+                for (unsigned j = 0; j < 8; ++j) v[j] = acc[n + j / 4][m][j % 4];
+                if (Whole || row < a.rows) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
+            }
+        }
+    };
+    if (tm + B <= a.rows && tn + B <= a.outer)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -371,14 +591,42 @@ template <typename T, bool Dense> void launchTokens(const Product& p, hipStream_
     checkHip(hipGetLastError());
 }
 
+// The tile of a product: the least estimated time, in microseconds, rounds of workgroups on the chip times the
+// blocks of the inner axis. A CU holds one workgroup of tiles of 256, two of 128 or 64. The constants fit
+// these times (rows x inner x outer: 256, 128, 64):
+//   4096 x 4096 x 8192 122, 192, 269    2048 x 1024 x 4096 22, 15.2, 20     2048 x 4096 x 1024 49, 28.8, 17.7
+//   1024 x 4096 x 4096 51, 31.3, 32.3   512 x 4096 x 4096 48, 26.9, 18.1    16384 x 512 x 512 16, 10.9, 14.4
+//   777 x 1001 x 1437 23, 9.9, 6.9      300 x 2000 x 6000 31, 13.8, 9.5     100000 x 256 x 256 29, 20.9, 30.7
+enum class Form { wide, middle, small };
+Form formOf(std::uint32_t rows, std::uint32_t outer, unsigned count) {
+    const auto tiles = [&](unsigned size) {
+        return std::uint64_t((rows + size - 1) / size) * ((outer + size - 1) / size);
+    };
+    const auto rounds = [](std::uint64_t n, unsigned slots) { return double((n + slots - 1) / slots); };
+    const std::uint64_t large = tiles(256), half = tiles(128), quarter = tiles(64);
+    const double wide = rounds(large, 256) * (11.5 + 1.5 * count);
+    const double middle = half <= 256 ? 5.0 + 0.75 * count : rounds(half, 512) * (5.0 + 1.3 * count);
+    const double small = quarter <= 256 ? 2.2 + 0.25 * count : rounds(quarter, 512) * (1.5 + 0.5 * count);
+    if (wide <= middle && wide <= small) return Form::wide;
+    return middle <= small ? Form::middle : Form::small;
+}
+
 template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages>
 void launchTiles(Product p, hipStream_t stream) {
-    p.tilesM = (p.rows + BM - 1) / BM;
-    const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + BN - 1) / BN);
+    p.tilesM = (p.rows + BM - 1) / BM, p.tilesN = (p.outer + BN - 1) / BN;
+    const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
     const std::size_t lds = Stages * (BM + BN) * kBlock;
     if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
     hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages>), dim3(unsigned(tiles)), dim3(64 * WM * WN), lds,
                        stream, p);
+    checkHip(hipGetLastError());
+}
+
+template <typename T> void launchWide(Product p, hipStream_t stream) {
+    p.tilesM = (p.rows + 255) / 256, p.tilesN = (p.outer + 255) / 256;
+    const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
+    if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+    hipLaunchKernelGGL((multiplyWide<T>), dim3(unsigned(tiles)), dim3(256), 2 * 2 * 256 * kBlock, stream, p);
     checkHip(hipGetLastError());
 }
 
@@ -391,7 +639,11 @@ template <typename T> void launchProduct(Product p, hipStream_t stream) {
         hipLaunchKernelGGL(multiplyTilesExact, dim3(unsigned(tiles)), dim3(256), 0, stream, p);
         checkHip(hipGetLastError());
     } else {
-        launchTiles<T, 128, 128, 2, 2, 2>(p, stream);
+        switch (formOf(p.rows, p.outer, p.count)) {
+        case Form::wide: launchWide<T>(p, stream); break;
+        case Form::middle: launchTiles<T, 128, 128, 4, 2, 2>(p, stream); break;
+        case Form::small: launchTiles<T, 64, 64, 2, 2, 4>(p, stream); break;
+        }
     }
 }
 

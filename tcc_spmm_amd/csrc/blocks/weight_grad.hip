@@ -1,112 +1,161 @@
 // The weight gradient dw = dy^T x from dense dy and the 8-bit blocks of x that the forward pass kept, and
 // the bias gradient (include/blocks.h).
 //
-// Both operands run along the rows, the axis of the sum, so an MFMA operand is a column of each: tiles of
-// 64 rows lie in LDS as they do in memory and are read with the transposing LDS load. x is converted to
-// bf16 on its way into LDS, exactly, its scales multiplied in. dy goes in as bf16 parts: itself, or for f16 two and
-// for f32 three parts of 8 bits each, every part the rest's nearest bf16; their products with x add
+// Both operands run along the rows, the axis of the sum, so an MFMA operand is a column of each: 64 rows
+// of a tile lie in LDS as they do in memory and are read with the transposing LDS load. x is converted to
+// bf16 on its way into LDS, exactly, its scales multiplied in. dy goes in as bf16 parts: itself, or for f16 two
+// and for f32 three parts of 8 bits each, every part the rest's nearest bf16; their products with x add
 // in the same FP32 accumulator, so an f32 gradient keeps its precision at three times the MFMA work.
-// The rows are split over workgroups, since a weight has few tiles; each writes its FP32 sums and a second
-// kernel adds the splits in order.
+// The bias gradient is the product of dy with a column of ones, an operand that needs no memory.
+// The rows are split over workgroups where a weight has few tiles; each writes its FP32 sums and a second
+// kernel adds the splits in order, so repeated calls give the same bits.
 #include "device_blocks.h"
 #include "hip_support.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
 using namespace blocks;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* LdsColumn;
 
-constexpr unsigned kTile = 128, kSteps = 64; // columns of dy and of x; rows of a step
-constexpr unsigned kRowBytes = kTile * 2, kPartBytes = kSteps * kRowBytes;
+constexpr unsigned kStep = 64; // rows of a step
 
 template <typename T> struct Parts { static constexpr unsigned count = 1; };
 template <> struct Parts<F16> { static constexpr unsigned count = 2; };
 template <> struct Parts<F32> { static constexpr unsigned count = 3; };
 
-// Byte of column c (a multiple of 4) of row r: 32-byte slots of a row are stored in an order that depends
-// on the row, so that the 16 rows that a wave's transposing load takes lie in different banks.
-__device__ __forceinline__ unsigned slotOf(unsigned r, unsigned c) {
-    return r * kRowBytes + ((c / 16) ^ ((r & 3) | ((r >> 1) & 4))) * 32 + c % 16 * 2;
-}
-
-// Eight consecutive rows of one column for each lane: rows r0 + 8 * (lane / 16) .., column c0 + lane % 16.
-__device__ __forceinline__ bf16x8 columnOf(const std::uint8_t* tile, unsigned r0, unsigned c0, unsigned lane) {
-    const unsigned r = r0 + lane / 16 * 8 + lane % 16 / 4, c = c0 + lane % 4 * 4;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(tile + slotOf(r, c)));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(tile + slotOf(r + 4, c)));
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
-    return __builtin_bit_cast(bf16x8, s16x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
-}
+// A tile of kStep rows of Columns bf16 values in LDS. The 32-byte slots of a row (16 values) are stored in
+// an order that depends on the row, its key: a wave's transposing load takes one slot of rows r0 + 8 i + j
+// (i, j < 4), which 64 banks of 4 bytes serve in two turns if they spread over all of them.
+template <unsigned Columns> struct Tile {
+    static constexpr unsigned rowBytes = Columns * 2, bytes = kStep * rowBytes;
+    static __device__ __forceinline__ unsigned key(unsigned r) {
+        if constexpr (Columns == 64) return ((r >> 1) & 1) | ((r >> 2) & 2);
+        return (r & 3) | ((r >> 1) & 4);
+    }
+    // Byte of column c, a multiple of 4, of row r.
+    static __device__ __forceinline__ unsigned at(unsigned r, unsigned c) {
+        return r * rowBytes + ((c / 16) ^ key(r)) * 32 + c % 16 * 2;
+    }
+    // Eight consecutive rows of a column: lane l has rows r0 + 8 * (l / 16) .. of column c0 + l % 16.
+    static __device__ __forceinline__ bf16x8 column(const std::uint8_t* tile, unsigned r0, unsigned c0, unsigned lane) {
+        const unsigned r = r0 + lane / 16 * 8 + lane % 16 / 4, c = c0 + lane % 4 * 4;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(tile + at(r, c)));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(tile + at(r + 4, c)));
+        return __builtin_bit_cast(bf16x8, s16x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
+    }
+};
 
 struct Gradient {
     const void* dy;
     std::uint64_t dyStride;
     const std::uint8_t *x, *xe;
     float *dw, *db; // the splits' sums, or the results where there is one split
+    std::uint64_t splitPitch;
     unsigned rows, outer, inner, codePitch, expPitch, tilesN, tilesK, rowsPerSplit;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void sumRows(Gradient a) {
-    constexpr unsigned P = Parts<T>::count;
-    extern __shared__ __align__(1024) std::uint8_t lds[]; // dy's parts, then x
-    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    const unsigned tile = blockIdx.x % (a.tilesN * a.tilesK), split = blockIdx.x / (a.tilesN * a.tilesK);
-    const unsigned n0 = tile % a.tilesN * kTile, k0 = tile / a.tilesN * kTile;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytesAt(const void* p, std::uint64_t count) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, unsigned(min(count, std::uint64_t(0x7FFFFFFF))), 0x00020000);
+}
+
+// Tiles of BN columns of dy by BK of x, WN x WK waves. A step's bytes are loaded to registers while the step
+// before is multiplied, and written to LDS into the other of two stages, or, where the parts of dy leave
+// no room for two, after a barrier. Aligned: dy of bf16 whose rows are 16-byte aligned, read by plain
+// buffer loads, which give zeros past the end.
+// The loads do not go to LDS directly: the compiler makes every transposing LDS load wait for all of
+// those in flight.
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, unsigned Stages, bool Aligned>
+__global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
+    constexpr unsigned P = Parts<T>::count, Threads = 64 * WN * WK, NT = BN / WN / 16, KT = BK / WK / 16;
+    constexpr unsigned StageBytes = P * Tile<BN>::bytes + Tile<BK>::bytes, DyLoads = kStep * BN / 8 / Threads;
+    constexpr unsigned XLoads = kStep * BK / 16 / Threads, BT = NT / WK; // BT: bias operands of a wave
+    static_assert(BT >= 1 && XLoads >= 1 && DyLoads >= 1, "every thread and wave has its share");
+    typedef typename T::Raw Raw;
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // per stage: dy's parts, then x
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const unsigned tiles = a.tilesN * a.tilesK, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+    const unsigned n0 = tile % a.tilesN * BN, k0 = tile / a.tilesN * BK;
     const unsigned first = split * a.rowsPerSplit, last = min(first + a.rowsPerSplit, a.rows);
-    const auto* dy = static_cast<const typename T::Raw*>(a.dy);
-    // A thread takes columns 8 * (t % 16) .. of rows t / 16 + 16 i of dy, and 16 codes of rows t / 8 + 32 i of x.
-    const unsigned dyColumn = t % 16 * 8, dyRow = t / 16, xColumn = t % 8 * 16, xRow = t / 8;
-    float v[4][8], sums[8] = {};
-    u32x4 q[2];
-    unsigned e[2];
-    auto fetch = [&](unsigned row) {
+    const Raw* dy = static_cast<const Raw*>(a.dy) + n0;
+    const std::uint64_t dyBytes = a.dyStride * sizeof(Raw);
+
+    typedef typename Group<T>::Vec Vec;
+    Vec raw[DyLoads];
+    auto fetchDy = [&](unsigned row) {
+        if constexpr (Aligned) {
+            const auto from = bytesAt(dy + row * a.dyStride, (last - row - 1) * dyBytes + (a.outer - n0) * sizeof(Raw));
 #pragma unroll
-        for (unsigned i = 0; i < 4; ++i) {
-            const unsigned r = row + dyRow + 16 * i;
-            if (r < last) {
-                load8<T>(dy + r * a.dyStride, n0 + dyColumn, a.outer, v[i]);
-            } else {
-#pragma unroll
-                for (unsigned j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            for (unsigned i = 0; i < DyLoads; ++i) {
+                const unsigned chunk = t + i * Threads, r = chunk / (BN / 8), c = chunk % (BN / 8) * 8;
+                const unsigned at = n0 + c < a.outer ? r * unsigned(dyBytes) + c * 2 : 0x80000000u;
+                raw[i] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
             }
-        }
+        } else {
 #pragma unroll
-        for (unsigned i = 0; i < 2; ++i) {
-            const std::uint64_t r = row + xRow + 32 * i;
-            q[i] = u32x4{0, 0, 0, 0};
-            e[i] = 127;
-            if (r < last) {
-                q[i] = *reinterpret_cast<const u32x4*>(a.x + r * a.codePitch + k0 + xColumn);
-                e[i] = a.xe[r * a.expPitch + k0 / kBlock];
+            for (unsigned i = 0; i < DyLoads; ++i) {
+                const unsigned chunk = t + i * Threads, r = row + chunk / (BN / 8), c = chunk % (BN / 8) * 8;
+                raw[i] = Vec{};
+                if (r >= last || n0 + c >= a.outer) continue;
+                const Raw* p = dy + r * a.dyStride + c;
+                if (n0 + c + 8 <= a.outer) {
+                    raw[i] = *reinterpret_cast<const typename Group<T>::Loose*>(p);
+                } else {
+#pragma unroll
+                    for (unsigned j = 0; j < 8; ++j)
+                        if (n0 + c + j < a.outer) raw[i][j] = p[j];
+                }
             }
         }
     };
-    auto stash = [&] {
+    auto stashDy = [&](unsigned stage) {
 #pragma unroll
-        for (unsigned i = 0; i < 4; ++i) {
-            float rest[8];
+        for (unsigned i = 0; i < DyLoads; ++i) {
+            const unsigned chunk = t + i * Threads, r = chunk / (BN / 8), c = chunk % (BN / 8) * 8;
+            std::uint8_t* to = lds + stage * StageBytes + Tile<BN>::at(r, c);
+            if constexpr (P == 1) {
+                *reinterpret_cast<Vec*>(to) = raw[i];
+            } else {
+                float rest[8];
 #pragma unroll
-            for (unsigned j = 0; j < 8; ++j) rest[j] = v[i][j], sums[j] += v[i][j];
+                for (unsigned j = 0; j < 8; ++j) rest[j] = T::get(raw[i][j]);
 #pragma unroll
-            for (unsigned p = 0; p < P; ++p) {
-                bf16x8 part;
+                for (unsigned p = 0; p < P; ++p) {
+                    bf16x8 part;
 #pragma unroll
-                for (unsigned j = 0; j < 8; ++j) {
-                    part[j] = __bf16(rest[j]);
-                    if (p + 1 < P) rest[j] -= float(part[j]);
+                    for (unsigned j = 0; j < 8; ++j) {
+                        part[j] = __bf16(rest[j]);
+                        if (p + 1 < P) rest[j] -= float(part[j]);
+                    }
+                    *reinterpret_cast<bf16x8*>(to + p * Tile<BN>::bytes) = part;
                 }
-                *reinterpret_cast<bf16x8*>(lds + p * kPartBytes + slotOf(dyRow + 16 * i, dyColumn)) = part;
             }
         }
+    };
+    u32x4 q[XLoads];
+    unsigned e[XLoads];
+    auto fetchX = [&](unsigned row) {
+        const auto codes = bytesAt(a.x + std::uint64_t(row) * a.codePitch + k0, (last - row) * std::uint64_t(a.codePitch) - k0);
+        const auto exponents = bytesAt(a.xe + std::uint64_t(row) * a.expPitch, (last - row) * std::uint64_t(a.expPitch));
 #pragma unroll
-        for (unsigned i = 0; i < 2; ++i) {
+        for (unsigned i = 0; i < XLoads; ++i) {
+            const unsigned chunk = t + i * Threads, r = chunk / (BK / 16), c = chunk % (BK / 16) * 16;
+            const bool in = k0 + c < a.codePitch;
+            q[i] = __builtin_amdgcn_raw_buffer_load_b128(codes, in ? r * a.codePitch + c : 0x80000000u, 0, 0);
+            e[i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, in ? r * a.expPitch + (k0 + c) / kBlock : 0x80000000u, 0, 0);
+        }
+    };
+    auto stashX = [&](unsigned stage) {
+        std::uint8_t* to = lds + stage * StageBytes + P * Tile<BN>::bytes;
+#pragma unroll
+        for (unsigned i = 0; i < XLoads; ++i) {
+            const unsigned chunk = t + i * Threads, r = chunk / (BK / 16), c = chunk % (BK / 16) * 16;
             const float s = scaleOf(e[i]);
-            std::uint8_t* to = lds + P * kPartBytes;
 #pragma unroll
             for (unsigned h = 0; h < 2; ++h) {
                 bf16x8 w;
@@ -116,85 +165,185 @@ __global__ __launch_bounds__(256) void sumRows(Gradient a) {
                     const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i][2 * h + j], s, true);
                     w[4 * j] = lo.x, w[4 * j + 1] = lo.y, w[4 * j + 2] = hi.x, w[4 * j + 3] = hi.y;
                 }
-                *reinterpret_cast<bf16x8*>(to + slotOf(xRow + 32 * i, xColumn + 8 * h)) = w;
+                *reinterpret_cast<bf16x8*>(to + Tile<BK>::at(r, c + 8 * h)) = w;
             }
         }
     };
-    const unsigned wn = wave % 2 * 64, wk = wave / 2 * 64;
-    f32x4 acc[4][4] = {}; // dy's columns by x's
-    if (first < last) fetch(first);
-    for (unsigned row = first; row < last; row += kSteps) {
-        stash();
-        __syncthreads();
-        if (row + kSteps < last) fetch(row + kSteps);
+    const unsigned wn = wave % WN * (BN / WN), wk = wave / WN, kk = wk * (BK / WK);
+    const bool bias = a.db && k0 == 0;
+    const bf16x8 ones = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+    f32x4 acc[NT][KT] = {}, sums[BT] = {};
+    auto half = [&](unsigned stage, unsigned r0, auto withBias) {
+        const std::uint8_t* base = lds + stage * StageBytes;
+        bf16x8 xf[KT];
 #pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-            bf16x8 xf[4];
+        for (unsigned k = 0; k < KT; ++k) xf[k] = Tile<BK>::column(base + P * Tile<BN>::bytes, r0, kk + 16 * k, lane);
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k) xf[k] = columnOf(lds + P * kPartBytes, 32 * h, wk + 16 * k, lane);
+        for (unsigned p = 0; p < P; ++p) {
+            bf16x8 df[NT];
 #pragma unroll
-            for (unsigned n = 0; n < 4; ++n)
+            for (unsigned n = 0; n < NT; ++n) df[n] = Tile<BN>::column(base + p * Tile<BN>::bytes, r0, wn + 16 * n, lane);
 #pragma unroll
-                for (unsigned p = 0; p < P; ++p) {
-                    const bf16x8 df = columnOf(lds + p * kPartBytes, 32 * h, wn + 16 * n, lane);
+            for (unsigned n = 0; n < NT; ++n)
 #pragma unroll
-                    for (unsigned k = 0; k < 4; ++k)
-                        acc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[k], df, acc[n][k], 0, 0, 0);
-                }
+                for (unsigned k = 0; k < KT; ++k)
+                    acc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[k], df[n], acc[n][k], 0, 0, 0);
+            // The WK waves of these columns share the bias operands.
+            if constexpr (decltype(withBias)::value)
+#pragma unroll
+                for (unsigned b = 0; b < BT; ++b)
+                    sums[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, Tile<BN>::column(base + p * Tile<BN>::bytes, r0,
+                                                                      wn + 16 * (wk * BT + b), lane), sums[b], 0, 0, 0);
         }
-        __syncthreads();
+    };
+    auto walk = [&](auto withBias) {
+        unsigned stage = 0;
+        for (unsigned row = first; row < last; row += kStep) {
+            const bool more = row + kStep < last;
+            // The last step loads itself again, for nobody, so that the loop has no branch.
+            fetchX(more ? row + kStep : row);
+            fetchDy(more ? row + kStep : row);
+            __builtin_amdgcn_sched_barrier(0); // the compiler would move the loads down to their use
+            half(stage, 0, withBias);
+            half(stage, 32, withBias);
+            __builtin_amdgcn_sched_barrier(0);
+            if (Stages == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (Stages == 2) stage = 1 - stage;
+            stashX(stage);
+            stashDy(stage);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+    };
+    if (first < last) {
+        fetchX(first);
+        fetchDy(first);
+        stashX(0);
+        stashDy(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (bias)
+            walk(std::true_type{});
+        else
+            walk(std::false_type{});
     }
     // x was the first operand: a lane has 4 consecutive columns of x for one of dy's.
-    float* dw = a.dw + std::uint64_t(split) * a.outer * a.inner;
+    float* dw = a.dw + split * a.splitPitch;
+    typedef f32x4 Loose4 __attribute__((aligned(4)));
 #pragma unroll
-    for (unsigned n = 0; n < 4; ++n) {
+    for (unsigned n = 0; n < NT; ++n) {
         const unsigned row = n0 + wn + 16 * n + lane % 16;
         if (row >= a.outer) continue;
 #pragma unroll
-        for (unsigned k = 0; k < 4; ++k) {
-            const unsigned column = k0 + wk + 16 * k + lane / 16 * 4;
+        for (unsigned k = 0; k < KT; ++k) {
+            const unsigned column = k0 + kk + 16 * k + lane / 16 * 4;
             float* to = dw + std::uint64_t(row) * a.inner + column;
+            if (column + 4 <= a.inner) {
+                *reinterpret_cast<Loose4*>(to) = acc[n][k];
+            } else {
 #pragma unroll
-            for (unsigned i = 0; i < 4; ++i)
-                if (column + i < a.inner) to[i] = acc[n][k][i];
+                for (unsigned i = 0; i < 4; ++i)
+                    if (column + i < a.inner) to[i] = acc[n][k][i];
+            }
         }
     }
-    if (a.db && k0 == 0) {
-        // Column sums: the 16 threads with the same columns add theirs through LDS.
-        float* part = reinterpret_cast<float*>(lds);
+    if (bias && lane < 16) {
+        // Every row of a product with ones is the sum.
 #pragma unroll
-        for (unsigned j = 0; j < 8; ++j) part[dyRow * kTile + dyColumn + j] = sums[j];
-        __syncthreads();
-        if (t < kTile && n0 + t < a.outer) {
-            float s = 0.0f;
-            for (unsigned r = 0; r < 16; ++r) s += part[r * kTile + t];
-            a.db[std::uint64_t(split) * a.outer + n0 + t] = s;
+        for (unsigned b = 0; b < BT; ++b) {
+            const unsigned column = n0 + wn + 16 * (wk * BT + b) + lane;
+            if (column < a.outer) a.db[split * a.splitPitch + column] = sums[b][0];
         }
     }
 }
 
-// out = the sum of `splits` arrays of n floats, in order.
-__global__ __launch_bounds__(256) void addSplits(const float* __restrict__ parts, float* __restrict__ out,
-                                                  std::uint64_t n, unsigned splits) {
-    const std::uint64_t i = std::uint64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.0f;
-    for (unsigned k = 0; k < splits; ++k) s += parts[k * n + i];
-    out[i] = s;
+// dw and db from the splits' sums, added in a fixed order: Ways threads add every Ways-th split of four
+// values, then their sums through LDS. A split's db follows its dw.
+template <unsigned Ways>
+__global__ __launch_bounds__(64 * Ways) void addSplits(const float* __restrict__ parts, float* __restrict__ dw,
+                                                        float* __restrict__ db, std::uint64_t size, std::uint64_t dbAt,
+                                                        unsigned outer, std::uint64_t pitch, unsigned splits) {
+    __shared__ f32x4 sums[Ways][64];
+    const unsigned lane = threadIdx.x % 64, way = threadIdx.x / 64;
+    const std::uint64_t at = (std::uint64_t(blockIdx.x) * 64 + lane) * 4;
+    f32x4 s = {};
+    if (at < pitch)
+#pragma unroll 4
+        for (unsigned k = way; k < splits; k += Ways) s += *reinterpret_cast<const f32x4*>(parts + k * pitch + at);
+    sums[way][lane] = s;
+    __syncthreads();
+    if (way || at >= pitch) return;
+#pragma unroll
+    for (unsigned w = 1; w < Ways; ++w) s += sums[w][lane];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+        if (at + i < size)
+            dw[at + i] = s[i];
+        else if (db && at >= dbAt && at + i - dbAt < outer)
+            db[at + i - dbAt] = s[i];
+    }
 }
 
-unsigned splitsOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer) {
-    const std::uint64_t tiles = std::uint64_t((inner + kTile - 1) / kTile) * ((outer + kTile - 1) / kTile);
-    const std::uint64_t steps = (std::uint64_t(rows) + kSteps - 1) / kSteps;
-    const std::uint64_t want = (1024 + tiles - 1) / tiles, most = std::max<std::uint64_t>(1, steps / 4);
-    return unsigned(std::max<std::uint64_t>(1, std::min(want, most)));
+// ------------------------------------------------------------------------------------------------
+// Host side
+
+// Form of a call: tile, and how many splits of the rows.
+struct Plan {
+    unsigned bn, bk, splits, steps; // steps of a split
+    bool aligned;
+};
+
+constexpr unsigned kUnits = 256; // compute units
+
+bool alignedRows(const DenseMatrix& dy, std::uint32_t outer) {
+    return dy.type == DenseType::bf16 && reinterpret_cast<std::uintptr_t>(dy.data) % 16 == 0 && dy.stride % 8 == 0 &&
+           outer % 8 == 0 && dy.stride < (1u << 23);
+}
+
+std::uint64_t rounded4(std::uint64_t n) { return (n + 3) / 4 * 4; }
+std::uint64_t pitchOf(std::uint32_t inner, std::uint32_t outer) {
+    return rounded4(std::uint64_t(outer) * inner) + rounded4(outer);
+}
+
+// The splits with the least estimated time, in microseconds: rounds of workgroups on the chip times the
+// steps of each, and the traffic of the partial sums, written once and read once.
+double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, double stepTime, unsigned perUnit) {
+    const std::uint64_t tiles = std::uint64_t((inner + p.bk - 1) / p.bk) * ((outer + p.bn - 1) / p.bn);
+    const std::uint64_t steps = std::max<std::uint64_t>(1, (std::uint64_t(rows) + kStep - 1) / kStep);
+    double best = 1e30;
+    auto consider = [&](std::uint64_t splits) {
+        splits = std::max<std::uint64_t>(1, std::min(splits, steps));
+        const std::uint64_t each = (steps + splits - 1) / splits, used = (steps + each - 1) / each;
+        const std::uint64_t rounds = (tiles * used + kUnits * perUnit - 1) / (kUnits * perUnit);
+        double time = double(rounds) * (double(each) * stepTime + 3.0);
+        if (used > 1) time += 4.0 + double(used) * double(pitchOf(inner, outer)) * 8.0 / 4.0e6;
+        if (time < best) best = time, p.splits = unsigned(used), p.steps = unsigned(each);
+    };
+    consider(1);
+    for (unsigned rounds = 1; rounds <= 8; ++rounds) consider(std::uint64_t(rounds) * kUnits * perUnit / tiles);
+    return best;
+}
+
+Plan planOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, bool aligned) {
+    Plan small = {outer <= 64 && !aligned ? 64u : 128u, 128, 1, 1, aligned}, large = {256, 256, 1, 1, aligned};
+    const unsigned parts = type == DenseType::f32 ? 3 : type == DenseType::f16 ? 2 : 1;
+    const double smallTime = planTime(small, rows, inner, outer, 0.6 + 0.3 * parts, 2);
+    if (!aligned) return small;
+    return planTime(large, rows, inner, outer, 1.5, 1) < smallTime ? large : small;
+}
+
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, unsigned Stages, bool Aligned>
+void launchSum(const Gradient& a, std::uint64_t blocks, hipStream_t stream) {
+    constexpr unsigned lds = Stages * (Parts<T>::count * Tile<BN>::bytes + Tile<BK>::bytes);
+    hipLaunchKernelGGL((sumRows<T, BN, BK, WN, WK, Stages, Aligned>), dim3(unsigned(blocks)), dim3(64 * WN * WK), lds, stream, a);
 }
 
 } // namespace
 
-std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType) {
-    const unsigned splits = splitsOf(rows, inner, outer);
-    return splits == 1 ? 0 : std::size_t(splits) * (std::size_t(outer) * inner + outer) * sizeof(float);
+std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
+    if (!rows || !inner || !outer) return 0;
+    // The larger of the two forms' needs: which one runs depends on dy's alignment.
+    std::uint64_t splits = planOf(rows, inner, outer, type, false).splits;
+    if (type == DenseType::bf16) splits = std::max<std::uint64_t>(splits, planOf(rows, inner, outer, type, true).splits);
+    return splits == 1 ? 0 : std::size_t(splits * pitchOf(inner, outer) * sizeof(float));
 }
 
 void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::uint32_t rows, std::uint32_t inner,
@@ -212,34 +361,46 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
         checkDense(where, dy.data, dy.stride, dy.type, outer);
         checkCodes(where, x.codes, x.exponents);
     }
-    const unsigned splits = splitsOf(rows, inner, outer);
     const std::size_t need = weightGradBlocksWorkspace(rows, inner, outer, dy.type);
     if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
+    const Plan p = planOf(rows, inner, outer, dy.type, alignedRows(dy, outer));
+    const std::uint64_t size = std::uint64_t(outer) * inner, pitch = pitchOf(inner, outer);
+    auto* parts = static_cast<float*>(workspace);
     Gradient a = {};
     a.dy = dy.data, a.dyStride = dy.stride, a.x = x.codes, a.xe = x.exponents;
     a.rows = rows, a.outer = outer, a.inner = inner;
     a.codePitch = unsigned(blockCodePitch(inner)), a.expPitch = unsigned(blockExponentPitch(inner));
-    a.tilesN = (outer + kTile - 1) / kTile, a.tilesK = (inner + kTile - 1) / kTile;
-    const unsigned steps = (rows + kSteps - 1) / kSteps;
-    a.rowsPerSplit = std::max(1u, (steps + splits - 1) / splits) * kSteps;
-    const std::uint64_t size = std::uint64_t(outer) * inner;
-    auto* parts = static_cast<float*>(workspace);
-    a.dw = splits == 1 ? dw : parts;
-    a.db = !db ? nullptr : splits == 1 ? db : parts + splits * size;
-    const std::uint64_t blocks = std::uint64_t(a.tilesN) * a.tilesK * splits;
+    a.tilesN = (outer + p.bn - 1) / p.bn, a.tilesK = (inner + p.bk - 1) / p.bk;
+    a.rowsPerSplit = p.steps * kStep;
+    a.dw = p.splits == 1 ? dw : parts;
+    a.db = !db ? nullptr : p.splits == 1 ? db : parts + rounded4(size);
+    a.splitPitch = p.splits == 1 ? 0 : pitch;
+    const std::uint64_t blocks = std::uint64_t(a.tilesN) * a.tilesK * p.splits;
     if (blocks >> 31) reject(where, "more than 2^31 tiles");
-    withType(dy.type, [&](auto tag) {
-        typedef decltype(tag) T;
-        hipLaunchKernelGGL((sumRows<T>), dim3(unsigned(blocks)), dim3(256), (Parts<T>::count + 1) * kPartBytes, stream,
-                           a);
-    });
+    if (p.aligned) {
+        if (p.bn == 256)
+            launchSum<BF16, 256, 256, 2, 4, 2, true>(a, blocks, stream);
+        else
+            launchSum<BF16, 128, 128, 2, 4, 2, true>(a, blocks, stream);
+    } else {
+        withType(dy.type, [&](auto tag) {
+            typedef decltype(tag) T;
+            if (p.bn == 64)
+                launchSum<T, 64, 128, 1, 4, 1, false>(a, blocks, stream);
+            else
+                launchSum<T, 128, 128, 2, 2, 1, false>(a, blocks, stream);
+        });
+    }
     checkHip(hipGetLastError());
-    if (splits > 1) {
-        hipLaunchKernelGGL(addSplits, dim3(unsigned((size + 255) / 256)), dim3(256), 0, stream, parts, dw, size, splits);
-        if (db)
-            hipLaunchKernelGGL(addSplits, dim3((outer + 255) / 256), dim3(256), 0, stream, parts + splits * size, db,
-                               std::uint64_t(outer), splits);
+    if (p.splits > 1) {
+        const dim3 grid(unsigned((pitch / 4 + 63) / 64));
+        if (p.splits >= 32)
+            hipLaunchKernelGGL(addSplits<16>, grid, dim3(1024), 0, stream, parts, dw, db, size, rounded4(size), outer,
+                               pitch, p.splits);
+        else
+            hipLaunchKernelGGL(addSplits<4>, grid, dim3(256), 0, stream, parts, dw, db, size, rounded4(size), outer,
+                               pitch, p.splits);
         checkHip(hipGetLastError());
     }
 }

@@ -142,6 +142,13 @@ SHAPES = [(1, 1, 1), (1, 128, 16), (1, 4096, 130), (3, 100, 77), (16, 512, 64), 
           (700, 2048, 1000), (1111, 96, 47), (5000, 128, 256)]
 
 
+@pytest.mark.parametrize("rows,inner,outer,dtype", [(4090, 200, 4100, "bf16"), (4091, 300, 4099, "f16"),
+                                                    (3900, 600, 4000, "bf16"), (4096, 1024, 4096, "bf16")])
+def test_linear_wide(gpu, rows, inner, outer, dtype):
+    """Products of many tiles, which the largest tile takes: one block more than its pairs, ragged edges."""
+    test_linear(gpu, rows, inner, outer, dtype)
+
+
 @pytest.mark.parametrize("rows,inner,outer", SHAPES)
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_linear(gpu, rows, inner, outer, dtype):
@@ -235,6 +242,18 @@ def test_linear_backward(gpu, rows, inner, outer, dtype):
         assert all(torch.equal(got[n], again[n]) for n in want), "repeated calls give the same bits"
     only = linear_blocks_backward(dy, kept, weight, need=(False, True, False))
     assert only[0] is None and only[2] is None and torch.equal(only[1], got["dw"])
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(1500, 2048, 4096), (1030, 4000, 4104), (4000, 1000, 520)])
+def test_weight_gradient_large(gpu, rows, inner, outer):
+    """Gradients of many tiles, which the largest tile takes, and of few, over many rows."""
+    from tcc_spmm_amd.blocks import quantize_blocks, weight_grad_blocks
+    x, dy = random((rows, inner), 1, "bf16"), random((rows, outer), 2, "bf16", 1e-2)
+    xv, g = O.quantize(f64(x))[2], f64(dy)
+    dw, db = weight_grad_blocks(dy, quantize_blocks(x))
+    near(dw, g.T @ xv, (rows / 4 + 64) * U * (np.abs(g).T @ np.abs(xv)) + 1e-30, "dw")
+    near(db, g.sum(0), (rows / 4 + 64) * U * np.abs(g).sum(0) + 1e-30, "db")
+    assert torch.equal(weight_grad_blocks(dy, quantize_blocks(x), bias=False)[0], dw)
 
 
 def test_weight_gradient_of_no_rows(gpu):
