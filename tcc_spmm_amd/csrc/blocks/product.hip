@@ -74,6 +74,27 @@ template <bool Whole> __device__ __forceinline__ void bias8(const float* bias, u
     }
 }
 
+// The same for four FP32 outputs.
+typedef f32x4 LooseF32x4 __attribute__((aligned(4)));
+__device__ __forceinline__ f32x4 bias4(const float* bias, unsigned at, unsigned n) {
+    f32x4 b = {};
+    if (!bias) return b;
+    if (at + 4 <= n) return *reinterpret_cast<const LooseF32x4*>(bias + at);
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i)
+        if (at + i < n) b[i] = bias[at + i];
+    return b;
+}
+__device__ __forceinline__ void put4(float* row, unsigned at, unsigned n, f32x4 v) {
+    if (at + 4 <= n) {
+        *reinterpret_cast<LooseF32x4*>(row + at) = v;
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i)
+            if (at + i < n) row[at + i] = v[i];
+    }
+}
+
 // Waits until at most N of this wave's memory loads are outstanding and its LDS reads are done, then
 // for the workgroup. One asm block with a memory clobber, so that no access moves across it.
 template <unsigned N> __device__ __forceinline__ void waitBarrier() {
@@ -476,14 +497,168 @@ __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
 #pragma unroll
     for (unsigned n = 0; n < 4; ++n) {
         const unsigned column = tn + wn + n * 16 + g * 4;
+        const f32x4 b = bias4(a.bias, column, a.outer);
 #pragma unroll
         for (unsigned m = 0; m < 4; ++m) {
             const unsigned row = tm + wm + m * 16 + l16;
-            if (row >= a.rows) continue;
+            if (row < a.rows) put4(y + row * a.yStride, column, a.outer, acc[n][m] + b);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many rows through a narrow layer (a graph's, after the sparse product): the weight fits in LDS. A workgroup
+// takes it there once, as MFMA operands, and then each of its waves goes through rows of its own, 16 at a
+// time, without a barrier: dense x is read once, quantized in the layout of an operand, kept if asked for, and
+// multiplied with every column. Bound by HBM; what it saves against the tiles is writing and reading codes.
+//
+// A lane reads 16 bytes of its row at a time, four lanes 64 bytes side by side. That gives it 32 elements of a
+// block in an order of their own; the order along the inner axis is free as long as both operands share it,
+// so the weight is laid out in the same order: element e of a block is in lane group e / 4 % 4 (FP32) or
+// e / 8 % 4, after those of the groups before it in the block.
+template <typename T, unsigned Blocks>
+__global__ __launch_bounds__(512) void multiplyRows(Product a) {
+    constexpr bool Exact = std::is_same<T, F32>::value;
+    constexpr unsigned Run = Exact ? 4 : 8, Image = Exact ? 256 : 128; // elements of a load; bytes of a weight block
+    constexpr unsigned Together = 4;                                   // column tiles multiplied at a time
+    typedef typename T::Raw Raw;
+    typedef Raw RunVec __attribute__((ext_vector_type(Run)));
+    typedef RunVec LooseRun __attribute__((aligned(alignof(Raw))));
+    extern __shared__ __align__(1024) std::uint8_t lds[];
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave, l16 = lane % 16, g = lane / 16;
+    const unsigned tiles = (a.outer + 16 * Together - 1) / (16 * Together) * Together, slots = tiles * 16;
+    // Column of slot s: a 16-bit y has 8 columns of two tiles in one lane.
+    auto columnOf = [](unsigned s) {
+        if constexpr (Exact) return s;
+        return s / 32 * 32 + s % 16 / 4 * 8 + s / 16 % 2 * 4 + s % 4;
+    };
+    for (unsigned i = t; i < slots * Blocks * 8; i += 512) {
+        const unsigned part = i % 8, block = i / 8 % Blocks, slot = i / 8 / Blocks, column = columnOf(slot);
+        u32x4 q = {0, 0, 0, 0};
+        float scale = 0.0f;
+        if (column < a.outer) {
+            q = *reinterpret_cast<const u32x4*>(a.w + (std::uint64_t(column) * Blocks + block) * kBlock + part * 16);
+            scale = scaleOf(a.we[std::uint64_t(column / kBlock) * a.expPitch + block]);
+        }
+        std::uint8_t* to = lds + (block * slots + slot) * Image;
+        if constexpr (Exact) {
+            // 16-byte chunks of a 256-byte row: 4 * group + (element of the group) / 8.
 #pragma unroll
-            for (unsigned i = 0; i < 4; ++i)
-                if (column + i < a.outer)
-                    y[row * a.yStride + column + i] = acc[n][m][i] + (a.bias ? a.bias[column + i] : 0.0f);
+            for (unsigned j = 0; j < 4; ++j) {
+                const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[j], scale, false);
+                const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[j], scale, true);
+                *reinterpret_cast<u32x2*>(to + ((4 * j + part / 2) ^ (slot & 15)) * 16 + part % 2 * 8) =
+                    u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
+            }
+        } else {
+#pragma unroll
+            for (unsigned j = 0; j < 2; ++j) {
+                const unsigned at = (part % 2 * 2 + j) * 32 + part / 2 * 8;
+                *reinterpret_cast<u32x2*>(to + ((at / 16) ^ (slot & 7)) * 16 + at % 16) = u32x2{q[2 * j], q[2 * j + 1]};
+            }
+        }
+    }
+    __syncthreads();
+    const unsigned groups = (a.rows + 15) / 16;
+    for (unsigned group = blockIdx.x * 8 + wave; group < groups; group += gridDim.x * 8) {
+        const unsigned row = group * 16 + l16;
+        const Raw* x = static_cast<const Raw*>(a.dense) + min(row, a.rows - 1) * a.denseStride;
+        RunVec raw[Blocks][32 / Run];
+#pragma unroll
+        for (unsigned b = 0; b < Blocks; ++b)
+#pragma unroll
+            for (unsigned i = 0; i < 32 / Run; ++i) {
+                const unsigned at = b * kBlock + (i * 4 + g) * Run;
+                if (at + Run <= a.inner) {
+                    raw[b][i] = __builtin_nontemporal_load(reinterpret_cast<const LooseRun*>(x + at));
+                } else {
+#pragma unroll
+                    for (unsigned j = 0; j < Run; ++j) raw[b][i][j] = at + j < a.inner ? x[at + j] : Raw(0.0f);
+                }
+            }
+        u32x4 q[Blocks][2];
+        unsigned xe[Blocks];
+#pragma unroll
+        for (unsigned b = 0; b < Blocks; ++b) {
+            float v[4][8];
+            unsigned peak = 0;
+#pragma unroll
+            for (unsigned i = 0; i < 4; ++i) {
+#pragma unroll
+                for (unsigned j = 0; j < 8; ++j) v[i][j] = T::get(raw[b][(i * 8 + j) / Run][j % Run]);
+                peak = max(peak, peakBits(v[i]));
+            }
+            peak = max(peak, unsigned(__shfl_xor(int(peak), 16)));
+            peak = max(peak, unsigned(__shfl_xor(int(peak), 32)));
+            xe[b] = exponentOf<BlockCodes::e4m3>(peak);
+            const u32x2 q0 = encode8<BlockCodes::e4m3>(v[0], xe[b]), q1 = encode8<BlockCodes::e4m3>(v[1], xe[b]);
+            const u32x2 q2 = encode8<BlockCodes::e4m3>(v[2], xe[b]), q3 = encode8<BlockCodes::e4m3>(v[3], xe[b]);
+            q[b][0] = u32x4{q0.x, q0.y, q1.x, q1.y};
+            q[b][1] = u32x4{q2.x, q2.y, q3.x, q3.y};
+            if (a.keep && row < a.rows) {
+                std::uint8_t* to = a.keep + (std::uint64_t(row) * Blocks + b) * kBlock;
+#pragma unroll
+                for (unsigned i = 0; i < 32 / Run; ++i) {
+                    if constexpr (Exact)
+                        *reinterpret_cast<unsigned*>(to + (i * 4 + g) * 4) = q[b][i / 4][i % 4];
+                    else
+                        *reinterpret_cast<u32x2*>(to + (i * 4 + g) * 8) =
+                            u32x2{q[b][i / 2][i % 2 * 2], q[b][i / 2][i % 2 * 2 + 1]};
+                }
+                if (b + g < (b + 1 == Blocks ? a.expPitch : b + 1))
+                    a.keepExp[std::uint64_t(row) * a.expPitch + b + g] = std::uint8_t(g ? 127u : xe[b]);
+            }
+        }
+        Raw* y = static_cast<Raw*>(a.y) + row * a.yStride;
+        for (unsigned tile = 0; tile < tiles; tile += Together) {
+            f32x4 acc[Together] = {};
+#pragma unroll
+            for (unsigned b = 0; b < Blocks; ++b) {
+                const std::uint8_t* w = lds + (b * slots + tile * 16 + l16) * Image;
+                if constexpr (Exact) {
+                    const float scale = scaleOf(xe[b]);
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i) {
+                        const bf16x8 xf = values8(q[b][i / 2][i % 2 * 2], q[b][i / 2][i % 2 * 2 + 1], scale);
+#pragma unroll
+                        for (unsigned n = 0; n < Together; ++n)
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                *reinterpret_cast<const bf16x8*>(w + n * 16 * Image + ((4 * g + i) ^ l16) * 16), xf,
+                                acc[n], 0, 0, 0);
+                    }
+                } else {
+                    const unsigned we = a.we[std::uint64_t(tile * 16 / kBlock) * a.expPitch + b];
+#pragma unroll
+                    for (unsigned n = 0; n < Together; ++n) {
+                        const u32x4* p = reinterpret_cast<const u32x4*>(w + n * 16 * Image);
+                        acc[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            join(p[(2 * g) ^ (l16 & 7)], p[(2 * g + 1) ^ (l16 & 7)]), join(q[b][0], q[b][1]), acc[n], 0, 0,
+                            0, int(we), 0, int(xe[b]));
+                    }
+                }
+            }
+            // The sums are needed here, by all lanes: left to itself the compiler moves the multiplication, with its reads
+            // of LDS, to where only the lanes with a row run.
+#pragma unroll
+            for (unsigned n = 0; n < Together; ++n) asm volatile("" ::"v"(acc[n]));
+            if (row >= a.rows) continue;
+            if constexpr (Exact) {
+#pragma unroll
+                for (unsigned n = 0; n < Together; ++n) {
+                    const unsigned column = (tile + n) * 16 + g * 4;
+                    put4(y, column, a.outer, acc[n] + bias4(a.bias, column, a.outer));
+                }
+            } else {
+#pragma unroll
+                for (unsigned n = 0; n < Together; n += 2) {
+                    const unsigned column = (tile + n) * 16 + g * 8;
+                    float v[8], b[8];
+#pragma unroll
+                    for (unsigned i = 0; i < 8; ++i) v[i] = acc[n + i / 4][i % 4];
+                    bias8<false>(a.bias, column, a.outer, b);
+                    put8<T, false>(y, column, a.outer, v, b);
+                }
+            }
         }
     }
 }
@@ -680,13 +855,33 @@ void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, De
 namespace {
 bool fusedTokens(std::uint32_t rows) { return rows <= kTokenRows; }
 
+// The weight's bytes in LDS if a narrow layer with many rows goes through multiplyRows, else 0.
+constexpr unsigned kRowsLds = 160 * 1024;
+std::size_t rowsImage(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
+    const std::uint64_t count = (inner + kBlock - 1) / kBlock, slots = (std::uint64_t(outer) + 63) / 64 * 64;
+    const std::uint64_t bytes = slots * count * (type == DenseType::f32 ? 256 : 128);
+    return rows >= 8192 && count <= 4 && bytes <= kRowsLds ? std::size_t(bytes) : 0;
+}
+
+template <typename T> void launchRows(const Product& p, std::size_t lds, hipStream_t stream) {
+    // Two workgroups a CU where their images fit; rows of at least one round of its waves for each.
+    const unsigned grid = std::min((p.rows + 127) / 128, lds <= kRowsLds / 2 ? 512u : 256u);
+    switch (p.count) {
+    case 1: hipLaunchKernelGGL((multiplyRows<T, 1>), dim3(grid), dim3(512), lds, stream, p); break;
+    case 2: hipLaunchKernelGGL((multiplyRows<T, 2>), dim3(grid), dim3(512), lds, stream, p); break;
+    case 3: hipLaunchKernelGGL((multiplyRows<T, 3>), dim3(grid), dim3(512), lds, stream, p); break;
+    case 4: hipLaunchKernelGGL((multiplyRows<T, 4>), dim3(grid), dim3(512), lds, stream, p); break;
+    }
+    checkHip(hipGetLastError());
+}
+
 std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
 } // namespace
 
 std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                   bool keep) {
     std::size_t bytes = matmulBlocksWorkspace(rows, inner, outer, type);
-    if (!keep && !fusedTokens(rows))
+    if (!keep && !fusedTokens(rows) && !rowsImage(rows, inner, outer, type))
         bytes += rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
     return bytes;
 }
@@ -709,14 +904,20 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
     const std::size_t need = linearBlocksWorkspace(rows, inner, outer, x.type, keep.codes);
     if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
-    if (fusedTokens(rows)) {
+    const std::size_t image = rowsImage(rows, inner, outer, x.type);
+    if (fusedTokens(rows) || image) {
         Product p = {};
         p.w = w.codes, p.we = w.exponents, p.bias = bias, p.y = y, p.yStride = yStride;
         p.rows = rows, p.outer = outer, p.inner = inner;
         p.count = (inner + kBlock - 1) / kBlock;
         p.expPitch = unsigned(blockExponentPitch(inner));
         p.dense = x.data, p.denseStride = x.stride, p.keep = keep.codes, p.keepExp = keep.exponents;
-        withType(x.type, [&](auto tag) { launchTokens<decltype(tag), true>(p, stream); });
+        withType(x.type, [&](auto tag) {
+            if (image)
+                launchRows<decltype(tag)>(p, image, stream);
+            else
+                launchTokens<decltype(tag), true>(p, stream);
+        });
         return;
     }
     auto* spare = static_cast<std::uint8_t*>(workspace);
