@@ -111,13 +111,6 @@ __global__ __launch_bounds__(kThreads) void activateBlocksBackward(Call a) {
     if constexpr (Gated) store8<T>(dx + a.width, at, a.width, du);
 }
 
-template <typename F> void withCodes(BlockCodes c, F f) {
-    if (c == BlockCodes::e4m3)
-        f(std::integral_constant<BlockCodes, BlockCodes::e4m3>{});
-    else
-        f(std::integral_constant<BlockCodes, BlockCodes::int8>{});
-}
-
 template <typename F> void withActivation(BlockActivation k, F f) {
     switch (k) {
     case BlockActivation::silu: f(std::integral_constant<BlockActivation, BlockActivation::silu>{}); break;

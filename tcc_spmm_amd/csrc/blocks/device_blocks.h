@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 namespace blocks {
 
@@ -225,6 +226,14 @@ template <typename F> void withType(DenseType t, F f) {
     case DenseType::bf16: f(BF16{}); break;
     case DenseType::f16: f(F16{}); break;
     }
+}
+
+// Calls f with the code type as a constant.
+template <typename F> void withCodes(BlockCodes c, F f) {
+    if (c == BlockCodes::e4m3)
+        f(std::integral_constant<BlockCodes, BlockCodes::e4m3>{});
+    else
+        f(std::integral_constant<BlockCodes, BlockCodes::int8>{});
 }
 
 } // namespace blocks

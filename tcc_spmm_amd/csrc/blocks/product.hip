@@ -129,14 +129,22 @@ __device__ __forceinline__ unsigned tileOf(unsigned id, unsigned total, unsigned
 // scale there: a lane takes chunks g and g + 4 of its row.
 // The weight is the MFMA's first operand, whose rows become consecutive values of one lane: rows are
 // dealt to pairs of MFMAs so that a lane ends with 8 consecutive outputs of one row of y.
-template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages>
-__global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
+//
+// Groups of waves share a tile where there are few: each takes a run of the inner axis, with stages of its own,
+// and the first adds the others' sums. A step costs its barrier and its LDS reads' latency, so half the
+// steps are nearly half the time.
+template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
+__global__ __launch_bounds__(64 * WM * WN * Groups) void multiplyTiles(Product a) {
     constexpr unsigned Waves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
     constexpr unsigned XL = BM / 8 / Waves, WL = BN / 8 / Waves;
     static_assert(Stages == 2 || Stages == 4, "the stage is a constant of the unrolled step");
     static_assert(BN / WN <= 128 && NT % 2 == 0, "a wave's columns share a weight tile");
-    extern __shared__ __align__(1024) std::uint8_t lds[];
-    const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    extern __shared__ __align__(1024) std::uint8_t shared[];
+    const unsigned lane = threadIdx.x % kWave, allWaves = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned wave = allWaves % Waves, part = Groups == 1 ? 0 : allWaves / Waves;
+    std::uint8_t* lds = shared + part * Stages * (BM + BN) * kBlock;
+    // This group's blocks: `steps` of them from `first` on, those past the last being zeros.
+    const unsigned steps = Groups == 1 ? a.count : (a.count + 4 * Groups - 1) / (4 * Groups) * 4, first = part * steps;
     const unsigned tile = tileOf(blockIdx.x, gridDim.x, a.tilesM, a.tilesN);
     const unsigned tm = tile % a.tilesM * BM, tn = tile / a.tilesM * BN;
     const unsigned pitch = a.count * kBlock;
@@ -148,11 +156,11 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
     const unsigned r = wave * 8 + lane / 8;
     const unsigned xo = r * pitch + ((lane % 8) ^ (r & 7)) * 16;
     const unsigned wo = r * pitch + ((lane % 8) ^ ((r & 3) | ((r >> 1) & 4))) * 16;
-    // Step k's bytes into stage s; past the last step the last one again, so that every wave has the
-    // same number of loads outstanding.
+    // Block k's bytes into stage s; past the last block zeros, from beyond the buffer, so that every wave has
+    // the same number of loads outstanding.
     auto load = [&](unsigned k, unsigned s) {
         std::uint8_t* to = lds + s * (BM + BN) * kBlock + wave * 1024;
-        const unsigned from = min(k, a.count - 1) * kBlock;
+        const unsigned from = k < a.count ? k * kBlock : 0x7FFFFFFFu;
 #pragma unroll
         for (unsigned j = 0; j < XL; ++j)
             loadToLds(xr, to + j * Waves * 1024, xo, from + j * Waves * 8 * pitch);
@@ -175,14 +183,15 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
         wsNext = *reinterpret_cast<const unsigned*>(we + k4);
     };
     f32x4 acc[NT][MT] = {};
-    loadExponents(0);
+    loadExponents(min(first, (a.count - 1) / 4 * 4));
 #pragma unroll
-    for (unsigned s = 0; s + 1 < Stages; ++s) load(s, s);
+    for (unsigned s = 0; s + 1 < Stages; ++s) load(first + s, s);
     const unsigned xKey = l16 & 7, wKey = (l16 & 3) | (l16 & 4);
     const std::uint8_t* xRead = lds + (wm + l16) * kBlock;
     const std::uint8_t* wRead = lds + BM * kBlock + (wn + l16 / 4 * 8 + l16 % 4) * kBlock;
     auto step = [&](unsigned k, auto sel) {
-        constexpr unsigned S = decltype(sel)::value, at = S % Stages * (BM + BN) * kBlock;
+        constexpr unsigned S = decltype(sel)::value;
+        constexpr unsigned at = S % Stages * (BM + BN) * kBlock;
         waitBarrier<(Stages - 2) * (XL + WL)>();
         load(k + Stages - 1, (S + Stages - 1) % Stages);
         i32x8 xf[MT];
@@ -207,22 +216,36 @@ __global__ __launch_bounds__(64 * WM * WN) void multiplyTiles(Product a) {
         ws = wsNext;
         loadExponents(min(k4 + 4, (a.count - 1) / 4 * 4));
     };
-    unsigned k = 0;
-    for (; k + 4 <= a.count; k += 4) {
+    unsigned k = first;
+    for (; k + 4 <= first + steps; k += 4) {
         nextExponents(k);
         step(k, std::integral_constant<unsigned, 0>{});
         step(k + 1, std::integral_constant<unsigned, 1>{});
         step(k + 2, std::integral_constant<unsigned, 2>{});
         step(k + 3, std::integral_constant<unsigned, 3>{});
     }
-    if (k < a.count) {
+    if (Groups == 1 && k < steps) {
         nextExponents(k);
         step(k, std::integral_constant<unsigned, 0>{});
-        if (k + 1 < a.count) step(k + 1, std::integral_constant<unsigned, 1>{});
-        if (k + 2 < a.count) step(k + 2, std::integral_constant<unsigned, 2>{});
+        if (k + 1 < steps) step(k + 1, std::integral_constant<unsigned, 1>{});
+        if (k + 2 < steps) step(k + 2, std::integral_constant<unsigned, 2>{});
     }
     // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (Groups > 1) {
+        __syncthreads();
+        f32x4* sums = reinterpret_cast<f32x4*>(shared) + wave * NT * MT * kWave + lane;
+        if (part)
+#pragma unroll
+            for (unsigned i = 0; i < NT * MT; ++i)
+                sums[((part - 1) * Waves * NT * MT + i) * kWave] = acc[i / MT][i % MT];
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (unsigned p = 0; p + 1 < Groups; ++p)
+#pragma unroll
+            for (unsigned i = 0; i < NT * MT; ++i) acc[i / MT][i % MT] += sums[(p * Waves * NT * MT + i) * kWave];
+    }
     typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
     auto store = [&](auto whole) {
         constexpr bool Whole = decltype(whole)::value;
@@ -666,73 +689,92 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
 // ------------------------------------------------------------------------------------------------
 // Few rows (single tokens, small batches): a workgroup takes 16 columns of y for all rows; its eight waves
 // share the blocks of the inner axis and add their sums through LDS in the waves' order. The weight's
-// codes go from memory to the MFMA's registers, each byte read once on the chip; a lane takes 32
-// consecutive codes of its row. Dense x is quantized by every workgroup for itself, in the operand's
-// layout: a row's block lies in lanes 16 apart.
-constexpr unsigned kTokenWaves = 8;
+// codes go from memory to the MFMA's registers, each byte read once on the chip, four blocks' loads at a
+// time before the first is used: what bounds this is how many bytes are on their way. A lane takes 32
+// consecutive codes of its row.
+// Dense: up to kFusedRows rows of dense x, which every workgroup quantizes for itself into LDS while its
+// first weights are on their way; more rows than that are cheaper to quantize once, in a launch of its own.
+constexpr unsigned kTokenWaves = 8, kFusedRows = 4;
 
 template <typename T, unsigned MT, bool Dense>
 __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) {
     constexpr bool Exact = std::is_same<T, F32>::value;
+    constexpr unsigned Ahead = 4; // blocks of a wave loaded at a time
     __shared__ f32x4 sums[kTokenWaves][MT][kWave];
-    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave, l16 = lane % 16, g = lane / 16;
-    const unsigned n0 = blockIdx.x * 16;
-    const std::uint64_t pitch = std::uint64_t(a.count) * kBlock;
-    const std::uint8_t* wp = a.w + min(n0 + l16, a.outer - 1) * pitch + g * 32;
+    extern __shared__ __align__(16) std::uint8_t lds[]; // Dense: x's codes, then its exponents
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const unsigned l16 = lane % 16, g = lane / 16, n0 = blockIdx.x * 16, pitch = a.count * kBlock;
+    const std::uint8_t* wp = a.w + min(n0 + l16, a.outer - 1) * std::uint64_t(pitch) + g * 32;
     const std::uint8_t* wep = a.we + std::uint64_t(n0 / kBlock) * a.expPitch;
-    f32x4 acc[MT] = {};
-    for (unsigned k = wave; k < a.count; k += kTokenWaves) {
-        const u32x4 w0 = *reinterpret_cast<const u32x4*>(wp + k * kBlock);
-        const u32x4 w1 = *reinterpret_cast<const u32x4*>(wp + k * kBlock + 16);
-        const unsigned we = wep[k];
+    std::uint8_t* exponents = lds + a.rows * pitch;
+    u32x4 w[Ahead][2];
+    auto fetch = [&](unsigned k) {
 #pragma unroll
-        for (unsigned m = 0; m < MT; ++m) {
-            const unsigned row = m * 16 + l16;
-            u32x4 x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
-            unsigned xe = 127;
-            if constexpr (Dense) {
-                float v[4][8];
-                unsigned peak = 0;
-                const auto* xp = static_cast<const typename T::Raw*>(a.dense) + min(row, a.rows - 1) * a.denseStride;
-#pragma unroll
-                for (unsigned i = 0; i < 4; ++i) {
-                    load8<T>(xp, k * kBlock + g * 32 + i * 8, a.inner, v[i]);
-                    peak = max(peak, peakBits(v[i]));
-                }
-                peak = max(peak, unsigned(__shfl_xor(int(peak), 16)));
-                peak = max(peak, unsigned(__shfl_xor(int(peak), 32)));
-                xe = exponentOf<BlockCodes::e4m3>(peak);
-                const u32x2 q0 = encode8<BlockCodes::e4m3>(v[0], xe), q1 = encode8<BlockCodes::e4m3>(v[1], xe);
-                const u32x2 q2 = encode8<BlockCodes::e4m3>(v[2], xe), q3 = encode8<BlockCodes::e4m3>(v[3], xe);
-                x0 = u32x4{q0.x, q0.y, q1.x, q1.y};
-                x1 = u32x4{q2.x, q2.y, q3.x, q3.y};
-                if (a.keep && blockIdx.x == 0 && row < a.rows) {
-                    u32x4* to = reinterpret_cast<u32x4*>(a.keep + row * pitch + k * kBlock + g * 32);
-                    to[0] = x0;
-                    to[1] = x1;
-                    if (k + g < (k + 1 == a.count ? a.expPitch : k + 1))
-                        a.keepExp[std::uint64_t(row) * a.expPitch + k + g] = std::uint8_t(g ? 127u : xe);
-                }
-            } else {
-                const std::uint64_t at = min(row, a.rows - 1);
-                x0 = *reinterpret_cast<const u32x4*>(a.x + at * pitch + k * kBlock + g * 32);
-                x1 = *reinterpret_cast<const u32x4*>(a.x + at * pitch + k * kBlock + g * 32 + 16);
-                xe = a.xe[at * a.expPitch + k];
-            }
-            if constexpr (Exact) {
-                const float xs = scaleOf(xe), ws = scaleOf(we);
-#pragma unroll
-                for (unsigned i = 0; i < 4; ++i) {
-                    const u32x4 wq = i < 2 ? w0 : w1, xq = i < 2 ? x0 : x1;
-                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values8(wq[i % 2 * 2], wq[i % 2 * 2 + 1], ws),
-                                                                     values8(xq[i % 2 * 2], xq[i % 2 * 2 + 1], xs),
-                                                                     acc[m], 0, 0, 0);
-                }
-            } else {
-                acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w0, w1), join(x0, x1), acc[m], 0, 0, 0,
-                                                                          int(we), 0, int(xe));
+        for (unsigned u = 0; u < Ahead; ++u) {
+            const std::uint8_t* p = wp + std::uint64_t(min(k + u * kTokenWaves, a.count - 1)) * kBlock;
+            w[u][0] = *reinterpret_cast<const u32x4*>(p);
+            w[u][1] = *reinterpret_cast<const u32x4*>(p + 16);
+        }
+    };
+    fetch(wave);
+    if constexpr (Dense) {
+        const unsigned sub = t % kBlockLanes;
+        for (unsigned item = t / kBlockLanes; item < a.rows * a.count; item += kWave * kTokenWaves / kBlockLanes) {
+            const unsigned row = item / a.count, block = item - row * a.count;
+            float v[8];
+            load8<T>(static_cast<const typename T::Raw*>(a.dense) + row * a.denseStride, block * kBlock + sub * 8, a.inner, v);
+            const unsigned e = exponentOf<BlockCodes::e4m3>(rowMax(peakBits(v)));
+            const u32x2 q = encode8<BlockCodes::e4m3>(v, e);
+            *reinterpret_cast<u32x2*>(lds + row * pitch + block * kBlock + sub * 8) = q;
+            if (sub == 0) exponents[item] = std::uint8_t(e);
+            if (a.keep && blockIdx.x == 0) {
+                *reinterpret_cast<u32x2*>(a.keep + row * std::uint64_t(pitch) + block * kBlock + sub * 8) = q;
+                if (block + sub < (block + 1 == a.count ? a.expPitch : block + 1))
+                    a.keepExp[row * std::uint64_t(a.expPitch) + block + sub] = std::uint8_t(sub ? 127u : e);
             }
         }
+        __syncthreads();
+    }
+    f32x4 acc[MT] = {};
+    for (unsigned k = wave; k < a.count; k += Ahead * kTokenWaves) {
+        u32x4 x[Ahead][MT][2];
+        unsigned xe[Ahead][MT];
+#pragma unroll
+        for (unsigned u = 0; u < Ahead; ++u) {
+            const unsigned block = min(k + u * kTokenWaves, a.count - 1);
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                const unsigned row = min(m * 16 + l16, a.rows - 1);
+                const std::uint8_t* p = Dense ? lds + row * pitch : a.x + row * std::uint64_t(pitch);
+                x[u][m][0] = *reinterpret_cast<const u32x4*>(p + block * kBlock + g * 32);
+                x[u][m][1] = *reinterpret_cast<const u32x4*>(p + block * kBlock + g * 32 + 16);
+                xe[u][m] = Dense ? exponents[row * a.count + block] : a.xe[row * std::uint64_t(a.expPitch) + block];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0); // the compiler would move the loads down to their use
+#pragma unroll
+        for (unsigned u = 0; u < Ahead; ++u) {
+            if (k + u * kTokenWaves >= a.count) break;
+            const unsigned we = wep[k + u * kTokenWaves];
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                if constexpr (Exact) {
+                    const float xs = scaleOf(xe[u][m]), ws = scaleOf(we);
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i) {
+                        const u32x4 wq = w[u][i / 2], xq = x[u][m][i / 2];
+                        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            values8(wq[i % 2 * 2], wq[i % 2 * 2 + 1], ws), values8(xq[i % 2 * 2], xq[i % 2 * 2 + 1], xs),
+                            acc[m], 0, 0, 0);
+                    }
+                } else {
+                    acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w[u][0], w[u][1]),
+                                                                              join(x[u][m][0], x[u][m][1]), acc[m], 0, 0,
+                                                                              0, int(we), 0, int(xe[u][m]));
+                }
+            }
+        }
+        if (k + Ahead * kTokenWaves < a.count) fetch(k + Ahead * kTokenWaves);
     }
 #pragma unroll
     for (unsigned m = 0; m < MT; ++m) sums[wave][m][lane] = acc[m];
@@ -753,47 +795,62 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) 
 // ------------------------------------------------------------------------------------------------
 // Host side
 
+// FP32 rows that multiplyTokens takes; its tiles are of 128.
 constexpr unsigned kTokenRows = 64;
 
-template <typename T, bool Dense> void launchTokens(const Product& p, hipStream_t stream) {
+void launchTokens(const Product& p, hipStream_t stream) {
     const dim3 grid((p.outer + 15) / 16), threads(kWave * kTokenWaves);
     if (p.rows <= 16)
-        hipLaunchKernelGGL((multiplyTokens<T, 1, Dense>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 1, false>), grid, threads, 0, stream, p);
     else if (p.rows <= 32)
-        hipLaunchKernelGGL((multiplyTokens<T, 2, Dense>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 2, false>), grid, threads, 0, stream, p);
     else
-        hipLaunchKernelGGL((multiplyTokens<T, 4, Dense>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 4, false>), grid, threads, 0, stream, p);
     checkHip(hipGetLastError());
 }
 
-// The tile of a product: the least estimated time, in microseconds, rounds of workgroups on the chip times the
-// blocks of the inner axis. A CU holds one workgroup of tiles of 256, two of 128 or 64. The constants fit
-// these times (rows x inner x outer: 256, 128, 64):
-//   4096 x 4096 x 8192 122, 192, 269    2048 x 1024 x 4096 22, 15.2, 20     2048 x 4096 x 1024 49, 28.8, 17.7
-//   1024 x 4096 x 4096 51, 31.3, 32.3   512 x 4096 x 4096 48, 26.9, 18.1    16384 x 512 x 512 16, 10.9, 14.4
-//   777 x 1001 x 1437 23, 9.9, 6.9      300 x 2000 x 6000 31, 13.8, 9.5     100000 x 256 x 256 29, 20.9, 30.7
-enum class Form { wide, middle, small };
+// LDS of x's codes and exponents in a fused product of few rows.
+std::size_t fusedLds(std::uint32_t rows, unsigned count) { return (std::size_t(rows) * count * (kBlock + 1) + 15) / 16 * 16; }
+bool fusedTokens(std::uint32_t rows, std::uint32_t inner) {
+    return rows <= kFusedRows && fusedLds(rows, (inner + kBlock - 1) / kBlock) <= 48 * 1024;
+}
+
+template <typename T> void launchFusedTokens(const Product& p, hipStream_t stream) {
+    hipLaunchKernelGGL((multiplyTokens<T, 1, true>), dim3((p.outer + 15) / 16), dim3(kWave * kTokenWaves),
+                       fusedLds(p.rows, p.count), stream, p);
+    checkHip(hipGetLastError());
+}
+
+// The tile of a 16-bit product: the least estimated time, in microseconds, rounds of workgroups on the chip
+// times the blocks of the inner axis. A CU holds one workgroup of tiles of 256 or, with its four groups of
+// waves, 32, two of 128 or 64. The constants fit these times (rows x inner x outer: 256, 128, 64, 32):
+//   4096 x 4096 x 8192 122, 192, 269, -     2048 x 1024 x 4096 22, 15.2, 20, -    2048 x 4096 x 1024 49, 28.8, 17.7, 40
+//   1024 x 4096 x 4096 51, 31.3, 31.0, 78   512 x 4096 x 4096 48, 26.9, 17.9, 40  16384 x 512 x 512 16, 10.9, 14.4, -
+//   777 x 1001 x 1437 23, 9.9, 6.7, 16      300 x 2000 x 6000 31, 13.8, 9.5, 27   100000 x 256 x 256 29, 20.9, 30.7, -
+//   128 x 4096 x 4096 48, 24, 8.9, 11.0     24 x 4096 x 8192 -, -, 9.7, 6.8       16 x 1024 x 4096 -, -, 4.2, 4.5
+enum class Form { wide, middle, small, few };
 Form formOf(std::uint32_t rows, std::uint32_t outer, unsigned count) {
     const auto tiles = [&](unsigned size) {
         return std::uint64_t((rows + size - 1) / size) * ((outer + size - 1) / size);
     };
     const auto rounds = [](std::uint64_t n, unsigned slots) { return double((n + slots - 1) / slots); };
-    const std::uint64_t large = tiles(256), half = tiles(128), quarter = tiles(64);
-    const double wide = rounds(large, 256) * (11.5 + 1.5 * count);
+    const std::uint64_t half = tiles(128), quarter = tiles(64);
+    const double wide = rounds(tiles(256), 256) * (11.5 + 1.5 * count);
     const double middle = half <= 256 ? 5.0 + 0.75 * count : rounds(half, 512) * (5.0 + 1.3 * count);
-    const double small = quarter <= 256 ? 2.2 + 0.25 * count : rounds(quarter, 512) * (1.5 + 0.5 * count);
-    if (wide <= middle && wide <= small) return Form::wide;
-    return middle <= small ? Form::middle : Form::small;
+    const double small = quarter <= 256 ? 2.9 + 0.18 * count : rounds(quarter, 512) * (1.5 + 0.5 * count);
+    const double few = rounds(tiles(32), 256) * (3.9 + 0.09 * count);
+    const double least = std::min(std::min(wide, middle), std::min(small, few));
+    return least == wide ? Form::wide : least == middle ? Form::middle : least == small ? Form::small : Form::few;
 }
 
-template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages>
+template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 void launchTiles(Product p, hipStream_t stream) {
     p.tilesM = (p.rows + BM - 1) / BM, p.tilesN = (p.outer + BN - 1) / BN;
     const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
-    const std::size_t lds = Stages * (BM + BN) * kBlock;
+    const std::size_t lds = Groups * Stages * (BM + BN) * kBlock;
     if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
-    hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages>), dim3(unsigned(tiles)), dim3(64 * WM * WN), lds,
-                       stream, p);
+    hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
+                       dim3(64 * WM * WN * Groups), lds, stream, p);
     checkHip(hipGetLastError());
 }
 
@@ -806,8 +863,8 @@ template <typename T> void launchWide(Product p, hipStream_t stream) {
 }
 
 template <typename T> void launchProduct(Product p, hipStream_t stream) {
-    if (p.rows <= kTokenRows) return launchTokens<T, false>(p, stream);
     if constexpr (std::is_same<T, F32>::value) {
+        if (p.rows <= kTokenRows) return launchTokens(p, stream);
         p.tilesM = (p.rows + 127) / 128;
         const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + 127) / 128);
         if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
@@ -816,8 +873,9 @@ template <typename T> void launchProduct(Product p, hipStream_t stream) {
     } else {
         switch (formOf(p.rows, p.outer, p.count)) {
         case Form::wide: launchWide<T>(p, stream); break;
-        case Form::middle: launchTiles<T, 128, 128, 4, 2, 2>(p, stream); break;
-        case Form::small: launchTiles<T, 64, 64, 2, 2, 4>(p, stream); break;
+        case Form::middle: launchTiles<T, 128, 128, 4, 2, 2, 1>(p, stream); break;
+        case Form::small: launchTiles<T, 64, 64, 2, 2, 4, 1>(p, stream); break;
+        case Form::few: launchTiles<T, 32, 32, 2, 1, 4, 4>(p, stream); break;
         }
     }
 }
@@ -853,8 +911,6 @@ void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, De
 }
 
 namespace {
-bool fusedTokens(std::uint32_t rows) { return rows <= kTokenRows; }
-
 // The weight's bytes in LDS if a narrow layer with many rows goes through multiplyRows, else 0.
 constexpr unsigned kRowsLds = 160 * 1024;
 std::size_t rowsImage(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
@@ -881,7 +937,7 @@ std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 25
 std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                   bool keep) {
     std::size_t bytes = matmulBlocksWorkspace(rows, inner, outer, type);
-    if (!keep && !fusedTokens(rows) && !rowsImage(rows, inner, outer, type))
+    if (!keep && !fusedTokens(rows, inner) && !rowsImage(rows, inner, outer, type))
         bytes += rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
     return bytes;
 }
@@ -905,7 +961,7 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
     if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
     const std::size_t image = rowsImage(rows, inner, outer, x.type);
-    if (fusedTokens(rows) || image) {
+    if (fusedTokens(rows, inner) || image) {
         Product p = {};
         p.w = w.codes, p.we = w.exponents, p.bias = bias, p.y = y, p.yStride = yStride;
         p.rows = rows, p.outer = outer, p.inner = inner;
@@ -916,7 +972,7 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
             if (image)
                 launchRows<decltype(tag)>(p, image, stream);
             else
-                launchTokens<decltype(tag), true>(p, stream);
+                launchFusedTokens<decltype(tag)>(p, stream);
         });
         return;
     }

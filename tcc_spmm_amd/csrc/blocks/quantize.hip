@@ -2,7 +2,7 @@
 //
 // Rows: 16 lanes take one block of 128 elements, 8 a lane: one load (two at FP32), the peak by four DPP
 // steps inside the lanes' DPP row, one 8-byte store of codes. A thread takes kItems blocks and issues all
-// their loads first. Bound by HBM.
+// their loads first: four, or one where that leaves units without work. Bound by HBM.
 //
 // Weights: a workgroup takes one tile of 128 x 128, 64 elements a thread in registers, finds the tile's
 // peak through LDS and writes the codes and, for the input gradient, the transposed codes, whose
@@ -14,10 +14,10 @@ namespace {
 
 using namespace blocks;
 
-constexpr unsigned kThreads = 256, kItems = 4;
+constexpr unsigned kThreads = 256;
 constexpr unsigned kGroups = kThreads / kBlockLanes;
 
-template <typename T, BlockCodes C>
+template <typename T, BlockCodes C, unsigned kItems>
 __global__ __launch_bounds__(kThreads) void quantizeRowBlocks(const typename T::Raw* __restrict__ x,
                                                                std::uint64_t stride,
                                                                std::uint8_t* __restrict__ codes,
@@ -138,9 +138,12 @@ __global__ __launch_bounds__(kThreads) void quantizeWeightTiles(const typename T
     }
 }
 
+// Blocks up to which a thread takes one: sixteen workgroups' for each of 256 units.
+constexpr unsigned kFewItems = 256 * 16 * 16;
+
 unsigned itemsOf(const char* where, std::uint32_t rows, unsigned count) {
     const std::uint64_t items = std::uint64_t(rows) * count;
-    if (items >= (std::uint64_t(1) << 32) - kGroups * kItems) reject(where, "more than 2^32 blocks");
+    if (items >= (std::uint64_t(1) << 32) - kGroups * 4) reject(where, "more than 2^32 blocks");
     return unsigned(items);
 }
 
@@ -154,16 +157,21 @@ void quantizeBlocks(DenseMatrix x, BlockRows out, std::uint32_t rows, std::uint3
     checkDense("quantize blocks", x.data, x.stride, x.type, columns);
     checkCodes("quantize blocks", out.codes, out.exponents);
     const unsigned count = (columns + kBlock - 1) / kBlock, items = itemsOf("quantize blocks", rows, count);
-    const unsigned grid = (items + kGroups * kItems - 1) / (kGroups * kItems);
-    withType(x.type, [&](auto tag) {
+    const auto launch = [&](auto tag, auto codes, auto each) {
         typedef decltype(tag) T;
-        const auto* data = static_cast<const typename T::Raw*>(x.data);
-        if (out.type == BlockCodes::e4m3)
-            hipLaunchKernelGGL((quantizeRowBlocks<T, BlockCodes::e4m3>), dim3(grid), dim3(kThreads), 0, stream, data,
-                               x.stride, out.codes, out.exponents, items, columns, count, rowMagic(count));
-        else
-            hipLaunchKernelGGL((quantizeRowBlocks<T, BlockCodes::int8>), dim3(grid), dim3(kThreads), 0, stream, data,
-                               x.stride, out.codes, out.exponents, items, columns, count, rowMagic(count));
+        constexpr unsigned kItems = decltype(each)::value;
+        const unsigned grid = (items + kGroups * kItems - 1) / (kGroups * kItems);
+        hipLaunchKernelGGL((quantizeRowBlocks<T, decltype(codes)::value, kItems>), dim3(grid), dim3(kThreads), 0, stream,
+                           static_cast<const typename T::Raw*>(x.data), x.stride, out.codes, out.exponents, items,
+                           columns, count, rowMagic(count));
+    };
+    withType(x.type, [&](auto tag) {
+        withCodes(out.type, [&](auto codes) {
+            if (items < kFewItems)
+                launch(tag, codes, std::integral_constant<unsigned, 1>{});
+            else
+                launch(tag, codes, std::integral_constant<unsigned, 4>{});
+        });
     });
     checkHip(hipGetLastError());
 }

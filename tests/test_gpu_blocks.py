@@ -139,7 +139,7 @@ def product_room(x, w, dtype):
 
 SHAPES = [(1, 1, 1), (1, 128, 16), (1, 4096, 130), (3, 100, 77), (16, 512, 64), (17, 1001, 200), (40, 640, 129),
           (64, 256, 300), (65, 128, 128), (129, 129, 127), (200, 1300, 257), (300, 384, 513), (513, 1024, 640),
-          (700, 2048, 1000), (1111, 96, 47), (5000, 128, 256)]
+          (700, 2048, 1000), (1111, 96, 47), (5000, 128, 256), (24, 4096, 1000), (32, 2900, 513), (5, 2048, 2050)]
 
 
 @pytest.mark.parametrize("rows,inner,outer,dtype", [(4090, 200, 4100, "bf16"), (4091, 300, 4099, "f16"),
