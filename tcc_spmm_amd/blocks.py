@@ -13,7 +13,6 @@ rows is copied first.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -43,11 +42,12 @@ def _check_stored(codes, exponents, columns: int, types, exponent_rows: int | No
         raise ValueError(f"{name} exponents must be torch.uint8, got {exponents.dtype}")
     if columns < 1:
         raise ValueError(f"{name} needs at least one column")
-    if codes.dim() != 2 or codes.shape[1] != _blocks(columns) * BLOCK or not codes.is_contiguous():
-        raise ValueError(f"{name} codes must be contiguous [rows, {_blocks(columns) * BLOCK}]")
-    rows = codes.shape[0] if exponent_rows is None else exponent_rows
-    if tuple(exponents.shape) != (rows, _exponent_pitch(columns)) or not exponents.is_contiguous():
-        raise ValueError(f"{name} exponents must be contiguous [{rows}, {_exponent_pitch(columns)}]")
+    blocks = _blocks(columns)
+    if codes.dim() != 2 or codes.shape[1] != blocks * BLOCK or not codes.is_contiguous():
+        raise ValueError(f"{name} codes must be contiguous [rows, {blocks * BLOCK}]")
+    rows, pitch = codes.shape[0] if exponent_rows is None else exponent_rows, -(-blocks // 4) * 4
+    if exponents.shape != (rows, pitch) or not exponents.is_contiguous():
+        raise ValueError(f"{name} exponents must be contiguous [{rows}, {pitch}]")
     if exponents.device != codes.device:
         raise ValueError(f"tensor on {exponents.device}, expected {codes.device}")
 
@@ -101,25 +101,32 @@ class BlockWeight:
         """The transposed weight's view of the same codes."""
         if self.codes_t is None:
             raise ValueError("the weight was quantized without its transposed copy")
-        return BlockWeight(self.codes_t, self.exponents_t, self.rows, self.codes, self.exponents)
+        return _weight(self.codes_t, self.exponents_t, self.rows, self.codes, self.exponents)
 
 
-_NOWHERE = contextlib.nullcontext()
+def _weight(codes, exponents, columns, codes_t, exponents_t) -> BlockWeight:
+    """A BlockWeight of tensors that are laid out as its constructor would check."""
+    out = BlockWeight.__new__(BlockWeight)
+    out.codes, out.exponents, out.columns = codes, exponents, columns
+    out.codes_t, out.exponents_t = codes_t, exponents_t
+    return out
 
 
-def _place(device, stream):
-    """Where a call's outputs are allocated and its kernels launched."""
+def _away(device, stream):
+    """None if a call's outputs and launches belong where the caller already is, else the context to make it
+    in: another stream than the current one, or another device."""
     if device.type != "cuda":
         raise ValueError("device entry points take CUDA (HIP) tensors")
-    if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"stream on {stream.device}, tensors on {device}")
-        return torch.cuda.stream(stream)
-    return _NOWHERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if stream is None:
+        return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream on {stream.device}, tensors on {device}")
+    return torch.cuda.stream(stream)
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+# The current stream's handle; making a torch.cuda.Stream of it would cost 3 us a call.
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _dense(t: torch.Tensor, name: str, columns: int | None = None) -> None:
@@ -160,8 +167,11 @@ def _bias(bias, outer: int, device):
 
 
 def _new_blocks(rows: int, columns: int, codes, device) -> BlockTensor:
-    return BlockTensor(torch.empty((rows, _blocks(columns) * BLOCK), dtype=codes, device=device),
-                       torch.empty((rows, _exponent_pitch(columns)), dtype=torch.uint8, device=device), columns)
+    out = BlockTensor.__new__(BlockTensor)  # laid out as its constructor would check
+    out.codes = torch.empty((rows, _blocks(columns) * BLOCK), dtype=codes, device=device)
+    out.exponents = torch.empty((rows, _exponent_pitch(columns)), dtype=torch.uint8, device=device)
+    out.columns = columns
+    return out
 
 
 def _workspace(query, args, device):
@@ -178,12 +188,16 @@ def quantize_blocks(x: torch.Tensor, codes=E4M3, stream=None) -> BlockTensor:
     _dense(x, "x")
     if codes not in _CODES:
         raise ValueError(f"codes must be float8_e4m3fn or int8, got {codes}")
-    with _place(x.device, stream):
-        x = _rows(x)
-        out = _new_blocks(x.shape[0], x.shape[1], codes, x.device)
-        check(lib().tcc_quantize_blocks(x.data_ptr(), _stride(x), _TYPES[x.dtype], out.codes.data_ptr(),
-                                        out.exponents.data_ptr(), _CODES[codes], x.shape[0], x.shape[1],
-                                        _stream()))
+    device = x.device
+    away = _away(device, stream)
+    if away:
+        with away:
+            return quantize_blocks(x, codes)
+    x = _rows(x)
+    out = _new_blocks(x.shape[0], x.shape[1], codes, device)
+    check(lib().tcc_quantize_blocks(x.data_ptr(), _stride(x), _TYPES[x.dtype], out.codes.data_ptr(),
+                                    out.exponents.data_ptr(), _CODES[codes], x.shape[0], x.shape[1],
+                                    _stream(device.index)))
     return out
 
 
@@ -192,11 +206,14 @@ def dequantize_blocks(x: BlockTensor, dtype=torch.float32, stream=None) -> torch
     if dtype not in _TYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     device = x.codes.device
-    with _place(device, stream):
-        out = torch.empty((x.rows, x.columns), dtype=dtype, device=device)
-        check(lib().tcc_dequantize_blocks(x.codes.data_ptr(), x.exponents.data_ptr(), _CODES[x.codes.dtype],
-                                          out.data_ptr(), x.columns, _TYPES[dtype], x.rows, x.columns,
-                                          _stream()))
+    away = _away(device, stream)
+    if away:
+        with away:
+            return dequantize_blocks(x, dtype)
+    out = torch.empty((x.rows, x.columns), dtype=dtype, device=device)
+    check(lib().tcc_dequantize_blocks(x.codes.data_ptr(), x.exponents.data_ptr(), _CODES[x.codes.dtype],
+                                      out.data_ptr(), x.columns, _TYPES[dtype], x.rows, x.columns,
+                                      _stream(device.index)))
     return out
 
 
@@ -208,20 +225,23 @@ def quantize_weight_blocks(w: torch.Tensor, transposed: bool = True, stream=None
         raise ValueError("w must be [outer, inner]")
     outer, inner = w.shape
     device = w.device
-    with _place(device, stream):
-        w = _rows(w)
+    away = _away(device, stream)
+    if away:
+        with away:
+            return quantize_weight_blocks(w, transposed)
+    w = _rows(w)
 
-        def space(rows, columns):
-            return (torch.empty((rows, _blocks(columns) * BLOCK), dtype=E4M3, device=device),
-                    torch.empty((_blocks(rows), _exponent_pitch(columns)), dtype=torch.uint8, device=device))
+    def space(rows, columns):
+        return (torch.empty((rows, _blocks(columns) * BLOCK), dtype=E4M3, device=device),
+                torch.empty((_blocks(rows), _exponent_pitch(columns)), dtype=torch.uint8, device=device))
 
-        codes, exponents = space(outer, inner)
-        codes_t, exponents_t = space(inner, outer) if transposed else (None, None)
-        check(lib().tcc_quantize_weight_blocks(
-            w.data_ptr(), _stride(w), _TYPES[w.dtype], codes.data_ptr(), exponents.data_ptr(),
-            codes_t.data_ptr() if transposed else 0, exponents_t.data_ptr() if transposed else 0, outer, inner,
-            _stream()))
-    return BlockWeight(codes, exponents, inner, codes_t, exponents_t)
+    codes, exponents = space(outer, inner)
+    codes_t, exponents_t = space(inner, outer) if transposed else (None, None)
+    check(lib().tcc_quantize_weight_blocks(
+        w.data_ptr(), _stride(w), _TYPES[w.dtype], codes.data_ptr(), exponents.data_ptr(),
+        codes_t.data_ptr() if transposed else 0, exponents_t.data_ptr() if transposed else 0, outer, inner,
+        _stream(device.index)))
+    return _weight(codes, exponents, inner, codes_t, exponents_t)
 
 
 def matmul_blocks(x: BlockTensor, weight: BlockWeight, bias: torch.Tensor | None = None,
@@ -235,14 +255,17 @@ def matmul_blocks(x: BlockTensor, weight: BlockWeight, bias: torch.Tensor | None
         raise ValueError(f"x has rows of {x.columns} elements, expected {weight.columns}")
     device, outer = x.codes.device, weight.rows
     _same_device(device, weight.codes)
-    bias = _bias(bias, outer, device)
-    with _place(device, stream):
-        y = torch.empty((x.rows, outer), dtype=dtype, device=device)
-        sizes = (x.rows, x.columns, outer, _TYPES[dtype])
-        _space, at, size = _workspace(lib().tcc_matmul_blocks_workspace, sizes, device)
-        check(lib().tcc_matmul_blocks(x.codes.data_ptr(), x.exponents.data_ptr(), weight.codes.data_ptr(),
-                                      weight.exponents.data_ptr(), bias, y.data_ptr(), outer, sizes[3], x.rows,
-                                      x.columns, outer, at, size, _stream()))
+    at_bias = _bias(bias, outer, device)
+    away = _away(device, stream)
+    if away:
+        with away:
+            return matmul_blocks(x, weight, bias, dtype)
+    y = torch.empty((x.rows, outer), dtype=dtype, device=device)
+    sizes = (x.rows, x.columns, outer, _TYPES[dtype])
+    _space, at, size = _workspace(lib().tcc_matmul_blocks_workspace, sizes, device)
+    check(lib().tcc_matmul_blocks(x.codes.data_ptr(), x.exponents.data_ptr(), weight.codes.data_ptr(),
+                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, sizes[3], x.rows,
+                                  x.columns, outer, at, size, _stream(device.index)))
     return y
 
 
@@ -254,19 +277,22 @@ def linear_blocks(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | Non
     _dense(x, "x", inner)
     device = x.device
     _same_device(device, weight.codes)
-    bias = _bias(bias, outer, device)
+    at_bias = _bias(bias, outer, device)
     kind = _TYPES[x.dtype]
-    with _place(device, stream):
-        flat = _rows(x)
-        rows = flat.shape[0]
-        y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
-        kept = _new_blocks(rows, inner, E4M3, device) if keep else None
-        _space, at, size = _workspace(lib().tcc_linear_blocks_workspace, (rows, inner, outer, kind, keep), device)
-        check(lib().tcc_linear_blocks(flat.data_ptr(), _stride(flat), kind, weight.codes.data_ptr(),
-                                      weight.exponents.data_ptr(), bias, y.data_ptr(), outer,
-                                      kept.codes.data_ptr() if keep else 0,
-                                      kept.exponents.data_ptr() if keep else 0, rows, inner, outer, at, size,
-                                      _stream()))
+    away = _away(device, stream)
+    if away:
+        with away:
+            return linear_blocks(x, weight, bias, keep=keep)
+    flat = _rows(x)
+    rows = flat.shape[0]
+    y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
+    kept = _new_blocks(rows, inner, E4M3, device) if keep else None
+    _space, at, size = _workspace(lib().tcc_linear_blocks_workspace, (rows, inner, outer, kind, keep), device)
+    check(lib().tcc_linear_blocks(flat.data_ptr(), _stride(flat), kind, weight.codes.data_ptr(),
+                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer,
+                                  kept.codes.data_ptr() if keep else 0,
+                                  kept.exponents.data_ptr() if keep else 0, rows, inner, outer, at, size,
+                                  _stream(device.index)))
     return (y, kept) if keep else y
 
 
@@ -280,15 +306,18 @@ def weight_grad_blocks(dy: torch.Tensor, x: BlockTensor, bias: bool = True, stre
     _same_device(device, x.codes)
     if dy.numel() != x.rows * outer:
         raise ValueError(f"dy has {dy.numel() // outer} rows, the kept blocks {x.rows}")
-    with _place(device, stream):
-        dy = _rows(dy)
-        dw = torch.empty((outer, x.columns), dtype=torch.float32, device=device)
-        db = torch.empty(outer, dtype=torch.float32, device=device) if bias else None
-        sizes = (x.rows, x.columns, outer, _TYPES[dy.dtype])
-        _space, at, size = _workspace(lib().tcc_weight_grad_blocks_workspace, sizes, device)
-        check(lib().tcc_weight_grad_blocks(dy.data_ptr(), _stride(dy), sizes[3], x.codes.data_ptr(),
-                                           x.exponents.data_ptr(), dw.data_ptr(), db.data_ptr() if bias else 0,
-                                           x.rows, x.columns, outer, at, size, _stream()))
+    away = _away(device, stream)
+    if away:
+        with away:
+            return weight_grad_blocks(dy, x, bias)
+    dy = _rows(dy)
+    dw = torch.empty((outer, x.columns), dtype=torch.float32, device=device)
+    db = torch.empty(outer, dtype=torch.float32, device=device) if bias else None
+    sizes = (x.rows, x.columns, outer, _TYPES[dy.dtype])
+    _space, at, size = _workspace(lib().tcc_weight_grad_blocks_workspace, sizes, device)
+    check(lib().tcc_weight_grad_blocks(dy.data_ptr(), _stride(dy), sizes[3], x.codes.data_ptr(),
+                                       x.exponents.data_ptr(), dw.data_ptr(), db.data_ptr() if bias else 0,
+                                       x.rows, x.columns, outer, at, size, _stream(device.index)))
     return dw, db
 
 
@@ -322,15 +351,18 @@ def activation_blocks(x: torch.Tensor, kind: str = "silu", *, gated: bool = Fals
         raise ValueError("a gated activation needs rows of an even number of elements")
     width = x.shape[-1] // 2 if gated else x.shape[-1]
     device = x.device
-    with _place(device, stream):
-        flat = _rows(x)
-        rows = flat.shape[0]
-        y = torch.empty((*x.shape[:-1], width), dtype=x.dtype, device=device)
-        kept = None if codes is None else _new_blocks(2 * rows if gated else rows, width, codes, device)
-        check(lib().tcc_activation_blocks(flat.data_ptr(), _stride(flat), _TYPES[x.dtype], function, gated,
-                                          y.data_ptr(), width, kept.codes.data_ptr() if kept else 0,
-                                          kept.exponents.data_ptr() if kept else 0,
-                                          _CODES[codes] if kept else 0, rows, width, _stream()))
+    away = _away(device, stream)
+    if away:
+        with away:
+            return activation_blocks(x, kind, gated=gated, codes=codes)
+    flat = _rows(x)
+    rows = flat.shape[0]
+    y = torch.empty((*x.shape[:-1], width), dtype=x.dtype, device=device)
+    kept = None if codes is None else _new_blocks(2 * rows if gated else rows, width, codes, device)
+    check(lib().tcc_activation_blocks(flat.data_ptr(), _stride(flat), _TYPES[x.dtype], function, gated,
+                                      y.data_ptr(), width, kept.codes.data_ptr() if kept else 0,
+                                      kept.exponents.data_ptr() if kept else 0,
+                                      _CODES[codes] if kept else 0, rows, width, _stream(device.index)))
     return y, kept
 
 
@@ -345,13 +377,16 @@ def activation_blocks_backward(dy: torch.Tensor, kept: BlockTensor, kind: str = 
     if dy.numel() // width * (2 if gated else 1) != kept.rows:
         raise ValueError(f"dy has {dy.numel() // width} rows, the kept blocks {kept.rows}")
     wide = 2 * width if gated else width
-    with _place(device, stream):
-        flat = _rows(dy)
-        dx = torch.empty((*dy.shape[:-1], wide), dtype=dy.dtype, device=device)
-        check(lib().tcc_activation_blocks_backward(flat.data_ptr(), _stride(flat), _TYPES[dy.dtype],
-                                                   kept.codes.data_ptr(), kept.exponents.data_ptr(),
-                                                   _CODES[kept.codes.dtype], function, gated, dx.data_ptr(), wide,
-                                                   flat.shape[0], width, _stream()))
+    away = _away(device, stream)
+    if away:
+        with away:
+            return activation_blocks_backward(dy, kept, kind, gated=gated)
+    flat = _rows(dy)
+    dx = torch.empty((*dy.shape[:-1], wide), dtype=dy.dtype, device=device)
+    check(lib().tcc_activation_blocks_backward(flat.data_ptr(), _stride(flat), _TYPES[dy.dtype],
+                                               kept.codes.data_ptr(), kept.exponents.data_ptr(),
+                                               _CODES[kept.codes.dtype], function, gated, dx.data_ptr(), wide,
+                                               flat.shape[0], width, _stream(device.index)))
     return dx
 
 
