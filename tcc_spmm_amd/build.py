@@ -68,25 +68,28 @@ def check_kernel_asm(src: pathlib.Path = CSRC / "kernel" / "spmm.hip") -> None:
         raise RuntimeError("SpMM kernel assembly check failed:\n  " + "\n  ".join(problems))
 
 
-def check_product_asm(src: pathlib.Path = CSRC / "blocks" / "product.hip") -> None:
-    """The same for the product of 8-bit blocks: multiplyWide's MFMAs are inline assembly, whose latency
-    the compiler does not know."""
+# Kernels whose MFMAs are inline assembly, whose latency the compiler does not know.
+INLINE_MFMA = {CSRC / "blocks" / "product.hip": "multiplyWide", CSRC / "blocks" / "weight_grad.hip": "sumRowsWide"}
+
+
+def check_inline_mfma(src: pathlib.Path) -> None:
+    """The same for a file of INLINE_MFMA."""
     from . import asm_check
-    out = BUILD / "product-gfx950.s"
+    out = BUILD / f"{src.stem}-gfx950.s"
     cmd = [str(ROCM / "bin" / "hipcc"), *HIP_FLAGS, "--cuda-device-only", "-S", str(src), "-o", str(out)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"assembly listing failed: {shlex.join(cmd)}\n{res.stderr}")
-    problems = asm_check.check(out.read_text(), "multiplyWide")
+    problems = asm_check.check(out.read_text(), INLINE_MFMA[src])
     if problems:
-        raise RuntimeError("Block product assembly check failed:\n  " + "\n  ".join(problems))
+        raise RuntimeError(f"{src.name}: assembly check failed:\n  " + "\n  ".join(problems))
 
 
 def build(verbose: bool = False) -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
-        checks = [pool.submit(check_kernel_asm), pool.submit(check_product_asm)]
+        checks = [pool.submit(check_kernel_asm), *(pool.submit(check_inline_mfma, src) for src in INLINE_MFMA)]
         objs = list(pool.map(_compile, srcs))
         for check in checks:
             check.result()

@@ -35,6 +35,8 @@ template <> struct Parts<F32> { static constexpr unsigned count = 3; };
 template <unsigned Columns> struct Tile {
     static constexpr unsigned rowBytes = Columns * 2, bytes = kStep * rowBytes;
     static __device__ __forceinline__ unsigned key(unsigned r) {
+        // For the operands of 32 columns half a wave takes two slots of four rows at a time.
+        if constexpr (Columns == 256) return (r & 3) << 1;
         if constexpr (Columns == 64) return ((r >> 1) & 1) | ((r >> 2) & 2);
         return (r & 3) | ((r >> 1) & 4);
     }
@@ -255,6 +257,204 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     }
 }
 
+// acc += a b in the accumulation registers, in place (the compiler moves accumulators that fill them about
+// between MFMAs). It does not know this instruction's latency: whoever reads acc has to let it finish.
+__device__ __forceinline__ void multiplyInPlace(f32x16& acc, bf16x8 a, bf16x8 b) {
+    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+// Tiles of 256 x 256 for gradients with enough of them, dy of bf16 with aligned rows. Four waves, one a SIMD, of
+// 128 x 128 each. A step is four chunks of 16 rows; while one is multiplied, the next one's operands are read
+// from LDS to a second set of registers, a read behind each MFMA. The 32 x 32 MFMA leaves 32 cycles for what
+// has to be issued beside it, the 16 x 16 one 16, which the reads, conversions and writes do not fit into.
+// A step's bytes are loaded to registers two steps ahead, and written to the other stage while the step before
+// is multiplied; one barrier a step, before its last chunk.
+// Bias: the workgroup also sums dy's columns, from the registers that they pass through.
+template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient& a, std::uint8_t* lds) {
+    constexpr unsigned B = 256, Tiles = 4, Threads = 256, StageBytes = 2 * Tile<B>::bytes;
+    constexpr unsigned DyLoads = kStep * B / 8 / Threads, XLoads = kStep * B / 16 / Threads;
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const unsigned tiles = a.tilesN * a.tilesK, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+    const unsigned n0 = tile % a.tilesN * B, k0 = tile / a.tilesN * B;
+    const unsigned first = split * a.rowsPerSplit, last = min(first + a.rowsPerSplit, a.rows);
+    const __bf16* dy = static_cast<const __bf16*>(a.dy) + n0;
+    // A thread's chunks: 8 columns of dy of rows t / 32 + 8 i, 16 of x of rows t / 16 + 16 i.
+    const unsigned dyRow = t / 32, dyColumn = t % 32 * 8, xRow = t / 16, xColumn = t % 16 * 16;
+    const unsigned dyPitch = unsigned(a.dyStride * 2);
+    const unsigned dyAt = n0 + dyColumn < a.outer ? dyRow * dyPitch + dyColumn * 2 : 0x80000000u;
+    const unsigned xAt = k0 + xColumn < a.codePitch ? xRow * a.codePitch + k0 + xColumn : 0x80000000u;
+    const unsigned eAt = k0 + xColumn < a.codePitch ? xRow * a.expPitch + (k0 + xColumn) / kBlock : 0x80000000u;
+    const unsigned dyTo = Tile<B>::at(dyRow, dyColumn), xTo = Tile<B>::at(xRow, xColumn), xTo8 = Tile<B>::at(xRow, xColumn + 8);
+    u32x4 raw[2][DyLoads], q[2][XLoads]; // two steps' bytes
+    unsigned e[2][XLoads];
+    float sums[8] = {};
+    // Load `i` of 12 of the step from `row` on, 8 of dy and 4 of x; past the split's end zeros, from beyond the
+    // buffers.
+    auto fetch = [&](unsigned row, unsigned set, unsigned i) {
+        const unsigned rows =
+            __builtin_amdgcn_readfirstlane(unsigned(min(max(int(last) - int(row), 0), int(kStep))));
+        const auto buffer = [](const void* p, unsigned bytes) {
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+        };
+        if (i < DyLoads) {
+            const auto from = buffer(dy + row * a.dyStride, rows * dyPitch);
+            raw[set][i] = __builtin_amdgcn_raw_buffer_load_b128(from, dyAt, i * 8 * dyPitch, 0);
+        } else {
+            i -= DyLoads;
+            const auto codes = buffer(a.x + std::uint64_t(row) * a.codePitch, rows * a.codePitch);
+            const auto exponents = buffer(a.xe + std::uint64_t(row) * a.expPitch, rows * a.expPitch);
+            q[set][i] = __builtin_amdgcn_raw_buffer_load_b128(codes, xAt, i * 16 * a.codePitch, 0);
+            e[set][i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, eAt, i * 16 * a.expPitch, 0);
+        }
+    };
+    constexpr unsigned Loads = DyLoads + XLoads;
+    // A step's parity is its stage and its set of registers.
+    auto stashDy = [&](unsigned stage, unsigned i) {
+        *reinterpret_cast<u32x4*>(lds + stage * StageBytes + dyTo + i * 8 * Tile<B>::rowBytes) = raw[stage][i];
+        if constexpr (Bias) {
+            const bf16x8 v = __builtin_bit_cast(bf16x8, raw[stage][i]);
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) sums[j] += float(v[j]);
+        }
+    };
+    // Half h of 16 codes.
+    auto stashX = [&](unsigned stage, unsigned i, unsigned h) {
+        const float s = scaleOf(e[stage][i]);
+        bf16x8 w;
+#pragma unroll
+        for (unsigned j = 0; j < 2; ++j) {
+            const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[stage][i][2 * h + j], s, false);
+            const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[stage][i][2 * h + j], s, true);
+            w[4 * j] = lo.x, w[4 * j + 1] = lo.y, w[4 * j + 2] = hi.x, w[4 * j + 3] = hi.y;
+        }
+        *reinterpret_cast<bf16x8*>(lds + stage * StageBytes + Tile<B>::bytes + i * 16 * Tile<B>::rowBytes +
+                                   (h ? xTo8 : xTo)) = w;
+    };
+    const unsigned wn = wave % 2 * 128, wk = wave / 2, kk = wk * 128;
+    // Where a lane reads its 4 rows of column 32 i + lane % 32 of the wave's 128: rows 8 * (lane / 32) on, of chunk 0.
+    // The keys of rows 4 or 16 further are the same.
+    unsigned xRead[2][Tiles], dyRead[2][Tiles];
+#pragma unroll
+    for (unsigned s = 0; s < 2; ++s)
+#pragma unroll
+        for (unsigned i = 0; i < Tiles; ++i) {
+            const unsigned r = lane / 32 * 8 + lane % 16 / 4, c = 32 * i + lane / 16 % 2 * 16 + lane % 4 * 4;
+            xRead[s][i] = s * StageBytes + Tile<B>::bytes + Tile<B>::at(r, kk + c);
+            dyRead[s][i] = s * StageBytes + Tile<B>::at(r, wn + c);
+            asm("" : "+v"(xRead[s][i]), "+v"(dyRead[s][i])); // kept, not computed again for every read
+        }
+    auto column = [&](unsigned at, unsigned chunk) {
+        const std::uint8_t* p = lds + at + chunk * 16 * Tile<B>::rowBytes;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(p + 4 * Tile<B>::rowBytes));
+        return __builtin_bit_cast(bf16x8, s16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
+    };
+    f32x16 acc[Tiles][Tiles] = {};
+    bf16x8 xf[2][Tiles], df[2][Tiles];
+    auto step = [&](unsigned row, auto sel) {
+        constexpr unsigned S = decltype(sel)::value;
+#pragma unroll
+        for (unsigned c = 0; c < 4; ++c) {
+            const unsigned set = c % 2;
+            if (c == 3) { // the next step's stage from here on
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+#pragma unroll
+            for (unsigned m = 0; m < Tiles * Tiles; ++m) {
+                const unsigned n = m / Tiles, k = m % Tiles;
+                // The next chunk's operands, one with every other MFMA.
+                if (m % 2 == 0) {
+                    const unsigned i = m / 4, stage = c == 3 ? 1 - S : S, next = c == 3 ? 0 : c + 1;
+                    if (m % 4 == 0)
+                        xf[1 - set][i] = column(xRead[stage][i], next);
+                    else
+                        df[1 - set][i] = column(dyRead[stage][i], next);
+                } else if (c < 3) {
+                    // The next step's bytes: 8 pieces of dy, then 8 of x, which are converted.
+                    const unsigned i = c * 8 + m / 2;
+                    if (i < 8)
+                        stashDy(1 - S, i);
+                    else if (i < 24 && i % 2 == 0)
+                        stashX(1 - S, (i - 8) / 4, (i - 8) / 2 % 2);
+                } else {
+                    // The loads of the step after the next two, into the registers that are free now.
+                    const unsigned i = m / 2 * 3 / 2;
+                    fetch(row + 3 * kStep, 1 - S, i);
+                    if (m % 4 == 3) fetch(row + 3 * kStep, 1 - S, i + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                multiplyInPlace(acc[n][k], xf[set][k], df[set][n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // Where the loop ends the compiler copies the sums: the last MFMAs, of 8 passes, have to be done by then.
+        if (S == 1) asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[3][2]), "+a"(acc[3][3]));
+    };
+#pragma unroll
+    for (unsigned i = 0; i < Loads; ++i) fetch(first, 0, i);
+#pragma unroll
+    for (unsigned i = 0; i < Loads; ++i) fetch(first + kStep, 1, i);
+#pragma unroll
+    for (unsigned i = 0; i < XLoads; ++i) stashX(0, i, 0), stashX(0, i, 1);
+#pragma unroll
+    for (unsigned i = 0; i < DyLoads; ++i) stashDy(0, i);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (unsigned i = 0; i < Loads; ++i) fetch(first + 2 * kStep, 0, i);
+#pragma unroll
+    for (unsigned i = 0; i < Tiles; ++i) xf[0][i] = column(xRead[0][i], 0), df[0][i] = column(dyRead[0][i], 0);
+    for (unsigned row = first; row < last; row += 2 * kStep) {
+        step(row, std::integral_constant<unsigned, 0>{});
+        step(row + kStep, std::integral_constant<unsigned, 1>{});
+    }
+    float* dw = a.dw + split * a.splitPitch;
+    typedef f32x4 Loose4 __attribute__((aligned(4)));
+#pragma unroll
+    for (unsigned n = 0; n < Tiles; ++n) {
+        const unsigned row = n0 + wn + 32 * n + lane % 32;
+        if (row >= a.outer) continue;
+#pragma unroll
+        for (unsigned k = 0; k < Tiles; ++k)
+#pragma unroll
+            for (unsigned j = 0; j < 4; ++j) {
+                const unsigned column = k0 + kk + 32 * k + 8 * j + lane / 32 * 4;
+                float* to = dw + std::uint64_t(row) * a.inner + column;
+                if (column + 4 <= a.inner) {
+                    *reinterpret_cast<Loose4*>(to) = f32x4{acc[n][k][4 * j], acc[n][k][4 * j + 1], acc[n][k][4 * j + 2],
+                                                          acc[n][k][4 * j + 3]};
+                } else {
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i)
+                        if (column + i < a.inner) to[i] = acc[n][k][4 * j + i];
+                }
+            }
+    }
+    if constexpr (Bias) {
+        // The eight threads with the same columns add theirs through LDS, which nobody reads any more.
+        __syncthreads();
+        float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (unsigned j = 0; j < 8; ++j) part[dyRow * B + dyColumn + j] = sums[j];
+        __syncthreads();
+        if (n0 + t < a.outer) {
+            float s = 0.0f;
+#pragma unroll
+            for (unsigned r = 0; r < 8; ++r) s += part[r * B + t];
+            a.db[split * a.splitPitch + n0 + t] = s;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void sumRowsWide(Gradient a) {
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages of dy, then x
+    // Two bodies, not a condition in one: accumulators that fill their registers leave no room to join paths.
+    if (a.db && blockIdx.x % (a.tilesN * a.tilesK) < a.tilesN)
+        sumTileWide<true>(a, lds);
+    else
+        sumTileWide<false>(a, lds);
+}
+
 // dw and db from the splits' sums, added in a fixed order: Ways threads add every Ways-th split of four
 // values, then their sums through LDS. A split's db follows its dw.
 template <unsigned Ways>
@@ -380,7 +580,7 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     if (blocks >> 31) reject(where, "more than 2^31 tiles");
     if (p.aligned) {
         if (p.bn == 256)
-            launchSum<BF16, 256, 256, 2, 4, 2, true>(a, blocks, stream);
+            hipLaunchKernelGGL(sumRowsWide, dim3(unsigned(blocks)), dim3(256), 2 * 2 * Tile<256>::bytes, stream, a);
         else
             launchSum<BF16, 128, 128, 2, 4, 2, true>(a, blocks, stream);
     } else {
