@@ -32,11 +32,11 @@ template <> struct Parts<F32> { static constexpr unsigned count = 3; };
 // A tile of kStep rows of Columns bf16 values in LDS. The 32-byte slots of a row (16 values) are stored in
 // an order that depends on the row, its key: a wave's transposing load takes one slot of rows r0 + 8 i + j
 // (i, j < 4), which 64 banks of 4 bytes serve in two turns if they spread over all of them.
-template <unsigned Columns> struct Tile {
+// (Pairs: for operands of 32 columns half a wave takes two slots of four rows at a time.)
+template <unsigned Columns, bool Pairs = false> struct Tile {
     static constexpr unsigned rowBytes = Columns * 2, bytes = kStep * rowBytes;
     static __device__ __forceinline__ unsigned key(unsigned r) {
-        // For the operands of 32 columns half a wave takes two slots of four rows at a time.
-        if constexpr (Columns == 256) return (r & 3) << 1;
+        if constexpr (Pairs) return (r & 3) << 1;
         if constexpr (Columns == 64) return ((r >> 1) & 1) | ((r >> 2) & 2);
         return (r & 3) | ((r >> 1) & 4);
     }
@@ -62,70 +62,62 @@ struct Gradient {
     unsigned rows, outer, inner, codePitch, expPitch, tilesN, tilesK, rowsPerSplit;
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytesAt(const void* p, std::uint64_t count) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, unsigned(min(count, std::uint64_t(0x7FFFFFFF))), 0x00020000);
-}
-
-// Tiles of BN columns of dy by BK of x, WN x WK waves. A step's bytes are loaded to registers while the step
-// before is multiplied, and written to LDS into the other of two stages, or, where the parts of dy leave
-// no room for two, after a barrier. Aligned: dy of bf16 whose rows are 16-byte aligned, read by plain
-// buffer loads, which give zeros past the end.
-// The loads do not go to LDS directly: the compiler makes every transposing LDS load wait for all of
-// those in flight.
-template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, unsigned Stages, bool Aligned>
+// Tiles of BN columns of dy by BK of x, WN x WK waves, for any dy. A step's bytes are loaded to registers while the
+// step before is multiplied; dy is split into its parts on the way to LDS, which has one stage, since its
+// parts leave little room and several workgroups share a CU.
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK>
 __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     constexpr unsigned P = Parts<T>::count, Threads = 64 * WN * WK, NT = BN / WN / 16, KT = BK / WK / 16;
-    constexpr unsigned StageBytes = P * Tile<BN>::bytes + Tile<BK>::bytes, DyLoads = kStep * BN / 8 / Threads;
+    constexpr unsigned DyLoads = kStep * BN / 8 / Threads;
     constexpr unsigned XLoads = kStep * BK / 16 / Threads, BT = NT / WK; // BT: bias operands of a wave
     static_assert(BT >= 1 && XLoads >= 1 && DyLoads >= 1, "every thread and wave has its share");
     typedef typename T::Raw Raw;
-    extern __shared__ __align__(1024) std::uint8_t lds[]; // per stage: dy's parts, then x
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // dy's parts, then x
     const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const unsigned tiles = a.tilesN * a.tilesK, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
     const unsigned n0 = tile % a.tilesN * BN, k0 = tile / a.tilesN * BK;
     const unsigned first = split * a.rowsPerSplit, last = min(first + a.rowsPerSplit, a.rows);
     const Raw* dy = static_cast<const Raw*>(a.dy) + n0;
-    const std::uint64_t dyBytes = a.dyStride * sizeof(Raw);
 
     typedef typename Group<T>::Vec Vec;
     Vec raw[DyLoads];
+    u32x4 q[XLoads];
+    unsigned e[XLoads];
+    const auto buffer = [](const void* p, unsigned bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+    };
+    // Rows of the step from `row` on; past the split's end there are none, and loads give zeros.
+    const auto rowsOf = [&](unsigned row) {
+        return __builtin_amdgcn_readfirstlane(min(row < last ? last - row : 0u, kStep));
+    };
     auto fetchDy = [&](unsigned row) {
-        if constexpr (Aligned) {
-            const auto from = bytesAt(dy + row * a.dyStride, (last - row - 1) * dyBytes + (a.outer - n0) * sizeof(Raw));
 #pragma unroll
-            for (unsigned i = 0; i < DyLoads; ++i) {
-                const unsigned chunk = t + i * Threads, r = chunk / (BN / 8), c = chunk % (BN / 8) * 8;
-                const unsigned at = n0 + c < a.outer ? r * unsigned(dyBytes) + c * 2 : 0x80000000u;
-                raw[i] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
-            }
-        } else {
+        for (unsigned i = 0; i < DyLoads; ++i) {
+            const unsigned chunk = t + i * Threads, r = row + chunk / (BN / 8), c = chunk % (BN / 8) * 8;
+            raw[i] = Vec{};
+            if (r >= last || n0 + c >= a.outer) continue;
+            const Raw* p = dy + r * a.dyStride + c;
+            if (n0 + c + 8 <= a.outer) {
+                raw[i] = *reinterpret_cast<const typename Group<T>::Loose*>(p);
+            } else {
 #pragma unroll
-            for (unsigned i = 0; i < DyLoads; ++i) {
-                const unsigned chunk = t + i * Threads, r = row + chunk / (BN / 8), c = chunk % (BN / 8) * 8;
-                raw[i] = Vec{};
-                if (r >= last || n0 + c >= a.outer) continue;
-                const Raw* p = dy + r * a.dyStride + c;
-                if (n0 + c + 8 <= a.outer) {
-                    raw[i] = *reinterpret_cast<const typename Group<T>::Loose*>(p);
-                } else {
-#pragma unroll
-                    for (unsigned j = 0; j < 8; ++j)
-                        if (n0 + c + j < a.outer) raw[i][j] = p[j];
-                }
+                for (unsigned j = 0; j < 8; ++j)
+                    if (n0 + c + j < a.outer) raw[i][j] = p[j];
             }
         }
     };
-    auto stashDy = [&](unsigned stage) {
+    auto stashDy = [&] {
 #pragma unroll
         for (unsigned i = 0; i < DyLoads; ++i) {
             const unsigned chunk = t + i * Threads, r = chunk / (BN / 8), c = chunk % (BN / 8) * 8;
-            std::uint8_t* to = lds + stage * StageBytes + Tile<BN>::at(r, c);
+            std::uint8_t* to = lds + Tile<BN>::at(r, c);
             if constexpr (P == 1) {
                 *reinterpret_cast<Vec*>(to) = raw[i];
             } else {
                 float rest[8];
 #pragma unroll
                 for (unsigned j = 0; j < 8; ++j) rest[j] = T::get(raw[i][j]);
+                const bool large = peakBits(rest) >= 0x7F7F8000u; // rounds to an infinity, or is one, or a NaN
 #pragma unroll
                 for (unsigned p = 0; p < P; ++p) {
                     bf16x8 part;
@@ -134,26 +126,38 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
                         part[j] = __bf16(rest[j]);
                         if (p + 1 < P) rest[j] -= float(part[j]);
                     }
+                    // An infinity or a NaN is its first part and leaves no rest; a finite number's first part is finite.
+                    if (p == 0 && large) {
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) {
+                            const float v = T::get(raw[i][j]), cut = __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+                            if (!__builtin_isfinite(v)) {
+                                rest[j] = 0.0f;
+                            } else if (!__builtin_isfinite(float(part[j]))) {
+                                part[j] = __bf16(cut);
+                                rest[j] = v - cut;
+                            }
+                        }
+                    }
                     *reinterpret_cast<bf16x8*>(to + p * Tile<BN>::bytes) = part;
                 }
             }
         }
     };
-    u32x4 q[XLoads];
-    unsigned e[XLoads];
     auto fetchX = [&](unsigned row) {
-        const auto codes = bytesAt(a.x + std::uint64_t(row) * a.codePitch + k0, (last - row) * std::uint64_t(a.codePitch) - k0);
-        const auto exponents = bytesAt(a.xe + std::uint64_t(row) * a.expPitch, (last - row) * std::uint64_t(a.expPitch));
+        const unsigned rows = rowsOf(row);
+        const auto codes = buffer(a.x + std::uint64_t(row) * a.codePitch, rows * a.codePitch);
+        const auto exponents = buffer(a.xe + std::uint64_t(row) * a.expPitch, rows * a.expPitch);
 #pragma unroll
         for (unsigned i = 0; i < XLoads; ++i) {
             const unsigned chunk = t + i * Threads, r = chunk / (BK / 16), c = chunk % (BK / 16) * 16;
             const bool in = k0 + c < a.codePitch;
-            q[i] = __builtin_amdgcn_raw_buffer_load_b128(codes, in ? r * a.codePitch + c : 0x80000000u, 0, 0);
+            q[i] = __builtin_amdgcn_raw_buffer_load_b128(codes, in ? r * a.codePitch + k0 + c : 0x80000000u, 0, 0);
             e[i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, in ? r * a.expPitch + (k0 + c) / kBlock : 0x80000000u, 0, 0);
         }
     };
-    auto stashX = [&](unsigned stage) {
-        std::uint8_t* to = lds + stage * StageBytes + P * Tile<BN>::bytes;
+    auto stashX = [&] {
+        std::uint8_t* to = lds + P * Tile<BN>::bytes;
 #pragma unroll
         for (unsigned i = 0; i < XLoads; ++i) {
             const unsigned chunk = t + i * Threads, r = chunk / (BK / 16), c = chunk % (BK / 16) * 16;
@@ -175,8 +179,8 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     const bool bias = a.db && k0 == 0;
     const bf16x8 ones = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
     f32x4 acc[NT][KT] = {}, sums[BT] = {};
-    auto half = [&](unsigned stage, unsigned r0, auto withBias) {
-        const std::uint8_t* base = lds + stage * StageBytes;
+    auto half = [&](unsigned r0, auto withBias) {
+        const std::uint8_t* base = lds;
         bf16x8 xf[KT];
 #pragma unroll
         for (unsigned k = 0; k < KT; ++k) xf[k] = Tile<BK>::column(base + P * Tile<BN>::bytes, r0, kk + 16 * k, lane);
@@ -199,28 +203,24 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
         }
     };
     auto walk = [&](auto withBias) {
-        unsigned stage = 0;
         for (unsigned row = first; row < last; row += kStep) {
-            const bool more = row + kStep < last;
-            // The last step loads itself again, for nobody, so that the loop has no branch.
-            fetchX(more ? row + kStep : row);
-            fetchDy(more ? row + kStep : row);
+            fetchX(row + kStep);
+            fetchDy(row + kStep);
             __builtin_amdgcn_sched_barrier(0); // the compiler would move the loads down to their use
-            half(stage, 0, withBias);
-            half(stage, 32, withBias);
+            half(0, withBias);
+            half(32, withBias);
             __builtin_amdgcn_sched_barrier(0);
-            if (Stages == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (Stages == 2) stage = 1 - stage;
-            stashX(stage);
-            stashDy(stage);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            stashX();
+            stashDy();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     };
     if (first < last) {
         fetchX(first);
         fetchDy(first);
-        stashX(0);
-        stashDy(0);
+        stashX();
+        stashDy();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (bias)
             walk(std::true_type{});
@@ -263,54 +263,57 @@ __device__ __forceinline__ void multiplyInPlace(f32x16& acc, bf16x8 a, bf16x8 b)
     asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
-// Tiles of 256 x 256 for gradients with enough of them, dy of bf16 with aligned rows. Four waves, one a SIMD, of
-// 128 x 128 each. A step is four chunks of 16 rows; while one is multiplied, the next one's operands are read
+// dy of bf16 with aligned rows: tiles of 256 x 256, or 128 x 128 where a weight has few. Four waves of a quarter
+// each; of the large tile one fills a SIMD's registers, of the small two share it. A step is four chunks of 16 rows; while one is multiplied, the next one's operands are read
 // from LDS to a second set of registers, a read behind each MFMA. The 32 x 32 MFMA leaves 32 cycles for what
 // has to be issued beside it, the 16 x 16 one 16, which the reads, conversions and writes do not fit into.
 // A step's bytes are loaded to registers two steps ahead, and written to the other stage while the step before
 // is multiplied; one barrier a step, before its last chunk.
 // Bias: the workgroup also sums dy's columns, from the registers that they pass through.
-template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient& a, std::uint8_t* lds) {
-    constexpr unsigned B = 256, Tiles = 4, Threads = 256, StageBytes = 2 * Tile<B>::bytes;
+template <unsigned B, bool Bias> __device__ __forceinline__ void sumTile(const Gradient& a, std::uint8_t* lds) {
+    typedef Tile<B, true> In;
+    constexpr unsigned Tiles = B / 64, Threads = 256, StageBytes = 2 * In::bytes;
     constexpr unsigned DyLoads = kStep * B / 8 / Threads, XLoads = kStep * B / 16 / Threads;
     const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const unsigned tiles = a.tilesN * a.tilesK, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
     const unsigned n0 = tile % a.tilesN * B, k0 = tile / a.tilesN * B;
     const unsigned first = split * a.rowsPerSplit, last = min(first + a.rowsPerSplit, a.rows);
     const __bf16* dy = static_cast<const __bf16*>(a.dy) + n0;
-    // A thread's chunks: 8 columns of dy of rows t / 32 + 8 i, 16 of x of rows t / 16 + 16 i.
-    const unsigned dyRow = t / 32, dyColumn = t % 32 * 8, xRow = t / 16, xColumn = t % 16 * 16;
+    // A thread's chunks: 8 columns of dy, 16 of x, of rows DyApart or XApart from each other, all with one key.
+    constexpr unsigned DyApart = Threads * 8 / B, XApart = Threads * 16 / B;
+    static_assert(DyApart % 4 == 0 && XApart % 4 == 0, "the key is the row's place among four");
+    const unsigned dyRow = t / (B / 8), dyColumn = t % (B / 8) * 8, xRow = t / (B / 16), xColumn = t % (B / 16) * 16;
     const unsigned dyPitch = unsigned(a.dyStride * 2);
     const unsigned dyAt = n0 + dyColumn < a.outer ? dyRow * dyPitch + dyColumn * 2 : 0x80000000u;
     const unsigned xAt = k0 + xColumn < a.codePitch ? xRow * a.codePitch + k0 + xColumn : 0x80000000u;
     const unsigned eAt = k0 + xColumn < a.codePitch ? xRow * a.expPitch + (k0 + xColumn) / kBlock : 0x80000000u;
-    const unsigned dyTo = Tile<B>::at(dyRow, dyColumn), xTo = Tile<B>::at(xRow, xColumn), xTo8 = Tile<B>::at(xRow, xColumn + 8);
+    const unsigned dyTo = In::at(dyRow, dyColumn), xTo = In::at(xRow, xColumn), xTo8 = In::at(xRow, xColumn + 8);
     u32x4 raw[2][DyLoads], q[2][XLoads]; // two steps' bytes
     unsigned e[2][XLoads];
     float sums[8] = {};
-    // Load `i` of 12 of the step from `row` on, 8 of dy and 4 of x; past the split's end zeros, from beyond the
+    // Load `i` of the step from `row` on, dy's, then x's; past the split's end zeros, from beyond the
     // buffers.
     auto fetch = [&](unsigned row, unsigned set, unsigned i) {
         const unsigned rows =
-            __builtin_amdgcn_readfirstlane(unsigned(min(max(int(last) - int(row), 0), int(kStep))));
+            __builtin_amdgcn_readfirstlane(min(row < last ? last - row : 0u, kStep));
         const auto buffer = [](const void* p, unsigned bytes) {
             return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
         };
         if (i < DyLoads) {
             const auto from = buffer(dy + row * a.dyStride, rows * dyPitch);
-            raw[set][i] = __builtin_amdgcn_raw_buffer_load_b128(from, dyAt, i * 8 * dyPitch, 0);
+            raw[set][i] = __builtin_amdgcn_raw_buffer_load_b128(from, dyAt, i * DyApart * dyPitch, 0);
         } else {
             i -= DyLoads;
             const auto codes = buffer(a.x + std::uint64_t(row) * a.codePitch, rows * a.codePitch);
             const auto exponents = buffer(a.xe + std::uint64_t(row) * a.expPitch, rows * a.expPitch);
-            q[set][i] = __builtin_amdgcn_raw_buffer_load_b128(codes, xAt, i * 16 * a.codePitch, 0);
-            e[set][i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, eAt, i * 16 * a.expPitch, 0);
+            q[set][i] = __builtin_amdgcn_raw_buffer_load_b128(codes, xAt, i * XApart * a.codePitch, 0);
+            e[set][i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, eAt, i * XApart * a.expPitch, 0);
         }
     };
     constexpr unsigned Loads = DyLoads + XLoads;
     // A step's parity is its stage and its set of registers.
     auto stashDy = [&](unsigned stage, unsigned i) {
-        *reinterpret_cast<u32x4*>(lds + stage * StageBytes + dyTo + i * 8 * Tile<B>::rowBytes) = raw[stage][i];
+        *reinterpret_cast<u32x4*>(lds + stage * StageBytes + dyTo + i * DyApart * In::rowBytes) = raw[stage][i];
         if constexpr (Bias) {
             const bf16x8 v = __builtin_bit_cast(bf16x8, raw[stage][i]);
 #pragma unroll
@@ -327,11 +330,11 @@ template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient&
             const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[stage][i][2 * h + j], s, true);
             w[4 * j] = lo.x, w[4 * j + 1] = lo.y, w[4 * j + 2] = hi.x, w[4 * j + 3] = hi.y;
         }
-        *reinterpret_cast<bf16x8*>(lds + stage * StageBytes + Tile<B>::bytes + i * 16 * Tile<B>::rowBytes +
+        *reinterpret_cast<bf16x8*>(lds + stage * StageBytes + In::bytes + i * XApart * In::rowBytes +
                                    (h ? xTo8 : xTo)) = w;
     };
-    const unsigned wn = wave % 2 * 128, wk = wave / 2, kk = wk * 128;
-    // Where a lane reads its 4 rows of column 32 i + lane % 32 of the wave's 128: rows 8 * (lane / 32) on, of chunk 0.
+    const unsigned wn = wave % 2 * (B / 2), kk = wave / 2 * (B / 2);
+    // Where a lane reads its 4 rows of column 32 i + lane % 32 of the wave's: rows 8 * (lane / 32) on, of chunk 0.
     // The keys of rows 4 or 16 further are the same.
     unsigned xRead[2][Tiles], dyRead[2][Tiles];
 #pragma unroll
@@ -339,18 +342,21 @@ template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient&
 #pragma unroll
         for (unsigned i = 0; i < Tiles; ++i) {
             const unsigned r = lane / 32 * 8 + lane % 16 / 4, c = 32 * i + lane / 16 % 2 * 16 + lane % 4 * 4;
-            xRead[s][i] = s * StageBytes + Tile<B>::bytes + Tile<B>::at(r, kk + c);
-            dyRead[s][i] = s * StageBytes + Tile<B>::at(r, wn + c);
+            xRead[s][i] = s * StageBytes + In::bytes + In::at(r, kk + c);
+            dyRead[s][i] = s * StageBytes + In::at(r, wn + c);
             asm("" : "+v"(xRead[s][i]), "+v"(dyRead[s][i])); // kept, not computed again for every read
         }
     auto column = [&](unsigned at, unsigned chunk) {
-        const std::uint8_t* p = lds + at + chunk * 16 * Tile<B>::rowBytes;
+        const std::uint8_t* p = lds + at + chunk * 16 * In::rowBytes;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)p);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(p + 4 * Tile<B>::rowBytes));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsColumn)(p + 4 * In::rowBytes));
         return __builtin_bit_cast(bf16x8, s16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
     };
     f32x16 acc[Tiles][Tiles] = {};
     bf16x8 xf[2][Tiles], df[2][Tiles];
+    // Of `count` things spread over `slots`, those before slot m.
+    constexpr auto share = [](unsigned m, unsigned count, unsigned slots) { return m * count / slots; };
+    constexpr unsigned Slots = Tiles * Tiles, Pieces = DyLoads + 2 * XLoads;
     auto step = [&](unsigned row, auto sel) {
         constexpr unsigned S = decltype(sel)::value;
 #pragma unroll
@@ -361,27 +367,32 @@ template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient&
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
 #pragma unroll
-            for (unsigned m = 0; m < Tiles * Tiles; ++m) {
+            for (unsigned m = 0; m < Slots; ++m) {
                 const unsigned n = m / Tiles, k = m % Tiles;
-                // The next chunk's operands, one with every other MFMA.
-                if (m % 2 == 0) {
-                    const unsigned i = m / 4, stage = c == 3 ? 1 - S : S, next = c == 3 ? 0 : c + 1;
-                    if (m % 4 == 0)
-                        xf[1 - set][i] = column(xRead[stage][i], next);
+                // What goes beside MFMA m: the next chunk's operands; the next step's bytes, dy's, then x's, which are
+                // converted; in the last chunk the loads of the step after the next two, into the registers that
+                // are free by then.
+#pragma unroll
+                for (unsigned i = share(m, 2 * Tiles, Slots); i < share(m + 1, 2 * Tiles, Slots); ++i) {
+                    const unsigned stage = c == 3 ? 1 - S : S, next = c == 3 ? 0 : c + 1;
+                    if (i % 2 == 0)
+                        xf[1 - set][i / 2] = column(xRead[stage][i / 2], next);
                     else
-                        df[1 - set][i] = column(dyRead[stage][i], next);
-                } else if (c < 3) {
-                    // The next step's bytes: 8 pieces of dy, then 8 of x, which are converted.
-                    const unsigned i = c * 8 + m / 2;
-                    if (i < 8)
-                        stashDy(1 - S, i);
-                    else if (i < 24 && i % 2 == 0)
-                        stashX(1 - S, (i - 8) / 4, (i - 8) / 2 % 2);
+                        df[1 - set][i / 2] = column(dyRead[stage][i / 2], next);
+                }
+                if (c < 3) {
+                    const unsigned at = c * Slots + m;
+#pragma unroll
+                    for (unsigned i = share(at, Pieces, 3 * Slots); i < share(at + 1, Pieces, 3 * Slots); ++i) {
+                        if (i < DyLoads)
+                            stashDy(1 - S, i);
+                        else
+                            stashX(1 - S, (i - DyLoads) / 2, (i - DyLoads) % 2);
+                    }
                 } else {
-                    // The loads of the step after the next two, into the registers that are free now.
-                    const unsigned i = m / 2 * 3 / 2;
-                    fetch(row + 3 * kStep, 1 - S, i);
-                    if (m % 4 == 3) fetch(row + 3 * kStep, 1 - S, i + 1);
+#pragma unroll
+                    for (unsigned i = share(m, Loads, Slots); i < share(m + 1, Loads, Slots); ++i)
+                        fetch(row + 3 * kStep, 1 - S, i);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 multiplyInPlace(acc[n][k], xf[set][k], df[set][n]);
@@ -389,7 +400,7 @@ template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient&
             }
         }
         // Where the loop ends the compiler copies the sums: the last MFMAs, of 8 passes, have to be done by then.
-        if (S == 1) asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[3][2]), "+a"(acc[3][3]));
+        if (S == 1) asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[Tiles - 1][Tiles - 2]), "+a"(acc[Tiles - 1][Tiles - 1]));
     };
 #pragma unroll
     for (unsigned i = 0; i < Loads; ++i) fetch(first, 0, i);
@@ -431,28 +442,35 @@ template <bool Bias> __device__ __forceinline__ void sumTileWide(const Gradient&
             }
     }
     if constexpr (Bias) {
-        // The eight threads with the same columns add theirs through LDS, which nobody reads any more.
+        // The threads with the same columns add theirs through LDS, which nobody reads any more.
         __syncthreads();
         float* part = reinterpret_cast<float*>(lds);
 #pragma unroll
         for (unsigned j = 0; j < 8; ++j) part[dyRow * B + dyColumn + j] = sums[j];
         __syncthreads();
-        if (n0 + t < a.outer) {
+        if (t < B && n0 + t < a.outer) {
             float s = 0.0f;
 #pragma unroll
-            for (unsigned r = 0; r < 8; ++r) s += part[r * B + t];
+            for (unsigned r = 0; r < DyApart; ++r) s += part[r * B + t];
             a.db[split * a.splitPitch + n0 + t] = s;
         }
     }
 }
 
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void sumRowsWide(Gradient a) {
-    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages of dy, then x
-    // Two bodies, not a condition in one: accumulators that fill their registers leave no room to join paths.
+// Two bodies, not a condition in one: accumulators that fill their registers leave no room to join paths.
+template <unsigned B> __device__ __forceinline__ void sumTileWithBias(const Gradient& a, std::uint8_t* lds) {
     if (a.db && blockIdx.x % (a.tilesN * a.tilesK) < a.tilesN)
-        sumTileWide<true>(a, lds);
+        sumTile<B, true>(a, lds);
     else
-        sumTileWide<false>(a, lds);
+        sumTile<B, false>(a, lds);
+}
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void sumRowsInPlace256(Gradient a) {
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages of dy, then x
+    sumTileWithBias<256>(a, lds);
+}
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void sumRowsInPlace128(Gradient a) {
+    extern __shared__ __align__(1024) std::uint8_t lds[];
+    sumTileWithBias<128>(a, lds);
 }
 
 // dw and db from the splits' sums, added in a fixed order: Ways threads add every Ways-th split of four
@@ -530,10 +548,10 @@ Plan planOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseT
     return planTime(large, rows, inner, outer, 1.5, 1) < smallTime ? large : small;
 }
 
-template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, unsigned Stages, bool Aligned>
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK>
 void launchSum(const Gradient& a, std::uint64_t blocks, hipStream_t stream) {
-    constexpr unsigned lds = Stages * (Parts<T>::count * Tile<BN>::bytes + Tile<BK>::bytes);
-    hipLaunchKernelGGL((sumRows<T, BN, BK, WN, WK, Stages, Aligned>), dim3(unsigned(blocks)), dim3(64 * WN * WK), lds, stream, a);
+    constexpr unsigned lds = Parts<T>::count * Tile<BN>::bytes + Tile<BK>::bytes;
+    hipLaunchKernelGGL((sumRows<T, BN, BK, WN, WK>), dim3(unsigned(blocks)), dim3(64 * WN * WK), lds, stream, a);
 }
 
 } // namespace
@@ -580,16 +598,16 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     if (blocks >> 31) reject(where, "more than 2^31 tiles");
     if (p.aligned) {
         if (p.bn == 256)
-            hipLaunchKernelGGL(sumRowsWide, dim3(unsigned(blocks)), dim3(256), 2 * 2 * Tile<256>::bytes, stream, a);
+            hipLaunchKernelGGL(sumRowsInPlace256, dim3(unsigned(blocks)), dim3(256), 4 * Tile<256>::bytes, stream, a);
         else
-            launchSum<BF16, 128, 128, 2, 4, 2, true>(a, blocks, stream);
+            hipLaunchKernelGGL(sumRowsInPlace128, dim3(unsigned(blocks)), dim3(256), 4 * Tile<128>::bytes, stream, a);
     } else {
         withType(dy.type, [&](auto tag) {
             typedef decltype(tag) T;
             if (p.bn == 64)
-                launchSum<T, 64, 128, 1, 4, 1, false>(a, blocks, stream);
+                launchSum<T, 64, 128, 1, 4>(a, blocks, stream);
             else
-                launchSum<T, 128, 128, 2, 2, 1, false>(a, blocks, stream);
+                launchSum<T, 128, 128, 2, 2>(a, blocks, stream);
         });
     }
     checkHip(hipGetLastError());

@@ -264,6 +264,27 @@ def test_weight_gradient_large(gpu, rows, inner, outer):
     assert torch.equal(weight_grad_blocks(dy, quantize_blocks(x), bias=False)[0], dw)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,inner,outer", [(100, 130, 40), (300, 256, 136)])
+def test_weight_gradient_of_infinities(gpu, rows, inner, outer, dtype):
+    """An infinity or a NaN in dy stays in its column of the gradient, an infinity an infinity where its row of x
+    has no zero; the largest finite numbers stay finite."""
+    from tcc_spmm_amd.blocks import quantize_blocks, weight_grad_blocks
+    x, dy = random((rows, inner), 1, dtype).abs() + 0.5, random((rows, outer), 2, dtype)
+    dy[3, 1], dy[5, 2], dy[7, 3] = float("inf"), float("-inf"), float("nan")
+    top = torch.finfo(DTYPES[dtype]).max
+    dy[:, 4] = 0.0
+    dy[9, 4] = top if dtype == "f16" else top / 4
+    xv, g = O.quantize(f64(x))[2], f64(dy)
+    dw, db = weight_grad_blocks(dy, quantize_blocks(x))
+    want = torch.from_numpy(np.nan_to_num(g, nan=0, posinf=0, neginf=0).T @ xv)
+    assert (dw[1] == float("inf")).all() and (dw[2] == float("-inf")).all() and dw[3].isnan().all()
+    assert db[1] == float("inf") and db[2] == float("-inf") and db[3].isnan()
+    rest = [i for i in range(outer) if i not in (1, 2, 3)]
+    terms = np.abs(np.nan_to_num(g, nan=0, posinf=0, neginf=0)).T @ xv
+    near(dw[rest], want[rest].numpy(), (rows / 4 + 64) * U * terms[rest], "dw")
+
+
 def test_weight_gradient_of_no_rows(gpu):
     from tcc_spmm_amd.blocks import quantize_blocks, weight_grad_blocks
     dw, db = weight_grad_blocks(torch.empty((0, 30), device="cuda"), quantize_blocks(torch.empty((0, 50), device="cuda")))
