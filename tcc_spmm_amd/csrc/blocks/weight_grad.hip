@@ -521,9 +521,11 @@ std::uint64_t pitchOf(std::uint32_t inner, std::uint32_t outer) {
     return rounded4(std::uint64_t(outer) * inner) + rounded4(outer);
 }
 
-// The splits with the least estimated time, in microseconds: rounds of workgroups on the chip times the
-// steps of each, and the traffic of the partial sums, written once and read once.
-double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, double stepTime, unsigned perUnit) {
+// The splits with the least estimated time, in microseconds: rounds of workgroups on the chip times the steps of
+// each, and the traffic of the partial sums, written once and read once. `alone` and `shared` are the time of
+// a step of a workgroup that has its CU to itself and of one that shares it with perUnit - 1 others.
+double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, double alone, double shared,
+                unsigned perUnit) {
     const std::uint64_t tiles = std::uint64_t((inner + p.bk - 1) / p.bk) * ((outer + p.bn - 1) / p.bn);
     const std::uint64_t steps = std::max<std::uint64_t>(1, (std::uint64_t(rows) + kStep - 1) / kStep);
     double best = 1e30;
@@ -531,21 +533,27 @@ double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t 
         splits = std::max<std::uint64_t>(1, std::min(splits, steps));
         const std::uint64_t each = (steps + splits - 1) / splits, used = (steps + each - 1) / each;
         const std::uint64_t rounds = (tiles * used + kUnits * perUnit - 1) / (kUnits * perUnit);
-        double time = double(rounds) * (double(each) * stepTime + 3.0);
+        double time = tiles * used <= kUnits ? 8.0 + double(each) * alone : double(rounds) * (8.0 + double(each) * shared);
         if (used > 1) time += 4.0 + double(used) * double(pitchOf(inner, outer)) * 8.0 / 4.0e6;
         if (time < best) best = time, p.splits = unsigned(used), p.steps = unsigned(each);
     };
     consider(1);
-    for (unsigned rounds = 1; rounds <= 8; ++rounds) consider(std::uint64_t(rounds) * kUnits * perUnit / tiles);
+    consider(kUnits / tiles);
+    for (unsigned rounds = 1; rounds <= 4; ++rounds) consider(std::uint64_t(rounds) * kUnits * perUnit / tiles);
     return best;
 }
 
+// Steps measured, in us: the large tile 2.0 (4096 x 4096 x 4096 135, 8192 x 4096 x 8192 545), the small one 0.75 alone
+// (2048 x 1024 x 4096 32) and 1.15 shared (2048 x 2048 x 4096 46).
 Plan planOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, bool aligned) {
     Plan small = {outer <= 64 && !aligned ? 64u : 128u, 128, 1, 1, aligned}, large = {256, 256, 1, 1, aligned};
-    const unsigned parts = type == DenseType::f32 ? 3 : type == DenseType::f16 ? 2 : 1;
-    const double smallTime = planTime(small, rows, inner, outer, 0.6 + 0.3 * parts, 2);
-    if (!aligned) return small;
-    return planTime(large, rows, inner, outer, 1.5, 1) < smallTime ? large : small;
+    if (!aligned) {
+        const double step = 0.6 + 0.3 * (type == DenseType::f32 ? 3 : type == DenseType::f16 ? 2 : 1);
+        planTime(small, rows, inner, outer, step, step, 2);
+        return small;
+    }
+    const double smallTime = planTime(small, rows, inner, outer, 0.75, 1.15, 2);
+    return planTime(large, rows, inner, outer, 2.0, 2.0, 1) < smallTime ? large : small;
 }
 
 template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK>
