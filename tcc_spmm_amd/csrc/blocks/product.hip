@@ -101,6 +101,11 @@ template <unsigned N> __device__ __forceinline__ void waitBarrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// The bytes of a dword of exponents, of blocks k to k + 3, that belong to blocks before `count`.
+__device__ __forceinline__ unsigned finiteExponents(unsigned k, unsigned count) {
+    return k + 4 <= count ? ~0u : k >= count ? 0u : (1u << 8 * (count - k)) - 1;
+}
+
 // Rows from `first` on of a matrix of `rows` rows of `pitch` bytes.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rowsAt(const std::uint8_t* p, unsigned pitch, unsigned first, unsigned rows) {
     const std::uint64_t bytes = std::uint64_t(rows - first) * pitch;
@@ -211,9 +216,11 @@ __global__ __launch_bounds__(64 * WM * WN * Groups) void multiplyTiles(Product a
         }
     };
     auto nextExponents = [&](unsigned k4) {
+        // Past the last block (of a group's steps) codes are zeros, and so that the products are, the exponents finite.
+        const unsigned keep = Groups == 1 ? ~0u : finiteExponents(k4, a.count);
 #pragma unroll
-        for (unsigned m = 0; m < MT; ++m) xs[m] = xsNext[m];
-        ws = wsNext;
+        for (unsigned m = 0; m < MT; ++m) xs[m] = (xsNext[m] & keep) | (0x7F7F7F7Fu & ~keep);
+        ws = (wsNext & keep) | (0x7F7F7F7Fu & ~keep);
         loadExponents(min(k4 + 4, (a.count - 1) / 4 * 4));
     };
     unsigned k = first;
@@ -410,9 +417,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[6][6]), "+a"(acc[7][6]), "+a"(acc[6][7]), "+a"(acc[7][7]));
     };
     for (unsigned k = 0; k < a.count; k += 2) {
+        // A block past the last has codes of zeros, and has to have finite exponents.
+        const unsigned keep = finiteExponents(k, a.count) & 0xFFFFu;
 #pragma unroll
-        for (unsigned m = 0; m < Tiles; ++m) xs[m] = xsNext[m];
-        ws = wsNext;
+        for (unsigned m = 0; m < Tiles; ++m) xs[m] = (xsNext[m] & keep) | (0x7F7Fu & ~keep);
+        ws = (wsNext & keep) | (0x7F7Fu & ~keep);
         loadExponents(k + 2);
         blockStep(k, std::integral_constant<unsigned, 0>{});
         blockStep(k, std::integral_constant<unsigned, 1>{});

@@ -225,6 +225,43 @@ def test_given_exponents_over_their_range(gpu, rows, dtype):
     near(y, want, product_room(xv, wv, dtype) + 4 * U * np.abs(want) + rounded(want, dtype), "y")
 
 
+@pytest.mark.parametrize("rows,outer", [(3, 40), (20, 300), (100, 200), (600, 500), (4096, 4100)])
+@pytest.mark.parametrize("columns", [128, 640, 1153])
+def test_exponents_past_the_last_block_do_not_count(gpu, rows, outer, columns):
+    """Bytes that fill up a row of exponents may be anything, 255 among them."""
+    from tcc_spmm_amd.blocks import matmul_blocks, quantize_blocks, quantize_weight_blocks, weight_grad_blocks
+    x, weight = quantize_blocks(random((rows, columns), 1)), quantize_weight_blocks(random((outer, columns), 2))
+    dy = random((rows, outer), 3, "bf16")
+    want = matmul_blocks(x, weight), weight_grad_blocks(dy, x)[0]
+    blocks = -(-columns // 128)
+    x.exponents[:, blocks:] = 255
+    weight.exponents[:, blocks:] = 255
+    assert torch.equal(matmul_blocks(x, weight), want[0]) and torch.equal(weight_grad_blocks(dy, x)[0], want[1])
+    assert matmul_blocks(x, weight, dtype=torch.float32).isfinite().all()
+
+
+def test_offsets_past_32_bits(gpu):
+    """Nine million rows of 256: x, y and the kept codes pass 2^31, x 2^32 bytes; the last rows are those of a call
+    on them alone."""
+    from tcc_spmm_amd import blocks as B
+    x = torch.randn((9_000_000, 256), device="cuda", dtype=torch.bfloat16)
+    weight = B.quantize_weight_blocks(random((64, 256), 2))
+    y, kept = B.linear_blocks(x, weight, keep=True)
+    tail, tail_kept = B.linear_blocks(x[-9000:], weight, keep=True)
+    assert torch.equal(y[-9000:], tail) and torch.equal(kept.codes[-9000:].float(), tail_kept.codes.float())
+    assert torch.equal(B.matmul_blocks(kept, weight)[-9000:], tail)
+    a, act = B.activation_blocks(x, "silu", gated=True)
+    b, tail_act = B.activation_blocks(x[-9000:], "silu", gated=True)
+    assert torch.equal(a[-9000:], b) and torch.equal(act.codes[-18000:], tail_act.codes)
+    assert torch.equal(B.activation_blocks_backward(a, act, gated=True)[-9000:],
+                       B.activation_blocks_backward(b, tail_act, gated=True))
+    dy = torch.zeros((9_000_000, 64), device="cuda", dtype=torch.bfloat16)
+    dy[-9000:] = random((9000, 64), 3, "bf16")
+    dw, _ = B.weight_grad_blocks(dy, kept)
+    want, _ = B.weight_grad_blocks(dy[-9000:], tail_kept)
+    assert (dw - want).abs().max() <= 1e-4 * want.abs().max()
+
+
 # --------------------------------------------------------------------------------------------------
 # Gradients of the layer
 
