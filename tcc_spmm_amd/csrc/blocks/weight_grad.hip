@@ -65,8 +65,9 @@ struct Gradient {
 // Tiles of BN columns of dy by BK of x, WN x WK waves, for any dy. A step's bytes are loaded to registers while the
 // step before is multiplied; dy is split into its parts on the way to LDS, which has one stage, since its
 // parts leave little room and several workgroups share a CU.
-template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK>
-__global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
+// Narrow: rows of dy of fewer than 8 elements.
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, bool Narrow>
+__global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(2))) void sumRows(Gradient a) {
     constexpr unsigned P = Parts<T>::count, Threads = 64 * WN * WK, NT = BN / WN / 16, KT = BK / WK / 16;
     constexpr unsigned DyLoads = kStep * BN / 8 / Threads;
     constexpr unsigned XLoads = kStep * BK / 16 / Threads, BT = NT / WK; // BT: bias operands of a wave
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     const unsigned tiles = a.tilesN * a.tilesK, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
     const unsigned n0 = tile % a.tilesN * BN, k0 = tile / a.tilesN * BK;
     const unsigned first = split * a.rowsPerSplit, last = min(first + a.rowsPerSplit, a.rows);
-    const Raw* dy = static_cast<const Raw*>(a.dy) + n0;
+    const Raw* dy = static_cast<const Raw*>(a.dy);
 
     typedef typename Group<T>::Vec Vec;
     Vec raw[DyLoads];
@@ -90,33 +91,45 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     const auto rowsOf = [&](unsigned row) {
         return __builtin_amdgcn_readfirstlane(min(row < last ? last - row : 0u, kStep));
     };
-    auto fetchDy = [&](unsigned row) {
+    // No load is conditional, since what a branch loads is waited for where it ends: rows past the split's end read
+    // its last row, and a chunk over the row's end the row's last 8 elements, put right on the way to LDS. The parts
+    // of a step are inlined by force: a call would take every register that they share through memory.
+    const bool ragged = !Narrow && n0 + BN > a.outer && a.outer % 8 != 0;
+    auto fetchDy = [&](unsigned row) __attribute__((always_inline)) {
 #pragma unroll
         for (unsigned i = 0; i < DyLoads; ++i) {
-            const unsigned chunk = t + i * Threads, r = row + chunk / (BN / 8), c = chunk % (BN / 8) * 8;
-            raw[i] = Vec{};
-            if (r >= last || n0 + c >= a.outer) continue;
-            const Raw* p = dy + r * a.dyStride + c;
-            if (n0 + c + 8 <= a.outer) {
-                raw[i] = *reinterpret_cast<const typename Group<T>::Loose*>(p);
-            } else {
+            const unsigned chunk = t + i * Threads, r = min(row + chunk / (BN / 8), last - 1), c = n0 + chunk % (BN / 8) * 8;
+            const Raw* p = dy + r * a.dyStride;
+            if constexpr (Narrow) {
 #pragma unroll
-                for (unsigned j = 0; j < 8; ++j)
-                    if (n0 + c + j < a.outer) raw[i][j] = p[j];
+                for (unsigned j = 0; j < 8; ++j) raw[i][j] = p[min(c + j, a.outer - 1)];
+            } else {
+                raw[i] = *reinterpret_cast<const typename Group<T>::Loose*>(p + min(c, a.outer - 8));
             }
         }
     };
-    auto stashDy = [&] {
+    auto stashDy = [&](unsigned row) __attribute__((always_inline)) {
 #pragma unroll
         for (unsigned i = 0; i < DyLoads; ++i) {
             const unsigned chunk = t + i * Threads, r = chunk / (BN / 8), c = chunk % (BN / 8) * 8;
             std::uint8_t* to = lds + Tile<BN>::at(r, c);
+            Vec v = raw[i];
+            if (ragged) {
+                const unsigned past = n0 + c - min(n0 + c, a.outer - 8);
+#pragma unroll
+                for (unsigned by = 4; by; by /= 2)
+#pragma unroll
+                    for (unsigned j = 0; j + by < 8; ++j) v[j] = past & by ? v[j + by] : v[j];
+            }
+            if (row + kStep > last)
+#pragma unroll
+                for (unsigned j = 0; j < 8; ++j) v[j] = row + r < last ? v[j] : Raw(0.0f);
             if constexpr (P == 1) {
-                *reinterpret_cast<Vec*>(to) = raw[i];
+                *reinterpret_cast<Vec*>(to) = v;
             } else {
                 float rest[8];
 #pragma unroll
-                for (unsigned j = 0; j < 8; ++j) rest[j] = T::get(raw[i][j]);
+                for (unsigned j = 0; j < 8; ++j) rest[j] = T::get(v[j]);
                 const bool large = peakBits(rest) >= 0x7F7F8000u; // rounds to an infinity, or is one, or a NaN
 #pragma unroll
                 for (unsigned p = 0; p < P; ++p) {
@@ -130,13 +143,10 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
                     if (p == 0 && large) {
 #pragma unroll
                         for (unsigned j = 0; j < 8; ++j) {
-                            const float v = T::get(raw[i][j]), cut = __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
-                            if (!__builtin_isfinite(v)) {
-                                rest[j] = 0.0f;
-                            } else if (!__builtin_isfinite(float(part[j]))) {
-                                part[j] = __bf16(cut);
-                                rest[j] = v - cut;
-                            }
+                            const float f = T::get(v[j]), cut = __uint_as_float(__float_as_uint(f) & 0xFFFF0000u);
+                            const bool finite = __builtin_isfinite(f), over = !__builtin_isfinite(float(part[j]));
+                            part[j] = finite && over ? __bf16(cut) : part[j];
+                            rest[j] = !finite ? 0.0f : over ? f - cut : rest[j];
                         }
                     }
                     *reinterpret_cast<bf16x8*>(to + p * Tile<BN>::bytes) = part;
@@ -144,7 +154,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
             }
         }
     };
-    auto fetchX = [&](unsigned row) {
+    auto fetchX = [&](unsigned row) __attribute__((always_inline)) {
         const unsigned rows = rowsOf(row);
         const auto codes = buffer(a.x + std::uint64_t(row) * a.codePitch, rows * a.codePitch);
         const auto exponents = buffer(a.xe + std::uint64_t(row) * a.expPitch, rows * a.expPitch);
@@ -156,7 +166,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
             e[i] = __builtin_amdgcn_raw_buffer_load_b8(exponents, in ? r * a.expPitch + (k0 + c) / kBlock : 0x80000000u, 0, 0);
         }
     };
-    auto stashX = [&] {
+    auto stashX = [&]() __attribute__((always_inline)) {
         std::uint8_t* to = lds + P * Tile<BN>::bytes;
 #pragma unroll
         for (unsigned i = 0; i < XLoads; ++i) {
@@ -179,7 +189,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
     const bool bias = a.db && k0 == 0;
     const bf16x8 ones = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
     f32x4 acc[NT][KT] = {}, sums[BT] = {};
-    auto half = [&](unsigned r0, auto withBias) {
+    auto half = [&](unsigned r0, auto withBias) __attribute__((always_inline)) {
         const std::uint8_t* base = lds;
         bf16x8 xf[KT];
 #pragma unroll
@@ -202,7 +212,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
                                                                       wn + 16 * (wk * BT + b), lane), sums[b], 0, 0, 0);
         }
     };
-    auto walk = [&](auto withBias) {
+    auto walk = [&](auto withBias) __attribute__((always_inline)) {
         for (unsigned row = first; row < last; row += kStep) {
             fetchX(row + kStep);
             fetchDy(row + kStep);
@@ -212,7 +222,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             stashX();
-            stashDy();
+            stashDy(row + kStep);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     };
@@ -220,7 +230,7 @@ __global__ __launch_bounds__(64 * WN * WK) void sumRows(Gradient a) {
         fetchX(first);
         fetchDy(first);
         stashX();
-        stashDy();
+        stashDy(first);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (bias)
             walk(std::true_type{});
@@ -544,22 +554,25 @@ double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t 
 }
 
 // Steps measured, in us: the large tile 2.0 (4096 x 4096 x 4096 135, 8192 x 4096 x 8192 545), the small one 0.75 alone
-// (2048 x 1024 x 4096 32) and 1.15 shared (2048 x 2048 x 4096 46).
+// (2048 x 1024 x 4096 32) and 1.15 shared (2048 x 2048 x 4096 46). Where dy is not bf16 in aligned rows: bf16 1.2 alone
+// (2048 x 1024 x 4095 46) and 1.65 shared (4096 x 4096 x 4095 212), f16 2.0 (71) and 2.9 (4096 x 4096 x 4096 372), f32
+// 2.75 (96; in two splits that share a CU 82) and 3.9 (514).
 Plan planOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, bool aligned) {
     Plan small = {outer <= 64 && !aligned ? 64u : 128u, 128, 1, 1, aligned}, large = {256, 256, 1, 1, aligned};
     if (!aligned) {
-        const double step = 0.6 + 0.3 * (type == DenseType::f32 ? 3 : type == DenseType::f16 ? 2 : 1);
-        planTime(small, rows, inner, outer, step, step, 2);
+        const double alone = type == DenseType::f32 ? 2.75 : type == DenseType::f16 ? 2.0 : 1.2;
+        const double shared = type == DenseType::f32 ? 3.9 : type == DenseType::f16 ? 2.9 : 1.65;
+        planTime(small, rows, inner, outer, alone, shared, 2);
         return small;
     }
     const double smallTime = planTime(small, rows, inner, outer, 0.75, 1.15, 2);
     return planTime(large, rows, inner, outer, 2.0, 2.0, 1) < smallTime ? large : small;
 }
 
-template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK>
+template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, bool Narrow>
 void launchSum(const Gradient& a, std::uint64_t blocks, hipStream_t stream) {
     constexpr unsigned lds = Parts<T>::count * Tile<BN>::bytes + Tile<BK>::bytes;
-    hipLaunchKernelGGL((sumRows<T, BN, BK, WN, WK>), dim3(unsigned(blocks)), dim3(64 * WN * WK), lds, stream, a);
+    hipLaunchKernelGGL((sumRows<T, BN, BK, WN, WK, Narrow>), dim3(unsigned(blocks)), dim3(64 * WN * WK), lds, stream, a);
 }
 
 } // namespace
@@ -612,10 +625,12 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     } else {
         withType(dy.type, [&](auto tag) {
             typedef decltype(tag) T;
-            if (p.bn == 64)
-                launchSum<T, 64, 128, 1, 4>(a, blocks, stream);
+            if (outer < 8)
+                launchSum<T, 64, 128, 1, 4, true>(a, blocks, stream);
+            else if (p.bn == 64)
+                launchSum<T, 64, 128, 1, 4, false>(a, blocks, stream);
             else
-                launchSum<T, 128, 128, 2, 2>(a, blocks, stream);
+                launchSum<T, 128, 128, 2, 2, false>(a, blocks, stream);
         });
     }
     checkHip(hipGetLastError());
