@@ -548,11 +548,19 @@ __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
 // block in an order of their own; the order along the inner axis is free as long as both operands share it,
 // so the weight is laid out in the same order: element e of a block is in lane group e / 4 % 4 (FP32) or
 // e / 8 % 4, after those of the groups before it in the block.
+// swapGroups<16>: where bit 4 of the lane is set, a takes the b of the lane without it, which takes a in turn;
+// swapGroups<32>: bit 5.
+template <unsigned Lanes> __device__ __forceinline__ void swapGroups(unsigned& a, unsigned& b) {
+    const auto r = Lanes == 16 ? __builtin_amdgcn_permlane16_swap(a, b, false, false)
+                               : __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+
 template <typename T, unsigned Blocks>
 __global__ __launch_bounds__(512) void multiplyRows(Product a) {
     constexpr bool Exact = std::is_same<T, F32>::value;
     constexpr unsigned Run = Exact ? 4 : 8, Image = Exact ? 256 : 128; // elements of a load; bytes of a weight block
-    constexpr unsigned Together = 4;                                   // column tiles multiplied at a time
+    constexpr unsigned Together = 4, Fill = 4; // column tiles multiplied at a time; loads of the weight in flight
     typedef typename T::Raw Raw;
     typedef Raw RunVec __attribute__((ext_vector_type(Run)));
     typedef RunVec LooseRun __attribute__((aligned(alignof(Raw))));
@@ -564,29 +572,41 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
         if constexpr (Exact) return s;
         return s / 32 * 32 + s % 16 / 4 * 8 + s / 16 % 2 * 4 + s % 4;
     };
-    for (unsigned i = t; i < slots * Blocks * 8; i += 512) {
-        const unsigned part = i % 8, block = i / 8 % Blocks, slot = i / 8 / Blocks, column = columnOf(slot);
-        u32x4 q = {0, 0, 0, 0};
-        float scale = 0.0f;
-        if (column < a.outer) {
-            q = *reinterpret_cast<const u32x4*>(a.w + (std::uint64_t(column) * Blocks + block) * kBlock + part * 16);
-            scale = scaleOf(a.we[std::uint64_t(column / kBlock) * a.expPitch + block]);
+    for (unsigned i0 = t; i0 < slots * Blocks * 8; i0 += 512 * Fill) {
+        u32x4 q[Fill];
+        unsigned e[Fill];
+#pragma unroll
+        for (unsigned f = 0; f < Fill; ++f) {
+            const unsigned i = i0 + f * 512, part = i % 8, block = i / 8 % Blocks;
+            const unsigned column = min(columnOf(i / 8 / Blocks), a.outer - 1);
+            q[f] = *reinterpret_cast<const u32x4*>(a.w + (std::uint64_t(column) * Blocks + block) * kBlock + part * 16);
+            e[f] = a.we[std::uint64_t(column / kBlock) * a.expPitch + block];
         }
-        std::uint8_t* to = lds + (block * slots + slot) * Image;
-        if constexpr (Exact) {
-            // 16-byte chunks of a 256-byte row: 4 * group + (element of the group) / 8.
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (unsigned j = 0; j < 4; ++j) {
-                const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[j], scale, false);
-                const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[j], scale, true);
-                *reinterpret_cast<u32x2*>(to + ((4 * j + part / 2) ^ (slot & 15)) * 16 + part % 2 * 8) =
-                    u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
-            }
-        } else {
+        for (unsigned f = 0; f < Fill; ++f) {
+            const unsigned i = i0 + f * 512, part = i % 8, block = i / 8 % Blocks, slot = i / 8 / Blocks;
+            if (slot >= slots) break;
+            const bool in = columnOf(slot) < a.outer;
+            std::uint8_t* to = lds + (block * slots + slot) * Image;
+            if constexpr (Exact) {
+                // 16-byte chunks of a 256-byte row: 4 * group + (element of the group) / 8.
+                const float scale = in ? scaleOf(e[f]) : 0.0f;
 #pragma unroll
-            for (unsigned j = 0; j < 2; ++j) {
-                const unsigned at = (part % 2 * 2 + j) * 32 + part / 2 * 8;
-                *reinterpret_cast<u32x2*>(to + ((at / 16) ^ (slot & 7)) * 16 + at % 16) = u32x2{q[2 * j], q[2 * j + 1]};
+                for (unsigned j = 0; j < 4; ++j) {
+                    const unsigned c = in ? q[f][j] : 0;
+                    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false);
+                    const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true);
+                    *reinterpret_cast<u32x2*>(to + ((4 * j + part / 2) ^ (slot & 15)) * 16 + part % 2 * 8) =
+                        u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
+                }
+            } else {
+#pragma unroll
+                for (unsigned j = 0; j < 2; ++j) {
+                    const unsigned at = (part % 2 * 2 + j) * 32 + part / 2 * 8;
+                    *reinterpret_cast<u32x2*>(to + ((at / 16) ^ (slot & 7)) * 16 + at % 16) =
+                        in ? u32x2{q[f][2 * j], q[f][2 * j + 1]} : u32x2{0, 0};
+                }
             }
         }
     }
@@ -600,14 +620,28 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
         for (unsigned b = 0; b < Blocks; ++b)
 #pragma unroll
             for (unsigned i = 0; i < 32 / Run; ++i) {
-                const unsigned at = b * kBlock + (i * 4 + g) * Run;
-                if (at + Run <= a.inner) {
+                const unsigned at = min(b * kBlock + (i * 4 + g) * Run, a.inner - Run);
+                raw[b][i] = RunVec{};
+                if (b + 1 < Blocks || b * kBlock + i * 4 * Run < a.inner)
                     raw[b][i] = __builtin_nontemporal_load(reinterpret_cast<const LooseRun*>(x + at));
-                } else {
-#pragma unroll
-                    for (unsigned j = 0; j < Run; ++j) raw[b][i][j] = at + j < a.inner ? x[at + j] : Raw(0.0f);
-                }
             }
+        __builtin_amdgcn_sched_barrier(0);
+        if (a.inner != Blocks * kBlock) {
+            // The last block ends early: runs past the row read its last elements, which move to their places.
+#pragma unroll
+            for (unsigned i = 0; i < 32 / Run; ++i) {
+                const unsigned at = (Blocks - 1) * kBlock + (i * 4 + g) * Run, past = at - min(at, a.inner - Run);
+                RunVec& v = raw[Blocks - 1][i];
+                if (a.inner % Run) {
+#pragma unroll
+                    for (unsigned by = Run / 2; by; by /= 2)
+#pragma unroll
+                        for (unsigned j = 0; j + by < Run; ++j) v[j] = past & by ? v[j + by] : v[j];
+                }
+#pragma unroll
+                for (unsigned j = 0; j < Run; ++j) v[j] = past + j < Run ? v[j] : Raw(0.0f);
+            }
+        }
         u32x4 q[Blocks][2];
         unsigned xe[Blocks];
 #pragma unroll
@@ -627,19 +661,28 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
             const u32x2 q2 = encode8<BlockCodes::e4m3>(v[2], xe[b]), q3 = encode8<BlockCodes::e4m3>(v[3], xe[b]);
             q[b][0] = u32x4{q0.x, q0.y, q1.x, q1.y};
             q[b][1] = u32x4{q2.x, q2.y, q3.x, q3.y};
-            if (a.keep && row < a.rows) {
+            if (a.keep) {
+                // Lane groups exchange codes until each has 16 bytes side by side: four store 64 bytes of a row.
                 std::uint8_t* to = a.keep + (std::uint64_t(row) * Blocks + b) * kBlock;
 #pragma unroll
-                for (unsigned i = 0; i < 32 / Run; ++i) {
-                    if constexpr (Exact)
-                        *reinterpret_cast<unsigned*>(to + (i * 4 + g) * 4) = q[b][i / 4][i % 4];
-                    else
-                        *reinterpret_cast<u32x2*>(to + (i * 4 + g) * 8) =
-                            u32x2{q[b][i / 2][i % 2 * 2], q[b][i / 2][i % 2 * 2 + 1]};
+                for (unsigned h = 0; h < 2; ++h) {
+                    unsigned c[4] = {q[b][h][0], q[b][h][1], q[b][h][2], q[b][h][3]};
+                    if constexpr (Exact) {
+                        swapGroups<16>(c[0], c[1]), swapGroups<16>(c[2], c[3]);
+                        swapGroups<32>(c[0], c[2]), swapGroups<32>(c[1], c[3]);
+                    } else {
+                        swapGroups<16>(c[0], c[2]), swapGroups<16>(c[1], c[3]);
+                    }
+                    const unsigned at = h * 64 + (Exact ? g * 16 : g % 2 * 32 + g / 2 * 16);
+                    if (row < a.rows) *reinterpret_cast<u32x4*>(to + at) = u32x4{c[0], c[1], c[2], c[3]};
                 }
-                if (b + g < (b + 1 == Blocks ? a.expPitch : b + 1))
-                    a.keepExp[std::uint64_t(row) * a.expPitch + b + g] = std::uint8_t(g ? 127u : xe[b]);
             }
+        }
+        if (a.keep && row < a.rows && g == 0) {
+            unsigned exponents = 0x7F7F7F7Fu;
+#pragma unroll
+            for (unsigned b = 0; b < Blocks; ++b) exponents ^= (xe[b] ^ 0x7Fu) << 8 * b;
+            reinterpret_cast<unsigned*>(a.keepExp)[row] = exponents;
         }
         Raw* y = static_cast<Raw*>(a.y) + row * a.yStride;
         for (unsigned tile = 0; tile < tiles; tile += Together) {
@@ -920,12 +963,18 @@ void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, De
 }
 
 namespace {
-// The weight's bytes in LDS if a narrow layer with many rows goes through multiplyRows, else 0.
+// The weight's bytes in LDS if a narrow layer with many rows goes through multiplyRows, else 0. A group of 128 rows
+// fills an image of its own, so the larger it is, the more rows it takes to pay. Measured in us, here against a
+// launch that quantizes and tiles: f32 128 -> 128 (32 KiB) at 4096 rows 8.3 : 9.0, 8192 8.3 : 10.2; bf16 128 -> 256
+// (32 KiB) at 4096 7.2 : 5.3, 8192 7.6 : 6.9, 20000 9.0 : 12.0; f32 128 -> 256 (64 KiB) at 8192 12.3 : 10.8, 20000
+// 13.4 : 16.3; bf16 512 -> 256 (128 KiB) at 8192 15.5 : 10.7, 16384 18 : 18, 300000 129 : 172. Rows of fewer than 8
+// elements cannot be read 8 at a time.
 constexpr unsigned kRowsLds = 160 * 1024;
 std::size_t rowsImage(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
     const std::uint64_t count = (inner + kBlock - 1) / kBlock, slots = (std::uint64_t(outer) + 63) / 64 * 64;
     const std::uint64_t bytes = slots * count * (type == DenseType::f32 ? 256 : 128);
-    return rows >= 8192 && count <= 4 && bytes <= kRowsLds ? std::size_t(bytes) : 0;
+    const bool enough = inner >= 8 && rows >= (bytes <= 32 * 1024 ? 8192u : 16384u);
+    return enough && count <= 4 && bytes <= kRowsLds ? std::size_t(bytes) : 0;
 }
 
 template <typename T> void launchRows(const Product& p, std::size_t lds, hipStream_t stream) {

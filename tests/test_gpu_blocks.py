@@ -150,7 +150,8 @@ def test_linear_wide(gpu, rows, inner, outer, dtype):
 
 
 @pytest.mark.parametrize("rows,inner,outer", [(8192, 128, 256), (20011, 47, 256), (10007, 256, 47), (9001, 300, 100),
-                                              (8200, 512, 130), (16385, 129, 3)])
+                                              (8200, 512, 130), (16385, 129, 3), (8199, 7, 40), (16391, 300, 100),
+                                              (16390, 509, 47), (16401, 512, 130), (17000, 250, 256)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_linear_narrow(gpu, rows, inner, outer, dtype):
     """Many rows through a layer whose weight fits in LDS, and the same layer where blocks are given."""
