@@ -739,7 +739,7 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Few rows (single tokens, small batches): a workgroup takes 16 columns of y for all rows; its eight waves
+// Few rows (single tokens, small batches): a workgroup takes 16 columns of y for up to 64 rows; its eight waves
 // share the blocks of the inner axis and add their sums through LDS in the waves' order. The weight's
 // codes go from memory to the MFMA's registers, each byte read once on the chip, four blocks' loads at a
 // time before the first is used: what bounds this is how many bytes are on their way. A lane takes 32
@@ -756,6 +756,7 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) 
     extern __shared__ __align__(16) std::uint8_t lds[]; // Dense: x's codes, then its exponents
     const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const unsigned l16 = lane % 16, g = lane / 16, n0 = blockIdx.x * 16, pitch = a.count * kBlock;
+    const unsigned m0 = Dense ? 0 : blockIdx.y * 16 * MT;
     const std::uint8_t* wp = a.w + min(n0 + l16, a.outer - 1) * std::uint64_t(pitch) + g * 32;
     const std::uint8_t* wep = a.we + std::uint64_t(n0 / kBlock) * a.expPitch;
     std::uint8_t* exponents = lds + a.rows * pitch;
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) 
             const unsigned block = min(k + u * kTokenWaves, a.count - 1);
 #pragma unroll
             for (unsigned m = 0; m < MT; ++m) {
-                const unsigned row = min(m * 16 + l16, a.rows - 1);
+                const unsigned row = min(m0 + m * 16 + l16, a.rows - 1);
                 const std::uint8_t* p = Dense ? lds + row * pitch : a.x + row * std::uint64_t(pitch);
                 x[u][m][0] = *reinterpret_cast<const u32x4*>(p + block * kBlock + g * 32);
                 x[u][m][1] = *reinterpret_cast<const u32x4*>(p + block * kBlock + g * 32 + 16);
@@ -834,11 +835,11 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) 
     // Output i of 256 * MT: column fastest.
     typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
     for (unsigned i = t; i < 256 * MT; i += kWave * kTokenWaves) {
-        const unsigned column = i % 16, row = i / 16;
+        const unsigned column = i % 16, r = i / 16, row = m0 + r;
         if (n0 + column >= a.outer || row >= a.rows) continue;
         float s = 0.0f;
 #pragma unroll
-        for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][row / 16][row % 16 + column / 4 * 16][column % 4];
+        for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][r / 16][r % 16 + column / 4 * 16][column % 4];
         if (a.bias) s += a.bias[n0 + column];
         y[row * a.yStride + n0 + column] = T::put(s);
     }
@@ -847,17 +848,28 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void multiplyTokens(Product a) 
 // ------------------------------------------------------------------------------------------------
 // Host side
 
-// FP32 rows that multiplyTokens takes; its tiles are of 128.
-constexpr unsigned kTokenRows = 64;
+// Whether multiplyTokens takes an FP32 product, by the least estimated time in microseconds: rounds of its
+// workgroups, 64 rows by 16 columns, against rounds of tiles of 128. The constants fit these times (rows x inner x
+// outer, this form : tiles): 64 x 4096 x 4096 18 : 58, 100 x 4096 x 4096 29 : 59, 256 x 4096 x 4096 61 : 69,
+// 512 x 4096 x 4096 119 : 72, 512 x 8192 x 512 31 : 115, 256 x 1024 x 1024 12.9 : 18.9, 300 x 1000 x 1000 22 : 19,
+// 1024 x 1024 x 1024 46 : 19, 256 x 512 x 8192 52 : 13, 4096 x 4096 x 4096 - : 178.
+bool exactTokens(std::uint32_t rows, std::uint32_t outer, unsigned count) {
+    const auto over = [](std::uint64_t n, std::uint64_t size) { return (n + size - 1) / size; };
+    const std::uint64_t groups = over(rows, 64) * over(outer, 16), tiles = over(rows, 128) * over(outer, 128);
+    const double tokens = double(over(groups, 256)) * (count <= 4 ? 6.0 : 14.5 * std::max(1.0, count / 32.0));
+    const double exact = tiles <= 256 ? 5.0 + 1.7 * count : double(over(tiles, 512)) * (5.0 + 2.6 * count);
+    return rows <= 64 || (over(rows, 64) < 65536 && tokens < exact);
+}
 
 void launchTokens(const Product& p, hipStream_t stream) {
-    const dim3 grid((p.outer + 15) / 16), threads(kWave * kTokenWaves);
+    const dim3 threads(kWave * kTokenWaves);
+    const unsigned across = (p.outer + 15) / 16;
     if (p.rows <= 16)
-        hipLaunchKernelGGL((multiplyTokens<F32, 1, false>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 1, false>), dim3(across), threads, 0, stream, p);
     else if (p.rows <= 32)
-        hipLaunchKernelGGL((multiplyTokens<F32, 2, false>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 2, false>), dim3(across), threads, 0, stream, p);
     else
-        hipLaunchKernelGGL((multiplyTokens<F32, 4, false>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((multiplyTokens<F32, 4, false>), dim3(across, (p.rows + 63) / 64), threads, 0, stream, p);
     checkHip(hipGetLastError());
 }
 
@@ -916,7 +928,7 @@ template <typename T> void launchWide(Product p, hipStream_t stream) {
 
 template <typename T> void launchProduct(Product p, hipStream_t stream) {
     if constexpr (std::is_same<T, F32>::value) {
-        if (p.rows <= kTokenRows) return launchTokens(p, stream);
+        if (exactTokens(p.rows, p.outer, p.count)) return launchTokens(p, stream);
         p.tilesM = (p.rows + 127) / 128;
         const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + 127) / 128);
         if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");

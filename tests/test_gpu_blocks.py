@@ -149,6 +149,12 @@ def test_linear_wide(gpu, rows, inner, outer, dtype):
     test_linear(gpu, rows, inner, outer, dtype)
 
 
+@pytest.mark.parametrize("rows,inner,outer", [(65, 4500, 100), (130, 1500, 200), (200, 8300, 33), (511, 1024, 65)])
+def test_linear_f32_few_tiles(gpu, rows, inner, outer):
+    """FP32 products of more than 64 rows that are too few tiles: 64 rows at a time, the last ones ragged."""
+    test_linear(gpu, rows, inner, outer, "f32")
+
+
 @pytest.mark.parametrize("rows,inner,outer", [(8192, 128, 256), (20011, 47, 256), (10007, 256, 47), (9001, 300, 100),
                                               (8200, 512, 130), (16385, 129, 3), (8199, 7, 40), (16391, 300, 100),
                                               (16390, 509, 47), (16401, 512, 130), (17000, 250, 256)])
