@@ -41,11 +41,11 @@ struct Call {
     unsigned items, width, count, magic, expPitch;
 };
 
-template <BlockCodes C>
+template <typename T, BlockCodes C>
 __device__ __forceinline__ void keepBlock(const Call& a, std::uint64_t row, unsigned block, unsigned lane,
                                           const float (&v)[8]) {
     const unsigned e = exponentOf<C>(rowMax(peakBits(v)));
-    *reinterpret_cast<u32x2*>(a.codes + row * a.count * kBlock + block * kBlock + lane * 8) = encode8<C>(v, e);
+    storeCodes<T>(a.codes + row * a.count * kBlock + block * kBlock, lane, encode8<C>(v, e));
     if (block + lane < (block + 1 == a.count ? a.expPitch : block + 1))
         a.exponents[row * a.expPitch + block + lane] = std::uint8_t(lane ? 127u : e);
 }
@@ -56,30 +56,30 @@ __global__ __launch_bounds__(kThreads) void activateBlocks(Call a) {
     const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
     if (item >= a.items) return;
     const unsigned row = rowOf(item, a.count, a.magic), block = item - row * a.count;
-    const unsigned at = block * kBlock + lane * 8;
+    const unsigned at = block * kBlock;
     const auto* x = static_cast<const typename T::Raw*>(a.in) + row * a.inStride;
     float g[8], u[8], y[8];
-    load8<T>(x, at, a.width, g);
-    if constexpr (Gated) load8<T>(x + a.width, at, a.width, u);
+    loadBlock<T>(x, at, lane, a.width, g);
+    if constexpr (Gated) loadBlock<T>(x + a.width, at, lane, a.width, u);
 #pragma unroll
     for (unsigned i = 0; i < 8; ++i) {
         float d;
         activate<F, false>(g[i], y[i], d);
         if constexpr (Gated) y[i] *= u[i];
     }
-    store8<T>(static_cast<typename T::Raw*>(a.out) + row * a.outStride, at, a.width, y);
+    storeBlock<T>(static_cast<typename T::Raw*>(a.out) + row * a.outStride, at, lane, a.width, y);
     if (!a.codes) return;
     if constexpr (Gated) {
-        keepBlock<C>(a, 2 * std::uint64_t(row), block, lane, g);
-        keepBlock<C>(a, 2 * std::uint64_t(row) + 1, block, lane, u);
+        keepBlock<T, C>(a, 2 * std::uint64_t(row), block, lane, g);
+        keepBlock<T, C>(a, 2 * std::uint64_t(row) + 1, block, lane, u);
     } else {
-        keepBlock<C>(a, row, block, lane, g);
+        keepBlock<T, C>(a, row, block, lane, g);
     }
 }
 
-template <BlockCodes C>
+template <typename T, BlockCodes C>
 __device__ __forceinline__ void keptBlock(const Call& a, std::uint64_t row, unsigned block, unsigned lane, float (&v)[8]) {
-    const u32x2 q = *reinterpret_cast<const u32x2*>(a.codes + row * a.count * kBlock + block * kBlock + lane * 8);
+    const u32x2 q = loadCodes<T>(a.codes + row * a.count * kBlock + block * kBlock, lane);
     decode8<C>(q, scaleOf(a.exponents[row * a.expPitch + block]), v);
 }
 
@@ -89,11 +89,11 @@ __global__ __launch_bounds__(kThreads) void activateBlocksBackward(Call a) {
     const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
     if (item >= a.items) return;
     const unsigned row = rowOf(item, a.count, a.magic), block = item - row * a.count;
-    const unsigned at = block * kBlock + lane * 8;
+    const unsigned at = block * kBlock;
     float dy[8], g[8], u[8];
-    load8<T>(static_cast<const typename T::Raw*>(a.in) + row * a.inStride, at, a.width, dy);
-    keptBlock<C>(a, Gated ? 2 * std::uint64_t(row) : row, block, lane, g);
-    if constexpr (Gated) keptBlock<C>(a, 2 * std::uint64_t(row) + 1, block, lane, u);
+    loadBlock<T>(static_cast<const typename T::Raw*>(a.in) + row * a.inStride, at, lane, a.width, dy);
+    keptBlock<T, C>(a, Gated ? 2 * std::uint64_t(row) : row, block, lane, g);
+    if constexpr (Gated) keptBlock<T, C>(a, 2 * std::uint64_t(row) + 1, block, lane, u);
     float dg[8], du[8];
 #pragma unroll
     for (unsigned i = 0; i < 8; ++i) {
@@ -107,8 +107,8 @@ __global__ __launch_bounds__(kThreads) void activateBlocksBackward(Call a) {
         }
     }
     auto* dx = static_cast<typename T::Raw*>(a.out) + row * a.outStride;
-    store8<T>(dx, at, a.width, dg);
-    if constexpr (Gated) store8<T>(dx + a.width, at, a.width, du);
+    storeBlock<T>(dx, at, lane, a.width, dg);
+    if constexpr (Gated) storeBlock<T>(dx + a.width, at, lane, a.width, du);
 }
 
 template <typename F> void withActivation(BlockActivation k, F f) {

@@ -15,7 +15,7 @@ namespace blocks {
 constexpr unsigned kWave = 64;
 // A block of 128 elements is held by 16 lanes, 8 consecutive elements each: one DPP row, so that the
 // block's maximum is four DPP steps, and 16 bytes a lane of a 16-bit type.
-constexpr unsigned kBlockLanes = 16, kLaneElements = 8;
+constexpr unsigned kBlockLanes = 16; // of eight elements each
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -76,6 +76,68 @@ __device__ __forceinline__ void store8(typename T::Raw* row, unsigned at, unsign
 #pragma unroll
         for (unsigned i = 0; i < 8; ++i)
             if (at + i < n) row[at + i] = T::put(v[i]);
+    }
+}
+
+// A lane's eight elements of the block that starts at column `at` of a row of n, with the codes of the same
+// elements. Of FP32 they are four of each half, so that every access of a block's lanes is 256 bytes side by side:
+// with eight in a row, 16 bytes of each 32, a nontemporal store wrote at half the rate (dequantizing 1,000,000 x 256,
+// 407 us to 204).
+template <typename T>
+__device__ __forceinline__ void loadBlock(const typename T::Raw* row, unsigned at, unsigned lane, unsigned n, float (&v)[8]) {
+    if constexpr (!std::is_same<T, F32>::value) {
+        load8<T>(row, at + lane * 8, n, v);
+    } else {
+        typedef f32x4 Loose __attribute__((aligned(4)));
+#pragma unroll
+        for (unsigned h = 0; h < 8; h += 4) {
+            const unsigned c = at + h * (kBlock / 8) + lane * 4;
+            if (c + 4 <= n) {
+                const f32x4 g = __builtin_nontemporal_load(reinterpret_cast<const Loose*>(row + c));
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) v[h + i] = g[i];
+            } else {
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) v[h + i] = c + i < n ? row[c + i] : 0.0f;
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void storeBlock(typename T::Raw* row, unsigned at, unsigned lane, unsigned n, const float (&v)[8]) {
+    if constexpr (!std::is_same<T, F32>::value) {
+        store8<T>(row, at + lane * 8, n, v);
+    } else {
+        typedef f32x4 Loose __attribute__((aligned(4)));
+#pragma unroll
+        for (unsigned h = 0; h < 8; h += 4) {
+            const unsigned c = at + h * (kBlock / 8) + lane * 4;
+            if (c + 4 <= n) {
+                __builtin_nontemporal_store(f32x4{v[h], v[h + 1], v[h + 2], v[h + 3]}, reinterpret_cast<Loose*>(row + c));
+            } else {
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i)
+                    if (c + i < n) row[c + i] = v[h + i];
+            }
+        }
+    }
+}
+
+template <typename T> __device__ __forceinline__ u32x2 loadCodes(const std::uint8_t* block, unsigned lane) {
+    if constexpr (!std::is_same<T, F32>::value)
+        return *reinterpret_cast<const u32x2*>(block + lane * 8);
+    else
+        return u32x2{*reinterpret_cast<const unsigned*>(block + lane * 4),
+                     *reinterpret_cast<const unsigned*>(block + kBlock / 2 + lane * 4)};
+}
+
+template <typename T> __device__ __forceinline__ void storeCodes(std::uint8_t* block, unsigned lane, u32x2 q) {
+    if constexpr (!std::is_same<T, F32>::value) {
+        *reinterpret_cast<u32x2*>(block + lane * 8) = q;
+    } else {
+        *reinterpret_cast<unsigned*>(block + lane * 4) = q.x;
+        *reinterpret_cast<unsigned*>(block + kBlock / 2 + lane * 4) = q.y;
     }
 }
 

@@ -33,8 +33,7 @@ __global__ __launch_bounds__(kThreads) void quantizeRowBlocks(const typename T::
     for (unsigned i = 0; i < kItems; ++i) {
         const unsigned item = first + i * kGroups;
         row[i] = rowOf(item, count, magic);
-        const unsigned at = (item - row[i] * count) * kBlock + lane * kLaneElements;
-        if (item < items) load8<T>(x + row[i] * stride, at, columns, v[i]);
+        if (item < items) loadBlock<T>(x + row[i] * stride, (item - row[i] * count) * kBlock, lane, columns, v[i]);
     }
 #pragma unroll
     for (unsigned i = 0; i < kItems; ++i) {
@@ -42,8 +41,7 @@ __global__ __launch_bounds__(kThreads) void quantizeRowBlocks(const typename T::
         if (item >= items) break;
         const unsigned block = item - row[i] * count;
         const unsigned e = exponentOf<C>(rowMax(peakBits(v[i])));
-        const u32x2 q = encode8<C>(v[i], e);
-        *reinterpret_cast<u32x2*>(codes + std::uint64_t(row[i]) * codePitch + block * kBlock + lane * 8) = q;
+        storeCodes<T>(codes + std::uint64_t(row[i]) * codePitch + block * kBlock, lane, encode8<C>(v[i], e));
         // The row's last block fills the exponents up to a multiple of four with it.
         const unsigned end = block + 1 == count ? exponentPitch : block + 1;
         if (block + lane < end)
@@ -62,10 +60,11 @@ __global__ __launch_bounds__(kThreads) void dequantizeRowBlocks(const std::uint8
     const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
     if (item >= items) return;
     const unsigned row = rowOf(item, count, magic), block = item - row * count;
-    const u32x2 q = *reinterpret_cast<const u32x2*>(codes + std::uint64_t(row) * count * kBlock + block * kBlock + lane * 8);
+    const std::uint8_t* from = codes + std::uint64_t(row) * count * kBlock + block * kBlock;
+    const float scale = scaleOf(exponents[std::uint64_t(row) * ((count + 3) / 4 * 4) + block]);
     float v[8];
-    decode8<C>(q, scaleOf(exponents[std::uint64_t(row) * ((count + 3) / 4 * 4) + block]), v);
-    store8<T>(out + row * stride, block * kBlock + lane * kLaneElements, columns, v);
+    decode8<C>(loadCodes<T>(from, lane), scale, v);
+    storeBlock<T>(out + row * stride, block * kBlock, lane, columns, v);
 }
 
 // Thread t takes row t / 2's half t % 2 of the tile in eight groups of 8 elements, in the order that
