@@ -120,20 +120,27 @@ __global__ __launch_bounds__(kThreads) void quantizeWeightTiles(const typename T
     }
     if (!out.codesT) return;
     __syncthreads();
-    // A thread gathers 16 bytes of a column: a transposed row is 8 threads.
+    // A thread turns 16 rows of 4 columns, dwords of 4 rows at a time: a transposed row is 8 threads.
     const std::uint64_t pitchT = up * std::uint64_t(kBlock);
+    const unsigned column = t / 8 * 4, from = t % 8 * 16;
+    u32x4 q[4];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+        unsigned r[4];
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i)
+            r[i] = *reinterpret_cast<const unsigned*>(turned + (from + 4 * j + i) * kRowBytes + column);
+        const unsigned ab0 = __builtin_amdgcn_perm(r[1], r[0], 0x05010400), ab2 = __builtin_amdgcn_perm(r[1], r[0], 0x07030602);
+        const unsigned cd0 = __builtin_amdgcn_perm(r[3], r[2], 0x05010400), cd2 = __builtin_amdgcn_perm(r[3], r[2], 0x07030602);
+        q[0][j] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100);
+        q[1][j] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302);
+        q[2][j] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100);
+        q[3][j] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302);
+    }
 #pragma unroll
     for (unsigned i = 0; i < 4; ++i) {
-        const unsigned column = i * 32 + t / 8, from = t % 8 * 16;
-        if (tileX * kBlock + column >= inner) continue;
-        u32x4 q;
-#pragma unroll
-        for (unsigned j = 0; j < 4; ++j) {
-            const std::uint8_t* p = turned + (from + 4 * j) * kRowBytes + column;
-            q[j] = unsigned(p[0]) | unsigned(p[kRowBytes]) << 8 | unsigned(p[2 * kRowBytes]) << 16 |
-                   unsigned(p[3 * kRowBytes]) << 24;
-        }
-        *reinterpret_cast<u32x4*>(out.codesT + (tileX * kBlock + column) * pitchT + tileY * kBlock + from) = q;
+        const unsigned to = tileX * kBlock + column + i;
+        if (to < inner) *reinterpret_cast<u32x4*>(out.codesT + to * pitchT + tileY * kBlock + from) = q[i];
     }
 }
 
