@@ -4,7 +4,7 @@
 // factor's), 8 a lane. Forward computes y from x itself and the kept blocks from the same registers;
 // backward makes x's values from the codes and needs nothing else of the forward pass. Measured: 2,449,029 x 128
 // FP32 silu 500 us and back 457, 5.6 and 6.2 TB/s; 16384 x 4096 bf16, gated, 87 and 86 us, 6.2 TB/s; 16384 x 8192
-// bf16 silu 133 us, gelu 148 (erf's arithmetic shows), gelu_tanh 135. 333 x 1000: 4.5 us, a launch and its latency.
+// bf16 silu 133 us, gelu 148 (erf's arithmetic shows), gelu_tanh 135. 333 x 1001: 4.6 us, a launch and its latency.
 //
 // __expf is off by about its argument times 2^-24 of its value. Where the argument is large, the exponential is
 // negligible beside 1 or the result is a small fraction of x; there alone it is off by more than its last bits.

@@ -643,7 +643,9 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     checkHip(hipGetLastError());
     if (p.splits > 1) {
         const dim3 grid(unsigned((pitch / 4 + 63) / 64));
-        if (p.splits >= 32)
+        // 16 ways where there are many splits of a small gradient (262,144 x 256 x 47, the call, 32 us : 35 with 4);
+        // 4 where workgroups abound (100,000 x 256 x 256 35.0 : 35.7, 8192 x 1024 x 1024 38 : 45).
+        if (p.splits >= 32 && grid.x <= 128)
             hipLaunchKernelGGL(addSplits<16>, grid, dim3(1024), 0, stream, parts, dw, db, size, rounded4(size), outer,
                                pitch, p.splits);
         else
