@@ -77,15 +77,13 @@ void quantizeWeightBlocks(DenseMatrix w, BlockWeightView out, std::uint32_t oute
 // gradient's blocks. Products of codes are exact. An FP32 y has its sums in FP32 (bf16 MFMA on the exact
 // values). For 16-bit types the 8-bit MFMA adds the 128 products of a block with about 17 bits below the
 // largest one (measured: 1.2e-5 of the sum's norm, a twentieth of an f16 rounding) and the blocks in FP32.
-// workspaceBytes must be at least matmulBlocksWorkspace(..) for the same sizes and type.
-std::size_t matmulBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type);
 void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, DenseType type,
                   std::uint64_t stride, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
-                  void* workspace, std::size_t workspaceBytes, hipStream_t stream = nullptr);
+                  hipStream_t stream = nullptr);
 
 // The linear layer on dense x: quantizeBlocks and matmulBlocks with y's type that of x, in one launch
 // where that is faster. `keep` with null codes keeps nothing; else it receives x's blocks, the backward
-// pass's checkpoint.
+// pass's checkpoint. workspaceBytes must be at least linearBlocksWorkspace(..) for the same sizes and type.
 std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                   bool keep);
 void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, std::uint64_t yStride,

@@ -131,11 +131,9 @@ int tcc_quantize_weight_blocks(const void* w, uint64_t stride, uint32_t type, ui
                                uint8_t* codesT, uint8_t* exponentsT, uint32_t outer, uint32_t inner,
                                void* stream);
 /* Workspace queries write the bytes that the call with the same arguments needs at least. */
-int tcc_matmul_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, size_t* bytes);
 int tcc_matmul_blocks(const uint8_t* xCodes, const uint8_t* xExponents, const uint8_t* wCodes,
                       const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type,
-                      uint32_t rows, uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes,
-                      void* stream);
+                      uint32_t rows, uint32_t inner, uint32_t outer, void* stream);
 int tcc_linear_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, int keep,
                                 size_t* bytes);
 /* keepCodes and keepExponents may be null: x's blocks are not kept then. */

@@ -87,11 +87,8 @@ SIGNATURES = {
                                         C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
     "tcc_quantize_weight_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
                                              C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]),
-    "tcc_matmul_blocks_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
-                                              C.POINTER(C.c_size_t)]),
     "tcc_matmul_blocks": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
-                                    C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p,
-                                    C.c_size_t, C.c_void_p]),
+                                    C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p]),
     "tcc_linear_blocks_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
                                               C.POINTER(C.c_size_t)]),
     "tcc_linear_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,

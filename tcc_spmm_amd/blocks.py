@@ -261,11 +261,9 @@ def matmul_blocks(x: BlockTensor, weight: BlockWeight, bias: torch.Tensor | None
         with away:
             return matmul_blocks(x, weight, bias, dtype)
     y = torch.empty((x.rows, outer), dtype=dtype, device=device)
-    sizes = (x.rows, x.columns, outer, _TYPES[dtype])
-    _space, at, size = _workspace(lib().tcc_matmul_blocks_workspace, sizes, device)
     check(lib().tcc_matmul_blocks(x.codes.data_ptr(), x.exponents.data_ptr(), weight.codes.data_ptr(),
-                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, sizes[3], x.rows,
-                                  x.columns, outer, at, size, _stream(device.index)))
+                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, _TYPES[dtype], x.rows,
+                                  x.columns, outer, _stream(device.index)))
     return y
 
 

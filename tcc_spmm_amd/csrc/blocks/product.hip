@@ -963,11 +963,8 @@ void checkWeight(const char* where, const BlockWeightView& w, const float* bias)
 
 } // namespace
 
-std::size_t matmulBlocksWorkspace(std::uint32_t, std::uint32_t, std::uint32_t, DenseType) { return 0; }
-
 void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, DenseType type, std::uint64_t stride,
-                  std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, void*, std::size_t,
-                  hipStream_t stream) {
+                  std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, hipStream_t stream) {
     const char* where = "matmul blocks";
     checkColumns(where, inner);
     checkColumns(where, outer);
@@ -1018,10 +1015,8 @@ std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 25
 
 std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                   bool keep) {
-    std::size_t bytes = matmulBlocksWorkspace(rows, inner, outer, type);
-    if (!keep && !fusedTokens(rows, inner) && !rowsImage(rows, inner, outer, type))
-        bytes += rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
-    return bytes;
+    if (keep || fusedTokens(rows, inner) || rowsImage(rows, inner, outer, type)) return 0;
+    return rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
 }
 
 void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, std::uint64_t yStride, BlockRows keep,
@@ -1059,11 +1054,7 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
         return;
     }
     auto* spare = static_cast<std::uint8_t*>(workspace);
-    if (!keep.codes) {
-        keep = {spare, spare + rounded(rows * blockCodePitch(inner)), BlockCodes::e4m3};
-        const std::size_t used = rounded(rows * blockCodePitch(inner)) + rounded(rows * blockExponentPitch(inner));
-        spare += used, workspaceBytes -= used;
-    }
+    if (!keep.codes) keep = {spare, spare + rounded(rows * blockCodePitch(inner)), BlockCodes::e4m3};
     quantizeBlocks(x, keep, rows, inner, stream);
-    matmulBlocks(keep, w, bias, y, x.type, yStride, rows, inner, outer, spare, workspaceBytes, stream);
+    matmulBlocks(keep, w, bias, y, x.type, yStride, rows, inner, outer, stream);
 }

@@ -280,21 +280,13 @@ int tcc_quantize_weight_blocks(const void* w, uint64_t stride, uint32_t type, ui
     });
 }
 
-int tcc_matmul_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, size_t* bytes) {
-    return guarded([&] {
-        need(bytes, "workspace size");
-        *bytes = matmulBlocksWorkspace(rows, inner, outer, DenseType(type));
-    });
-}
-
 int tcc_matmul_blocks(const uint8_t* xCodes, const uint8_t* xExponents, const uint8_t* wCodes,
                       const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type,
-                      uint32_t rows, uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes,
-                      void* stream) {
+                      uint32_t rows, uint32_t inner, uint32_t outer, void* stream) {
     return guarded([&] {
         matmulBlocks({input(xCodes), input(xExponents), BlockCodes::e4m3},
                      {input(wCodes), input(wExponents), nullptr, nullptr}, bias, y, DenseType(type), stride, rows,
-                     inner, outer, workspace, workspaceBytes, static_cast<hipStream_t>(stream));
+                     inner, outer, static_cast<hipStream_t>(stream));
     });
 }
 

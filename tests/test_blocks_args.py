@@ -45,7 +45,7 @@ def test_product_refusals():
     from tcc_spmm_amd._lib import lib
     L = lib()
     matmul = lambda x=P, w=P, bias=None, y=P, stride=64, t=0, rows=100, k=128, n=64: L.tcc_matmul_blocks(  # noqa: E731
-        x, P, w, P, bias, y, stride, t, rows, k, n, None, 0, None)
+        x, P, w, P, bias, y, stride, t, rows, k, n, None)
     rejected(matmul(x=None), b"null codes")
     rejected(matmul(w=None), b"null codes")
     rejected(matmul(bias=P + 2), b"bias")
