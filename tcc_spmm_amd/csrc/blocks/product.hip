@@ -551,8 +551,10 @@ __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
 // takes it there once, as MFMA operands, and then each of its waves goes through rows of its own, 16 at a
 // time, without a barrier: dense x is read once, quantized in the layout of an operand, kept if asked for, and
 // multiplied with every column. Bound by HBM; what it saves against the tiles is writing and reading codes.
-// Measured, FP32: 2,449,029 x 128 -> 256 838 us, 4.5 TB/s; 262,144 x 256 -> 47 with x kept 87 us, 4.4 TB/s;
-// 262,144 x 47 -> 256 89, 3.6 TB/s, where rows of 188 bytes are read 16 at a time, 64 bytes of each.
+// Measured, FP32: 2,449,029 x 128 -> 256 804 us, 4.7 TB/s; 262,144 x 256 -> 47 with x kept 88 us, 4.4 TB/s;
+// 262,144 x 47 -> 256 83, 3.8 TB/s, where rows of 188 bytes are read 16 at a time, 64 bytes of each. Loads and stores
+// are ordinary ones: a row's lines come and go in two or more accesses, and nontemporal loads took 3 to 10% longer
+// (1,000,000 x 128 -> 128 255 us : 230), nontemporal stores up to 17% (1,000,000 x 128 -> 256 406 : 350).
 //
 // A lane reads 16 bytes of its row at a time, four lanes 64 bytes side by side. That gives it 32 elements of a
 // block in an order of their own; the order along the inner axis is free as long as both operands share it,
@@ -633,7 +635,7 @@ __global__ __launch_bounds__(512) void multiplyRows(Product a) {
                 const unsigned at = min(b * kBlock + (i * 4 + g) * Run, a.inner - Run);
                 raw[b][i] = RunVec{};
                 if (b + 1 < Blocks || b * kBlock + i * 4 * Run < a.inner)
-                    raw[b][i] = __builtin_nontemporal_load(reinterpret_cast<const LooseRun*>(x + at));
+                    raw[b][i] = *reinterpret_cast<const LooseRun*>(x + at);
             }
         __builtin_amdgcn_sched_barrier(0);
         if (a.inner != Blocks * kBlock) {
