@@ -75,8 +75,10 @@ void quantizeWeightBlocks(DenseMatrix w, BlockWeightView out, std::uint32_t oute
 // y = x w^T + bias for x in E4M3 blocks [rows][inner] and w in E4M3 tiles [outer][inner]; bias null or
 // FP32 [outer]. Called with the transposed weight it gives the input gradient from the output
 // gradient's blocks. Products of codes are exact. An FP32 y has its sums in FP32 (bf16 MFMA on the exact
-// values). For 16-bit types the 8-bit MFMA adds the 128 products of a block with about 17 bits below the
-// largest one (measured: 1.2e-5 of the sum's norm, a twentieth of an f16 rounding) and the blocks in FP32.
+// values). For 16-bit types the sums are the 8-bit MFMA's: of 8 consecutive products each is cut off, towards
+// zero, 13 bits below the power of two of the largest, and from there on sums are FP32's. So a sum is at most
+// 7 * 2^-13 of its terms' magnitudes off; on random numbers 1.2e-5 of the sums' norm, a twentieth of an f16
+// rounding, which shows as a last place here and there. Who needs FP32 sums in 16 bits takes an FP32 y and rounds it.
 void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, DenseType type,
                   std::uint64_t stride, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
                   hipStream_t stream = nullptr);

@@ -125,7 +125,8 @@ __device__ __forceinline__ unsigned tileOf(unsigned id, unsigned total, unsigned
 }
 
 // ------------------------------------------------------------------------------------------------
-// 16-bit outputs: the scaled 8-bit MFMA on tiles of BM x BN.
+// 16-bit outputs: the scaled 8-bit MFMA on tiles of BM x BN. Its sums, here and in the kernels below, are those that
+// include/blocks.h states for 16-bit types: fewer bits than FP32's within eight products, at twice the bf16 MFMA's rate.
 //
 // A block of 128 along the inner axis is one step: 128 bytes of each of the tile's rows, loaded to LDS
 // without passing registers, Stages deep. The 16-byte chunks of a row are stored in an order that
@@ -462,8 +463,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 // FP32 outputs: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
 // 128 x 128, steps of half a block: a row's 64 values are 128 bytes of LDS, stored in the chunk order of
 // the 8-bit kernel. Codes pass through registers to be converted, in every tile anew, which with the bf16 MFMA's
-// half rate bounds it: 4096 x 4096 x 8192 367 us, 0.75 PFLOP/s (a library's product in FP32 0.15). The 8-bit MFMA adds
-// its 128 products with about 17 bits, 1.2e-5 of the sum off, which 16-bit outputs hide and FP32 ones would show.
+// half rate bounds it: 4096 x 4096 x 8192 367 us, 0.75 PFLOP/s (a library's product in FP32 0.15). The 8-bit MFMA cuts
+// products off 13 bits below the largest of eight, 1.2e-5 of the sum off on random numbers, which a 16-bit output's
+// rounding is twenty times as large as and an FP32 one's far smaller.
 __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
     constexpr unsigned B = 128;
     __shared__ __align__(1024) std::uint8_t lds[2][2][B * 128];
