@@ -74,8 +74,10 @@ void quantizeWeightBlocks(DenseMatrix w, BlockWeightView out, std::uint32_t oute
 
 // y = x w^T + bias for x in E4M3 blocks [rows][inner] and w in E4M3 tiles [outer][inner]; bias null or
 // FP32 [outer]. Called with the transposed weight it gives the input gradient from the output
-// gradient's blocks. Products of codes are exact. An FP32 y has its sums in FP32 (bf16 MFMA on the exact
-// values). For 16-bit types the sums are the 8-bit MFMA's: of 8 consecutive products each is cut off, towards
+// gradient's blocks. An FP32 y has its sums in FP32, through the bf16 MFMA on the codes' values. Those are exact for
+// exponents of 3 to 246; below, a value is rounded to a multiple of 2^-133, bf16's last, and one of 2^128 or more, which
+// FP32 rows never give, is infinite (as in dequantizeBlocks). For 16-bit types products of codes are exact at every
+// exponent, and the sums are the 8-bit MFMA's: of 8 consecutive products each is cut off, towards
 // zero, 13 bits below the power of two of the largest, and from there on sums are FP32's. So a sum is at most
 // 7 * 2^-13 of its terms' magnitudes off; on random numbers 1.2e-5 of the sums' norm, a twentieth of an f16
 // rounding, which shows as a last place here and there. Who needs FP32 sums in 16 bits takes an FP32 y and rounds it.
@@ -93,8 +95,9 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
                   void* workspace, std::size_t workspaceBytes, hipStream_t stream = nullptr);
 
 // dw = dy^T x for dense dy [rows][outer] and x's E4M3 blocks [rows][inner], FP32 [outer][inner]
-// contiguous, and, if db is not null, db = the sums of dy's columns. All sums in FP32; a dy of f16 or f32
-// goes through the bf16 MFMA as two or three bf16 parts, which together hold it exactly (FP32: to 2^-25).
+// contiguous, and, if db is not null, db = the sums of dy's columns. All sums in FP32, of x's values as in an FP32 y of
+// matmulBlocks; a dy of f16 or f32 goes through the bf16 MFMA as two or three bf16 parts, which together hold it exactly
+// (FP32: to 2^-25 of it, or 2^-134 where that is more).
 // Repeated calls give the same bits. Zero rows give zero gradients.
 std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
                                       DenseType type);

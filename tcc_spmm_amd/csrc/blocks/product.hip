@@ -28,7 +28,8 @@ __device__ __forceinline__ i32x8 join(u32x4 p, u32x4 q) {
     return i32x8{int(p.x), int(p.y), int(p.z), int(p.w), int(q.x), int(q.y), int(q.z), int(q.w)};
 }
 
-// The values of 8 E4M3 codes as bf16, exact: the conversion multiplies by the scale's power of two.
+// The values of 8 E4M3 codes as bf16: the conversion multiplies by the scale's power of two. Exact but for the ends of
+// the range: multiples of 2^-134 and less (exponents below 3) are rounded, values of 2^128 and more infinite.
 __device__ __forceinline__ bf16x8 values8(unsigned lo, unsigned hi, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
     const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 }
 
 // ------------------------------------------------------------------------------------------------
-// FP32 outputs: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
+// FP32 outputs: the codes' values, exact in bf16 (values8), through the bf16 MFMA, whose sums are FP32's. Tiles of
 // 128 x 128, steps of half a block: a row's 64 values are 128 bytes of LDS, stored in the chunk order of
 // the 8-bit kernel. Codes pass through registers to be converted, in every tile anew, which with the bf16 MFMA's
 // half rate bounds it: 4096 x 4096 x 8192 367 us, 0.75 PFLOP/s (a library's product in FP32 0.15). The 8-bit MFMA cuts

@@ -3,7 +3,8 @@
 //
 // Both operands run along the rows, the axis of the sum, so an MFMA operand is a column of each: 64 rows
 // of a tile lie in LDS as they do in memory and are read with the transposing LDS load. x is converted to
-// bf16 on its way into LDS, exactly, its scales multiplied in. dy goes in as bf16 parts: itself, or for f16 two
+// bf16 on its way into LDS, its scales multiplied in, exactly for exponents of 3 to 246 (below, bf16's last
+// place is 2^-133; above, values end at 2^128). dy goes in as bf16 parts: itself, or for f16 two
 // and for f32 three parts of 8 bits each, every part the rest's nearest bf16; their products with x add
 // in the same FP32 accumulator, so an f32 gradient keeps its precision at three times the MFMA work.
 // The bias gradient is the product of dy with a column of ones, an operand that needs no memory.

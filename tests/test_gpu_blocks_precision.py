@@ -57,3 +57,55 @@ def test_random_sums_differ_from_fp32_ones_by_few_roundings(gpu, rows, inner, ou
     off = (y.float() - exact.to(DTYPES[dtype]).float()).norm() / exact.norm()
     assert float(off) <= np.sqrt(2.4e-5 * 2 * ROUNDING[dtype])
     assert torch.equal(y, matmul_blocks(x, weight, dtype=DTYPES[dtype])), "repeated calls give the same bits"
+
+
+# Codes of every kind: subnormal ones, an odd one among them, the smallest normal one, the largest.
+KINDS = np.array([2.0 ** -9, 3 * 2.0 ** -9, 7 * 2.0 ** -9, 2.0 ** -6, 1.0, 1.875, 240.0, 448.0])
+
+
+def in_bf16(v):
+    return torch.from_numpy(v).float().bfloat16().double().numpy()
+
+
+@pytest.mark.parametrize("e", [0, 1, 2, 3, 4, 127, 245, 246, 247, 248, 254])
+@pytest.mark.parametrize("rows,outer", [(8, 40), (600, 600)])
+def test_values_at_the_ends_of_the_range(gpu, rows, outer, e):
+    """One product a sum, so that it shows what a code and its exponent stand for: in a 16-bit output always the value,
+    in an FP32 output and in the weight gradient the value as bf16 has it, which is the same for exponents of 3 to 246."""
+    from tcc_spmm_amd.blocks import matmul_blocks, weight_grad_blocks
+    f = min(max(254 - e, 30), 220)  # brings the products back to the middle of the range
+    value, factor = KINDS * 2.0 ** (e - 127), 2.0 ** (f - 127)
+    if 3 <= e <= 246:
+        assert np.array_equal(in_bf16(value), value)
+    one, kinds = np.zeros((outer, 128)), np.zeros((rows, 128))
+    one[:, 0], kinds[:8, 0] = 1.0, KINDS
+    x, w = given(kinds, [e]), given(one, [f], weight=True)
+    assert np.array_equal(f64(matmul_blocks(x, w, dtype=torch.bfloat16))[:8, 0], value * factor)
+    assert np.array_equal(f64(matmul_blocks(x, w, dtype=torch.float32))[:8, 0], in_bf16(value) * factor)
+    # the same codes in the weight
+    one, kinds = np.zeros((rows, 128)), np.zeros((outer, 128))
+    one[:, 0], kinds[:8, 0] = 1.0, KINDS
+    y = matmul_blocks(given(one, [f]), given(kinds, [e], weight=True), dtype=torch.float32)
+    assert np.array_equal(f64(y)[0, :8], in_bf16(value) * factor)
+    if e > 246:  # an infinite value of another row makes the sum NaN
+        return
+    factor = 2.0 ** (100 if e < 100 else -100 if e > 200 else 0)
+    for dtype in (torch.float32, torch.bfloat16):
+        for columns in (outer, outer + 1):
+            dy = torch.zeros((rows, columns), device="cuda", dtype=dtype)
+            dy[torch.arange(8), torch.arange(8)] = factor
+            assert np.array_equal(f64(weight_grad_blocks(dy, x)[0])[:8, 0], in_bf16(value) * factor)
+
+
+@pytest.mark.parametrize("rows", [3, 40, 500, 9000])
+def test_rows_near_the_smallest_numbers(gpu, rows):
+    """FP32 rows whose blocks have the least exponents, through a layer: bf16 keeps a value to 2^-134."""
+    from tcc_spmm_amd.blocks import linear_blocks, quantize_blocks
+    x = torch.zeros((rows, 128), device="cuda")
+    x[:, 0], x[:, 1] = 2.0 ** -118, 3 * 2.0 ** -135
+    kept = quantize_blocks(x)
+    assert (kept.exponents[:, 0] == 1).all() and np.array_equal(f64(kept.dequantize()), f64(x))
+    w = np.zeros((64, 128))
+    w[:, 1] = 1.0
+    y = linear_blocks(x, given(w, [227], weight=True))
+    assert np.array_equal(f64(y), np.full((rows, 64), in_bf16(np.array(3 * 2.0 ** -135)) * 2.0 ** 100))
