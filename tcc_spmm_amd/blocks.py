@@ -446,11 +446,17 @@ class _Activation(torch.autograd.Function):
 def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """x w^T + bias with both operands in E4M3 blocks, differentiable; w is the master weight, quantized
     in every call."""
+    if not torch.is_grad_enabled():
+        # Inside a Function the mode is off and its arguments still say that they require a gradient.
+        weight = quantize_weight_blocks(w, transposed=False)
+        return linear_blocks(x, weight, None if bias is None else bias.float())
     return _Linear.apply(x, w, bias)
 
 
 def block_activation(x: torch.Tensor, kind: str = "silu", *, gated: bool = False, codes=INT8) -> torch.Tensor:
     """activation_blocks, differentiable: what autograd keeps of x is its blocks."""
+    if not torch.is_grad_enabled():
+        return activation_blocks(x, kind, gated=gated, codes=None)[0]
     return _Activation.apply(x, kind, gated, codes)
 
 

@@ -1,0 +1,47 @@
+"""What block_linear, block_activation and BlockLinear do, and leave out, in the modes that torch calls them in."""
+import pytest
+import torch
+
+from test_gpu_blocks import random
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(function, what it keeps or makes besides the result) of each call that the layers make."""
+    from tcc_spmm_amd import blocks as B
+    seen = []
+    linear, activation, quantize = B.linear_blocks, B.activation_blocks, B.quantize_weight_blocks
+
+    def see_linear(*args, keep=False, **more):
+        seen.append(("linear", keep))
+        return linear(*args, keep=keep, **more)
+
+    def see_activation(*args, codes=B.INT8, **more):
+        seen.append(("activation", codes is not None))
+        return activation(*args, codes=codes, **more)
+
+    def see_quantize(w, transposed=True, **more):
+        seen.append(("weight", transposed))
+        return quantize(w, transposed, **more)
+
+    monkeypatch.setattr(B, "linear_blocks", see_linear)
+    monkeypatch.setattr(B, "activation_blocks", see_activation)
+    monkeypatch.setattr(B, "quantize_weight_blocks", see_quantize)
+    return seen
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_nothing_is_kept_without_gradients(gpu, calls, mode):
+    from tcc_spmm_amd import blocks as B
+    layer, x = B.BlockLinear(100, 64).cuda(), random((300, 100), 1).requires_grad_()
+    want = layer(x)
+    act = B.block_activation(want, "silu")
+    assert calls == [("weight", True), ("linear", True), ("activation", True)]
+    calls.clear()
+    with mode():
+        y = layer(x)
+        a = B.block_activation(y.clone().requires_grad_() if mode is torch.no_grad else y, "silu")
+    assert torch.equal(y, want) and torch.equal(a, act)
+    assert calls == [("weight", False), ("linear", False), ("activation", False)]
