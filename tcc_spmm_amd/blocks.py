@@ -454,9 +454,12 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
 
 
 def block_activation(x: torch.Tensor, kind: str = "silu", *, gated: bool = False, codes=INT8) -> torch.Tensor:
-    """activation_blocks, differentiable: what autograd keeps of x is its blocks."""
+    """activation_blocks, differentiable: what autograd keeps of x is its blocks, so codes=None is for inputs that
+    need no gradient."""
     if not torch.is_grad_enabled():
         return activation_blocks(x, kind, gated=gated, codes=None)[0]
+    if codes is None and x.requires_grad:
+        raise ValueError("x requires a gradient, which codes=None keeps nothing for")
     return _Activation.apply(x, kind, gated, codes)
 
 

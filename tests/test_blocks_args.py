@@ -131,3 +131,12 @@ def test_torch_side_refusals_need_no_gpu():
             make()
     with pytest.raises(ValueError, match="CUDA"):
         B.quantize_blocks(x)
+
+
+def test_an_activation_that_keeps_nothing_has_no_gradient():
+    """Said by the call itself, not by an error in its backward pass."""
+    from tcc_spmm_amd import blocks as B
+    with pytest.raises(ValueError, match="requires a gradient"):
+        B.block_activation(torch.zeros((4, 128), requires_grad=True), codes=None)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing to say against the call itself
+        B.block_activation(torch.zeros((4, 128), requires_grad=True), codes=None)

@@ -45,3 +45,9 @@ def test_nothing_is_kept_without_gradients(gpu, calls, mode):
         a = B.block_activation(y.clone().requires_grad_() if mode is torch.no_grad else y, "silu")
     assert torch.equal(y, want) and torch.equal(a, act)
     assert calls == [("weight", False), ("linear", False), ("activation", False)]
+
+
+def test_an_activation_without_gradient_may_keep_nothing(gpu):
+    from tcc_spmm_amd import blocks as B
+    x = random((20, 64), 1)
+    assert torch.equal(B.block_activation(x, "gelu", codes=None), B.activation_blocks(x, "gelu")[0])
