@@ -397,13 +397,18 @@ def activation_blocks_backward(dy: torch.Tensor, kept: BlockTensor, kind: str = 
 # Under autograd
 
 
+def _float_bias(bias):
+    """A bias of any type and layout as the products take it."""
+    return None if bias is None else bias.float().contiguous()
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias):
         grad_x, grad_w, grad_b = ctx.needs_input_grad
         weight = quantize_weight_blocks(w, transposed=grad_x)
         keep = grad_w or grad_b
-        out = linear_blocks(x, weight, None if bias is None else bias.float(), keep=keep)
+        out = linear_blocks(x, weight, _float_bias(bias), keep=keep)
         y, kept = out if keep else (out, None)
         # x itself is not saved: the weight gradient reads its blocks, a byte an element.
         ctx.save_for_backward(*((kept.codes, kept.exponents) if keep else (None, None)),
@@ -449,7 +454,7 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if not torch.is_grad_enabled():
         # Inside a Function the mode is off and its arguments still say that they require a gradient.
         weight = quantize_weight_blocks(w, transposed=False)
-        return linear_blocks(x, weight, None if bias is None else bias.float())
+        return linear_blocks(x, weight, _float_bias(bias))
     return _Linear.apply(x, w, bias)
 
 
@@ -471,5 +476,5 @@ class BlockLinear(torch.nn.Linear):
 
     def serving(self):
         """(BlockWeight, float32 bias or None) for linear_blocks, quantized once."""
-        bias = None if self.bias is None else self.bias.detach().float()
-        return quantize_weight_blocks(self.weight.detach(), transposed=False), bias
+        bias = None if self.bias is None else self.bias.detach()
+        return quantize_weight_blocks(self.weight.detach(), transposed=False), _float_bias(bias)

@@ -51,3 +51,25 @@ def test_an_activation_without_gradient_may_keep_nothing(gpu):
     from tcc_spmm_amd import blocks as B
     x = random((20, 64), 1)
     assert torch.equal(B.block_activation(x, "gelu", codes=None), B.activation_blocks(x, "gelu")[0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bias_of_any_layout(gpu, dtype):
+    """A column of a wider tensor and one number for all, with their gradients."""
+    from tcc_spmm_amd import blocks as B
+    x, w, dy = random((30, 70), 1), random((40, 70), 2), random((30, 40), 3)
+    for make in (lambda t: t[:, 1], lambda t: t[0, :1].expand(40)):
+        base = random((40, 3), 4, dtype).requires_grad_()
+        plain = make(base.detach().clone()).contiguous().requires_grad_()
+        want, got = B.block_linear(x, w, plain), B.block_linear(x, w, make(base))
+        assert torch.equal(got, want)
+        with torch.no_grad():
+            assert torch.equal(B.block_linear(x, w, make(base)), want)
+        got.backward(dy)
+        want.backward(dy)
+        grad = torch.zeros_like(base)
+        if make(base).stride(0):
+            grad[:, 1] = plain.grad
+        else:
+            grad[0, 0] = plain.grad.sum()
+        assert torch.equal(base.grad, grad)
