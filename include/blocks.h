@@ -98,7 +98,8 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
 // contiguous, and, if db is not null, db = the sums of dy's columns. All sums in FP32, of x's values as in an FP32 y of
 // matmulBlocks; a dy of f16 or f32 goes through the bf16 MFMA as two or three bf16 parts, which together hold it exactly
 // (FP32: to 2^-25 of it, or 2^-134 where that is more).
-// Repeated calls give the same bits. Zero rows give zero gradients.
+// Repeated calls give the same bits. Zero rows give zero gradients. A null dw asks for db alone: neither x nor inner is
+// read, and the workspace is that of inner = 0.
 std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
                                       DenseType type);
 void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::uint32_t rows,

@@ -143,7 +143,7 @@ int tcc_linear_blocks(const void* x, uint64_t stride, uint32_t type, const uint8
                       void* workspace, size_t workspaceBytes, void* stream);
 int tcc_weight_grad_blocks_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type,
                                      size_t* bytes);
-/* db may be null. */
+/* db may be null, or dw: x and inner are not read then, and the workspace is that of inner = 0. */
 int tcc_weight_grad_blocks(const void* dy, uint64_t stride, uint32_t type, const uint8_t* xCodes,
                            const uint8_t* xExponents, float* dw, float* db, uint32_t rows, uint32_t inner,
                            uint32_t outer, void* workspace, size_t workspaceBytes, void* stream);

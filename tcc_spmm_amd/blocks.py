@@ -299,41 +299,48 @@ def linear_blocks(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | Non
     return (y, kept) if keep else y
 
 
-def weight_grad_blocks(dy: torch.Tensor, x: BlockTensor, bias: bool = True, stream=None):
+def weight_grad_blocks(dy: torch.Tensor, x: BlockTensor | None, bias: bool = True, stream=None):
     """weightGradBlocks: (dw float32 [outer, inner], db float32 [outer] or None) from the output gradient
-    [..., outer] and the forward pass's kept blocks."""
+    [..., outer] and the forward pass's kept blocks; without them (None, db)."""
     _dense(dy, "dy")
-    if x.codes.dtype != E4M3:
-        raise ValueError("x must have float8_e4m3fn codes")
     device, outer = dy.device, dy.shape[-1]
-    _same_device(device, x.codes)
-    if dy.numel() != x.rows * outer:
-        raise ValueError(f"dy has {dy.numel() // outer} rows, the kept blocks {x.rows}")
+    rows = dy.numel() // outer
+    if x is None:
+        if not bias:
+            raise ValueError("neither a weight's nor a bias's gradient is asked for")
+    else:
+        if x.codes.dtype != E4M3:
+            raise ValueError("x must have float8_e4m3fn codes")
+        _same_device(device, x.codes)
+        if rows != x.rows:
+            raise ValueError(f"dy has {rows} rows, the kept blocks {x.rows}")
     away = _away(device, stream)
     if away:
         with away:
             return weight_grad_blocks(dy, x, bias)
     dy = _rows(dy)
-    dw = torch.empty((outer, x.columns), dtype=torch.float32, device=device)
+    inner = 0 if x is None else x.columns
+    dw = None if x is None else torch.empty((outer, inner), dtype=torch.float32, device=device)
     db = torch.empty(outer, dtype=torch.float32, device=device) if bias else None
-    sizes = (x.rows, x.columns, outer, _TYPES[dy.dtype])
+    sizes = (rows, inner, outer, _TYPES[dy.dtype])
     _space, at, size = _workspace(lib().tcc_weight_grad_blocks_workspace, sizes, device)
-    check(lib().tcc_weight_grad_blocks(dy.data_ptr(), _stride(dy), sizes[3], x.codes.data_ptr(),
-                                       x.exponents.data_ptr(), dw.data_ptr(), db.data_ptr() if bias else 0,
-                                       x.rows, x.columns, outer, at, size, _stream(device.index)))
+    check(lib().tcc_weight_grad_blocks(dy.data_ptr(), _stride(dy), sizes[3], x.codes.data_ptr() if x else 0,
+                                       x.exponents.data_ptr() if x else 0, dw.data_ptr() if x else 0,
+                                       db.data_ptr() if bias else 0, rows, inner, outer, at, size,
+                                       _stream(device.index)))
     return dw, db
 
 
 def linear_blocks_backward(dy: torch.Tensor, kept: BlockTensor | None, weight: BlockWeight | None, *,
                            need=(True, True, True), stream=None):
     """(dx, dw, db) of linear_blocks, None for what `need` leaves out. dx = Q(dy) weight in dy's type, from the
-    weight's transposed copy; dw and db are float32, from the kept blocks and dy in full."""
+    weight's transposed copy; dw and db are float32, dw from the kept blocks and dy in full, db from dy."""
     dx = dw = db = None
     if need[0]:
         dx = linear_blocks(dy, weight.transposed(), stream=stream)
     if need[1] or need[2]:
-        dw, db = weight_grad_blocks(dy, kept, bias=bool(need[2]), stream=stream)
-    return dx, dw if need[1] else None, db
+        dw, db = weight_grad_blocks(dy, kept if need[1] else None, bias=bool(need[2]), stream=stream)
+    return dx, dw, db
 
 
 def _activation(kind: str) -> int:
@@ -405,13 +412,12 @@ def _float_bias(bias):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias):
-        grad_x, grad_w, grad_b = ctx.needs_input_grad
+        grad_x, grad_w, _ = ctx.needs_input_grad
         weight = quantize_weight_blocks(w, transposed=grad_x)
-        keep = grad_w or grad_b
-        out = linear_blocks(x, weight, _float_bias(bias), keep=keep)
-        y, kept = out if keep else (out, None)
-        # x itself is not saved: the weight gradient reads its blocks, a byte an element.
-        ctx.save_for_backward(*((kept.codes, kept.exponents) if keep else (None, None)),
+        out = linear_blocks(x, weight, _float_bias(bias), keep=grad_w)
+        y, kept = out if grad_w else (out, None)
+        # x itself is not saved: the weight gradient reads its blocks, a byte an element, and nothing else does.
+        ctx.save_for_backward(*((kept.codes, kept.exponents) if grad_w else (None, None)),
                               *((weight.codes_t, weight.exponents_t) if grad_x else (None, None)))
         ctx.shape, ctx.types = w.shape, (w.dtype, None if bias is None else bias.dtype)
         return y
@@ -424,9 +430,10 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         if codes_t is not None:
             dx = linear_blocks(dy, BlockWeight(codes_t, exponents_t, outer))
-        if codes is not None:
-            dw, db = weight_grad_blocks(dy, BlockTensor(codes, exponents, inner), bias=ctx.needs_input_grad[2])
-            dw = dw.to(ctx.types[0]) if ctx.needs_input_grad[1] else None
+        if codes is not None or ctx.needs_input_grad[2]:
+            kept = None if codes is None else BlockTensor(codes, exponents, inner)
+            dw, db = weight_grad_blocks(dy, kept, bias=ctx.needs_input_grad[2])
+            dw = None if dw is None else dw.to(ctx.types[0])
             db = None if db is None else db.to(ctx.types[1])
         return dx, dw, db
 

@@ -534,6 +534,9 @@ bool alignedRows(const DenseMatrix& dy, std::uint32_t outer) {
            outer % 8 == 0 && dy.stride < (1u << 23);
 }
 
+// The bias gradient alone is a weight gradient of no columns, whose one column of tiles has nothing else to store.
+unsigned tilesOf(std::uint32_t n, unsigned size) { return n ? (n + size - 1) / size : 1; }
+
 std::uint64_t rounded4(std::uint64_t n) { return (n + 3) / 4 * 4; }
 std::uint64_t pitchOf(std::uint32_t inner, std::uint32_t outer) {
     return rounded4(std::uint64_t(outer) * inner) + rounded4(outer);
@@ -544,7 +547,7 @@ std::uint64_t pitchOf(std::uint32_t inner, std::uint32_t outer) {
 // a step of a workgroup that has its CU to itself and of one that shares it with perUnit - 1 others.
 double planTime(Plan& p, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, double alone, double shared,
                 unsigned perUnit) {
-    const std::uint64_t tiles = std::uint64_t((inner + p.bk - 1) / p.bk) * ((outer + p.bn - 1) / p.bn);
+    const std::uint64_t tiles = tilesOf(inner, p.bk) * std::uint64_t(tilesOf(outer, p.bn));
     const std::uint64_t steps = std::max<std::uint64_t>(1, (std::uint64_t(rows) + kStep - 1) / kStep);
     double best = 1e30;
     auto consider = [&](std::uint64_t splits) {
@@ -586,7 +589,7 @@ void launchSum(const Gradient& a, std::uint64_t blocks, hipStream_t stream) {
 } // namespace
 
 std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
-    if (!rows || !inner || !outer) return 0;
+    if (!rows || !outer) return 0;
     // The larger of the two forms' needs: which one runs depends on dy's alignment.
     std::uint64_t splits = planOf(rows, inner, outer, type, false).splits;
     if (type == DenseType::bf16) splits = std::max<std::uint64_t>(splits, planOf(rows, inner, outer, type, true).splits);
@@ -596,17 +599,18 @@ std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, s
 void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::uint32_t rows, std::uint32_t inner,
                       std::uint32_t outer, void* workspace, std::size_t workspaceBytes, hipStream_t stream) {
     const char* where = "weight gradient";
-    checkColumns(where, inner);
+    if (!dw && db) inner = 0, x = {nullptr, nullptr, BlockCodes::e4m3};
+    if (dw) checkColumns(where, inner);
     checkColumns(where, outer);
     checkRows(where, rows);
     checkType(where, dy.type);
     if (x.type != BlockCodes::e4m3) reject(where, "x must have E4M3 codes");
-    if (!dw) reject(where, "null weight gradient");
+    if (!dw && !db) reject(where, "null weight gradient");
     if (reinterpret_cast<std::uintptr_t>(dw) % 4 || reinterpret_cast<std::uintptr_t>(db) % 4)
         reject(where, "gradients must be float-aligned");
     if (rows) {
         checkDense(where, dy.data, dy.stride, dy.type, outer);
-        checkCodes(where, x.codes, x.exponents);
+        if (dw) checkCodes(where, x.codes, x.exponents);
     }
     const std::size_t need = weightGradBlocksWorkspace(rows, inner, outer, dy.type);
     if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
@@ -618,7 +622,7 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     a.dy = dy.data, a.dyStride = dy.stride, a.x = x.codes, a.xe = x.exponents;
     a.rows = rows, a.outer = outer, a.inner = inner;
     a.codePitch = unsigned(blockCodePitch(inner)), a.expPitch = unsigned(blockExponentPitch(inner));
-    a.tilesN = (outer + p.bn - 1) / p.bn, a.tilesK = (inner + p.bk - 1) / p.bk;
+    a.tilesN = tilesOf(outer, p.bn), a.tilesK = tilesOf(inner, p.bk);
     a.rowsPerSplit = p.steps * kStep;
     a.dw = p.splits == 1 ? dw : parts;
     a.db = !db ? nullptr : p.splits == 1 ? db : parts + rounded4(size);

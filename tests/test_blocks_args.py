@@ -140,3 +140,23 @@ def test_an_activation_that_keeps_nothing_has_no_gradient():
         B.block_activation(torch.zeros((4, 128), requires_grad=True), codes=None)
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing to say against the call itself
         B.block_activation(torch.zeros((4, 128), requires_grad=True), codes=None)
+
+
+def test_a_bias_gradient_needs_no_blocks():
+    """Without dw nothing of x is looked at, and the workspace is for db alone."""
+    from tcc_spmm_amd._lib import lib
+    from tcc_spmm_amd import blocks as B
+    L = lib()
+    whole, alone = ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tcc_weight_grad_blocks_workspace(1000000, 128, 256, 1, ctypes.byref(whole)) == 0
+    assert L.tcc_weight_grad_blocks_workspace(1000000, 0, 256, 1, ctypes.byref(alone)) == 0
+    assert 0 < alone.value < whole.value / 16
+    call = lambda dy=P, x=None, dw=None, db=P, k=0, n=alone.value: L.tcc_weight_grad_blocks(  # noqa: E731
+        dy, 256, 1, x, x, dw, db, 1000000, k, 256, P, n, None)
+    rejected(call(dy=None), b"null dense")
+    rejected(call(db=None), b"null weight gradient")
+    rejected(call(n=alone.value - 1), b"workspace too small")
+    rejected(call(dw=P), b"zero elements")  # a weight gradient of no columns
+    rejected(call(dw=P, k=128), b"null codes")
+    with pytest.raises(ValueError, match="asked for"):
+        B.weight_grad_blocks(torch.zeros((4, 128)), None, bias=False)

@@ -1,8 +1,10 @@
 """What block_linear, block_activation and BlockLinear do, and leave out, in the modes that torch calls them in."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_blocks import random
+from blocks_oracle import f64
+from test_gpu_blocks import U, cut, near, random
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +75,42 @@ def test_bias_of_any_layout(gpu, dtype):
         else:
             grad[0, 0] = plain.grad.sum()
         assert torch.equal(base.grad, grad)
+
+
+@pytest.mark.parametrize("rows,outer", [(0, 40), (1, 1), (7, 5), (300, 47), (65, 128), (1000, 129), (5003, 520), (40000, 64),
+                                        (9000, 4104)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_bias_gradient_alone(gpu, rows, outer, dtype):
+    """Sums of n numbers through the MFMA, which adds at least four at once, in a few splits: (n / 4 + 64) roundings of
+    2^-24 of the magnitudes' sum. NaN beside a slice and in the other columns stays there."""
+    from tcc_spmm_amd.blocks import linear_blocks_backward, weight_grad_blocks
+    dy = random((rows, outer), 1, dtype)
+    want, terms = f64(dy).sum(0), np.abs(f64(dy)).sum(0)
+    for d in (dy, cut(dy)):
+        dw, db = weight_grad_blocks(d, None)
+        assert dw is None
+        near(db, want, (rows / 4 + 64) * U * terms, "db")
+        assert torch.equal(db, weight_grad_blocks(d, None)[1]), "repeated calls give the same bits"
+        assert torch.equal(linear_blocks_backward(d, None, None, need=(False, False, True))[2], db)
+    if rows and outer > 1:
+        dy[0, 1] = float("nan")
+        bad = weight_grad_blocks(dy, None)[1]
+        assert bad[1].isnan() and bad.isnan().sum() == 1
+
+
+def test_a_frozen_weight_keeps_nothing_of_its_input(gpu, calls):
+    from tcc_spmm_amd import blocks as B
+    layer, x, dy = B.BlockLinear(100, 64).cuda(), random((300, 100), 1), random((300, 64), 2)
+    layer(x).backward(dy)
+    want = layer.bias.grad.clone()
+    layer.zero_grad()
+    layer.weight.requires_grad_(False)
+    calls.clear()
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t) or t, lambda t: t):
+        y = layer(x)
+    assert calls == [("weight", False), ("linear", False)] and not saved
+    y.backward(dy)
+    # Both are FP32 sums of the same 300 numbers, in an order of their own.
+    assert layer.weight.grad is None
+    assert ((layer.bias.grad - want).abs() <= 2 * (300 / 4 + 64) * U * dy.abs().sum(0)).all()
