@@ -457,7 +457,10 @@ class _Activation(torch.autograd.Function):
 
 def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """x w^T + bias with both operands in E4M3 blocks, differentiable; w is the master weight, quantized
-    in every call."""
+    in every call. Under autocast x is cast to its type first, as torch's linear casts it; w is quantized and the bias
+    added at their own precision."""
+    if x.dtype in _TYPES and torch.is_autocast_enabled(x.device.type):
+        x = x.to(torch.get_autocast_dtype(x.device.type))
     if not torch.is_grad_enabled():
         # Inside a Function the mode is off and its arguments still say that they require a gradient.
         weight = quantize_weight_blocks(w, transposed=False)

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from blocks_oracle import f64
+from blocks_oracle import DTYPES, f64
 from test_gpu_blocks import U, cut, near, random
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +114,32 @@ def test_a_frozen_weight_keeps_nothing_of_its_input(gpu, calls):
     # Both are FP32 sums of the same 300 numbers, in an order of their own.
     assert layer.weight.grad is None
     assert ((layer.bias.grad - want).abs() <= 2 * (300 / 4 + 64) * U * dy.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("autocast", ["bf16", "f16"])
+def test_under_autocast(gpu, autocast):
+    """FP32 rows go through the layers in autocast's type, there and back; parameters and x have gradients of their own
+    type; within a disabled region nothing is cast."""
+    from tcc_spmm_amd import blocks as B
+    layer, x = B.BlockLinear(100, 128).cuda(), random((300, 100), 1).requires_grad_()
+    dy = random((300, 64), 2, autocast)
+
+    def step(x):
+        y = B.block_activation(layer(x), "silu", gated=True)
+        assert y.dtype == DTYPES[autocast]
+        y.backward(dy)
+        grads = [p.grad.clone() for p in layer.parameters()]
+        layer.zero_grad()
+        return y, grads
+
+    half = x.detach().to(DTYPES[autocast]).requires_grad_()
+    want, want_grads = step(half)
+    with torch.autocast("cuda", DTYPES[autocast]):
+        got, grads = step(x)
+        with torch.no_grad():
+            assert layer(x).dtype == DTYPES[autocast]
+        with torch.autocast("cuda", enabled=False):
+            assert layer(x).dtype == torch.float32
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+    assert x.grad.dtype == torch.float32 and torch.equal(x.grad, half.grad.float())
+    assert layer(x).dtype == torch.float32
