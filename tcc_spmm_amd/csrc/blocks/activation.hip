@@ -58,7 +58,7 @@ __device__ __forceinline__ void keepBlock(const Call& a, std::uint64_t row, unsi
 template <typename T, BlockCodes C, BlockActivation F, bool Gated>
 __global__ __launch_bounds__(kThreads) void activateBlocks(Call a) {
     const unsigned lane = threadIdx.x % kBlockLanes;
-    const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
+    const unsigned item = flatGroup() * kGroups + threadIdx.x / kBlockLanes;
     if (item >= a.items) return;
     const unsigned row = rowOf(item, a.count, a.magic), block = item - row * a.count;
     const unsigned at = block * kBlock;
@@ -91,7 +91,7 @@ __device__ __forceinline__ void keptBlock(const Call& a, std::uint64_t row, unsi
 template <typename T, BlockCodes C, BlockActivation F, bool Gated>
 __global__ __launch_bounds__(kThreads) void activateBlocksBackward(Call a) {
     const unsigned lane = threadIdx.x % kBlockLanes;
-    const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
+    const unsigned item = flatGroup() * kGroups + threadIdx.x / kBlockLanes;
     if (item >= a.items) return;
     const unsigned row = rowOf(item, a.count, a.magic), block = item - row * a.count;
     const unsigned at = block * kBlock;
@@ -154,7 +154,7 @@ void activationBlocks(DenseMatrix x, BlockActivation f, bool gated, void* y, std
     Call a = {};
     if (!setUp("activation blocks", a, y, yStride, x.data, x.stride, x.type, keep, false, f, gated, rows, width)) return;
     a.in = x.data, a.inStride = x.stride, a.out = y, a.outStride = yStride;
-    const dim3 grid((a.items + kGroups - 1) / kGroups), threads(kThreads);
+    const dim3 grid = flatGrid((a.items + kGroups - 1) / kGroups), threads(kThreads);
     withType(x.type, [&](auto tag) {
         withCodes(keep.type, [&](auto codes) {
             withActivation(f, [&](auto kind) {
@@ -178,7 +178,7 @@ void activationBlocksBackward(DenseMatrix dy, BlockRows kept, BlockActivation f,
                width))
         return;
     a.in = dy.data, a.inStride = dy.stride, a.out = dx, a.outStride = dxStride;
-    const dim3 grid((a.items + kGroups - 1) / kGroups), threads(kThreads);
+    const dim3 grid = flatGrid((a.items + kGroups - 1) / kGroups), threads(kThreads);
     withType(dy.type, [&](auto tag) {
         withCodes(kept.type, [&](auto codes) {
             withActivation(f, [&](auto kind) {

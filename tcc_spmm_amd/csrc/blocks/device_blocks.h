@@ -229,6 +229,11 @@ template <BlockCodes C> __device__ __forceinline__ void decode8(u32x2 q, float s
     }
 }
 
+// Workgroups of a walk over the blocks of all rows, 256 threads each: a launch takes fewer than 2^32 threads a
+// dimension, so from kGridRow on they are dealt to rows of a second one.
+constexpr unsigned kGridRow = 1u << 23;
+__device__ __forceinline__ unsigned flatGroup() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 // item / count for a flat index over rows of `count` blocks: magic = ceil(2^32 / count) makes the high
 // word at most one too large.
 __device__ __forceinline__ unsigned rowOf(unsigned item, unsigned count, unsigned magic) {
@@ -244,6 +249,10 @@ namespace blocks {
 
 inline unsigned rowMagic(unsigned count) {
     return unsigned(((std::uint64_t(1) << 32) + count - 1) / count);
+}
+
+inline dim3 flatGrid(unsigned groups) {
+    return groups <= kGridRow ? dim3(groups) : dim3(kGridRow, (groups + kGridRow - 1) / kGridRow);
 }
 
 inline void reject(const char* where, const char* what) {

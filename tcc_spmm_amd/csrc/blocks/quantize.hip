@@ -27,7 +27,7 @@ __global__ __launch_bounds__(kThreads) void quantizeRowBlocks(const typename T::
                                                                unsigned items, unsigned columns,
                                                                unsigned count, unsigned magic) {
     const unsigned lane = threadIdx.x % kBlockLanes;
-    const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
+    const unsigned item = flatGroup() * kGroups + threadIdx.x / kBlockLanes;
     if (item >= items) return;
     const unsigned codePitch = count * kBlock, exponentPitch = (count + 3) / 4 * 4;
     const unsigned row = rowOf(item, count, magic), block = item - row * count;
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kThreads) void dequantizeRowBlocks(const std::uint8
                                                                  unsigned columns, unsigned count,
                                                                  unsigned magic) {
     const unsigned lane = threadIdx.x % kBlockLanes;
-    const unsigned item = blockIdx.x * kGroups + threadIdx.x / kBlockLanes;
+    const unsigned item = flatGroup() * kGroups + threadIdx.x / kBlockLanes;
     if (item >= items) return;
     const unsigned row = rowOf(item, count, magic), block = item - row * count;
     const std::uint8_t* from = codes + std::uint64_t(row) * count * kBlock + block * kBlock;
@@ -152,11 +152,11 @@ void quantizeBlocks(DenseMatrix x, BlockRows out, std::uint32_t rows, std::uint3
     checkDense("quantize blocks", x.data, x.stride, x.type, columns);
     checkCodes("quantize blocks", out.codes, out.exponents);
     const unsigned count = (columns + kBlock - 1) / kBlock, items = itemsOf("quantize blocks", rows, count);
-    const unsigned grid = (items + kGroups - 1) / kGroups;
+    const dim3 grid = flatGrid((items + kGroups - 1) / kGroups);
     withType(x.type, [&](auto tag) {
         withCodes(out.type, [&](auto kind) {
             typedef decltype(tag) T;
-            hipLaunchKernelGGL((quantizeRowBlocks<T, decltype(kind)::value>), dim3(grid), dim3(kThreads), 0, stream,
+            hipLaunchKernelGGL((quantizeRowBlocks<T, decltype(kind)::value>), grid, dim3(kThreads), 0, stream,
                                static_cast<const typename T::Raw*>(x.data), x.stride, out.codes, out.exponents, items,
                                columns, count, rowMagic(count));
         });
@@ -173,15 +173,15 @@ void dequantizeBlocks(BlockRows x, void* out, DenseType type, std::uint64_t stri
     checkDense("dequantize blocks", out, stride, type, columns);
     checkCodes("dequantize blocks", x.codes, x.exponents);
     const unsigned count = (columns + kBlock - 1) / kBlock, items = itemsOf("dequantize blocks", rows, count);
-    const unsigned grid = (items + kGroups - 1) / kGroups;
+    const dim3 grid = flatGrid((items + kGroups - 1) / kGroups);
     withType(type, [&](auto tag) {
         typedef decltype(tag) T;
         auto* data = static_cast<typename T::Raw*>(out);
         if (x.type == BlockCodes::e4m3)
-            hipLaunchKernelGGL((dequantizeRowBlocks<T, BlockCodes::e4m3>), dim3(grid), dim3(kThreads), 0, stream,
+            hipLaunchKernelGGL((dequantizeRowBlocks<T, BlockCodes::e4m3>), grid, dim3(kThreads), 0, stream,
                                x.codes, x.exponents, data, stride, items, columns, count, rowMagic(count));
         else
-            hipLaunchKernelGGL((dequantizeRowBlocks<T, BlockCodes::int8>), dim3(grid), dim3(kThreads), 0, stream,
+            hipLaunchKernelGGL((dequantizeRowBlocks<T, BlockCodes::int8>), grid, dim3(kThreads), 0, stream,
                                x.codes, x.exponents, data, stride, items, columns, count, rowMagic(count));
     });
     checkHip(hipGetLastError());
