@@ -259,6 +259,14 @@ inline void reject(const char* where, const char* what) {
     throw std::invalid_argument(std::string(where) + ": " + what);
 }
 
+// Whether a launch takes that many workgroups: it has fewer than 2^32 threads.
+constexpr bool launchTakes(std::uint64_t groups, unsigned threads) {
+    return groups < (std::uint64_t(1) << 32) / threads;
+}
+inline void checkGrid(const char* where, std::uint64_t groups, unsigned threads) {
+    if (!launchTakes(groups, threads)) reject(where, "more tiles than a launch takes");
+}
+
 inline std::size_t elementBytes(DenseType t) { return t == DenseType::f32 ? 4 : 2; }
 
 inline void checkType(const char* where, DenseType t) {

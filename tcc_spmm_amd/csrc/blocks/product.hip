@@ -917,9 +917,13 @@ Form formOf(std::uint32_t rows, std::uint32_t outer, unsigned count) {
     const auto rounds = [](std::uint64_t n, unsigned slots) { return double((n + slots - 1) / slots); };
     const std::uint64_t half = tiles(128), quarter = tiles(64);
     const double wide = rounds(tiles(256), 256) * (11.5 + 1.5 * count);
-    const double middle = half <= 256 ? 5.0 + 0.75 * count : rounds(half, 512) * (5.0 + 1.3 * count);
-    const double small = quarter <= 256 ? 2.9 + 0.18 * count : rounds(quarter, 512) * (1.5 + 0.5 * count);
-    const double few = rounds(tiles(32), 256) * (3.9 + 0.09 * count);
+    double middle = half <= 256 ? 5.0 + 0.75 * count : rounds(half, 512) * (5.0 + 1.3 * count);
+    double small = quarter <= 256 ? 2.9 + 0.18 * count : rounds(quarter, 512) * (1.5 + 0.5 * count);
+    double few = rounds(tiles(32), 256) * (3.9 + 0.09 * count);
+    // 2^27 rows and more can be too many tiles of these for a launch.
+    if (!launchTakes(half, 512)) middle = wide + 1.0;
+    if (!launchTakes(quarter, 256)) small = wide + 1.0;
+    if (!launchTakes(tiles(32), 512)) few = wide + 1.0;
     const double least = std::min(std::min(wide, middle), std::min(small, few));
     return least == wide ? Form::wide : least == middle ? Form::middle : least == small ? Form::small : Form::few;
 }
@@ -929,7 +933,7 @@ void launchTiles(Product p, hipStream_t stream) {
     p.tilesM = (p.rows + BM - 1) / BM, p.tilesN = (p.outer + BN - 1) / BN;
     const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
     const std::size_t lds = Groups * Stages * (BM + BN) * kBlock;
-    if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+    checkGrid("matmul blocks", tiles, 64 * WM * WN * Groups);
     hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
                        dim3(64 * WM * WN * Groups), lds, stream, p);
     checkHip(hipGetLastError());
@@ -938,7 +942,7 @@ void launchTiles(Product p, hipStream_t stream) {
 template <typename T> void launchWide(Product p, hipStream_t stream) {
     p.tilesM = (p.rows + 255) / 256, p.tilesN = (p.outer + 255) / 256;
     const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
-    if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+    checkGrid("matmul blocks", tiles, 256);
     hipLaunchKernelGGL((multiplyWide<T>), dim3(unsigned(tiles)), dim3(256), 2 * 2 * 256 * kBlock, stream, p);
     checkHip(hipGetLastError());
 }
@@ -948,7 +952,7 @@ template <typename T> void launchProduct(Product p, hipStream_t stream) {
         if (exactTokens(p.rows, p.outer, p.count)) return launchTokens(p, stream);
         p.tilesM = (p.rows + 127) / 128;
         const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + 127) / 128);
-        if (tiles >> 31) reject("matmul blocks", "more than 2^31 tiles");
+        checkGrid("matmul blocks", tiles, 256);
         hipLaunchKernelGGL(multiplyTilesExact, dim3(unsigned(tiles)), dim3(256), 0, stream, p);
         checkHip(hipGetLastError());
     } else {

@@ -197,7 +197,7 @@ void quantizeWeightBlocks(DenseMatrix w, BlockWeightView out, std::uint32_t oute
     if (!out.codesT != !out.exponentsT) reject(where, "transposed codes and exponents come together");
     if (out.codesT) checkCodes(where, out.codesT, out.exponentsT);
     const std::uint64_t tiles = std::uint64_t((inner + kBlock - 1) / kBlock) * ((outer + kBlock - 1) / kBlock);
-    if (tiles >> 31) reject(where, "more than 2^31 tiles");
+    checkGrid(where, tiles, kThreads);
     withType(w.type, [&](auto tag) {
         typedef decltype(tag) T;
         hipLaunchKernelGGL((quantizeWeightTiles<T>), dim3(unsigned(tiles)), dim3(kThreads), 0, stream,

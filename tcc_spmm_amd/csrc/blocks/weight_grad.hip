@@ -628,7 +628,7 @@ void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::ui
     a.db = !db ? nullptr : p.splits == 1 ? db : parts + rounded4(size);
     a.splitPitch = p.splits == 1 ? 0 : pitch;
     const std::uint64_t blocks = std::uint64_t(a.tilesN) * a.tilesK * p.splits;
-    if (blocks >> 31) reject(where, "more than 2^31 tiles");
+    checkGrid(where, blocks, 256);
     if (p.aligned) {
         if (p.bn == 256)
             hipLaunchKernelGGL(sumRowsInPlace256, dim3(unsigned(blocks)), dim3(256), 4 * Tile<256>::bytes, stream, a);

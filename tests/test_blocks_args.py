@@ -160,3 +160,19 @@ def test_a_bias_gradient_needs_no_blocks():
     rejected(call(dw=P, k=128), b"null codes")
     with pytest.raises(ValueError, match="asked for"):
         B.weight_grad_blocks(torch.zeros((4, 128)), None, bias=False)
+
+
+def test_products_of_more_tiles_than_a_launch_takes():
+    """A launch has fewer than 2^32 threads: 2^24 tiles, of 256 x 256 for 16 bits, else of 128 x 128, are refused by the
+    call, not by the runtime."""
+    from tcc_spmm_amd._lib import lib
+    L = lib()
+    most = (1 << 31) - 1
+    matmul = lambda t, rows, n: L.tcc_matmul_blocks(P, P, P, P, None, P, n, t, rows, 128, n, None)  # noqa: E731
+    for t, rows, n in ((1, most, 512), (2, most, 257), (1, 1 << 22, 1 << 18), (0, most, 128), (0, 1 << 30, 129)):
+        rejected(matmul(t, rows, n), b"more tiles than a launch takes")
+    rejected(L.tcc_quantize_weight_blocks(P, 1 << 20, 0, P, P, None, None, 1 << 20, 1 << 20, None), b"than a launch takes")
+    size = ctypes.c_size_t()
+    assert L.tcc_weight_grad_blocks_workspace(64, 1 << 21, 1 << 20, 1, ctypes.byref(size)) == 0 and size.value == 0
+    rejected(L.tcc_weight_grad_blocks(P, 1 << 20, 0, P, P, P, None, 64, 1 << 20, 1 << 20, P, 1 << 40, None),
+             b"than a launch takes")

@@ -39,3 +39,24 @@ def test_more_blocks_than_a_launch_takes_threads_for(room):
         want, want_act = B.activation_blocks(x[p], "silu")
         assert torch.equal(y[p], want) and torch.equal(act.codes[p], want_act.codes)
         assert torch.equal(dx[p], B.activation_blocks_backward(y[p], want_act, "silu"))
+
+
+def test_product_of_more_rows_than_small_tiles_have_threads_for(room):
+    """2^30 + 300 rows are too many tiles of 64 rows for a launch. Most rows are zeros; the others are those of a product
+    of them alone."""
+    from tcc_spmm_amd import blocks as B
+    room(190)
+    rows, outer = (1 << 30) + 300, 8
+    codes = torch.zeros((rows, 128), device="cuda", dtype=torch.uint8).view(B.E4M3)
+    exponents = torch.full((rows, 4), 127, device="cuda", dtype=torch.uint8)
+    weight = B.quantize_weight_blocks(random((outer, 128), 1))
+    parts = [slice(at, at + 300) for at in (0, (1 << 29) - 100, rows - 300)]
+    for i, p in enumerate(parts):
+        some = B.quantize_blocks(random((300, 128), 2 + i))
+        codes[p], exponents[p] = some.codes, some.exponents
+    y = B.matmul_blocks(B.BlockTensor(codes, exponents, 128), weight)
+    for p in parts:
+        alone = B.BlockTensor(codes[p].contiguous(), exponents[p].contiguous(), 128)
+        # One block is one instruction's sum in every form of the product.
+        assert torch.equal(y[p], B.matmul_blocks(alone, weight))
+    assert not y[1000:100000].any()
