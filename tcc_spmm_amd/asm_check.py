@@ -14,7 +14,11 @@ if the next pair's rows are the only loads to LDS among the N youngest, on every
 merged, dropped or moved one of the instructions in between would make it a silent race; the build
 refuses such a kernel.
 
-check(asm_text) returns a list of problems (empty when the kernels are clean).
+The block products' rings of stages wait in the same way, in front of a barrier. check_counted_waits holds each such
+wait to what the source counts on: how many of the N youngest instructions are loads to LDS, and how many of those
+follow the wait before.
+
+check(asm_text) and check_counted_waits return a list of problems (empty when the kernels are clean).
 """
 from __future__ import annotations
 
@@ -101,6 +105,14 @@ def _successors(instrs, labels, i):
     return [i + 1]
 
 
+def _predecessors(instrs, labels):
+    before = [[] for _ in range(len(instrs) + 1)]
+    for i in range(len(instrs)):
+        for j in _successors(instrs, labels, i):
+            before[j].append(i)
+    return before
+
+
 def _kernel_hazards(instrs, labels):
     infos = [_info(x) for x in instrs]
     found = []
@@ -140,10 +152,7 @@ def _ring_waits(instrs, labels, asm_blocks, rows):
               if any(x.startswith("ds_read") for x in instrs[i:end])]
     if not any(map(_loads_to_lds, instrs)):
         return []
-    before = [[] for _ in range(len(instrs) + 1)]
-    for i in range(len(instrs)):
-        for j in _successors(instrs, labels, i):
-            before[j].append(i)
+    before = _predecessors(instrs, labels)
     found = []
     for i, wait in blocks:
         m = re.match(r"s_waitcnt .*?vmcnt\((\d+)\)", wait)
@@ -180,16 +189,69 @@ def _ring_waits(instrs, labels, asm_blocks, rows):
     return found
 
 
+def _counted_waits(instrs, labels, asm_blocks, waits):
+    """`waits`: for each N of an inline `s_waitcnt vmcnt(N)` in front of a barrier, how many of the N youngest memory
+    instructions may be loads to LDS, and the numbers of loads to LDS that may lie between it and the inline wait before
+    (or the kernel's start)."""
+    before = _predecessors(instrs, labels)
+    starts = {i for i, end in asm_blocks if "s_barrier" in instrs[i:end] and "vmcnt" in instrs[i]}
+    found = []
+    for i in sorted(starts):
+        n = int(re.search(r"vmcnt\((\d+)\)", instrs[i]).group(1))
+        if n == 0:
+            continue
+        if n not in waits:
+            found.append(f"`{instrs[i]}` is a wait that no count is known of")
+            continue
+        most, between = waits[n]
+        # Backwards on every path: instructions that count, loads to LDS among them, and whether the wait before is passed.
+        stack, seen = [(j, 0, 0, False) for j in before[i]] or [(-1, 0, 0, False)], set()
+        while stack:
+            state = stack.pop()
+            j, count, loads, passed = state
+            if state in seen:
+                continue
+            seen.add(state)
+            if not passed and (j < 0 or j in starts):
+                if loads not in between:
+                    found.append(f"{loads} loads to LDS between `{instrs[i]}` and the wait before, not "
+                                 f"{' or '.join(map(str, sorted(between)))}")
+                passed = True
+            if j < 0 or passed and count >= n:
+                continue
+            if instrs[j].startswith(_VMEM):
+                count += 1
+                loads += _loads_to_lds(instrs[j])
+                if count <= n and loads > most:
+                    found.append(f"`{instrs[i]}` may leave {loads} loads to LDS outstanding, not {most}")
+                    break
+            stack.extend((k, count, loads, passed) for k in before[j] or [-1])
+    return found
+
+
+def _kernels(lines, kernels):
+    """(name, body) of every kernel whose name contains `kernels`."""
+    for k, line in enumerate(lines):
+        if re.match(r"^_Z\S+:", line) and kernels in line:
+            end = next((j for j in range(k, len(lines)) if lines[j].startswith(".Lfunc_end")), len(lines))
+            yield line.split(":")[0], lines[k + 1:end]
+
+
+def check_counted_waits(asm_text: str, kernels: str, waits: dict) -> list:
+    """Problems with the inline counted waits of every kernel whose name contains `kernels` (_counted_waits)."""
+    problems, some = [], False
+    for name, body in _kernels(asm_text.split("\n"), kernels):
+        some = True
+        problems += [f"{name}: {wait}" for wait in _counted_waits(*_parse(body), waits)]
+    return problems if some else ["no kernels found in the assembly"]
+
+
 def check(asm_text: str, kernels: str = "Kernel") -> list:
     """Problems in every kernel of a gfx950 assembly listing (hipcc --cuda-device-only -S) whose name
     contains `kernels`; spills are looked for in all of them."""
-    lines = asm_text.split("\n")
-    problems = []
-    starts = [k for k, l in enumerate(lines) if re.match(r"^_Z\S+:", l) and kernels in l]
-    for k in starts:
-        name = lines[k].split(":")[0]
-        end = next((j for j in range(k, len(lines)) if lines[j].startswith(".Lfunc_end")), len(lines))
-        body = lines[k + 1:end]
+    problems, some = [], False
+    for name, body in _kernels(asm_text.split("\n"), kernels):
+        some = True
         if any(l.strip().startswith(("scratch_store", "scratch_load", "buffer_store_dword off"))
                for l in body):
             problems.append(f"{name}: spills to scratch")
@@ -203,6 +265,6 @@ def check(asm_text: str, kernels: str = "Kernel") -> list:
                          asm_text):
         if int(m.group(2)):
             problems.append(f"{m.group(1)}: {m.group(2)} VGPR spills")
-    if not starts:
+    if not some:
         problems.append("no kernels found in the assembly")
     return problems

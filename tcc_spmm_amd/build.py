@@ -71,9 +71,18 @@ def check_kernel_asm(src: pathlib.Path = CSRC / "kernel" / "spmm.hip") -> None:
 # Kernels whose MFMAs are inline assembly, whose latency the compiler does not know.
 INLINE_MFMA = {CSRC / "blocks" / "product.hip": "multiplyWide", CSRC / "blocks" / "weight_grad.hip": "sumRowsInPlace"}
 
+# Inline waits in front of barriers, as asm_check.check_counted_waits takes them: by kernel, for each vmcnt(N) how many
+# loads to LDS it may leave outstanding and how many there are since the wait before. multiplyWide: what its quarters
+# load, 4 or 8 a wait, after 28 in front of the loop, and nine loads of exponents a pair of blocks (25 - 16, 21 - 12).
+# multiplyTiles of four stages: two stages of 4 loads, after three in front of the loop.
+COUNTED_WAITS = {CSRC / "blocks" / "product.hip": {
+    "multiplyWide": {25: (16, {4, 8}), 21: (12, {8}), 16: (16, {8}), 12: (12, {8, 28})},
+    "multiplyTiles": {8: (8, {4, 12})},
+}}
+
 
 def check_inline_mfma(src: pathlib.Path) -> None:
-    """The same for a file of INLINE_MFMA."""
+    """The same for a file of INLINE_MFMA, and its COUNTED_WAITS."""
     from . import asm_check
     out = BUILD / f"{src.stem}-gfx950.s"
     cmd = [str(ROCM / "bin" / "hipcc"), *HIP_FLAGS, "--cuda-device-only", "-S", str(src), "-o", str(out)]
@@ -81,6 +90,8 @@ def check_inline_mfma(src: pathlib.Path) -> None:
     if res.returncode != 0:
         raise RuntimeError(f"assembly listing failed: {shlex.join(cmd)}\n{res.stderr}")
     problems = asm_check.check(out.read_text(), INLINE_MFMA[src])
+    for kernels, waits in COUNTED_WAITS.get(src, {}).items():
+        problems += asm_check.check_counted_waits(out.read_text(), kernels, waits)
     if problems:
         raise RuntimeError(f"{src.name}: assembly check failed:\n  " + "\n  ".join(problems))
 

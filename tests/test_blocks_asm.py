@@ -37,3 +37,53 @@ def test_kernels_as_built(src):
     name = build.INLINE_MFMA[src]
     planted, count = re.subn(r"(\tv_mfma_\S+ a\[(\d+):\d+\].*\n)", r"\1\tv_accvgpr_read_b32 v0, a\2\n", listing)
     assert count > 64 and any("MFMA result read" in p for p in asm_check.check(planted, name))
+
+
+def _ring(between, wait=8, extra=""):
+    """A loop of one counted wait: `between` loads to LDS a turn, and before it eight."""
+    row = "\tbuffer_load_dwordx4 v9, s[4:7], 0 offen lds\n"
+    body = row * 8 + ".LBB0_1:\n" + extra + f"\t;;#ASMSTART\n\ts_waitcnt vmcnt({wait}) lgkmcnt(0)\n\ts_barrier\n\t;;#ASMEND\n"
+    return _listing(body + row * between + "\ts_cbranch_scc1 .LBB0_1\n")
+
+
+def test_counted_waits_are_held_to_their_counts():
+    load = "\tglobal_load_ushort v3, v4, s[2:3]\n"
+    check = lambda text, waits: asm_check.check_counted_waits(text, "multiplyWide", waits)  # noqa: E731
+    assert check(_ring(4), {8: (8, {4, 8})}) == []
+    assert check(_ring(4, extra=load), {9: (8, {4, 8})})[0].endswith("no count is known of")
+    assert check(_ring(4, 9, load), {9: (8, {4, 8})}) == []
+    # the load that was counted on is not there
+    assert check(_ring(4, 9), {9: (8, {4, 8})}) == [
+        "_ZN4test12multiplyWideEv: `s_waitcnt vmcnt(9) lgkmcnt(0)` may leave 9 loads to LDS outstanding, not 8"]
+    # a load to LDS too few, or one that is not a load to LDS any more
+    assert "3 loads to LDS between" in check(_ring(3), {8: (8, {4, 8})})[0]
+    assert check("", {8: (8, {4})}) == ["no kernels found in the assembly"]
+
+
+@pytest.mark.parametrize("src", list(build.COUNTED_WAITS), ids=lambda src: src.stem)
+def test_counted_waits_as_built(src):
+    """They pass; a memory load taken out of a loop, moved to the other side of the next wait, or made an ordinary one
+    does not, whichever it is."""
+    build.BUILD.mkdir(exist_ok=True)
+    build.check_inline_mfma(src)
+    listing = (build.BUILD / f"{src.stem}-gfx950.s").read_text()
+    for kernels, waits in build.COUNTED_WAITS[src].items():
+        lines = listing.split("\n")
+        starts = [i for i, line in enumerate(lines) if re.match(r"^_Z\S+:", line) and kernels in line]
+        checked = 0
+        for start in starts:
+            end = next(i for i in range(start, len(lines)) if lines[i].startswith(".Lfunc_end"))
+            kernel = lines[start:end + 1]
+            ring = [i for i, line in enumerate(kernel) if re.search(r"s_waitcnt vmcnt\([1-9]\d*\) lgkmcnt", line)
+                    and "s_barrier" in kernel[i + 1]]
+            if not ring:  # a form of two stages, whose waits are for everything
+                continue
+            for at in (i for i in range(ring[0] + 2, ring[-1]) if " lds" in kernel[i] or "load_ushort" in kernel[i]):
+                gone = kernel[:at] + kernel[at + 1:]
+                wait = next(i for i in ring if i > at) - 1
+                late = gone[:wait + 1] + [kernel[at]] + gone[wait + 1:]
+                plain = kernel[:at] + [kernel[at].replace(" lds", "")] + kernel[at + 1:]
+                for text in (gone, late) + ((plain,) if " lds" in kernel[at] else ()):
+                    assert asm_check.check_counted_waits("\n".join(text), kernels, waits), kernel[at]
+                checked += 1
+        assert checked > 10
