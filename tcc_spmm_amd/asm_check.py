@@ -2,10 +2,12 @@
 
 On gfx950 a VALU, memory or LDS instruction that reads a VGPR written by an MFMA is not interlocked:
 the compiler must separate them by wait states (16-pass MFMAs such as v_mfma_f32_32x32x8_f16 need
-18, which the compiler itself pads to). Kernel variants built during development showed ROCm 7.2's
+18, which the compiler itself pads to). The other way round an MFMA that reads a register that a VALU instruction wrote
+has to come OPERAND wait states after it, which the compiler pads to, but not for an MFMA in inline assembly. Kernel variants built during development showed ROCm 7.2's
 compiler issuing such reads 2 to 8 wait states after the MFMA, always next to register-spill code
 at a loop exit; the variant that did so produced wrong results. The build therefore refuses a kernel
-that spills to scratch or reads an MFMA result within REQUIRED wait states on any control-flow path.
+that spills to scratch, reads an MFMA result within REQUIRED wait states or has an inline MFMA read a VALU result within
+OPERAND of them, on any control-flow path.
 
 The panel walk reads X rows from LDS that memory loads put there (`buffer_load ... lds`), in inline
 assembly that waits with a hand-counted vmcnt(N): all but the N youngest vector memory instructions have
@@ -25,6 +27,7 @@ from __future__ import annotations
 import re
 
 REQUIRED = 18
+OPERAND = 2
 
 
 def _regs(tok: str) -> set:
@@ -140,8 +143,30 @@ def _kernel_hazards(instrs, labels):
                 continue
             if not op2.startswith("v_mfma"):
                 pending = pending - w2
-            cost = int(instrs[j].split()[1], 0) + 1 if op2 == "s_nop" else 1
-            stack.extend((s, waits + cost, pending) for s in _successors(instrs, labels, j))
+            stack.extend((s, waits + _wait_states(instrs[j]), pending) for s in _successors(instrs, labels, j))
+    return found
+
+
+def _wait_states(ins: str) -> int:
+    return int(ins.split()[1], 0) + 1 if ins.startswith("s_nop") else 1
+
+
+def _operand_hazards(instrs, labels, asm_blocks):
+    """MFMAs in inline assembly that read what a VALU instruction wrote less than OPERAND wait states before."""
+    before = _predecessors(instrs, labels)
+    found = []
+    for i in {i for start, end in asm_blocks for i in range(start, end) if instrs[i].startswith("v_mfma")}:
+        reads = _info(instrs[i])[2]
+        stack = [(j, 0) for j in before[i]]
+        while stack:
+            j, waits = stack.pop()
+            if waits >= OPERAND:
+                continue
+            op, writes, _, _ = _info(instrs[j])
+            if op.startswith("v_") and not op.startswith("v_mfma") and writes & reads:
+                found.append((waits, instrs[j], instrs[i]))
+                continue
+            stack.extend((k, waits + _wait_states(instrs[j])) for k in before[j])
     return found
 
 
@@ -259,6 +284,8 @@ def check(asm_text: str, kernels: str = "Kernel") -> list:
         for waits, mfma, reader in _kernel_hazards(instrs, labels):
             problems.append(f"{name}: MFMA result read {waits} wait states after `{mfma}` by "
                             f"`{reader}` (needs {REQUIRED})")
+        for waits, writer, mfma in _operand_hazards(instrs, labels, asm_blocks):
+            problems.append(f"{name}: `{mfma}` reads what `{writer}` wrote {waits} wait states before (needs {OPERAND})")
         for wait in _ring_waits(instrs, labels, asm_blocks, 4 if "256" in name else 2):
             problems.append(f"{name}: {wait}")
     for m in re.finditer(r"\.name:\s+(\S+)\n(?:.*\n){0,40}?\s+\.vgpr_spill_count:\s+(\d+)",

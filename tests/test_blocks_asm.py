@@ -87,3 +87,32 @@ def test_counted_waits_as_built(src):
                     assert asm_check.check_counted_waits("\n".join(text), kernels, waits), kernel[at]
                 checked += 1
         assert checked > 10
+
+
+INLINE = "\t;;#ASMSTART\n" + MFMA + "\t;;#ASMEND\n"
+
+
+@pytest.mark.parametrize("writes", ["v_mov_b32_e32 v3, v30", "v_and_or_b32 v16, v30, v31, v32", "v_accvgpr_write_b32 a2, 0",
+                                    "v_perm_b32 v15, v30, v31, s0"])
+def test_an_inline_mfma_right_behind_its_operand(writes):
+    """Any operand, the sum and the scales among them; not for other registers, or two wait states later, or where the
+    compiler itself places the MFMA."""
+    check = lambda between, mfma=INLINE: asm_check.check(_listing(f"\t{writes}\n" + between + mfma), "multiplyWide")  # noqa: E731
+    assert len(check("")) == 1 and "0 wait states before" in check("")[0]
+    assert len(check("\ts_mov_b32 s0, s1\n")) == 1
+    assert len(check(".LBB0_2:\n\ts_nop 0\n")) == 1  # a label is no instruction
+    assert check("\ts_nop 1\n") == [] and check("\ts_mov_b32 s0, s1\n\tds_read_b32 v40, v41\n") == []
+    assert check("", MFMA) == []
+    other = writes.replace(" v3,", " v33,").replace(" v16,", " v36,").replace(" a2,", " a22,").replace(" v15,", " v35,")
+    assert asm_check.check(_listing(f"\t{other}\n" + INLINE), "multiplyWide") == []
+
+
+@pytest.mark.parametrize("src", list(build.INLINE_MFMA), ids=lambda src: src.stem)
+def test_operands_as_built(src):
+    """With a write of an operand planted right in front of every inline MFMA the kernels do not pass."""
+    build.BUILD.mkdir(exist_ok=True)
+    build.check_inline_mfma(src)
+    listing = (build.BUILD / f"{src.stem}-gfx950.s").read_text()
+    planted, count = re.subn(r"(\t;;?#ASMSTART\n\tv_mfma_\S+ a\[\d+:\d+\], v\[(\d+):)", r"\tv_mov_b32_e32 v\2, 0\n\1", listing)
+    problems = asm_check.check(planted, build.INLINE_MFMA[src])
+    assert count > 64 and sum("wait states before" in p for p in problems) >= count
