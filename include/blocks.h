@@ -95,6 +95,11 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
                   BlockRows keep, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
                   void* workspace, std::size_t workspaceBytes, hipStream_t stream = nullptr);
 
+// The kernel that a call of these sizes takes, by name, for tests and measurements; its splits of the rows for a gradient.
+// matmulBlocks and linearBlocks; linearBlocks calls matmulBlocks where the names are the same.
+const char* matmulBlocksForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type);
+const char* linearBlocksForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type);
+
 // dw = dy^T x for dense dy [rows][outer] and x's E4M3 blocks [rows][inner], FP32 [outer][inner]
 // contiguous, and, if db is not null, db = the sums of dy's columns. All sums in FP32, of x's values as in an FP32 y of
 // matmulBlocks; a dy of f16 or f32 goes through the bf16 MFMA as two or three bf16 parts, which together hold it exactly
@@ -106,6 +111,9 @@ std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, s
 void weightGradBlocks(DenseMatrix dy, BlockRows x, float* dw, float* db, std::uint32_t rows,
                       std::uint32_t inner, std::uint32_t outer, void* workspace, std::size_t workspaceBytes,
                       hipStream_t stream = nullptr);
+
+const char* weightGradBlocksForm(DenseMatrix dy, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
+                                 std::uint32_t* splits);
 
 // y = f(x) for x [rows][width], or, gated, y = f(g) u for x = [g | u] of [rows][2 * width]; y has x's
 // type. `keep` receives x's blocks for the backward pass (null codes: nothing is kept): rows of `width`,

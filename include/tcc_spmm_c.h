@@ -154,6 +154,13 @@ int tcc_activation_blocks_backward(const void* dy, uint64_t stride, uint32_t typ
                                    const uint8_t* exponents, uint32_t codeType, uint32_t kind, int gated, void* dx,
                                    uint64_t dxStride, uint32_t rows, uint32_t width, void* stream);
 
+/* The kernel that a call takes, by name, and a gradient's splits of the rows (null: not asked for): for tests and
+ * measurements. No device is touched, and dy only looked at for its alignment. */
+int tcc_matmul_blocks_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, const char** form);
+int tcc_linear_blocks_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, const char** form);
+int tcc_weight_grad_blocks_form(const void* dy, uint64_t stride, uint32_t type, uint32_t rows, uint32_t inner,
+                                uint32_t outer, const char** form, uint32_t* splits);
+
 /* DeviceMatrix — reference src/device_matrix.cuh:8-37: uploads every array of a bucketed format,
  * allocates partials (partialCount*8*features floats) and counters (nSW*(features/128) uint32,
  * zeroed) when partialCount > 0, and hands out the view and the workspace. */

@@ -99,6 +99,10 @@ SIGNATURES = {
     "tcc_weight_grad_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p,
                                          C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
                                          C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tcc_matmul_blocks_form": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_char_p)]),
+    "tcc_linear_blocks_form": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(C.c_char_p)]),
+    "tcc_weight_grad_blocks_form": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32,
+                                              C.c_uint32, C.POINTER(C.c_char_p), C.POINTER(C.c_uint32)]),
     "tcc_activation_blocks": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p,
                                         C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
                                         C.c_uint32, C.c_void_p]),

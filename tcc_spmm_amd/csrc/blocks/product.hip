@@ -1022,6 +1022,25 @@ template <typename T> void launchRows(const Product& p, std::size_t lds, hipStre
 std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
 } // namespace
 
+const char* matmulBlocksForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
+    checkColumns("matmul blocks", inner);
+    checkColumns("matmul blocks", outer);
+    checkType("matmul blocks", type);
+    const unsigned count = (inner + kBlock - 1) / kBlock;
+    if (type == DenseType::f32) return exactTokens(rows, outer, count) ? "multiplyTokens" : "multiplyTilesExact";
+    switch (formOf(rows, outer, count)) {
+    case Form::wide: return "multiplyWide";
+    case Form::middle: return "multiplyTiles128";
+    case Form::small: return "multiplyTiles64";
+    default: return "multiplyTiles32";
+    }
+}
+
+const char* linearBlocksForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
+    const char* product = matmulBlocksForm(rows, inner, outer, type);
+    return rowsImage(rows, inner, outer, type) ? "multiplyRows" : fusedTokens(rows, inner) ? "multiplyTokensDense" : product;
+}
+
 std::size_t linearBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                   bool keep) {
     if (keep || fusedTokens(rows, inner) || rowsImage(rows, inner, outer, type)) return 0;

@@ -588,6 +588,16 @@ void launchSum(const Gradient& a, std::uint64_t blocks, hipStream_t stream) {
 
 } // namespace
 
+const char* weightGradBlocksForm(DenseMatrix dy, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer,
+                                 std::uint32_t* splits) {
+    checkType("weight gradient", dy.type);
+    checkColumns("weight gradient", outer);
+    const Plan p = planOf(rows, inner, outer, dy.type, alignedRows(dy, outer));
+    if (splits) *splits = p.splits;
+    if (p.aligned) return p.bn == 256 ? "sumRowsInPlace256" : "sumRowsInPlace128";
+    return outer < 8 ? "sumRowsNarrow" : p.bn == 64 ? "sumRows64" : "sumRows128";
+}
+
 std::size_t weightGradBlocksWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type) {
     if (!rows || !outer) return 0;
     // The larger of the two forms' needs: which one runs depends on dy's alignment.

@@ -326,6 +326,28 @@ int tcc_weight_grad_blocks(const void* dy, uint64_t stride, uint32_t type, const
     });
 }
 
+int tcc_matmul_blocks_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, const char** form) {
+    return guarded([&] {
+        need(form, "form");
+        *form = matmulBlocksForm(rows, inner, outer, DenseType(type));
+    });
+}
+
+int tcc_linear_blocks_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, const char** form) {
+    return guarded([&] {
+        need(form, "form");
+        *form = linearBlocksForm(rows, inner, outer, DenseType(type));
+    });
+}
+
+int tcc_weight_grad_blocks_form(const void* dy, uint64_t stride, uint32_t type, uint32_t rows, uint32_t inner,
+                                uint32_t outer, const char** form, uint32_t* splits) {
+    return guarded([&] {
+        need(form, "form");
+        *form = weightGradBlocksForm({dy, stride, DenseType(type)}, rows, inner, outer, splits);
+    });
+}
+
 int tcc_activation_blocks(const void* x, uint64_t stride, uint32_t type, uint32_t kind, int gated, void* y,
                           uint64_t yStride, uint8_t* keepCodes, uint8_t* keepExponents, uint32_t codeType,
                           uint32_t rows, uint32_t width, void* stream) {
