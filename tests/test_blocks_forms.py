@@ -107,3 +107,43 @@ def test_gradients(gpu, form, splits, dtype, rows, inner, outer):
     again = weight_grad_blocks(dy, kept)
     assert torch.equal(dw, again[0]) and torch.equal(db, again[1]), "repeated calls give the same bits"
     assert torch.equal(weight_grad_blocks(dy, kept, bias=False)[0], dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dtype,rows,inner,outer", [p for i, p in enumerate(PRODUCTS) if p[:2] not in
+                                                         {q[:2] for q in PRODUCTS[:i]} or p[0] in ("multiplyRows", "multiplyTokens")])
+def test_nan_stays_in_its_rows_and_columns(gpu, form, dtype, rows, inner, outer):
+    """A NaN or an infinity in x makes its row NaN, in the weight the columns of its tile, and everything else is what it
+    is without it."""
+    from tcc_spmm_amd.blocks import linear_blocks, quantize_weight_blocks
+    x, w = random((rows, inner), 1, dtype), random((outer, inner), 2)
+    clean = linear_blocks(x, quantize_weight_blocks(w))
+    bad = torch.zeros((rows, outer), dtype=torch.bool, device="cuda")
+    if outer > 128:
+        w[outer - 1, inner - 1] = float("nan")
+        bad[:, (outer - 1) // 128 * 128:] = True
+    for row, column, value in ((0, 0, float("nan")), (rows // 2, inner - 1, float("inf")), (rows - 1, inner // 2, float("-inf"))):
+        x[row, column] = value
+        bad[row] = True
+    y = linear_blocks(x, quantize_weight_blocks(w))
+    assert y[bad].isnan().all() and torch.equal(y[~bad], clean[~bad])
+    kept = linear_blocks(x, quantize_weight_blocks(w), keep=True)[1]
+    base.check_blocks(kept, x, "e4m3")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,splits,dtype,rows,inner,outer", GRADIENTS)
+def test_nan_stays_in_its_columns_of_the_gradient(gpu, form, splits, dtype, rows, inner, outer):
+    """A NaN in dy makes its row of dw NaN and its sum, one in x the columns of its block."""
+    from tcc_spmm_amd.blocks import quantize_blocks, weight_grad_blocks
+    x, dy = random((rows, inner), 1, dtype), random((rows, outer), 2, dtype)
+    clean, clean_db = weight_grad_blocks(dy, quantize_blocks(x))
+    bad = torch.zeros((outer, inner), dtype=torch.bool, device="cuda")
+    if inner > 128:
+        x[rows - 1, inner - 1] = float("inf")
+        bad[:, (inner - 1) // 128 * 128:] = True
+    dy[rows // 2, outer - 1] = float("nan")
+    bad[outer - 1] = True
+    dw, db = weight_grad_blocks(dy, quantize_blocks(x))
+    assert dw[bad].isnan().all() and torch.equal(dw[~bad], clean[~bad])
+    assert db[-1].isnan() and torch.equal(db[:-1], clean_db[:-1])
