@@ -147,3 +147,21 @@ def test_nan_stays_in_its_columns_of_the_gradient(gpu, form, splits, dtype, rows
     dw, db = weight_grad_blocks(dy, quantize_blocks(x))
     assert dw[bad].isnan().all() and torch.equal(dw[~bad], clean[~bad])
     assert db[-1].isnan() and torch.equal(db[:-1], clean_db[:-1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,splits,dtype,rows,inner,outer", [g for g in GRADIENTS if "InPlace" in g[0]] +
+                         [("sumRowsInPlace128", 1, "bf16", 300, 256, 136), ("sumRowsInPlace128", 1, "bf16", 1, 300, 8)])
+@pytest.mark.parametrize("left,right", [(8, 0), (16, 8), (0, 72)])
+def test_gradients_of_aligned_slices(gpu, form, splits, dtype, rows, inner, outer, left, right):
+    """A slice of a wider dy whose rows keep their alignment takes the same kernel as dy by itself, gives the same bits, and
+    reads nothing beside it."""
+    from tcc_spmm_amd.blocks import quantize_blocks, weight_grad_blocks
+    kept, dy = quantize_blocks(random((rows, inner), 1, dtype)), random((rows, outer), 2, dtype)
+    wide = base.cut(dy, left, right)
+    assert rows == 1 or wide.stride(0) > outer
+    assert gradient_form(wide.data_ptr(), wide.stride(0), dtype, rows, inner, outer) == (form, splits)
+    want, got = weight_grad_blocks(dy, kept), weight_grad_blocks(wide, kept)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    odd = base.cut(dy, 3, 2)
+    assert not gradient_form(odd.data_ptr(), odd.stride(0), dtype, rows, inner, outer)[0].startswith("sumRowsInPlace")
