@@ -459,8 +459,8 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     """x w^T + bias with both operands in E4M3 blocks, differentiable; w is the master weight, quantized
     in every call. Under autocast x is cast to its type first, as torch's linear casts it; w is quantized and the bias
     added at their own precision."""
-    if x.dtype in _TYPES and torch.is_autocast_enabled(x.device.type):
-        x = x.to(torch.get_autocast_dtype(x.device.type))
+    if x.is_cuda and x.dtype in _TYPES and torch.is_autocast_enabled("cuda"):
+        x = x.to(torch.get_autocast_dtype("cuda"))
     if not torch.is_grad_enabled():
         # Inside a Function the mode is off and its arguments still say that they require a gradient.
         weight = quantize_weight_blocks(w, transposed=False)

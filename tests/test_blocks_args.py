@@ -176,3 +176,15 @@ def test_products_of_more_tiles_than_a_launch_takes():
     assert L.tcc_weight_grad_blocks_workspace(64, 1 << 21, 1 << 20, 1, ctypes.byref(size)) == 0 and size.value == 0
     rejected(L.tcc_weight_grad_blocks(P, 1 << 20, 0, P, P, P, None, 64, 1 << 20, 1 << 20, P, 1 << 40, None),
              b"than a launch takes")
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_layers_refuse_other_devices(device):
+    """With the call's own error, with and without gradients and autocast."""
+    from tcc_spmm_amd import blocks as B
+    x, w = torch.zeros((4, 128), device=device), torch.zeros((8, 128), device=device, requires_grad=True)
+    for context in (torch.enable_grad, torch.no_grad, lambda: torch.autocast("cuda", torch.bfloat16, enabled=False)):
+        with context(), pytest.raises(ValueError, match="CUDA"):
+            B.block_linear(x, w)
+        with context(), pytest.raises(ValueError, match="CUDA"):
+            B.block_activation(x)
