@@ -16,8 +16,9 @@
 // launch. Errors are thrown before any launch: std::invalid_argument for null or misaligned buffers,
 // sizes and strides out of range and workspaces that are too small, std::runtime_error for the
 // runtime's. Rows may be up to 2^31 - 1, their elements up to 2^22, and a product's or weight's tiles fewer than 2^24
-// (of 256 x 256 for a 16-bit y, 128 x 128 otherwise), which is what a launch takes. Codes must be 16-byte aligned and exponents 4-byte aligned (anything from hipMalloc or
-// torch); dense matrices need only their element's alignment, with any row stride of at least a row.
+// (of 256 x 256 for a 16-bit y, 128 x 128 otherwise), which is what a launch takes. Codes must be 16-byte aligned and
+// exponents 4-byte aligned (anything from hipMalloc or torch); dense matrices need only their element's alignment, with
+// any row stride of at least a row.
 #pragma once
 
 #include <hip/hip_runtime_api.h>

@@ -275,7 +275,8 @@ def matmul_blocks(x: BlockTensor, weight: BlockWeight, bias: torch.Tensor | None
 def linear_blocks(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = None, *,
                   keep: bool = False, stream=None):
     """linearBlocks: y = Q(x) weight^T + bias in x's type, for x [..., inner] quantized into E4M3 blocks on
-    the way; sums are those of matmul_blocks with x's type. With keep=True returns (y, x's BlockTensor): what the weight gradient needs of x, in 8 bits."""
+    the way; sums are those of matmul_blocks with x's type. With keep=True returns (y, x's BlockTensor): what the weight
+    gradient needs of x, in 8 bits."""
     inner, outer = weight.columns, weight.rows
     _dense(x, "x", inner)
     device = x.device
@@ -479,7 +480,7 @@ def block_activation(x: torch.Tensor, kind: str = "silu", *, gated: bool = False
 
 
 class BlockLinear(torch.nn.Linear):
-    """torch.nn.Linear whose product and gradients run on 8-bit blocks."""
+    """torch.nn.Linear whose product and gradients run on 8-bit blocks, autocast included (block_linear)."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return block_linear(x, self.weight, self.bias)

@@ -464,7 +464,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 // FP32 outputs: the codes' values, exact in bf16 (values8), through the bf16 MFMA, whose sums are FP32's. Tiles of
 // 128 x 128, steps of half a block: a row's 64 values are 128 bytes of LDS, stored in the chunk order of
 // the 8-bit kernel. Codes pass through registers to be converted, in every tile anew, which with the bf16 MFMA's
-// half rate bounds it: 4096 x 4096 x 8192 367 us, 0.75 PFLOP/s (a library's product in FP32 0.15). The 8-bit MFMA cuts
+// half rate bounds it: 4096 x 4096 x 8192 360 us, 0.76 PFLOP/s (a library's product in FP32 0.15). The 8-bit MFMA cuts
 // products off 13 bits below the largest of eight, 1.2e-5 of the sum off on random numbers, which a 16-bit output's
 // rounding is twenty times as large as and an FP32 one's far smaller.
 __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void multiplyTilesExact(Product a) {
 // time, without a barrier: dense x is read once, quantized in the layout of an operand, kept if asked for, and
 // multiplied with every column. Bound by HBM; what it saves against the tiles is writing and reading codes.
 // Measured, FP32: 2,449,029 x 128 -> 256 804 us, 4.7 TB/s; 262,144 x 256 -> 47 with x kept 88 us, 4.4 TB/s;
-// 262,144 x 47 -> 256 83, 3.8 TB/s, where rows of 188 bytes are read 16 at a time, 64 bytes of each. Loads and stores
+// 262,144 x 47 -> 256 92, 3.4 TB/s, where rows of 188 bytes are read 16 at a time, 64 bytes of each. bf16: 1,000,000 x
+// 128 -> 256 179, 4.3 TB/s; 300,000 x 512 -> 256 120, 3.8; f16, 1,000,000 x 100 -> 47 94, 3.1. Loads and stores
 // are ordinary ones: a row's lines come and go in two or more accesses, and nontemporal loads took 3 to 10% longer
 // (1,000,000 x 128 -> 128 255 us : 230), nontemporal stores up to 17% (1,000,000 x 128 -> 256 406 : 350).
 //

@@ -67,9 +67,9 @@ struct Gradient {
 // step before is multiplied; dy is split into its parts on the way to LDS, which has one stage, since its
 // parts leave little room and several workgroups share a CU.
 // Narrow: rows of dy of fewer than 8 elements.
-// Measured, 4096 x 4096 x 4096: FP32 508 us and f16 374, 270 and 370 TFLOP/s (810 and 740 of the MFMA's), bound by the
-// split into parts and by LDS, which each part passes through; bf16 of odd rows 212. 262,144 x 256 x 47 FP32 46 us,
-// 2.5 TB/s; 1,000,000 x 128 x 256 330.
+// Measured, 4096 x 4096 x 4096: FP32 454 us and f16 332, 303 and 414 TFLOP/s (910 and 830 of the MFMA's), bound by the
+// split into parts and by LDS, which each part passes through; bf16 of odd rows 210. 262,144 x 256 x 47 FP32 46 us,
+// 2.5 TB/s, without columns of x (the bias gradient alone) 24, 2.1 TB/s of dy; 1,000,000 x 128 x 256 268.
 template <typename T, unsigned BN, unsigned BK, unsigned WN, unsigned WK, bool Narrow>
 __global__ __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(2))) void sumRows(Gradient a) {
     constexpr unsigned P = Parts<T>::count, Threads = 64 * WN * WK, NT = BN / WN / 16, KT = BK / WK / 16;
@@ -285,7 +285,7 @@ __device__ __forceinline__ void multiplyInPlace(f32x16& acc, bf16x8 a, bf16x8 b)
 // A step's bytes are loaded to registers two steps ahead, and written to the other stage while the step before
 // is multiplied; one barrier a step, before its last chunk.
 // Bias: the workgroup also sums dy's columns, from the registers that they pass through.
-// Measured: 8192 x 4096 x 8192 537 us, 1.02 PFLOP/s, and 4096 x 4096 x 4096 140 (a library's product of bf16 matrices
+// Measured: 8192 x 4096 x 8192 537 us, 1.02 PFLOP/s, and 4096 x 4096 x 4096 129 (a library's product of bf16 matrices
 // 372 and 96); the MFMAs' cycles are 58% of it, the rest is issuing conversions, LDS writes and transposing reads beside
 // them. 2048 x 1024 x 4096 32 us in tiles of 128, one a unit.
 template <unsigned B, bool Bias> __device__ __forceinline__ void sumTile(const Gradient& a, std::uint8_t* lds) {
