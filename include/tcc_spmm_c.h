@@ -161,6 +161,59 @@ int tcc_linear_blocks_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32
 int tcc_weight_grad_blocks_form(const void* dy, uint64_t stride, uint32_t type, uint32_t rows, uint32_t inner,
                                 uint32_t outer, const char** form, uint32_t* splits);
 
+/* ---- layers with weights in microscaled 4-bit blocks, and of many experts (HIP; include/micro.h and
+ * include/experts.h, no reference counterpart) ----
+ * Dense matrices as above. Rows of codes are E4M3 blocks of 128 (format 0) or microscaled blocks (format 1), weights
+ * microscaled blocks, laid out as the headers say. Zero rows or choices return TCC_OK without a launch. */
+int tcc_quantize_micro(const void* x, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                       uint32_t rows, uint32_t columns, void* stream);
+int tcc_dequantize_micro(const uint8_t* codes, const uint8_t* exponents, void* out, uint64_t stride, uint32_t type,
+                         uint32_t rows, uint32_t columns, void* stream);
+/* Weights in tiles, with their transposed copies if codesT and exponentsT are given. */
+int tcc_quantize_weight_micro(const void* w, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                              uint8_t* codesT, uint8_t* exponentsT, uint32_t experts, uint32_t outer, uint32_t inner,
+                              void* stream);
+int tcc_matmul_micro(const uint8_t* xCodes, const uint8_t* xExponents, uint32_t format, const uint8_t* wCodes,
+                     const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type, uint32_t rows,
+                     uint32_t inner, uint32_t outer, void* stream);
+int tcc_linear_micro_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format, int keep,
+                               size_t* bytes);
+/* keepCodes and keepExponents may be null: x's E4M3 blocks are not kept then. */
+int tcc_linear_micro(const void* x, uint64_t stride, uint32_t type, uint32_t format, const uint8_t* wCodes,
+                     const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride, uint8_t* keepCodes,
+                     uint8_t* keepExponents, uint32_t rows, uint32_t inner, uint32_t outer, void* workspace,
+                     size_t workspaceBytes, void* stream);
+int tcc_matmul_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format,
+                          const char** form);
+/* A plan is offsets [experts + 1], order and places [choices], int32 in device memory. */
+int tcc_sort_experts_workspace(uint32_t choices, uint32_t experts, size_t* bytes);
+int tcc_sort_experts(const void* ids, uint32_t idBytes, int32_t* offsets, int32_t* order, int32_t* places,
+                     uint32_t choices, uint32_t experts, void* workspace, size_t workspaceBytes, void* stream);
+int tcc_gather_experts(const void* x, uint64_t stride, uint32_t type, const int32_t* offsets, const int32_t* places,
+                       uint32_t choices, uint32_t each, uint32_t experts, void* rows, uint64_t rowsStride, uint32_t width,
+                       void* stream);
+/* weights may be null: ones. */
+int tcc_combine_experts(const void* rows, uint64_t stride, uint32_t type, const int32_t* offsets, const int32_t* places,
+                        uint32_t choices, uint32_t each, uint32_t experts, const void* weights, uint32_t weightType,
+                        void* y, uint64_t yStride, uint32_t width, void* stream);
+/* drows or dweights may be null; without dweights rows are not read. */
+int tcc_combine_experts_backward(const void* dy, uint64_t dyStride, const void* rows, uint64_t stride, uint32_t type,
+                                 const int32_t* offsets, const int32_t* places, uint32_t choices, uint32_t each,
+                                 uint32_t experts, const void* weights, uint32_t weightType, void* drows,
+                                 uint64_t drowsStride, void* dweights, uint32_t width, void* stream);
+int tcc_matmul_experts(const uint8_t* xCodes, const uint8_t* xExponents, uint32_t format, int byToken,
+                       const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t stride,
+                       uint32_t type, const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each,
+                       uint32_t experts, uint32_t inner, uint32_t outer, void* stream);
+int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, int byToken, uint32_t inner, uint32_t format,
+                                 size_t* bytes);
+int tcc_linear_experts(const void* x, uint64_t stride, uint32_t type, uint32_t format, int byToken,
+                       const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride,
+                       const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each, uint32_t experts,
+                       uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes, void* stream);
+int tcc_matmul_experts_form(uint32_t choices, uint32_t experts, uint32_t inner, uint32_t outer, uint32_t type,
+                            uint32_t format, const char** form);
+
 /* DeviceMatrix — reference src/device_matrix.cuh:8-37: uploads every array of a bucketed format,
  * allocates partials (partialCount*8*features floats) and counters (nSW*(features/128) uint32,
  * zeroed) when partialCount > 0, and hands out the view and the workspace. */

@@ -5,6 +5,7 @@
 
 #include "blocks.h"
 #include "device_matrix.h"
+#include "experts.h"
 #include "format/csr.h"
 #include "format/int8_features.h"
 #include "format/sw32.h"
@@ -63,6 +64,8 @@ void need(const void* p, const char* what) {
 
 // The library's functions only read through the pointers of an input's blocks.
 std::uint8_t* input(const uint8_t* p) { return const_cast<std::uint8_t*>(p); }
+
+std::int32_t* input(const int32_t* p) { return const_cast<std::int32_t*>(p); }
 
 Sw32DeviceView toView(const tcc_device_view* v) {
     Sw32DeviceView out;
@@ -365,6 +368,152 @@ int tcc_activation_blocks_backward(const void* dy, uint64_t stride, uint32_t typ
         activationBlocksBackward({dy, stride, DenseType(type)}, {input(codes), input(exponents), BlockCodes(codeType)},
                                  BlockActivation(kind), gated != 0, dx, dxStride, rows, width,
                                  static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_quantize_micro(const void* x, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                       uint32_t rows, uint32_t columns, void* stream) {
+    return guarded([&] {
+        quantizeMicro({x, stride, DenseType(type)}, {codes, exponents}, rows, columns, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_dequantize_micro(const uint8_t* codes, const uint8_t* exponents, void* out, uint64_t stride, uint32_t type,
+                         uint32_t rows, uint32_t columns, void* stream) {
+    return guarded([&] {
+        dequantizeMicro({input(codes), input(exponents)}, out, DenseType(type), stride, rows, columns,
+                        static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_quantize_weight_micro(const void* w, uint64_t stride, uint32_t type, uint8_t* codes, uint8_t* exponents,
+                              uint8_t* codesT, uint8_t* exponentsT, uint32_t experts, uint32_t outer, uint32_t inner,
+                              void* stream) {
+    return guarded([&] {
+        quantizeWeightMicro({w, stride, DenseType(type)}, {codes, exponents}, {codesT, exponentsT}, experts, outer, inner,
+                            static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_matmul_micro(const uint8_t* xCodes, const uint8_t* xExponents, uint32_t format, const uint8_t* wCodes,
+                     const uint8_t* wExponents, const float* bias, void* y, uint64_t stride, uint32_t type, uint32_t rows,
+                     uint32_t inner, uint32_t outer, void* stream) {
+    return guarded([&] {
+        matmulMicro({input(xCodes), input(xExponents), RowFormat(format)}, {input(wCodes), input(wExponents)}, bias, y,
+                    DenseType(type), stride, rows, inner, outer, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_linear_micro_workspace(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format, int keep,
+                               size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = linearMicroWorkspace(rows, inner, outer, DenseType(type), RowFormat(format), keep != 0);
+    });
+}
+
+int tcc_linear_micro(const void* x, uint64_t stride, uint32_t type, uint32_t format, const uint8_t* wCodes,
+                     const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride, uint8_t* keepCodes,
+                     uint8_t* keepExponents, uint32_t rows, uint32_t inner, uint32_t outer, void* workspace,
+                     size_t workspaceBytes, void* stream) {
+    return guarded([&] {
+        linearMicro({x, stride, DenseType(type)}, RowFormat(format), {input(wCodes), input(wExponents)}, bias, y, yStride,
+                    {keepCodes, keepExponents, BlockCodes::e4m3}, rows, inner, outer, workspace, workspaceBytes,
+                    static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_matmul_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format,
+                          const char** form) {
+    return guarded([&] {
+        need(form, "name of the form");
+        *form = matmulMicroForm(rows, inner, outer, DenseType(type), RowFormat(format));
+    });
+}
+
+int tcc_sort_experts_workspace(uint32_t choices, uint32_t experts, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = sortExpertsWorkspace(choices, experts);
+    });
+}
+
+int tcc_sort_experts(const void* ids, uint32_t idBytes, int32_t* offsets, int32_t* order, int32_t* places,
+                     uint32_t choices, uint32_t experts, void* workspace, size_t workspaceBytes, void* stream) {
+    return guarded([&] {
+        sortExperts(ids, idBytes, {offsets, order, places, choices, 1, experts}, workspace, workspaceBytes,
+                    static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_gather_experts(const void* x, uint64_t stride, uint32_t type, const int32_t* offsets, const int32_t* places,
+                       uint32_t choices, uint32_t each, uint32_t experts, void* rows, uint64_t rowsStride, uint32_t width,
+                       void* stream) {
+    return guarded([&] {
+        gatherExperts({x, stride, DenseType(type)}, {input(offsets), nullptr, input(places), choices, each, experts}, rows,
+                      rowsStride, width, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_combine_experts(const void* rows, uint64_t stride, uint32_t type, const int32_t* offsets, const int32_t* places,
+                        uint32_t choices, uint32_t each, uint32_t experts, const void* weights, uint32_t weightType,
+                        void* y, uint64_t yStride, uint32_t width, void* stream) {
+    return guarded([&] {
+        combineExperts({rows, stride, DenseType(type)}, {input(offsets), nullptr, input(places), choices, each, experts},
+                       weights, DenseType(weightType), y, yStride, width, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_combine_experts_backward(const void* dy, uint64_t dyStride, const void* rows, uint64_t stride, uint32_t type,
+                                 const int32_t* offsets, const int32_t* places, uint32_t choices, uint32_t each,
+                                 uint32_t experts, const void* weights, uint32_t weightType, void* drows,
+                                 uint64_t drowsStride, void* dweights, uint32_t width, void* stream) {
+    return guarded([&] {
+        combineExpertsBackward({dy, dyStride, DenseType(type)}, {rows, stride, DenseType(type)},
+                               {input(offsets), nullptr, input(places), choices, each, experts}, weights,
+                               DenseType(weightType), drows, drowsStride, dweights, width,
+                               static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_matmul_experts(const uint8_t* xCodes, const uint8_t* xExponents, uint32_t format, int byToken,
+                       const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t stride,
+                       uint32_t type, const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each,
+                       uint32_t experts, uint32_t inner, uint32_t outer, void* stream) {
+    return guarded([&] {
+        matmulExperts({input(xCodes), input(xExponents), RowFormat(format)}, byToken != 0,
+                      {input(wCodes), input(wExponents)}, bias, y, DenseType(type), stride,
+                      {input(offsets), input(order), nullptr, choices, each, experts}, inner, outer,
+                      static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, int byToken, uint32_t inner, uint32_t format,
+                                 size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "workspace size");
+        *bytes = linearExpertsWorkspace({nullptr, nullptr, nullptr, choices, each, 1}, byToken != 0, inner,
+                                        RowFormat(format));
+    });
+}
+
+int tcc_linear_experts(const void* x, uint64_t stride, uint32_t type, uint32_t format, int byToken,
+                       const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride,
+                       const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each, uint32_t experts,
+                       uint32_t inner, uint32_t outer, void* workspace, size_t workspaceBytes, void* stream) {
+    return guarded([&] {
+        linearExperts({x, stride, DenseType(type)}, RowFormat(format), byToken != 0, {input(wCodes), input(wExponents)},
+                      bias, y, yStride, {input(offsets), input(order), nullptr, choices, each, experts}, inner, outer,
+                      workspace, workspaceBytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+int tcc_matmul_experts_form(uint32_t choices, uint32_t experts, uint32_t inner, uint32_t outer, uint32_t type,
+                            uint32_t format, const char** form) {
+    return guarded([&] {
+        need(form, "name of the form");
+        *form = matmulExpertsForm({nullptr, nullptr, nullptr, choices, 1, experts}, inner, outer, DenseType(type),
+                                  RowFormat(format));
     });
 }
 

@@ -1,0 +1,837 @@
+// Products with weights in microscaled 4-bit blocks, y = x w^T + bias (include/micro.h), the linear layer on dense x, and
+// the experts' products (include/experts.h).
+//
+// What the kernels share. The weight is the scaled MFMA's first operand, x its second; 16 rows of each by 128 elements of
+// the inner axis, a step. Of a row in 4 bits a lane takes 32 elements in a row, 16 bytes, block g = lane / 16 of the
+// step, and gives that block's scale; of a row in 8 bits it takes elements 16 g to 16 g + 15 and 64 more, which is how
+// the instruction pairs them, and the row's one scale. A dword of exponents has four steps, a byte each, for
+// either (include/micro.h), so that no kernel moves them about.
+#include "blocks/device_product.h"
+#include "experts.h"
+#include "hip_support.h"
+#include "micro/device_micro.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace micro;
+
+struct Product {
+    const std::uint8_t *x, *xe;
+    const std::uint8_t *w, *we;
+    const float* bias;
+    void* y;
+    std::uint64_t yStride;
+    unsigned rows, inner, outer, count; // count: steps of a row
+    unsigned tilesM, tilesN;            // experts: tilesM is the most that their rows can make
+    const void* dense;
+    std::uint64_t denseStride;
+    std::uint8_t *keep, *keepExp;
+    // Experts: rows are the plan's choices.
+    const std::int32_t *offsets, *order; // null order: x has a row for each
+    unsigned experts, each;
+};
+
+// Bytes of rows of codes and of exponents.
+template <bool X8> __device__ __forceinline__ unsigned xPitch(const Product& a) { return a.count * (X8 ? kStep : kStep / 2); }
+template <bool X8> __device__ __forceinline__ unsigned xExpPitch(const Product& a) { return (a.count + 3) / 4 * (X8 ? 4 : 16); }
+__device__ __forceinline__ unsigned wPitch(const Product& a) { return a.count * (kStep / 2); }
+__device__ __forceinline__ unsigned wExpPitch(const Product& a) { return (a.count + 3) / 4 * 16; }
+
+// Steps in which block g of the four holds elements of the row.
+__device__ __forceinline__ unsigned stepsOfLane(const Product& a, unsigned g) {
+    return ((a.inner + kMicroBlock - 1) / kMicroBlock + 3 - g) / 4;
+}
+
+// acc += w x of one step; ws and xs have the scales in byte S.
+template <bool X8, unsigned S>
+__device__ __forceinline__ f32x4 multiply(u32x4 w, u32x4 x0, u32x4 x1, f32x4 acc, unsigned ws, unsigned xs) {
+    const u32x4 none = {};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(w, none), X8 ? join(x0, x1) : join(x0, none), acc, 4,
+                                                            X8 ? 0 : 4, S, int(ws), S, int(xs));
+}
+
+// The values of 8 E2M1 codes as bf16, exact at every finite scale.
+__device__ __forceinline__ bf16x8 microValues8(unsigned q, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3);
+    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// ------------------------------------------------------------------------------------------------
+// Experts: which rows a workgroup multiplies with which weight.
+//
+// The row tiles of all experts, one expert after the other and at last the rows of none, are numbered; how many each has
+// is known to the device alone. A wave counts them, 64 experts at a time, and finds the one that its number falls
+// into. A launch has as many workgroups as any plan of these sizes can need; those past the last tile end at once.
+struct Span {
+    unsigned expert, first, end; // rows [first, end) of the tile's expert
+};
+
+__device__ __forceinline__ unsigned tilesOfLane(const Product& a, unsigned e, unsigned tile, unsigned& lo, unsigned& hi) {
+    lo = e <= a.experts ? min(unsigned(a.offsets[e]), a.rows) : a.rows;
+    hi = e < a.experts ? min(unsigned(a.offsets[e + 1]), a.rows) : a.rows;
+    hi = max(lo, hi);
+    return (hi - lo + tile - 1) / tile;
+}
+
+__device__ __forceinline__ unsigned scanWave(unsigned v, unsigned lane) {
+#pragma unroll
+    for (unsigned by = 1; by < kWave; by *= 2) {
+        const unsigned up = unsigned(__shfl_up(int(v), by));
+        v += lane >= by ? up : 0;
+    }
+    return v;
+}
+
+// Row tiles of `tile` rows in all.
+__device__ __forceinline__ unsigned countTiles(const Product& a, unsigned tile, unsigned lane) {
+    unsigned total = 0, lo, hi;
+    for (unsigned base = 0; base <= a.experts; base += kWave) {
+        unsigned n = tilesOfLane(a, base + lane, tile, lo, hi);
+#pragma unroll
+        for (unsigned by = kWave / 2; by; by /= 2) n += unsigned(__shfl_xor(int(n), by));
+        total += n;
+    }
+    return __builtin_amdgcn_readfirstlane(total);
+}
+
+// The rows of row tile `id`, which countTiles has found to be one.
+__device__ __forceinline__ Span spanOf(const Product& a, unsigned id, unsigned tile, unsigned lane) {
+    unsigned before = 0;
+    for (unsigned base = 0; base <= a.experts; base += kWave) {
+        unsigned lo, hi;
+        const unsigned n = tilesOfLane(a, base + lane, tile, lo, hi);
+        const unsigned upTo = scanWave(n, lane) + before;
+        const unsigned last = __builtin_amdgcn_readlane(upTo, kWave - 1);
+        if (id < last) {
+            const unsigned at = unsigned(__builtin_ctzll(__ballot(upTo > id)));
+            const unsigned start = __builtin_amdgcn_readlane(upTo - n, at);
+            return {base + at, unsigned(__builtin_amdgcn_readlane(lo, at)) + (id - start) * tile,
+                    unsigned(__builtin_amdgcn_readlane(hi, at))};
+        }
+        before = last;
+    }
+    return {a.experts, a.rows, a.rows};
+}
+
+// The row of x that sorted row r takes.
+__device__ __forceinline__ unsigned sourceOf(const Product& a, unsigned r) {
+    r = min(r, a.rows - 1);
+    return a.order ? min(unsigned(a.order[r]), a.rows - 1) / a.each : r;
+}
+
+// Zeros for rows of no expert.
+template <typename T>
+__device__ __forceinline__ void zeroTile(const Product& a, const Span& s, unsigned rows, unsigned tn, unsigned columns) {
+    const unsigned end = min(s.end, s.first + rows);
+    for (unsigned i = threadIdx.x; i < rows * columns; i += blockDim.x) {
+        const unsigned row = s.first + i / columns, column = tn + i % columns;
+        if (row < end && column < a.outer) static_cast<typename T::Raw*>(a.y)[row * a.yStride + column] = T::put(0.0f);
+    }
+}
+
+// A workgroup's tile, of rows [first, end) of its weight, which `a` has afterwards. False: it has nothing left to do.
+template <typename T, bool Experts, unsigned BM, unsigned BN>
+__device__ __forceinline__ bool findTile(Product& a, unsigned lane, unsigned& first, unsigned& end, unsigned& tn) {
+    if constexpr (Experts) {
+        const unsigned tilesM = countTiles(a, BM, lane), total = tilesM * a.tilesN;
+        if (blockIdx.x >= total) return false;
+        const unsigned tile = tileOf(blockIdx.x, total, tilesM, a.tilesN);
+        const Span s = spanOf(a, tile % tilesM, BM, lane);
+        tn = tile / tilesM * BN;
+        if (s.expert >= a.experts) {
+            zeroTile<T>(a, s, BM, tn, BN);
+            return false;
+        }
+        first = s.first, end = s.end;
+        a.w += std::uint64_t(s.expert) * a.outer * wPitch(a);
+        a.we += std::uint64_t(s.expert) * a.outer * wExpPitch(a);
+        if (a.bias) a.bias += std::uint64_t(s.expert) * a.outer;
+    } else {
+        const unsigned tile = tileOf(blockIdx.x, gridDim.x, a.tilesM, a.tilesN);
+        first = tile % a.tilesM * BM, end = a.rows, tn = tile / a.tilesM * BN;
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Tiles of BM x BN. A step of the loop is 128 bytes of each of x's rows: 128 elements in 8 bits, 256 in 4, of which each
+// half is an MFMA's. They and the weight's rows are loaded to LDS without passing registers, Stages deep. The
+// 16-byte chunks of a row are stored in an order that depends on the row, so that the rows an MFMA operand takes at once
+// lie in different banks. Rows of the weight are dealt to pairs of MFMAs so that a lane ends with 8
+// consecutive outputs of one row of y. Groups of waves share a tile where there are few, each with a run of the inner axis
+// and stages of its own; the first adds the others' sums.
+template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
+__global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
+    constexpr unsigned Waves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+    constexpr unsigned Halves = X8 ? 1 : 2, Dword = 4 / Halves; // MFMAs of a step; steps of a dword of exponents
+    constexpr unsigned WRow = Halves * 64, Stage = BM * 128 + BN * WRow; // bytes
+    constexpr unsigned XL = BM / 8 / Waves, WL = BN * WRow / 1024 / Waves;
+    static_assert(XL * Waves * 8 == BM && WL * Waves * 1024 == BN * WRow, "whole loads of a wave");
+    static_assert((Stages == 2 || Stages == 4) && Dword % Halves == 0, "the stage is a constant of the unrolled step");
+    static_assert(NT % 2 == 0 && Waves % 2 == 0, "pairs of operands; keys take bit 3 of the row");
+    extern __shared__ __align__(1024) std::uint8_t shared[];
+    const unsigned lane = threadIdx.x % kWave, allWaves = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned wave = allWaves % Waves, part = Groups == 1 ? 0 : allWaves / Waves;
+    std::uint8_t* lds = shared + part * Stages * Stage;
+    unsigned tm, end, tn;
+    if (!findTile<T, Experts, BM, BN>(a, lane, tm, end, tn)) return;
+    const unsigned all = (a.count + Halves - 1) / Halves; // steps; this group's are `steps` from `first` on
+    const unsigned steps = Groups == 1 ? all : (all + Dword * Groups - 1) / (Dword * Groups) * Dword, first = part * steps;
+    const unsigned pitch = xPitch<X8>(a), pitchW = wPitch(a);
+    // Rows past the end are past the buffer and read as zeros, or another expert's; their results are not stored.
+    const bool byToken = Experts && a.order;
+    const auto xr = rowsAt(a.x, pitch, byToken ? 0 : tm, byToken ? a.rows / a.each : a.rows);
+    const auto wr = rowsAt(a.w, pitchW, tn, a.outer);
+    const unsigned fill = wave * 8 + lane / 8, chunk = (lane % 8) ^ (fill & 7);
+    unsigned xo[XL];
+#pragma unroll
+    for (unsigned j = 0; j < XL; ++j) {
+        const unsigned r = fill + j * Waves * 8;
+        xo[j] = (byToken ? sourceOf(a, tm + r) : r) * pitch + chunk * 16;
+    }
+    const unsigned fillW = X8 ? wave * 16 + lane / 4 : fill;
+    auto keyW = [](unsigned r) { return X8 ? (r >> 1 & 1) | (r >> 2 & 2) : (r & 3) | (r >> 1 & 4); };
+    const unsigned chunkW = X8 ? (lane % 4) ^ keyW(fillW) : (lane % 8) ^ keyW(fillW);
+    const unsigned wo = fillW * pitchW + chunkW * 16;
+    // An odd number of steps of 128 ends in the middle of the last 256: the weight's second half is zeros there, and x's,
+    // finite codes of the next row, count nothing.
+    const unsigned woLast = a.count % Halves && chunkW >= 4 ? 0x7FFFFFFFu : wo;
+    // Step k's bytes into stage s; past the last zeros, from beyond the buffer, so that every wave has the same number
+    // of loads outstanding.
+    auto load = [&](unsigned k, unsigned s) {
+        std::uint8_t* to = lds + s * Stage + wave * 1024;
+        const unsigned w = k + 1 == all ? woLast : wo, fromX = k < all ? k * 128 : 0x7FFFFFFFu;
+        const unsigned fromW = k < all ? k * WRow : 0x7FFFFFFFu;
+#pragma unroll
+        for (unsigned j = 0; j < XL; ++j) loadToLds(xr, to + j * Waves * 1024, xo[j], fromX);
+#pragma unroll
+        for (unsigned j = 0; j < WL; ++j)
+            loadToLds(wr, to + BM * 128 + j * Waves * 1024, w, fromW + j * Waves * (1024 / WRow) * pitchW);
+    };
+    const unsigned wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    const unsigned l16 = lane % 16, g = lane / 16, wRow = l16 / 4 * 8 + l16 % 4;
+    // Exponents of four MFMAs a dword: of this lane's row of each operand.
+    const std::uint8_t *xe[MT], *we[NT];
+    unsigned xs[MT], ws[NT], xsNext[MT], wsNext[NT];
+#pragma unroll
+    for (unsigned m = 0; m < MT; ++m) {
+        const unsigned r = min(tm + wm + m * 16 + l16, a.rows - 1);
+        xe[m] = a.xe + std::uint64_t(byToken ? sourceOf(a, r) : r) * xExpPitch<X8>(a) + (X8 ? 0 : 4 * g);
+    }
+#pragma unroll
+    for (unsigned n = 0; n < NT; ++n)
+        we[n] = a.we + std::uint64_t(min(tn + wn + n / 2 * 32 + n % 2 * 4 + wRow, a.outer - 1)) * wExpPitch(a) + 4 * g;
+    const unsigned lastDword = (a.count - 1) / 4, mine = stepsOfLane(a, g);
+    auto loadExponents = [&](unsigned dword) {
+        dword = min(dword, lastDword);
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) xsNext[m] = *reinterpret_cast<const unsigned*>(xe[m] + dword * (X8 ? 4 : 16));
+#pragma unroll
+        for (unsigned n = 0; n < NT; ++n) wsNext[n] = *reinterpret_cast<const unsigned*>(we[n] + dword * 16);
+    };
+    f32x4 acc[NT][MT] = {};
+    loadExponents(first / Dword);
+#pragma unroll
+    for (unsigned s = 0; s + 1 < Stages; ++s) load(first + s, s);
+    const unsigned xKey = l16 & 7, wKey = keyW(wRow);
+    const std::uint8_t* xRead = lds + (wm + l16) * 128;
+    const std::uint8_t* wRead = lds + BM * 128 + (wn + wRow) * WRow;
+    auto step = [&](unsigned k, auto sel) {
+        constexpr unsigned S = decltype(sel)::value;
+        constexpr unsigned at = S % Stages * Stage;
+        waitBarrier<(Stages - 2) * (XL + WL)>();
+        load(k + Stages - 1, (S + Stages - 1) % Stages);
+        u32x4 xf[MT][2];
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) {
+            xf[m][0] = *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * 128 + ((g ^ xKey) * 16));
+            xf[m][1] = *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * 128 + (((g + 4) ^ xKey) * 16));
+        }
+#pragma unroll
+        for (unsigned n = 0; n < NT; ++n) {
+            const std::uint8_t* r = wRead + at + (n / 2 * 32 + n % 2 * 4) * WRow;
+            const u32x4 w0 = *reinterpret_cast<const u32x4*>(r + ((g ^ wKey) * 16));
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m)
+                acc[n][m] = multiply<X8, S * Halves % 4>(w0, xf[m][0], xf[m][1], acc[n][m], ws[n], xs[m]);
+            if constexpr (!X8) {
+                const u32x4 w1 = *reinterpret_cast<const u32x4*>(r + (((g + 4) ^ wKey) * 16));
+#pragma unroll
+                for (unsigned m = 0; m < MT; ++m)
+                    acc[n][m] = multiply<X8, (S * Halves + 1) % 4>(w1, xf[m][1], xf[m][1], acc[n][m], ws[n], xs[m]);
+            }
+        }
+    };
+    auto nextExponents = [&](unsigned k) {
+        // Past the last block codes are zeros, and so that the products are, the exponents finite.
+        const unsigned keepW = finiteExponents(k * Halves, mine), keepX = X8 ? finiteExponents(k * Halves, a.count) : keepW;
+#pragma unroll
+        for (unsigned m = 0; m < MT; ++m) xs[m] = (xsNext[m] & keepX) | (0x7F7F7F7Fu & ~keepX);
+#pragma unroll
+        for (unsigned n = 0; n < NT; ++n) ws[n] = (wsNext[n] & keepW) | (0x7F7F7F7Fu & ~keepW);
+        loadExponents(k / Dword + 1);
+    };
+    // Steps in runs of four, whose stages are constants, of one or two dwords of exponents.
+    unsigned k = first;
+    auto four = [&](unsigned most) {
+        nextExponents(k);
+        step(k, std::integral_constant<unsigned, 0>{});
+        if (most > 1) step(k + 1, std::integral_constant<unsigned, 1>{});
+        if (most > 2) {
+            if constexpr (Dword == 2) nextExponents(k + 2);
+            step(k + 2, std::integral_constant<unsigned, 2>{});
+        }
+        if (most > 3) step(k + 3, std::integral_constant<unsigned, 3>{});
+    };
+    for (; k + 4 <= first + steps; k += 4) four(4);
+    if (k < first + steps) four(first + steps - k);
+    // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (Groups > 1) {
+        __syncthreads();
+        f32x4* sums = reinterpret_cast<f32x4*>(shared) + wave * NT * MT * kWave + lane;
+        if (part)
+#pragma unroll
+            for (unsigned i = 0; i < NT * MT; ++i)
+                sums[((part - 1) * Waves * NT * MT + i) * kWave] = acc[i / MT][i % MT];
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (unsigned p = 0; p + 1 < Groups; ++p)
+#pragma unroll
+            for (unsigned i = 0; i < NT * MT; ++i) acc[i / MT][i % MT] += sums[(p * Waves * NT * MT + i) * kWave];
+    }
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    auto store = [&](auto whole) {
+        constexpr bool Whole = decltype(whole)::value;
+#pragma unroll
+        for (unsigned n = 0; n < NT; n += 2) {
+            const unsigned column = tn + wn + n * 16 + g * 8;
+            float b[8];
+            bias8<Whole>(a.bias, column, a.outer, b);
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                const unsigned row = tm + wm + m * 16 + l16;
+                float v[8];
+#pragma unroll
+                for (unsigned i = 0; i < 8; ++i) v[i] = acc[n + i / 4][m][i % 4];
+                if (Whole || row < end) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
+            }
+        }
+    };
+    if (tm + BM <= end && tn + BN <= a.outer)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
+}
+
+// ------------------------------------------------------------------------------------------------
+// FP32 outputs of E4M3 rows: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
+// 128 x 128, half a step at a time: a row's 64 values are 128 bytes of LDS.
+template <bool Experts> __global__ __launch_bounds__(256) void microTilesExact(Product a) {
+    constexpr unsigned B = 128;
+    __shared__ __align__(1024) std::uint8_t lds[2][2][B * 128];
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave;
+    unsigned tm, end, tn;
+    if (!findTile<F32, Experts, B, B>(a, lane, tm, end, tn)) return;
+    const unsigned r = t / 4, part = t % 4; // 16 codes of rows r and r + 64 of each operand
+    const std::uint8_t *xp[2], *wp[2], *xep[2], *wep[2];
+#pragma unroll
+    for (unsigned h = 0; h < 2; ++h) {
+        const unsigned row = min(tm + r + 64 * h, a.rows - 1);
+        const std::uint64_t xrow = Experts ? sourceOf(a, row) : row, wrow = min(tn + r + 64 * h, a.outer - 1);
+        xp[h] = a.x + xrow * xPitch<true>(a) + part * 16;
+        xep[h] = a.xe + xrow * xExpPitch<true>(a);
+        wp[h] = a.w + wrow * wPitch(a) + part * 8;
+        wep[h] = a.we + wrow * wExpPitch(a) + part / 2 * 4;
+    }
+    const unsigned blocks = (a.inner + kMicroBlock - 1) / kMicroBlock;
+    u32x4 xq[2];
+    u32x2 wq[2];
+    unsigned xb[2], wb[2];
+    auto fetch = [&](unsigned k) { // half k
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            xq[h] = *reinterpret_cast<const u32x4*>(xp[h] + k * 64);
+            wq[h] = *reinterpret_cast<const u32x2*>(wp[h] + k * 32);
+            xb[h] = xep[h][k / 2];
+            wb[h] = k * 2 + part / 2 < blocks ? wep[h][exponentAt(k / 2, k % 2 * 2)] : 127u;
+        }
+    };
+    auto put = [&](std::uint8_t* to, unsigned row, unsigned i, bf16x8 v) {
+        *reinterpret_cast<bf16x8*>(to + row * 128 + ((2 * part + i) ^ (row & 7)) * 16) = v;
+    };
+    auto stash = [&](unsigned s) {
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            const float xs = scaleOf(xb[h]), ws = scaleOf(wb[h]);
+            put(lds[s][0], r + 64 * h, 0, values8(xq[h].x, xq[h].y, xs));
+            put(lds[s][0], r + 64 * h, 1, values8(xq[h].z, xq[h].w, xs));
+            put(lds[s][1], r + 64 * h, 0, microValues8(wq[h].x, ws));
+            put(lds[s][1], r + 64 * h, 1, microValues8(wq[h].y, ws));
+        }
+    };
+    const unsigned wm = wave % 2 * 64, wn = wave / 2 * 64, l16 = lane % 16, g = lane / 16;
+    f32x4 acc[4][4] = {};
+    const unsigned halves = 2 * a.count;
+    fetch(0);
+    stash(0);
+    __syncthreads();
+    for (unsigned k = 0; k < halves; ++k) {
+        if (k + 1 < halves) fetch(k + 1);
+        const std::uint8_t *bx = lds[k % 2][0], *bw = lds[k % 2][1];
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+            bf16x8 xf[4];
+#pragma unroll
+            for (unsigned m = 0; m < 4; ++m) {
+                const unsigned row = wm + m * 16 + l16;
+                xf[m] = *reinterpret_cast<const bf16x8*>(bx + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
+            }
+#pragma unroll
+            for (unsigned n = 0; n < 4; ++n) {
+                const unsigned row = wn + n * 16 + l16;
+                const bf16x8 wf = *reinterpret_cast<const bf16x8*>(bw + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
+#pragma unroll
+                for (unsigned m = 0; m < 4; ++m)
+                    acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[m], acc[n][m], 0, 0, 0);
+            }
+        }
+        if (k + 1 < halves) {
+            stash((k + 1) % 2);
+            __syncthreads();
+        }
+    }
+    float* y = static_cast<float*>(a.y);
+#pragma unroll
+    for (unsigned n = 0; n < 4; ++n) {
+        const unsigned column = tn + wn + n * 16 + g * 4;
+        const f32x4 b = bias4(a.bias, column, a.outer);
+#pragma unroll
+        for (unsigned m = 0; m < 4; ++m) {
+            const unsigned row = tm + wm + m * 16 + l16;
+            if (row < end) put4(y + row * a.yStride, column, a.outer, acc[n][m] + b);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few rows (single tokens, small batches, experts with a row or a few): a workgroup takes 16 columns of y for up to 64
+// rows; its eight waves share the inner axis, a run of steps each, and add their sums through LDS in the waves' order. The
+// weight's codes go from memory to the MFMA's registers, each byte read once for those rows, four steps' loads at a time
+// before the first is used.
+// Dense: up to kFusedRows rows of dense x, which every workgroup codes for itself into LDS while its first weights are on
+// their way.
+constexpr unsigned kTokenWaves = 8, kFusedRows = 4;
+
+template <typename T, bool X8, unsigned MT, bool Dense, bool Experts>
+__global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
+    constexpr bool Exact = X8 && std::is_same<T, F32>::value;
+    constexpr unsigned Ahead = 4, Rows = 16 * MT; // steps of a wave loaded at a time
+    static_assert(!(Dense && Experts), "experts' rows are coded in a launch of their own");
+    __shared__ f32x4 sums[kTokenWaves][MT][kWave];
+    extern __shared__ __align__(16) std::uint8_t lds[]; // Dense: x's codes, then its exponents
+    const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const unsigned l16 = lane % 16, g = lane / 16, n0 = blockIdx.x * 16;
+    unsigned m0 = Dense ? 0 : blockIdx.y * Rows, end = a.rows;
+    if constexpr (Experts) {
+        if (blockIdx.y >= countTiles(a, Rows, lane)) return;
+        const Span s = spanOf(a, blockIdx.y, Rows, lane);
+        if (s.expert >= a.experts) return zeroTile<T>(a, s, Rows, n0, 16);
+        m0 = s.first, end = s.end;
+        a.w += std::uint64_t(s.expert) * a.outer * wPitch(a);
+        a.we += std::uint64_t(s.expert) * a.outer * wExpPitch(a);
+        if (a.bias) a.bias += std::uint64_t(s.expert) * a.outer;
+    }
+    const unsigned pitch = xPitch<X8>(a), each = (a.count + kTokenWaves - 1) / kTokenWaves;
+    const unsigned from = wave * each, to = min(from + each, a.count);
+    const std::uint64_t wrow = min(n0 + l16, a.outer - 1);
+    const std::uint8_t* wp = a.w + wrow * wPitch(a) + g * 16;
+    const std::uint8_t* wep = a.we + wrow * wExpPitch(a) + g * 4;
+    const unsigned mine = stepsOfLane(a, g);
+    u32x4 w[Ahead];
+    unsigned ws[Ahead];
+    auto fetch = [&](unsigned k) {
+#pragma unroll
+        for (unsigned u = 0; u < Ahead; ++u) {
+            const unsigned at = min(k + u, a.count - 1);
+            w[u] = *reinterpret_cast<const u32x4*>(wp + std::uint64_t(at) * 64);
+            ws[u] = at < mine ? wep[at / 4 * 16 + at % 4] : 127u;
+        }
+    };
+    fetch(from);
+    std::uint8_t* exponents = lds + a.rows * pitch; // Dense: a byte a block, [row][step] or [row][step][4]
+    if constexpr (Dense) {
+        const unsigned sub = t % kBlockLanes;
+        for (unsigned item = t / kBlockLanes; item < a.rows * a.count; item += kWave * kTokenWaves / kBlockLanes) {
+            const unsigned row = item / a.count, step = item - row * a.count;
+            float v[8];
+            load8<T>(static_cast<const typename T::Raw*>(a.dense) + row * a.denseStride, step * kStep + sub * 8, a.inner, v);
+            if constexpr (X8) {
+                const unsigned e = exponentOf<BlockCodes::e4m3>(rowMax(peakBits(v)));
+                const u32x2 q = encode8<BlockCodes::e4m3>(v, e);
+                *reinterpret_cast<u32x2*>(lds + row * pitch + step * kStep + sub * 8) = q;
+                if (sub == 0) exponents[item] = std::uint8_t(e);
+                if (a.keep && blockIdx.x == 0) {
+                    *reinterpret_cast<u32x2*>(a.keep + row * std::uint64_t(pitch) + step * kStep + sub * 8) = q;
+                    if (step + sub < (step + 1 == a.count ? xExpPitch<true>(a) : step + 1))
+                        a.keepExp[row * std::uint64_t(xExpPitch<true>(a)) + step + sub] = std::uint8_t(sub ? 127u : e);
+                }
+            } else {
+                const unsigned e = microExponent(max4(peakBits(v)));
+                *reinterpret_cast<unsigned*>(lds + row * pitch + step * (kStep / 2) + sub * 4) = microEncode<8>(v, e);
+                if (sub % 4 == 0) exponents[item * 4 + sub / 4] = std::uint8_t(e);
+            }
+        }
+        __syncthreads();
+    }
+    const std::uint8_t *xp[MT], *xep[MT];
+#pragma unroll
+    for (unsigned m = 0; m < MT; ++m) {
+        const unsigned r = min(m0 + m * 16 + l16, a.rows - 1), row = Experts ? sourceOf(a, r) : r;
+        xp[m] = (Dense ? lds : a.x) + row * std::uint64_t(pitch) + (Exact ? g * 32 : g * 16);
+        if constexpr (Dense)
+            xep[m] = exponents + row * a.count * (X8 ? 1 : 4) + (X8 ? 0 : g);
+        else
+            xep[m] = a.xe + row * std::uint64_t(xExpPitch<X8>(a)) + (X8 ? 0 : g * 4);
+    }
+    f32x4 acc[MT] = {};
+    for (unsigned k = from; k < to; k += Ahead) {
+        u32x4 x[Ahead][MT][X8 ? 2 : 1];
+        unsigned xs[Ahead][MT];
+#pragma unroll
+        for (unsigned u = 0; u < Ahead; ++u) {
+            const unsigned at = min(k + u, a.count - 1);
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                const std::uint8_t* p = xp[m] + at * (X8 ? kStep : kStep / 2);
+                x[u][m][0] = *reinterpret_cast<const u32x4*>(p);
+                if constexpr (X8) x[u][m][1] = *reinterpret_cast<const u32x4*>(p + (Exact ? 16 : 64));
+                xs[u][m] = X8 || at < mine ? xep[m][X8 ? at : Dense ? at * 4 : at / 4 * 16 + at % 4] : 127u;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0); // the compiler would move the loads down to their use
+#pragma unroll
+        for (unsigned u = 0; u < Ahead; ++u) {
+            if (k + u >= to) break;
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m) {
+                if constexpr (Exact) {
+                    // A lane has elements 32 g to 32 g + 31 of both rows.
+                    const float wScale = scaleOf(ws[u]), xScale = scaleOf(xs[u][m]);
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i)
+                        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            microValues8(w[u][i], wScale),
+                            values8(x[u][m][i / 2][i % 2 * 2], x[u][m][i / 2][i % 2 * 2 + 1], xScale), acc[m], 0, 0, 0);
+                } else {
+                    acc[m] = multiply<X8, 0>(w[u], x[u][m][0], x[u][m][X8 ? 1 : 0], acc[m], ws[u], xs[u][m]);
+                }
+            }
+        }
+        if (k + Ahead < to) fetch(k + Ahead);
+    }
+#pragma unroll
+    for (unsigned m = 0; m < MT; ++m) sums[wave][m][lane] = acc[m];
+    __syncthreads();
+    // Output i of 256 * MT: column fastest.
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    for (unsigned i = t; i < 256 * MT; i += kWave * kTokenWaves) {
+        const unsigned column = i % 16, r = i / 16, row = m0 + r;
+        if (n0 + column >= a.outer || row >= end) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][r / 16][r % 16 + column / 4 * 16][column % 4];
+        if (a.bias) s += a.bias[n0 + column];
+        y[row * a.yStride + n0 + column] = T::put(s);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+
+enum class Form { middle, small, few, tokens, exact };
+const char* formName(Form f) {
+    switch (f) {
+    case Form::middle: return "microTiles128";
+    case Form::small: return "microTiles64";
+    case Form::few: return "microTiles32";
+    case Form::tokens: return "microTokens";
+    default: return "microTilesExact";
+    }
+}
+
+std::uint64_t over(std::uint64_t n, std::uint64_t size) { return (n + size - 1) / size; }
+
+// The most row tiles that `rows` sorted rows of `experts` experts and of none can make.
+std::uint64_t mostTiles(std::uint64_t rows, std::uint64_t experts, unsigned tile) {
+    return std::min(rows, rows / tile + experts + 1);
+}
+
+Form formOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    (void)inner;
+    if (rows <= 64) return Form::tokens;
+    if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
+    const std::uint64_t half = over(rows, 128) * over(outer, 128);
+    return half >= 256 ? Form::middle : over(rows, 64) * over(outer, 64) >= 128 ? Form::small : Form::few;
+}
+
+Form expertFormOf(const ExpertPlan& plan, std::uint32_t outer, DenseType type, RowFormat format) {
+    (void)outer;
+    const std::uint64_t mean = plan.choices / plan.experts;
+    if (mean <= 16) return Form::tokens;
+    if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
+    return mean <= 64 ? Form::small : Form::middle;
+}
+
+template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
+void launchTiles(Product p, hipStream_t stream) {
+    const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, BM) : over(p.rows, BM);
+    p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, BN));
+    const std::uint64_t tiles = up * p.tilesN;
+    constexpr unsigned lds = Groups * Stages * (BM * 128 + BN * (X8 ? 64 : 128));
+    checkGrid("matmul micro", tiles, 64 * WM * WN * Groups);
+    hipLaunchKernelGGL((microTiles<T, X8, Experts, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
+                       dim3(64 * WM * WN * Groups), lds, stream, p);
+    checkHip(hipGetLastError());
+}
+
+template <typename T, bool X8, bool Experts> void launchTokens(const Product& p, hipStream_t stream) {
+    const dim3 threads(kWave * kTokenWaves);
+    const unsigned across = unsigned(over(p.outer, 16));
+    if constexpr (Experts) {
+        const unsigned up = unsigned(mostTiles(p.rows, p.experts, 16)); // expertFormOf: at most 16 rows an expert
+        hipLaunchKernelGGL((microTokens<T, X8, 1, false, true>), dim3(across, up), threads, 0, stream, p);
+    } else if (p.rows <= 16) {
+        hipLaunchKernelGGL((microTokens<T, X8, 1, false, false>), dim3(across), threads, 0, stream, p);
+    } else if (p.rows <= 32) {
+        hipLaunchKernelGGL((microTokens<T, X8, 2, false, false>), dim3(across), threads, 0, stream, p);
+    } else {
+        hipLaunchKernelGGL((microTokens<T, X8, 4, false, false>), dim3(across, unsigned(over(p.rows, 64))), threads, 0,
+                           stream, p);
+    }
+    checkHip(hipGetLastError());
+}
+
+template <typename T, bool X8, bool Experts> void launchForm(Form form, Product p, hipStream_t stream) {
+    switch (form) {
+    case Form::middle: return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
+    case Form::small: return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
+    case Form::few: return launchTiles<T, X8, Experts, 32, 32, 2, 1, 4, 4>(p, stream);
+    case Form::tokens: return launchTokens<T, X8, Experts>(p, stream);
+    case Form::exact: break;
+    }
+    const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 128) : over(p.rows, 128);
+    p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 128));
+    checkGrid("matmul micro", up * p.tilesN, 256);
+    hipLaunchKernelGGL((microTilesExact<Experts>), dim3(unsigned(up * p.tilesN)), dim3(256), 0, stream, p);
+    checkHip(hipGetLastError());
+}
+
+// Calls f with the element type's tag and whether rows are in 8 bits.
+template <typename F> void withRows(DenseType type, RowFormat format, F f) {
+    withType(type, [&](auto tag) {
+        if (format == RowFormat::e4m3)
+            f(tag, std::true_type{});
+        else
+            f(tag, std::false_type{});
+    });
+}
+
+void checkRowCodes(const char* where, const CodedRows& x) {
+    if (x.format == RowFormat::e4m3)
+        checkCodes(where, x.codes, x.exponents);
+    else
+        checkMicro(where, {x.codes, x.exponents});
+}
+
+std::uint64_t codePitch(std::uint32_t inner, RowFormat f) {
+    return f == RowFormat::e4m3 ? blockCodePitch(inner) : microCodePitch(inner);
+}
+std::uint64_t exponentPitch(std::uint32_t inner, RowFormat f) {
+    return f == RowFormat::e4m3 ? blockExponentPitch(inner) : microExponentPitch(inner);
+}
+std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
+
+void encode(DenseMatrix x, CodedRows out, std::uint32_t rows, std::uint32_t inner, hipStream_t stream) {
+    if (out.format == RowFormat::e4m3)
+        quantizeBlocks(x, {out.codes, out.exponents, BlockCodes::e4m3}, rows, inner, stream);
+    else
+        quantizeMicro(x, {out.codes, out.exponents}, rows, inner, stream);
+}
+
+// LDS of x's codes and exponents in a fused product of few rows.
+std::size_t fusedLds(std::uint32_t rows, std::uint32_t inner, RowFormat f) {
+    const std::size_t count = over(inner, kStep);
+    return (rows * count * (f == RowFormat::e4m3 ? kStep + 1 : kStep / 2 + 4) + 15) / 16 * 16;
+}
+bool fusedTokens(std::uint32_t rows, std::uint32_t inner, RowFormat f) {
+    return rows <= kFusedRows && fusedLds(rows, inner, f) <= 48 * 1024;
+}
+
+Product productOf(MicroRows w, const float* bias, void* y, std::uint64_t stride, std::uint32_t rows, std::uint32_t inner,
+                  std::uint32_t outer) {
+    Product p = {};
+    p.w = w.codes, p.we = w.exponents, p.bias = bias, p.y = y, p.yStride = stride;
+    p.rows = rows, p.inner = inner, p.outer = outer, p.count = unsigned(over(inner, kStep));
+    return p;
+}
+
+void checkWeight(const char* where, const MicroRows& w, const float* bias) {
+    checkMicro(where, w);
+    if (reinterpret_cast<std::uintptr_t>(bias) % 4) reject(where, "bias not float-aligned");
+}
+
+} // namespace
+
+const char* matmulMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const char* where = "matmul micro";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkType(where, type);
+    checkFormat(where, format);
+    return formName(formOf(rows, inner, outer, type, format));
+}
+
+void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
+                 std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, hipStream_t stream) {
+    const char* where = "matmul micro";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkRows(where, rows);
+    checkType(where, type);
+    checkFormat(where, x.format);
+    if (!rows) return;
+    checkRowCodes(where, x);
+    checkWeight(where, w, bias);
+    checkDense(where, y, stride, type, outer);
+    Product p = productOf(w, bias, y, stride, rows, inner, outer);
+    p.x = x.codes, p.xe = x.exponents;
+    withRows(type, x.format, [&](auto tag, auto x8) {
+        launchForm<decltype(tag), decltype(x8)::value, false>(formOf(rows, inner, outer, type, x.format), p, stream);
+    });
+}
+
+std::size_t linearMicroWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
+                                 RowFormat format, bool keep) {
+    (void)outer, (void)type;
+    if (keep || fusedTokens(rows, inner, format)) return 0;
+    return rounded(rows * codePitch(inner, format)) + rounded(rows * exponentPitch(inner, format));
+}
+
+void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias, void* y, std::uint64_t yStride,
+                 BlockRows keep, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, void* workspace,
+                 std::size_t workspaceBytes, hipStream_t stream) {
+    const char* where = "linear micro";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkRows(where, rows);
+    checkType(where, x.type);
+    checkFormat(where, format);
+    if (!keep.codes != !keep.exponents) reject(where, "kept codes and exponents come together");
+    if (keep.codes && (format != RowFormat::e4m3 || keep.type != BlockCodes::e4m3))
+        reject(where, "kept blocks must have E4M3 codes");
+    if (!rows) return;
+    checkDense(where, x.data, x.stride, x.type, inner);
+    checkDense(where, y, yStride, x.type, outer);
+    checkWeight(where, w, bias);
+    if (keep.codes) checkCodes(where, keep.codes, keep.exponents);
+    const std::size_t need = linearMicroWorkspace(rows, inner, outer, x.type, format, keep.codes);
+    if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
+    if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
+    if (fusedTokens(rows, inner, format)) {
+        Product p = productOf(w, bias, y, yStride, rows, inner, outer);
+        p.dense = x.data, p.denseStride = x.stride, p.keep = keep.codes, p.keepExp = keep.exponents;
+        withRows(x.type, format, [&](auto tag, auto x8) {
+            hipLaunchKernelGGL((microTokens<decltype(tag), decltype(x8)::value, 1, true, false>),
+                               dim3(unsigned(over(outer, 16))), dim3(kWave * kTokenWaves), fusedLds(rows, inner, format),
+                               stream, p);
+        });
+        return checkHip(hipGetLastError());
+    }
+    auto* spare = static_cast<std::uint8_t*>(workspace);
+    CodedRows coded = {keep.codes, keep.exponents, format};
+    if (!keep.codes) coded = {spare, spare + rounded(rows * codePitch(inner, format)), format};
+    encode(x, coded, rows, inner, stream);
+    matmulMicro(coded, w, bias, y, x.type, yStride, rows, inner, outer, stream);
+}
+
+namespace {
+void checkExperts(const char* where, const ExpertPlan& plan) {
+    if (!plan.experts || plan.experts > kMaxExperts) reject(where, "experts must be 1 to 1024");
+    if (!plan.each || plan.each > kMaxEach) reject(where, "choices of a token must be 1 to 1024");
+    if (plan.choices >> 31) reject(where, "2^31 choices or more");
+    if (plan.choices % plan.each) reject(where, "choices are not whole tokens'");
+    if (!plan.choices) return;
+    if (!plan.offsets || !plan.order) reject(where, "null plan");
+    if (reinterpret_cast<std::uintptr_t>(plan.offsets) % 4 || reinterpret_cast<std::uintptr_t>(plan.order) % 4)
+        reject(where, "plan not aligned to its elements");
+}
+} // namespace
+
+const char* matmulExpertsForm(ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const char* where = "matmul experts";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkType(where, type);
+    checkFormat(where, format);
+    if (!plan.experts || plan.experts > kMaxExperts) reject(where, "experts must be 1 to 1024");
+    return formName(expertFormOf(plan, outer, type, format));
+}
+
+void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
+                   ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, hipStream_t stream) {
+    const char* where = "matmul experts";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkType(where, type);
+    checkFormat(where, x.format);
+    checkExperts(where, plan);
+    if (!plan.choices) return;
+    checkRowCodes(where, x);
+    checkWeight(where, w, bias);
+    checkDense(where, y, stride, type, outer);
+    if (byToken && plan.choices / plan.each * codePitch(inner, x.format) >> 31)
+        reject(where, "codes of tokens of 2^31 bytes or more: gather them");
+    Product p = productOf(w, bias, y, stride, plan.choices, inner, outer);
+    p.x = x.codes, p.xe = x.exponents;
+    p.offsets = plan.offsets, p.order = byToken ? plan.order : nullptr;
+    p.experts = plan.experts, p.each = plan.each;
+    withRows(type, x.format, [&](auto tag, auto x8) {
+        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, outer, type, x.format), p, stream);
+    });
+}
+
+std::size_t linearExpertsWorkspace(ExpertPlan plan, bool byToken, std::uint32_t inner, RowFormat format) {
+    const std::uint64_t rows = byToken && plan.each ? plan.choices / plan.each : plan.choices;
+    return rounded(rows * codePitch(inner, format)) + rounded(rows * exponentPitch(inner, format));
+}
+
+void linearExperts(DenseMatrix x, RowFormat format, bool byToken, MicroRows w, const float* bias, void* y,
+                   std::uint64_t yStride, ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, void* workspace,
+                   std::size_t workspaceBytes, hipStream_t stream) {
+    const char* where = "linear experts";
+    checkColumns(where, inner);
+    checkColumns(where, outer);
+    checkType(where, x.type);
+    checkFormat(where, format);
+    checkExperts(where, plan);
+    if (!plan.choices) return;
+    const std::uint32_t rows = byToken ? plan.choices / plan.each : plan.choices;
+    checkDense(where, x.data, x.stride, x.type, inner);
+    checkDense(where, y, yStride, x.type, outer);
+    checkWeight(where, w, bias);
+    const std::size_t need = linearExpertsWorkspace(plan, byToken, inner, format);
+    if (need > workspaceBytes || !workspace) reject(where, "workspace too small");
+    if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
+    if (byToken && rows * codePitch(inner, format) >> 31) reject(where, "codes of tokens of 2^31 bytes or more: gather them");
+    auto* spare = static_cast<std::uint8_t*>(workspace);
+    const CodedRows coded = {spare, spare + rounded(rows * codePitch(inner, format)), format};
+    encode(x, coded, rows, inner, stream);
+    matmulExperts(coded, byToken, w, bias, y, x.type, yStride, plan, inner, outer, stream);
+}
