@@ -245,8 +245,9 @@ def _counted_waits(instrs, labels, asm_blocks, waits):
             if j < 0 or passed and count >= n:
                 continue
             if instrs[j].startswith(_VMEM):
-                count += 1
-                loads += _loads_to_lds(instrs[j])
+                # Past these numbers more of either change nothing; without a bound a loop of loads would have no end.
+                count = min(count + 1, n + 1)
+                loads = min(loads + _loads_to_lds(instrs[j]), max(most, *between) + 1)
                 if count <= n and loads > most:
                     found.append(f"`{instrs[i]}` may leave {loads} loads to LDS outstanding, not {most}")
                     break

@@ -69,15 +69,22 @@ def check_kernel_asm(src: pathlib.Path = CSRC / "kernel" / "spmm.hip") -> None:
 
 
 # Kernels whose MFMAs are inline assembly, whose latency the compiler does not know.
-INLINE_MFMA = {CSRC / "blocks" / "product.hip": "multiplyWide", CSRC / "blocks" / "weight_grad.hip": "sumRowsInPlace"}
+INLINE_MFMA = {CSRC / "blocks" / "product.hip": "multiplyWide", CSRC / "blocks" / "weight_grad.hip": "sumRowsInPlace",
+               CSRC / "micro" / "multiply.hip": "microWide"}
 
 # Inline waits in front of barriers, as asm_check.check_counted_waits takes them: by kernel, for each vmcnt(N) how many
 # loads to LDS it may leave outstanding and how many there are since the wait before. multiplyWide: what its quarters
 # load, 4 or 8 a wait, after 28 in front of the loop, and nine loads of exponents a pair of blocks (25 - 16, 21 - 12).
-# multiplyTiles of four stages: two stages of 4 loads, after three in front of the loop.
+# multiplyTiles of four stages: two stages of 4 loads, after three in front of the loop. microWide4 and microWide8 as
+# multiplyWide, with 16 loads of exponents, and of rows in 8 bits half as many of the weight; microTiles as multiplyTiles,
+# a stage of 4 loads for rows in 4 bits and of 3 in 8.
 COUNTED_WAITS = {CSRC / "blocks" / "product.hip": {
     "multiplyWide": {25: (16, {4, 8}), 21: (12, {8}), 16: (16, {8}), 12: (12, {8, 28})},
     "multiplyTiles": {8: (8, {4, 12})},
+}, CSRC / "micro" / "multiply.hip": {
+    "microWide4": {32: (16, {4, 8}), 28: (12, {8}), 16: (16, {8}), 12: (12, {8, 28})},
+    "microWide8": {28: (12, {2, 4}), 26: (10, {8}), 12: (12, {4}), 10: (10, {8, 22})},
+    "microTiles": {8: (8, {4, 12}), 6: (6, {3, 9})},
 }}
 
 

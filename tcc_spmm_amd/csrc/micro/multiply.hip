@@ -134,28 +134,38 @@ __device__ __forceinline__ void zeroTile(const Product& a, const Span& s, unsign
     }
 }
 
-// A workgroup's tile, of rows [first, end) of its weight, which `a` has afterwards. False: it has nothing left to do.
+// A workgroup's tile: rows [first, end) of an expert's and columns from tn on. False: it has nothing left to do.
+struct Tile {
+    unsigned expert, first, end, tn;
+};
 template <typename T, bool Experts, unsigned BM, unsigned BN>
-__device__ __forceinline__ bool findTile(Product& a, unsigned lane, unsigned& first, unsigned& end, unsigned& tn) {
+__device__ __forceinline__ bool findTile(const Product& a, unsigned lane, Tile& t) {
     if constexpr (Experts) {
         const unsigned tilesM = countTiles(a, BM, lane), total = tilesM * a.tilesN;
         if (blockIdx.x >= total) return false;
         const unsigned tile = tileOf(blockIdx.x, total, tilesM, a.tilesN);
         const Span s = spanOf(a, tile % tilesM, BM, lane);
-        tn = tile / tilesM * BN;
-        if (s.expert >= a.experts) {
-            zeroTile<T>(a, s, BM, tn, BN);
-            return false;
-        }
-        first = s.first, end = s.end;
-        a.w += std::uint64_t(s.expert) * a.outer * wPitch(a);
-        a.we += std::uint64_t(s.expert) * a.outer * wExpPitch(a);
-        if (a.bias) a.bias += std::uint64_t(s.expert) * a.outer;
+        t = {s.expert, s.first, s.end, tile / tilesM * BN};
+        if (s.expert < a.experts) return true;
+        zeroTile<T>(a, s, BM, t.tn, BN);
+        return false;
     } else {
         const unsigned tile = tileOf(blockIdx.x, gridDim.x, a.tilesM, a.tilesN);
-        first = tile % a.tilesM * BM, end = a.rows, tn = tile / a.tilesM * BN;
+        t = {0, tile % a.tilesM * BM, a.rows, tile / a.tilesM * BN};
+        return true;
     }
-    return true;
+}
+
+// The expert's weight and bias. The tile is the same in all lanes, and said to be: the compiler does not see it behind
+// spanOf's loop, and would read buffers lane by lane.
+template <bool Experts> __device__ __forceinline__ void take(Product& a, Tile& t) {
+    if constexpr (Experts) {
+        t = {unsigned(__builtin_amdgcn_readfirstlane(t.expert)), unsigned(__builtin_amdgcn_readfirstlane(t.first)),
+             unsigned(__builtin_amdgcn_readfirstlane(t.end)), unsigned(__builtin_amdgcn_readfirstlane(t.tn))};
+        const std::uint64_t rows = std::uint64_t(t.expert) * a.outer;
+        a.w += rows * wPitch(a), a.we += rows * wExpPitch(a);
+        if (a.bias) a.bias += rows;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -178,8 +188,10 @@ __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
     const unsigned lane = threadIdx.x % kWave, allWaves = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const unsigned wave = allWaves % Waves, part = Groups == 1 ? 0 : allWaves / Waves;
     std::uint8_t* lds = shared + part * Stages * Stage;
-    unsigned tm, end, tn;
-    if (!findTile<T, Experts, BM, BN>(a, lane, tm, end, tn)) return;
+    Tile found;
+    if (!findTile<T, Experts, BM, BN>(a, lane, found)) return;
+    take<Experts>(a, found);
+    const unsigned tm = found.first, end = found.end, tn = found.tn;
     const unsigned all = (a.count + Halves - 1) / Halves; // steps; this group's are `steps` from `first` on
     const unsigned steps = Groups == 1 ? all : (all + Dword * Groups - 1) / (Dword * Groups) * Dword, first = part * steps;
     const unsigned pitch = xPitch<X8>(a), pitchW = wPitch(a);
@@ -330,6 +342,253 @@ __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
         store(std::false_type{});
 }
 
+// acc += w x of one step, with the scales in byte S of ws and xs, in the accumulation registers: asm with one operand for
+// both the sum and the result, since the compiler moves accumulators that fill the register file about. It does not
+// know this instruction's latency: whoever reads acc has to let the last one finish.
+template <bool X8, unsigned S>
+__device__ __forceinline__ void multiplyInPlace(f32x4& acc, u32x4 w, u32x4 x0, u32x4 x1, unsigned ws, unsigned xs) {
+    const i32x8 x = join(x0, x1);
+    if constexpr (X8) {
+        if constexpr (S == 0)
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
+                : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+        else
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4"
+                : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+    } else {
+        if constexpr (S == 0)
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                : "+a"(acc) : "v"(w), "v"(x0), "v"(ws), "v"(xs));
+        else if constexpr (S == 1)
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                : "+a"(acc) : "v"(w), "v"(x0), "v"(ws), "v"(xs));
+        else if constexpr (S == 2)
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0] cbsz:4 blgp:4"
+                : "+a"(acc) : "v"(w), "v"(x0), "v"(ws), "v"(xs));
+        else
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0] cbsz:4 blgp:4"
+                : "+a"(acc) : "v"(w), "v"(x0), "v"(ws), "v"(xs));
+    }
+}
+
+// The same on tiles of 256 x 256, for products with enough of them: four waves, one a SIMD, of 128 x 128 each, whose
+// accumulators fill the accumulation registers. LDS holds two stages. A step is multiplied in four quarters, a pair of
+// the weight's operands with all of x's in each, first half by half where x is in 4 bits: in a quarter the next pair is read
+// from LDS, and in the last one also, as each operand of x is used for the last time, its place is filled with the next
+// step's. So no MFMA waits for LDS. The loads into LDS are spread over the quarters, each into a place that was read
+// for the last time a quarter or more before, and each has at least a step's time to arrive:
+//   quarter 0: pairs 2 and 3 of step k + 1;  1 and 2: x of step k + 2;  3: pairs 0 and 1 of step k + 2
+// with a barrier before quarters 1 and 3.
+template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wideTile(Product& a) {
+    constexpr unsigned B = 256, Tiles = 8, Halves = X8 ? 1 : 2, WRow = Halves * 64, Stage = B * (128 + WRow);
+    constexpr unsigned WL = B * WRow / 1024 / 4, WRows = 4096 / WRow; // a wave's loads of a step's weight; rows of all four's
+    constexpr unsigned Exps = 2 * Tiles;                               // loads of exponents, for two steps
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages: 256 rows of x, 256 of w
+    const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    Tile found;
+    if (!findTile<T, Experts, B, B>(a, lane, found)) return;
+    take<Experts>(a, found);
+    const unsigned tm = found.first, end = found.end, tn = found.tn;
+    const unsigned all = (a.count + Halves - 1) / Halves, pitch = xPitch<X8>(a), pitchW = wPitch(a);
+    const bool byToken = Experts && a.order;
+    const unsigned xFirst = byToken ? 0 : tm, xRows = byToken ? a.rows / a.each : a.rows;
+    const auto xr = rowsAt(a.x, pitch, xFirst, xRows), wr = rowsAt(a.w, pitchW, tn, a.outer);
+    // Chunks and rows are dealt as in microTiles.
+    auto keyX = [](unsigned r) { return r & 7; };
+    auto keyW = [](unsigned r) { return X8 ? (r >> 1 & 1) | (r >> 2 & 2) : (r & 3) | (r >> 1 & 4); };
+    const unsigned fill = wave * 8 + lane / 8, fillW = X8 ? wave * 16 + lane / 4 : fill;
+    const unsigned chunk = (lane % 8) ^ keyX(fill), chunkW = X8 ? (lane % 4) ^ keyW(fillW) : (lane % 8) ^ keyW(fillW);
+    // A wave's loads are 32 rows of x apart, with the same keys; a token's rows may lie anywhere.
+    unsigned xo[Experts ? 8 : 1];
+#pragma unroll
+    for (unsigned i = 0; i < (Experts ? 8 : 1); ++i)
+        xo[i] = (byToken ? sourceOf(a, tm + fill + i * 32) : fill + i * 32) * pitch + chunk * 16;
+    const unsigned wo = fillW * pitchW + chunkW * 16;
+    const unsigned woLast = a.count % Halves && chunkW >= 4 ? 0x7FFFFFFFu : wo; // the half of a step that is not there
+    // Step k's rows of x or w into stage s; past the last zeros, from beyond the buffer.
+    auto loadX = [&](unsigned k, unsigned s, unsigned part) {
+        const unsigned from = k < all ? k * 128 : 0x7FFFFFFFu;
+        std::uint8_t* to = lds + s * Stage + wave * 1024 + part * 4096;
+        if constexpr (Experts)
+            loadToLds(xr, to, xo[part], from);
+        else
+            loadToLds(xr, to, xo[0], from + part * 32 * pitch);
+    };
+    auto loadW = [&](unsigned k, unsigned s, unsigned part) {
+        const unsigned from = k < all ? k * WRow : 0x7FFFFFFFu;
+        loadToLds(wr, lds + s * Stage + B * 128 + wave * 1024 + part * 4096, k + 1 == all ? woLast : wo,
+                  from + part * WRows * pitchW);
+    };
+    // Load i of the first or the last two pairs of both halves of the waves.
+    auto partW = [](unsigned last, unsigned i) { return X8 ? i * 2 + last : i / 2 + i % 2 * 4 + last * 2; };
+    const unsigned wm = wave % 2 * 128, wn = wave / 2 * 128, l16 = lane % 16, g = lane / 16;
+    const unsigned wRow = l16 / 4 * 8 + l16 % 4;
+    // A lane's chunks of its row in either stage: bytes of LDS, which the loads' offsets reach a stage of.
+    unsigned xRead[2][2], wRead[2][Halves];
+#pragma unroll
+    for (unsigned s = 0; s < 2; ++s) {
+#pragma unroll
+        for (unsigned c = 0; c < 2; ++c) {
+            xRead[s][c] = s * Stage + (wm + l16) * 128 + ((g + 4 * c) ^ keyX(l16)) * 16;
+            asm("" : "+v"(xRead[s][c])); // kept, not computed again for every load
+        }
+#pragma unroll
+        for (unsigned c = 0; c < Halves; ++c) {
+            wRead[s][c] = s * Stage + B * 128 + (wn + wRow) * WRow + ((g + 4 * c) ^ keyW(wRow)) * 16;
+            asm("" : "+v"(wRead[s][c]));
+        }
+    }
+    u32x4 xf[Tiles][2], wf[2][2][Halves];
+    auto readX = [&](unsigned s, unsigned m, unsigned c) {
+        xf[m][c] = *reinterpret_cast<const u32x4*>(lds + m * 16 * 128 + xRead[s][c]);
+    };
+    auto readW = [&](unsigned s, unsigned n) {
+#pragma unroll
+        for (unsigned c = 0; c < Halves; ++c)
+            wf[n / 2 % 2][n % 2][c] = *reinterpret_cast<const u32x4*>(lds + (n / 2 * 32 + n % 2 * 4) * WRow + wRead[s][c]);
+    };
+    // Two steps' exponents at a time, of this lane's row of each operand: a byte for each MFMA.
+    const unsigned pitchXe = xExpPitch<X8>(a), pitchWe = wExpPitch(a), mine = stepsOfLane(a, g);
+    const auto xer = rowsAt(a.xe, pitchXe, xFirst, xRows), wer = rowsAt(a.we, pitchWe, tn, a.outer);
+    unsigned xeo[Experts ? Tiles : 1];
+#pragma unroll
+    for (unsigned m = 0; m < (Experts ? Tiles : 1); ++m) {
+        const unsigned r = wm + m * 16 + l16;
+        xeo[m] = (byToken ? sourceOf(a, tm + r) : r) * pitchXe + (X8 ? 0 : 4 * g);
+    }
+    const unsigned weo = (wn + wRow) * pitchWe + 4 * g;
+    unsigned xs[Tiles], ws[Tiles], xsNext[Tiles], wsNext[Tiles];
+    auto loadExponents = [&](unsigned k) { // of steps k and k + 1, k even
+        k = min(k, (all - 1) / 2 * 2);
+        const unsigned fromX = X8 ? k : k / 2 * 16, fromW = X8 ? k / 4 * 16 + k % 4 : k / 2 * 16;
+#pragma unroll
+        for (unsigned m = 0; m < Tiles; ++m) {
+            const unsigned at = Experts ? xeo[m] : xeo[0], from = fromX + (Experts ? 0 : m * 16 * pitchXe);
+            const unsigned fromN = fromW + (m / 2 * 32 + m % 2 * 4) * pitchWe;
+            if constexpr (X8) {
+                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(xer, at, from, 0);
+                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(wer, weo, fromN, 0);
+            } else {
+                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(xer, at, from, 0);
+                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(wer, weo, fromN, 0);
+            }
+        }
+    };
+    f32x4 acc[Tiles][Tiles] = {};
+    loadExponents(0);
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) loadX(0, 0, i);
+#pragma unroll
+    for (unsigned i = 0; i < WL; ++i) loadW(0, 0, i);
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) loadX(1, 1, i);
+#pragma unroll
+    for (unsigned i = 0; i < WL / 2; ++i) loadW(1, 1, partW(0, i));
+    waitBarrier<8 + WL / 2>();
+#pragma unroll
+    for (unsigned i = 0; i < 2; ++i) readW(0, i);
+#pragma unroll
+    for (unsigned i = 0; i < Tiles; ++i) readX(0, i, 0), readX(0, i, 1);
+    // Step S of the pair that the exponents are for. The fences keep the compiler from moving the reads and loads between
+    // the MFMAs down to where their results are needed, which is where they would be waited for.
+    auto blockStep = [&](unsigned k, auto block) {
+        constexpr unsigned S = decltype(block)::value;
+#pragma unroll
+        for (unsigned q = 0; q < 4; ++q) {
+            // Before quarter 1 pairs 2 and 3 of this step have to be there, before 3 x and pairs 0 and 1 of the next. What
+            // was loaded since stays outstanding, and in a pair's first step the exponents.
+            if (q == 1) waitBarrier<8 + WL + (S == 0 ? Exps : 0)>();
+            if (q == 3) waitBarrier<8 + WL / 2 + (S == 0 ? Exps : 0)>();
+#pragma unroll
+            for (unsigned h = 0; h < Halves; ++h)
+#pragma unroll
+                for (unsigned m = 0; m < Tiles; ++m) {
+                    const unsigned i = h * Tiles + m, turns = Halves * Tiles; // of a quarter
+                    if (i % (turns / 2) == 0) {
+                        if (q < 3)
+                            readW(S, 2 * q + 2 + i / (turns / 2));
+                        else
+                            readW(1 - S, i / (turns / 2));
+                    }
+                    if (i % (turns / 4) == turns / 4 - 1) {
+                        const unsigned j = i / (turns / 4);
+                        if (q == 0 && j < WL / 2) loadW(k + S + 1, 1 - S, partW(1, j));
+                        if (q == 1) loadX(k + S + 2, S, j);
+                        if (q == 2) loadX(k + S + 2, S, 4 + j);
+                        if (q == 3 && j < WL / 2) loadW(k + S + 2, S, partW(0, j));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    auto multiply = [&](unsigned n, auto byte) {
+                        multiplyInPlace<X8, decltype(byte)::value>(acc[n][m], wf[n / 2 % 2][n % 2][h], xf[m][h], xf[m][1],
+                                                                   ws[n], xs[m]);
+                    };
+#pragma unroll
+                    for (unsigned n = 2 * q; n < 2 * q + 2; ++n) {
+                        if (h == 0)
+                            multiply(n, std::integral_constant<unsigned, S * Halves>{});
+                        else
+                            multiply(n, std::integral_constant<unsigned, S * Halves + Halves - 1>{});
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (q == 3) {
+                        readX(1 - S, m, h);
+                        if constexpr (X8) readX(1 - S, m, 1);
+                    }
+                }
+        }
+        // Where the loop ends the compiler copies the sums, without knowing that they come from an MFMA: the last
+        // ones, of up to 8 passes, have to be done by then.
+        if (S == 1)
+            asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[6][6]), "+a"(acc[7][6]), "+a"(acc[6][7]), "+a"(acc[7][7]));
+    };
+    for (unsigned k = 0; k < all; k += 2) {
+        // Past the last block codes are zeros, and have to have finite exponents.
+        const unsigned keepW = finiteExponents(k * Halves, mine), keepX = X8 ? finiteExponents(k, a.count) : keepW;
+#pragma unroll
+        for (unsigned m = 0; m < Tiles; ++m) {
+            xs[m] = (xsNext[m] & keepX) | (0x7F7F7F7Fu & ~keepX);
+            ws[m] = (wsNext[m] & keepW) | (0x7F7F7F7Fu & ~keepW);
+        }
+        loadExponents(k + 2);
+        blockStep(k, std::integral_constant<unsigned, 0>{});
+        blockStep(k, std::integral_constant<unsigned, 1>{});
+    }
+    // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+    auto store = [&](auto whole) {
+        constexpr bool Whole = decltype(whole)::value;
+#pragma unroll
+        for (unsigned n = 0; n < Tiles; n += 2) {
+            const unsigned column = tn + wn + n * 16 + g * 8;
+            float b[8];
+            bias8<Whole>(a.bias, column, a.outer, b);
+#pragma unroll
+            for (unsigned m = 0; m < Tiles; ++m) {
+                const unsigned row = tm + wm + m * 16 + l16;
+                float v[8];
+#pragma unroll
+                for (unsigned j = 0; j < 8; ++j) // one by one: the compiler would move all sums at once, and spill
+                    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[j]) : "a"(acc[n + j / 4][m][j % 4]));
+                if (Whole || row < end) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
+            }
+        }
+    };
+    if (tm + B <= end && tn + B <= a.outer)
+        store(std::true_type{});
+    else
+        store(std::false_type{});
+}
+
+template <typename T, bool Experts>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void microWide8(Product a) {
+    wideTile<T, true, Experts>(a);
+}
+template <typename T, bool Experts>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void microWide4(Product a) {
+    wideTile<T, false, Experts>(a);
+}
+
 // ------------------------------------------------------------------------------------------------
 // FP32 outputs of E4M3 rows: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
 // 128 x 128, half a step at a time: a row's 64 values are 128 bytes of LDS.
@@ -337,8 +596,10 @@ template <bool Experts> __global__ __launch_bounds__(256) void microTilesExact(P
     constexpr unsigned B = 128;
     __shared__ __align__(1024) std::uint8_t lds[2][2][B * 128];
     const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    unsigned tm, end, tn;
-    if (!findTile<F32, Experts, B, B>(a, lane, tm, end, tn)) return;
+    Tile found;
+    if (!findTile<F32, Experts, B, B>(a, lane, found)) return;
+    take<Experts>(a, found);
+    const unsigned tm = found.first, end = found.end, tn = found.tn;
     const unsigned r = t / 4, part = t % 4; // 16 codes of rows r and r + 64 of each operand
     const std::uint8_t *xp[2], *wp[2], *xep[2], *wep[2];
 #pragma unroll
@@ -438,16 +699,15 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
     extern __shared__ __align__(16) std::uint8_t lds[]; // Dense: x's codes, then its exponents
     const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const unsigned l16 = lane % 16, g = lane / 16, n0 = blockIdx.x * 16;
-    unsigned m0 = Dense ? 0 : blockIdx.y * Rows, end = a.rows;
+    Tile found = {0, Dense ? 0 : blockIdx.y * Rows, a.rows, n0};
     if constexpr (Experts) {
         if (blockIdx.y >= countTiles(a, Rows, lane)) return;
         const Span s = spanOf(a, blockIdx.y, Rows, lane);
         if (s.expert >= a.experts) return zeroTile<T>(a, s, Rows, n0, 16);
-        m0 = s.first, end = s.end;
-        a.w += std::uint64_t(s.expert) * a.outer * wPitch(a);
-        a.we += std::uint64_t(s.expert) * a.outer * wExpPitch(a);
-        if (a.bias) a.bias += std::uint64_t(s.expert) * a.outer;
+        found = {s.expert, s.first, s.end, n0};
+        take<true>(a, found);
     }
+    const unsigned m0 = found.first, end = found.end;
     const unsigned pitch = xPitch<X8>(a), each = (a.count + kTokenWaves - 1) / kTokenWaves;
     const unsigned from = wave * each, to = min(from + each, a.count);
     const std::uint64_t wrow = min(n0 + l16, a.outer - 1);
@@ -555,9 +815,10 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
 // ------------------------------------------------------------------------------------------------
 // Host side
 
-enum class Form { middle, small, few, tokens, exact };
+enum class Form { wide, middle, small, few, tokens, exact };
 const char* formName(Form f) {
     switch (f) {
+    case Form::wide: return "microWide";
     case Form::middle: return "microTiles128";
     case Form::small: return "microTiles64";
     case Form::few: return "microTiles32";
@@ -578,15 +839,15 @@ Form formOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseT
     if (rows <= 64) return Form::tokens;
     if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
     const std::uint64_t half = over(rows, 128) * over(outer, 128);
+    if (half >= 1024) return Form::wide;
     return half >= 256 ? Form::middle : over(rows, 64) * over(outer, 64) >= 128 ? Form::small : Form::few;
 }
 
 Form expertFormOf(const ExpertPlan& plan, std::uint32_t outer, DenseType type, RowFormat format) {
-    (void)outer;
     const std::uint64_t mean = plan.choices / plan.experts;
     if (mean <= 16) return Form::tokens;
     if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
-    return mean <= 64 ? Form::small : Form::middle;
+    return mean <= 64 ? Form::small : mean * outer < 512 * 1024 ? Form::middle : Form::wide;
 }
 
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
@@ -598,6 +859,18 @@ void launchTiles(Product p, hipStream_t stream) {
     checkGrid("matmul micro", tiles, 64 * WM * WN * Groups);
     hipLaunchKernelGGL((microTiles<T, X8, Experts, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
                        dim3(64 * WM * WN * Groups), lds, stream, p);
+    checkHip(hipGetLastError());
+}
+
+template <typename T, bool X8, bool Experts> void launchWide(Product p, hipStream_t stream) {
+    const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 256) : over(p.rows, 256);
+    p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 256));
+    checkGrid("matmul micro", up * p.tilesN, 256);
+    const dim3 grid(unsigned(up * p.tilesN)), threads(256);
+    if constexpr (X8)
+        hipLaunchKernelGGL((microWide8<T, Experts>), grid, threads, 2 * 256 * 192, stream, p);
+    else
+        hipLaunchKernelGGL((microWide4<T, Experts>), grid, threads, 2 * 256 * 256, stream, p);
     checkHip(hipGetLastError());
 }
 
@@ -619,12 +892,14 @@ template <typename T, bool X8, bool Experts> void launchTokens(const Product& p,
 }
 
 template <typename T, bool X8, bool Experts> void launchForm(Form form, Product p, hipStream_t stream) {
-    switch (form) {
-    case Form::middle: return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
-    case Form::small: return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
-    case Form::few: return launchTiles<T, X8, Experts, 32, 32, 2, 1, 4, 4>(p, stream);
-    case Form::tokens: return launchTokens<T, X8, Experts>(p, stream);
-    case Form::exact: break;
+    if (form == Form::tokens) return launchTokens<T, X8, Experts>(p, stream);
+    if constexpr (!X8 || !std::is_same<T, F32>::value) {
+        switch (form) {
+        case Form::wide: return launchWide<T, X8, Experts>(p, stream);
+        case Form::middle: return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
+        case Form::small: return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
+        default: return launchTiles<T, X8, Experts, 32, 32, 2, 1, 4, 4>(p, stream);
+        }
     }
     const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 128) : over(p.rows, 128);
     p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 128));

@@ -166,6 +166,13 @@ def test_linear_experts(gpu, tokens, each, experts, inner, outer, dtype, codes, 
     assert not y[offsets[-1]:].any()
 
 
+@pytest.mark.parametrize("tokens,each,experts,inner,outer", [(2100, 3, 5, 500, 600), (1100, 2, 2, 1153, 520), (900, 4, 7, 100, 3000)])
+@pytest.mark.parametrize("dtype,codes", [("bf16", "e4m3"), ("f32", "e2m1"), ("f16", "e2m1")])
+def test_linear_experts_wide(gpu, tokens, each, experts, inner, outer, dtype, codes):
+    """Experts of many rows, which the largest tile takes."""
+    test_linear_experts(gpu, tokens, each, experts, inner, outer, dtype, codes, 0.1, "any")
+
+
 @pytest.mark.parametrize("tokens", [7, 500])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("codes", ["e4m3", "e2m1"])

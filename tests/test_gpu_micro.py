@@ -167,6 +167,13 @@ def test_linear(gpu, rows, inner, outer, dtype, codes):
     near(matmul_micro(coded, weight, bias, dtype=DTYPES[dtype]), want, allowed, "y of coded rows")
 
 
+@pytest.mark.parametrize("rows,inner,outer", [(4090, 200, 4100), (4091, 300, 4099), (3900, 600, 4300), (4097, 1153, 4000)])
+@pytest.mark.parametrize("dtype,codes", [("bf16", "e4m3"), ("f16", "e4m3"), ("f32", "e2m1"), ("bf16", "e2m1"), ("f16", "e2m1")])
+def test_linear_wide(gpu, rows, inner, outer, dtype, codes):
+    """Products of many tiles, which the largest tile takes: odd and even numbers of its steps, ragged edges."""
+    test_linear(gpu, rows, inner, outer, dtype, codes)
+
+
 @pytest.mark.parametrize("codes", ["e4m3", "e2m1"])
 def test_linear_leading_dimensions_and_layouts(gpu, codes):
     from tcc_spmm_amd.micro import linear_micro, quantize_weight_micro
