@@ -18,7 +18,7 @@
 //
 // Every function is asynchronous on `stream` and allocates nothing. Sizes of zero rows return without a
 // launch. Errors are thrown before any launch, as in blocks.h. Rows may be up to 2^31 - 1, their elements up to 2^22, and a
-// product's tiles fewer than 2^24 (of 128 x 128). Codes and exponents must be 16-byte aligned; dense matrices
+// product's tiles fewer than 2^24 (of 64 x 64 for an FP32 y of E4M3 rows, else of 256 x 256). Codes and exponents must be 16-byte aligned; dense matrices
 // need only their element's alignment, with any row stride of at least a row.
 #pragma once
 
@@ -74,4 +74,6 @@ void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias
                  std::size_t workspaceBytes, hipStream_t stream = nullptr);
 
 // The kernel that a call of these sizes takes, by name, for tests and measurements.
+// linearMicro calls matmulMicro where the names are the same.
 const char* matmulMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format);
+const char* linearMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format);

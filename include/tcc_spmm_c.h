@@ -185,6 +185,8 @@ int tcc_linear_micro(const void* x, uint64_t stride, uint32_t type, uint32_t for
                      size_t workspaceBytes, void* stream);
 int tcc_matmul_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format,
                           const char** form);
+int tcc_linear_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format,
+                          const char** form);
 /* A plan is offsets [experts + 1], order and places [choices], int32 in device memory. */
 int tcc_sort_experts_workspace(uint32_t choices, uint32_t experts, size_t* bytes);
 int tcc_sort_experts(const void* ids, uint32_t idBytes, int32_t* offsets, int32_t* order, int32_t* places,

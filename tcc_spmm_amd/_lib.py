@@ -124,6 +124,8 @@ SIGNATURES = {
                                    C.c_void_p, C.c_size_t, C.c_void_p]),
     "tcc_matmul_micro_form": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
                                         C.POINTER(C.c_char_p)]),
+    "tcc_linear_micro_form": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                        C.POINTER(C.c_char_p)]),
     "tcc_sort_experts_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.POINTER(C.c_size_t)]),
     "tcc_sort_experts": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
                                    C.c_void_p, C.c_size_t, C.c_void_p]),

@@ -431,6 +431,14 @@ int tcc_matmul_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_
     });
 }
 
+int tcc_linear_micro_form(uint32_t rows, uint32_t inner, uint32_t outer, uint32_t type, uint32_t format,
+                          const char** form) {
+    return guarded([&] {
+        need(form, "name of the form");
+        *form = linearMicroForm(rows, inner, outer, DenseType(type), RowFormat(format));
+    });
+}
+
 int tcc_sort_experts_workspace(uint32_t choices, uint32_t experts, size_t* bytes) {
     return guarded([&] {
         need(bytes, "workspace size");

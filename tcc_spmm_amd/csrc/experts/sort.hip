@@ -1,9 +1,10 @@
 // Tokens' choices sorted by expert (include/experts.h): a stable counting sort.
 //
-// A workgroup takes kRun choices in order, 64 to a wave at a time. A choice's rank in its wave is the number of lanes
+// A workgroup takes a run of choices in order, 64 to a wave at a time. A choice's rank in its wave is the number of lanes
 // before it with the same expert, found by ballots on the bits of its number, and the wave's own count of that expert
-// so far, which the first such lane then raises. Up to kRun choices one workgroup does it all; more take three
-// launches: each run's counts, their prefix sums for each expert, and the ranks. No order depends on an atomic.
+// so far, which the first such lane then raises. Up to kAlone choices one workgroup does it all. More are runs of kRun, first
+// each run's counts, then the ranks; up to kFewRuns runs each adds the counts before it by itself, for more a launch
+// between the two makes their prefix sums. No order depends on an atomic.
 #include "experts.h"
 #include "hip_support.h"
 #include "blocks/device_blocks.h"
@@ -13,6 +14,7 @@ namespace {
 using namespace blocks;
 
 constexpr unsigned kThreads = 1024, kWaves = kThreads / kWave, kTurns = 4, kRun = kThreads * kTurns;
+constexpr unsigned kAloneTurns = 16, kAlone = kThreads * kAloneTurns, kFewRuns = 64;
 
 struct Sort {
     const void* ids;
@@ -77,8 +79,9 @@ __global__ __launch_bounds__(kThreads) void scanCounts(Sort a) {
     if (threadIdx.x == 0) a.counts[std::uint64_t(a.experts + 1) * a.runs + blockIdx.x] = before;
 }
 
-// Alone: the only run, whose own counts are all there are.
-template <typename Id, bool Alone> __global__ __launch_bounds__(kThreads) void placeChoices(Sort a) {
+// Alone: the only run, whose own counts are all there are. Scanned: counts are those before each run.
+enum class Counts { alone, each, scanned };
+template <typename Id, unsigned Turns, Counts C> __global__ __launch_bounds__(kThreads) void placeChoices(Sort a) {
     extern __shared__ unsigned lds[]; // counts of each wave, [kWaves][experts + 1]; then the first row of each expert
     __shared__ unsigned waves[kWaves];
     const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave, run = blockIdx.x, all = a.experts + 1;
@@ -86,16 +89,16 @@ template <typename Id, bool Alone> __global__ __launch_bounds__(kThreads) void p
     for (unsigned i = t; i < kWaves * all; i += kThreads) lds[i] = 0;
     __syncthreads();
     // A wave's choices lie in a row.
-    const std::uint64_t first = std::uint64_t(run) * kRun + wave * (kTurns * kWave) + lane;
-    unsigned expert[kTurns], rank[kTurns];
+    const std::uint64_t first = std::uint64_t(run) * kRun + wave * (Turns * kWave) + lane;
+    unsigned expert[Turns], rank[Turns];
 #pragma unroll
-    for (unsigned i = 0; i < kTurns; ++i) {
+    for (unsigned i = 0; i < Turns; ++i) {
         const std::uint64_t c = first + i * kWave;
         expert[i] = c < a.choices ? expertOf<Id>(a, unsigned(c)) : ~0u;
     }
     const unsigned bits = 32 - __builtin_clz(a.experts);
 #pragma unroll
-    for (unsigned i = 0; i < kTurns; ++i) {
+    for (unsigned i = 0; i < Turns; ++i) {
         const bool in = expert[i] != ~0u;
         std::uint64_t same = __ballot(in);
         for (unsigned b = 0; b < bits; ++b) {
@@ -121,18 +124,30 @@ template <typename Id, bool Alone> __global__ __launch_bounds__(kThreads) void p
                 lds[w * all + e] = mine;
                 mine += n;
             }
-        if (!Alone) mine = e < all ? a.counts[std::uint64_t(all) * a.runs + e] : 0;
+        unsigned earlier = 0; // of this expert, in the runs before
+        if (C == Counts::scanned && e < all) {
+            mine = a.counts[std::uint64_t(all) * a.runs + e];
+            earlier = a.counts[std::uint64_t(e) * a.runs + run];
+        }
+        if (C == Counts::each && e < all) {
+            mine = 0;
+            for (unsigned r = 0; r < a.runs; ++r) {
+                const unsigned n = a.counts[std::uint64_t(e) * a.runs + r];
+                earlier += r < run ? n : 0;
+                mine += n;
+            }
+        }
         unsigned total;
         const unsigned start = before + scanGroup(mine, waves, total);
         before += total;
         if (e < all) {
-            starts[e] = start + (Alone ? 0 : a.counts[std::uint64_t(e) * a.runs + run]);
+            starts[e] = start + earlier;
             if (run == 0) a.offsets[e] = std::int32_t(start);
         }
     }
     __syncthreads();
 #pragma unroll
-    for (unsigned i = 0; i < kTurns; ++i) {
+    for (unsigned i = 0; i < Turns; ++i) {
         if (expert[i] == ~0u) continue;
         const unsigned c = unsigned(first + i * kWave), row = starts[expert[i]] + counts[expert[i]] + rank[i];
         a.places[c] = std::int32_t(row);
@@ -145,7 +160,7 @@ std::uint64_t runsOf(std::uint32_t choices) { return (std::uint64_t(choices) + k
 } // namespace
 
 std::size_t sortExpertsWorkspace(std::uint32_t choices, std::uint32_t experts) {
-    if (choices <= kRun) return 0;
+    if (choices <= kAlone) return 0;
     return std::size_t((runsOf(choices) + 1) * (std::uint64_t(experts) + 1) * 4 + 255) / 256 * 256;
 }
 
@@ -168,12 +183,18 @@ void sortExperts(const void* ids, std::uint32_t idBytes, ExpertPlan plan, void* 
     const unsigned all = plan.experts + 1, lds = (kWaves + 1) * all * 4;
     const auto sort = [&](auto id) {
         typedef decltype(id) Id;
-        if (!need) {
-            hipLaunchKernelGGL((placeChoices<Id, true>), dim3(1), dim3(kThreads), lds, stream, a);
-        } else {
-            hipLaunchKernelGGL((countChoices<Id>), dim3(a.runs), dim3(kThreads), all * 4, stream, a);
-            hipLaunchKernelGGL(scanCounts, dim3(all), dim3(kThreads), 0, stream, a);
-            hipLaunchKernelGGL((placeChoices<Id, false>), dim3(a.runs), dim3(kThreads), lds, stream, a);
+        const dim3 one(1), runs(a.runs), threads(kThreads);
+        if (plan.choices <= kRun)
+            hipLaunchKernelGGL((placeChoices<Id, kTurns, Counts::alone>), one, threads, lds, stream, a);
+        else if (!need)
+            hipLaunchKernelGGL((placeChoices<Id, kAloneTurns, Counts::alone>), one, threads, lds, stream, a);
+        else
+            hipLaunchKernelGGL((countChoices<Id>), runs, threads, all * 4, stream, a);
+        if (need && a.runs <= kFewRuns)
+            hipLaunchKernelGGL((placeChoices<Id, kTurns, Counts::each>), runs, threads, lds, stream, a);
+        if (need && a.runs > kFewRuns) {
+            hipLaunchKernelGGL(scanCounts, dim3(all), threads, 0, stream, a);
+            hipLaunchKernelGGL((placeChoices<Id, kTurns, Counts::scanned>), runs, threads, lds, stream, a);
         }
     };
     if (idBytes == 4)

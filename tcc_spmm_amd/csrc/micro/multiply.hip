@@ -12,6 +12,7 @@
 #include "micro/device_micro.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -87,35 +88,28 @@ __device__ __forceinline__ unsigned scanWave(unsigned v, unsigned lane) {
     return v;
 }
 
-// Row tiles of `tile` rows in all.
-__device__ __forceinline__ unsigned countTiles(const Product& a, unsigned tile, unsigned lane) {
-    unsigned total = 0, lo, hi;
-    for (unsigned base = 0; base <= a.experts; base += kWave) {
-        unsigned n = tilesOfLane(a, base + lane, tile, lo, hi);
+// Row tile `id` of `tile` rows each, `id` being any function of their number. False: there is no such tile.
+template <typename F>
+__device__ __forceinline__ bool spanOf(const Product& a, unsigned tile, unsigned lane, F idOf, Span& s) {
+    unsigned lo, hi, n = tilesOfLane(a, lane, tile, lo, hi), upTo = scanWave(n, lane), before = 0;
+    unsigned total = __builtin_amdgcn_readlane(upTo, kWave - 1);
+    for (unsigned base = kWave; base <= a.experts; base += kWave) { // more experts than lanes: their tiles too
+        unsigned l, h, m = tilesOfLane(a, base + lane, tile, l, h);
 #pragma unroll
-        for (unsigned by = kWave / 2; by; by /= 2) n += unsigned(__shfl_xor(int(n), by));
-        total += n;
+        for (unsigned by = kWave / 2; by; by /= 2) m += unsigned(__shfl_xor(int(m), by));
+        total += __builtin_amdgcn_readfirstlane(m);
     }
-    return __builtin_amdgcn_readfirstlane(total);
-}
-
-// The rows of row tile `id`, which countTiles has found to be one.
-__device__ __forceinline__ Span spanOf(const Product& a, unsigned id, unsigned tile, unsigned lane) {
-    unsigned before = 0;
-    for (unsigned base = 0; base <= a.experts; base += kWave) {
-        unsigned lo, hi;
-        const unsigned n = tilesOfLane(a, base + lane, tile, lo, hi);
-        const unsigned upTo = scanWave(n, lane) + before;
-        const unsigned last = __builtin_amdgcn_readlane(upTo, kWave - 1);
-        if (id < last) {
-            const unsigned at = unsigned(__builtin_ctzll(__ballot(upTo > id)));
-            const unsigned start = __builtin_amdgcn_readlane(upTo - n, at);
-            return {base + at, unsigned(__builtin_amdgcn_readlane(lo, at)) + (id - start) * tile,
-                    unsigned(__builtin_amdgcn_readlane(hi, at))};
-        }
-        before = last;
+    const unsigned id = idOf(total);
+    if (id >= total) return false;
+    unsigned base = 0;
+    while (id >= unsigned(__builtin_amdgcn_readlane(upTo, kWave - 1))) {
+        before = __builtin_amdgcn_readlane(upTo, kWave - 1), base += kWave;
+        n = tilesOfLane(a, base + lane, tile, lo, hi), upTo = scanWave(n, lane) + before;
     }
-    return {a.experts, a.rows, a.rows};
+    const unsigned at = unsigned(__builtin_ctzll(__ballot(upTo > id)));
+    const unsigned start = __builtin_amdgcn_readlane(upTo - n, at);
+    s = {base + at, unsigned(__builtin_amdgcn_readlane(lo, at)) + (id - start) * tile, unsigned(__builtin_amdgcn_readlane(hi, at))};
+    return true;
 }
 
 // The row of x that sorted row r takes.
@@ -141,11 +135,15 @@ struct Tile {
 template <typename T, bool Experts, unsigned BM, unsigned BN>
 __device__ __forceinline__ bool findTile(const Product& a, unsigned lane, Tile& t) {
     if constexpr (Experts) {
-        const unsigned tilesM = countTiles(a, BM, lane), total = tilesM * a.tilesN;
-        if (blockIdx.x >= total) return false;
-        const unsigned tile = tileOf(blockIdx.x, total, tilesM, a.tilesN);
-        const Span s = spanOf(a, tile % tilesM, BM, lane);
-        t = {s.expert, s.first, s.end, tile / tilesM * BN};
+        Span s;
+        const bool some = spanOf(a, BM, lane, [&](unsigned tilesM) {
+            const unsigned total = tilesM * a.tilesN;
+            const unsigned tile = blockIdx.x < total ? tileOf(blockIdx.x, total, tilesM, a.tilesN) : 0;
+            t.tn = blockIdx.x < total ? tile / tilesM * BN : 0;
+            return blockIdx.x < total ? tile % tilesM : tilesM;
+        }, s);
+        if (!some) return false;
+        t = {s.expert, s.first, s.end, t.tn};
         if (s.expert < a.experts) return true;
         zeroTile<T>(a, s, BM, t.tn, BN);
         return false;
@@ -178,6 +176,7 @@ template <bool Experts> __device__ __forceinline__ void take(Product& a, Tile& t
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
     constexpr unsigned Waves = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+    constexpr bool Exact = X8 && std::is_same<T, F32>::value;
     constexpr unsigned Halves = X8 ? 1 : 2, Dword = 4 / Halves; // MFMAs of a step; steps of a dword of exponents
     constexpr unsigned WRow = Halves * 64, Stage = BM * 128 + BN * WRow; // bytes
     constexpr unsigned XL = BM / 8 / Waves, WL = BN * WRow / 1024 / Waves;
@@ -260,9 +259,32 @@ __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
         load(k + Stages - 1, (S + Stages - 1) % Stages);
         u32x4 xf[MT][2];
 #pragma unroll
-        for (unsigned m = 0; m < MT; ++m) {
-            xf[m][0] = *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * 128 + ((g ^ xKey) * 16));
-            xf[m][1] = *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * 128 + (((g + 4) ^ xKey) * 16));
+        for (unsigned m = 0; m < MT; ++m)
+#pragma unroll
+            for (unsigned c = 0; c < 2; ++c)
+                xf[m][c] = *reinterpret_cast<const u32x4*>(xRead + at + m * 16 * 128 +
+                                                           (((Exact ? 2 * g + c : g + 4 * c) ^ xKey) * 16));
+        if constexpr (Exact) {
+            // The bf16 MFMA on the values: a lane has elements 32 g to 32 g + 31 of both rows, 8 a time.
+            bf16x8 xv[MT][4];
+#pragma unroll
+            for (unsigned m = 0; m < MT; ++m)
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i)
+                    xv[m][i] = values8(xf[m][i / 2][i % 2 * 2], xf[m][i / 2][i % 2 * 2 + 1], scaleOf(xs[m] >> 8 * S & 255));
+#pragma unroll
+            for (unsigned n = 0; n < NT; ++n) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(wRead + at + (n / 2 * 32 + n % 2 * 4) * WRow + ((g ^ wKey) * 16));
+                const float scale = scaleOf(ws[n] >> 8 * S & 255);
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) {
+                    const bf16x8 wv = microValues8(w[i], scale);
+#pragma unroll
+                    for (unsigned m = 0; m < MT; ++m)
+                        acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[m][i], acc[n][m], 0, 0, 0);
+                }
+            }
+            return;
         }
 #pragma unroll
         for (unsigned n = 0; n < NT; ++n) {
@@ -590,124 +612,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 }
 
 // ------------------------------------------------------------------------------------------------
-// FP32 outputs of E4M3 rows: the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's. Tiles of
-// 128 x 128, half a step at a time: a row's 64 values are 128 bytes of LDS.
-template <bool Experts> __global__ __launch_bounds__(256) void microTilesExact(Product a) {
-    constexpr unsigned B = 128;
-    __shared__ __align__(1024) std::uint8_t lds[2][2][B * 128];
-    const unsigned t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    Tile found;
-    if (!findTile<F32, Experts, B, B>(a, lane, found)) return;
-    take<Experts>(a, found);
-    const unsigned tm = found.first, end = found.end, tn = found.tn;
-    const unsigned r = t / 4, part = t % 4; // 16 codes of rows r and r + 64 of each operand
-    const std::uint8_t *xp[2], *wp[2], *xep[2], *wep[2];
-#pragma unroll
-    for (unsigned h = 0; h < 2; ++h) {
-        const unsigned row = min(tm + r + 64 * h, a.rows - 1);
-        const std::uint64_t xrow = Experts ? sourceOf(a, row) : row, wrow = min(tn + r + 64 * h, a.outer - 1);
-        xp[h] = a.x + xrow * xPitch<true>(a) + part * 16;
-        xep[h] = a.xe + xrow * xExpPitch<true>(a);
-        wp[h] = a.w + wrow * wPitch(a) + part * 8;
-        wep[h] = a.we + wrow * wExpPitch(a) + part / 2 * 4;
-    }
-    const unsigned blocks = (a.inner + kMicroBlock - 1) / kMicroBlock;
-    u32x4 xq[2];
-    u32x2 wq[2];
-    unsigned xb[2], wb[2];
-    auto fetch = [&](unsigned k) { // half k
-#pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-            xq[h] = *reinterpret_cast<const u32x4*>(xp[h] + k * 64);
-            wq[h] = *reinterpret_cast<const u32x2*>(wp[h] + k * 32);
-            xb[h] = xep[h][k / 2];
-            wb[h] = k * 2 + part / 2 < blocks ? wep[h][exponentAt(k / 2, k % 2 * 2)] : 127u;
-        }
-    };
-    auto put = [&](std::uint8_t* to, unsigned row, unsigned i, bf16x8 v) {
-        *reinterpret_cast<bf16x8*>(to + row * 128 + ((2 * part + i) ^ (row & 7)) * 16) = v;
-    };
-    auto stash = [&](unsigned s) {
-#pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-            const float xs = scaleOf(xb[h]), ws = scaleOf(wb[h]);
-            put(lds[s][0], r + 64 * h, 0, values8(xq[h].x, xq[h].y, xs));
-            put(lds[s][0], r + 64 * h, 1, values8(xq[h].z, xq[h].w, xs));
-            put(lds[s][1], r + 64 * h, 0, microValues8(wq[h].x, ws));
-            put(lds[s][1], r + 64 * h, 1, microValues8(wq[h].y, ws));
-        }
-    };
-    const unsigned wm = wave % 2 * 64, wn = wave / 2 * 64, l16 = lane % 16, g = lane / 16;
-    f32x4 acc[4][4] = {};
-    const unsigned halves = 2 * a.count;
-    fetch(0);
-    stash(0);
-    __syncthreads();
-    for (unsigned k = 0; k < halves; ++k) {
-        if (k + 1 < halves) fetch(k + 1);
-        const std::uint8_t *bx = lds[k % 2][0], *bw = lds[k % 2][1];
-#pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-            bf16x8 xf[4];
-#pragma unroll
-            for (unsigned m = 0; m < 4; ++m) {
-                const unsigned row = wm + m * 16 + l16;
-                xf[m] = *reinterpret_cast<const bf16x8*>(bx + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
-            }
-#pragma unroll
-            for (unsigned n = 0; n < 4; ++n) {
-                const unsigned row = wn + n * 16 + l16;
-                const bf16x8 wf = *reinterpret_cast<const bf16x8*>(bw + row * 128 + ((4 * h + g) ^ (row & 7)) * 16);
-#pragma unroll
-                for (unsigned m = 0; m < 4; ++m)
-                    acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[m], acc[n][m], 0, 0, 0);
-            }
-        }
-        if (k + 1 < halves) {
-            stash((k + 1) % 2);
-            __syncthreads();
-        }
-    }
-    float* y = static_cast<float*>(a.y);
-#pragma unroll
-    for (unsigned n = 0; n < 4; ++n) {
-        const unsigned column = tn + wn + n * 16 + g * 4;
-        const f32x4 b = bias4(a.bias, column, a.outer);
-#pragma unroll
-        for (unsigned m = 0; m < 4; ++m) {
-            const unsigned row = tm + wm + m * 16 + l16;
-            if (row < end) put4(y + row * a.yStride, column, a.outer, acc[n][m] + b);
-        }
-    }
-}
-
-// ------------------------------------------------------------------------------------------------
-// Few rows (single tokens, small batches, experts with a row or a few): a workgroup takes 16 columns of y for up to 64
-// rows; its eight waves share the inner axis, a run of steps each, and add their sums through LDS in the waves' order. The
-// weight's codes go from memory to the MFMA's registers, each byte read once for those rows, four steps' loads at a time
-// before the first is used.
-// Dense: up to kFusedRows rows of dense x, which every workgroup codes for itself into LDS while its first weights are on
-// their way.
+// Up to kFusedRows rows of dense x (single tokens), in one launch: a workgroup takes 16 columns of y; its eight waves share the
+// inner axis, a run of steps each, and add their sums through LDS in the waves' order. The weight's codes go from memory to
+// the MFMA's registers, each byte read once on the chip, four steps' loads at a time before the first is used; every
+// workgroup codes x for itself into LDS while its first weights are on their way.
 constexpr unsigned kTokenWaves = 8, kFusedRows = 4;
 
-template <typename T, bool X8, unsigned MT, bool Dense, bool Experts>
-__global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
+template <typename T, bool X8> __global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
     constexpr bool Exact = X8 && std::is_same<T, F32>::value;
-    constexpr unsigned Ahead = 4, Rows = 16 * MT; // steps of a wave loaded at a time
-    static_assert(!(Dense && Experts), "experts' rows are coded in a launch of their own");
-    __shared__ f32x4 sums[kTokenWaves][MT][kWave];
-    extern __shared__ __align__(16) std::uint8_t lds[]; // Dense: x's codes, then its exponents
+    constexpr unsigned Ahead = 4; // steps of a wave loaded at a time
+    __shared__ f32x4 sums[kTokenWaves][kWave];
+    extern __shared__ __align__(16) std::uint8_t lds[]; // x's codes, then its exponents
     const unsigned t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const unsigned l16 = lane % 16, g = lane / 16, n0 = blockIdx.x * 16;
-    Tile found = {0, Dense ? 0 : blockIdx.y * Rows, a.rows, n0};
-    if constexpr (Experts) {
-        if (blockIdx.y >= countTiles(a, Rows, lane)) return;
-        const Span s = spanOf(a, blockIdx.y, Rows, lane);
-        if (s.expert >= a.experts) return zeroTile<T>(a, s, Rows, n0, 16);
-        found = {s.expert, s.first, s.end, n0};
-        take<true>(a, found);
-    }
-    const unsigned m0 = found.first, end = found.end;
     const unsigned pitch = xPitch<X8>(a), each = (a.count + kTokenWaves - 1) / kTokenWaves;
     const unsigned from = wave * each, to = min(from + each, a.count);
     const std::uint64_t wrow = min(n0 + l16, a.outer - 1);
@@ -725,105 +642,83 @@ __global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
         }
     };
     fetch(from);
-    std::uint8_t* exponents = lds + a.rows * pitch; // Dense: a byte a block, [row][step] or [row][step][4]
-    if constexpr (Dense) {
-        const unsigned sub = t % kBlockLanes;
-        for (unsigned item = t / kBlockLanes; item < a.rows * a.count; item += kWave * kTokenWaves / kBlockLanes) {
-            const unsigned row = item / a.count, step = item - row * a.count;
-            float v[8];
-            load8<T>(static_cast<const typename T::Raw*>(a.dense) + row * a.denseStride, step * kStep + sub * 8, a.inner, v);
-            if constexpr (X8) {
-                const unsigned e = exponentOf<BlockCodes::e4m3>(rowMax(peakBits(v)));
-                const u32x2 q = encode8<BlockCodes::e4m3>(v, e);
-                *reinterpret_cast<u32x2*>(lds + row * pitch + step * kStep + sub * 8) = q;
-                if (sub == 0) exponents[item] = std::uint8_t(e);
-                if (a.keep && blockIdx.x == 0) {
-                    *reinterpret_cast<u32x2*>(a.keep + row * std::uint64_t(pitch) + step * kStep + sub * 8) = q;
-                    if (step + sub < (step + 1 == a.count ? xExpPitch<true>(a) : step + 1))
-                        a.keepExp[row * std::uint64_t(xExpPitch<true>(a)) + step + sub] = std::uint8_t(sub ? 127u : e);
-                }
-            } else {
-                const unsigned e = microExponent(max4(peakBits(v)));
-                *reinterpret_cast<unsigned*>(lds + row * pitch + step * (kStep / 2) + sub * 4) = microEncode<8>(v, e);
-                if (sub % 4 == 0) exponents[item * 4 + sub / 4] = std::uint8_t(e);
+    std::uint8_t* exponents = lds + a.rows * pitch; // a byte a block: [row][step] or [row][step][4]
+    const unsigned sub = t % kBlockLanes;
+    for (unsigned item = t / kBlockLanes; item < a.rows * a.count; item += kWave * kTokenWaves / kBlockLanes) {
+        const unsigned row = item / a.count, step = item - row * a.count;
+        float v[8];
+        load8<T>(static_cast<const typename T::Raw*>(a.dense) + row * a.denseStride, step * kStep + sub * 8, a.inner, v);
+        if constexpr (X8) {
+            const unsigned e = exponentOf<BlockCodes::e4m3>(rowMax(peakBits(v)));
+            const u32x2 q = encode8<BlockCodes::e4m3>(v, e);
+            *reinterpret_cast<u32x2*>(lds + row * pitch + step * kStep + sub * 8) = q;
+            if (sub == 0) exponents[item] = std::uint8_t(e);
+            if (a.keep && blockIdx.x == 0) {
+                *reinterpret_cast<u32x2*>(a.keep + row * std::uint64_t(pitch) + step * kStep + sub * 8) = q;
+                if (step + sub < (step + 1 == a.count ? xExpPitch<true>(a) : step + 1))
+                    a.keepExp[row * std::uint64_t(xExpPitch<true>(a)) + step + sub] = std::uint8_t(sub ? 127u : e);
             }
+        } else {
+            const unsigned e = microExponent(max4(peakBits(v)));
+            *reinterpret_cast<unsigned*>(lds + row * pitch + step * (kStep / 2) + sub * 4) = microEncode<8>(v, e);
+            if (sub % 4 == 0) exponents[item * 4 + sub / 4] = std::uint8_t(e);
         }
-        __syncthreads();
     }
-    const std::uint8_t *xp[MT], *xep[MT];
-#pragma unroll
-    for (unsigned m = 0; m < MT; ++m) {
-        const unsigned r = min(m0 + m * 16 + l16, a.rows - 1), row = Experts ? sourceOf(a, r) : r;
-        xp[m] = (Dense ? lds : a.x) + row * std::uint64_t(pitch) + (Exact ? g * 32 : g * 16);
-        if constexpr (Dense)
-            xep[m] = exponents + row * a.count * (X8 ? 1 : 4) + (X8 ? 0 : g);
-        else
-            xep[m] = a.xe + row * std::uint64_t(xExpPitch<X8>(a)) + (X8 ? 0 : g * 4);
-    }
-    f32x4 acc[MT] = {};
+    __syncthreads();
+    const unsigned row = min(l16, a.rows - 1);
+    const std::uint8_t* xp = lds + row * pitch + (Exact ? g * 32 : g * 16);
+    const std::uint8_t* xep = exponents + row * a.count * (X8 ? 1 : 4) + (X8 ? 0 : g);
+    f32x4 acc = {};
     for (unsigned k = from; k < to; k += Ahead) {
-        u32x4 x[Ahead][MT][X8 ? 2 : 1];
-        unsigned xs[Ahead][MT];
+        u32x4 x[Ahead][2];
+        unsigned xs[Ahead];
 #pragma unroll
         for (unsigned u = 0; u < Ahead; ++u) {
             const unsigned at = min(k + u, a.count - 1);
-#pragma unroll
-            for (unsigned m = 0; m < MT; ++m) {
-                const std::uint8_t* p = xp[m] + at * (X8 ? kStep : kStep / 2);
-                x[u][m][0] = *reinterpret_cast<const u32x4*>(p);
-                if constexpr (X8) x[u][m][1] = *reinterpret_cast<const u32x4*>(p + (Exact ? 16 : 64));
-                xs[u][m] = X8 || at < mine ? xep[m][X8 ? at : Dense ? at * 4 : at / 4 * 16 + at % 4] : 127u;
-            }
+            x[u][0] = x[u][1] = *reinterpret_cast<const u32x4*>(xp + at * (X8 ? kStep : kStep / 2));
+            if constexpr (X8) x[u][1] = *reinterpret_cast<const u32x4*>(xp + at * kStep + (Exact ? 16 : 64));
+            xs[u] = xep[at * (X8 ? 1 : 4)];
         }
         __builtin_amdgcn_sched_barrier(0); // the compiler would move the loads down to their use
 #pragma unroll
         for (unsigned u = 0; u < Ahead; ++u) {
             if (k + u >= to) break;
+            if constexpr (Exact) {
+                // A lane has elements 32 g to 32 g + 31 of both rows.
+                const float wScale = scaleOf(ws[u]), xScale = scaleOf(xs[u]);
 #pragma unroll
-            for (unsigned m = 0; m < MT; ++m) {
-                if constexpr (Exact) {
-                    // A lane has elements 32 g to 32 g + 31 of both rows.
-                    const float wScale = scaleOf(ws[u]), xScale = scaleOf(xs[u][m]);
-#pragma unroll
-                    for (unsigned i = 0; i < 4; ++i)
-                        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            microValues8(w[u][i], wScale),
-                            values8(x[u][m][i / 2][i % 2 * 2], x[u][m][i / 2][i % 2 * 2 + 1], xScale), acc[m], 0, 0, 0);
-                } else {
-                    acc[m] = multiply<X8, 0>(w[u], x[u][m][0], x[u][m][X8 ? 1 : 0], acc[m], ws[u], xs[u][m]);
-                }
+                for (unsigned i = 0; i < 4; ++i)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        microValues8(w[u][i], wScale), values8(x[u][i / 2][i % 2 * 2], x[u][i / 2][i % 2 * 2 + 1], xScale),
+                        acc, 0, 0, 0);
+            } else {
+                acc = multiply<X8, 0>(w[u], x[u][0], x[u][1], acc, ws[u], xs[u]);
             }
         }
         if (k + Ahead < to) fetch(k + Ahead);
     }
-#pragma unroll
-    for (unsigned m = 0; m < MT; ++m) sums[wave][m][lane] = acc[m];
+    sums[wave][lane] = acc;
     __syncthreads();
-    // Output i of 256 * MT: column fastest.
-    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
-    for (unsigned i = t; i < 256 * MT; i += kWave * kTokenWaves) {
-        const unsigned column = i % 16, r = i / 16, row = m0 + r;
-        if (n0 + column >= a.outer || row >= end) continue;
-        float s = 0.0f;
+    // Output t: column fastest.
+    const unsigned column = n0 + t % 16, r = t / 16;
+    if (r >= a.rows || column >= a.outer) return;
+    float s = 0.0f;
 #pragma unroll
-        for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][r / 16][r % 16 + column / 4 * 16][column % 4];
-        if (a.bias) s += a.bias[n0 + column];
-        y[row * a.yStride + n0 + column] = T::put(s);
-    }
+    for (unsigned v = 0; v < kTokenWaves; ++v) s += sums[v][r + t % 16 / 4 * 16][t % 4];
+    if (a.bias) s += a.bias[column];
+    static_cast<typename T::Raw*>(a.y)[r * a.yStride + column] = T::put(s);
 }
 
 // ------------------------------------------------------------------------------------------------
 // Host side
 
-enum class Form { wide, middle, small, few, tokens, exact };
+enum class Form { wide, middle, small, few };
 const char* formName(Form f) {
     switch (f) {
     case Form::wide: return "microWide";
     case Form::middle: return "microTiles128";
     case Form::small: return "microTiles64";
-    case Form::few: return "microTiles32";
-    case Form::tokens: return "microTokens";
-    default: return "microTilesExact";
+    default: return "microTiles32";
     }
 }
 
@@ -834,20 +729,50 @@ std::uint64_t mostTiles(std::uint64_t rows, std::uint64_t experts, unsigned tile
     return std::min(rows, rows / tile + experts + 1);
 }
 
-Form formOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
-    (void)inner;
-    if (rows <= 64) return Form::tokens;
-    if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
-    const std::uint64_t half = over(rows, 128) * over(outer, 128);
-    if (half >= 1024) return Form::wide;
-    return half >= 256 ? Form::middle : over(rows, 64) * over(outer, 64) >= 128 ? Form::small : Form::few;
+// The tile of a product: the least estimated time, in microseconds. A CU holds one workgroup of tiles of 256 or, with its
+// four groups of waves, 32, two of 128 and two or three of 64; while tiles of 128 or 64 are at most one a CU, each step is
+// quicker. tilesOf says how many row tiles of a size there are, launched how many workgroups a launch of it has. The constants
+// fit these times (rows x inner x outer: 256, 128, 64, 32; 8-bit rows in bf16, 4-bit rows, 8-bit rows in FP32):
+//   16 x 4096 x 4096   46 22 8.2 6.1, 28 20 7.4 5.8, - 41 14.8 7.0      48 x 4096 x 8192  47 24 9.6 11.6, 29 22 8.3 10.9, - 43 15.7 13.7
+//   200 x 1024 x 1024  21 8.7 4.3 4.8, 18 9.1 4.5 5.1, - 14 6.1 5.5     512 x 4096 x 4096 58 27 18 41, 35 24 16 38, - 47 26 48
+//   777 x 1001 x 1437  23 10.5 7.1 18, 20 11 7.4 20, - 15 9.3 21        2048 x 512 x 2048 14 7.4 8.2 52, 12 7.5 9.0 54, - 13 12 63
+//   1024 x 8192 x 2048 108 58 35 70, 63 49 28 61, - 96 49 78            4096 x 2048 x 4096 36 48 61 -, 27 46 61 -, - 105 92 -
+//   100000 x 256 x 256 25 21 26 -, 26 29 41 -, - 39 36 -                3000 x 2000 x 3000 34 37 38 120, 26 35 36 126, - 77 53 140
+template <typename Tiles, typename Launched>
+Form leastOf(std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format, bool few, Tiles tilesOf, Launched launched) {
+    const double k = double(over(inner, kStep));
+    const bool x8 = format == RowFormat::e4m3, exact = x8 && type == DenseType::f32;
+    const auto tiles = [&](unsigned size) { return tilesOf(size) * double(over(outer, size)); };
+    const auto rounds = [](double n, unsigned slots) { return std::ceil(n / slots); };
+    const auto takes = [&](unsigned size, unsigned threads) { return launchTakes(launched(size) * over(outer, size), threads); };
+    const double never = 1e300, half = tiles(128), quarter = tiles(64);
+    double wide = rounds(tiles(256), 256) * (x8 ? 9.0 + 1.56 * k : 11.0 + 0.84 * k);
+    double middle = half <= 256 ? (x8 ? 3.5 + 0.8 * k : 4.5 + 0.68 * k) : rounds(half, 512) * (x8 ? 2.7 + 1.32 * k : 5.2 + 1.1 * k);
+    double small = quarter <= 256 ? (exact ? 2.6 + 0.42 * k : x8 ? 2.3 + 0.235 * k : 2.8 + 0.18 * k)
+                                  : 2.2 + quarter / 512 * (exact ? 2.2 + 0.66 * k : x8 ? 1.1 + 0.44 * k : 2.2 + 0.38 * k);
+    double fewest = 0.7 + rounds(tiles(32), 256) * (exact ? 3.6 + 0.085 * k : 3.2 + 0.075 * k);
+    if (exact) wide = middle = never; // of no size the quickest: half the wave's conversions are of operands that others have too
+    if (!takes(128, 512)) middle = never;
+    if (!takes(64, 256)) small = never;
+    if (!few || !takes(32, 512)) fewest = never;
+    const double least = std::min(std::min(wide, middle), std::min(small, fewest));
+    if (least == never) return exact ? Form::small : Form::wide; // more tiles than a launch takes: refused there
+    return least == small ? Form::small : least == fewest ? Form::few : least == middle ? Form::middle : Form::wide;
 }
 
-Form expertFormOf(const ExpertPlan& plan, std::uint32_t outer, DenseType type, RowFormat format) {
-    const std::uint64_t mean = plan.choices / plan.experts;
-    if (mean <= 16) return Form::tokens;
-    if (format == RowFormat::e4m3 && type == DenseType::f32) return Form::exact;
-    return mean <= 64 ? Form::small : mean * outer < 512 * 1024 ? Form::middle : Form::wide;
+Form formOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const auto up = [&](unsigned size) { return over(rows, size); };
+    return leastOf(inner, outer, type, format, true, [&](unsigned size) { return double(up(size)); }, up);
+}
+
+// The same for experts, of whose rows only the mean is known: each of those that can have any makes whole tiles and, by the
+// spread of their numbers, three quarters of one more. (24 tokens to 4 of 32, 2048 x 4096: 57, 39, 23 in tiles of 64; 1024 tokens
+// 111, 91, 89; 8192 in 4 bits 297, 423, 571.) Tiles of 32 were the quickest for none.
+Form expertFormOf(const ExpertPlan& plan, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const double used = std::min(plan.choices, plan.experts);
+    const auto tiles = [&](unsigned size) { return std::max(used, plan.choices / double(size) + 0.75 * used); };
+    return leastOf(inner, outer, type, format, false, tiles,
+                   [&](unsigned size) { return mostTiles(plan.choices, plan.experts, size); });
 }
 
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
@@ -874,38 +799,15 @@ template <typename T, bool X8, bool Experts> void launchWide(Product p, hipStrea
     checkHip(hipGetLastError());
 }
 
-template <typename T, bool X8, bool Experts> void launchTokens(const Product& p, hipStream_t stream) {
-    const dim3 threads(kWave * kTokenWaves);
-    const unsigned across = unsigned(over(p.outer, 16));
-    if constexpr (Experts) {
-        const unsigned up = unsigned(mostTiles(p.rows, p.experts, 16)); // expertFormOf: at most 16 rows an expert
-        hipLaunchKernelGGL((microTokens<T, X8, 1, false, true>), dim3(across, up), threads, 0, stream, p);
-    } else if (p.rows <= 16) {
-        hipLaunchKernelGGL((microTokens<T, X8, 1, false, false>), dim3(across), threads, 0, stream, p);
-    } else if (p.rows <= 32) {
-        hipLaunchKernelGGL((microTokens<T, X8, 2, false, false>), dim3(across), threads, 0, stream, p);
-    } else {
-        hipLaunchKernelGGL((microTokens<T, X8, 4, false, false>), dim3(across, unsigned(over(p.rows, 64))), threads, 0,
-                           stream, p);
-    }
-    checkHip(hipGetLastError());
-}
-
 template <typename T, bool X8, bool Experts> void launchForm(Form form, Product p, hipStream_t stream) {
-    if (form == Form::tokens) return launchTokens<T, X8, Experts>(p, stream);
-    if constexpr (!X8 || !std::is_same<T, F32>::value) {
-        switch (form) {
-        case Form::wide: return launchWide<T, X8, Experts>(p, stream);
-        case Form::middle: return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
-        case Form::small: return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
-        default: return launchTiles<T, X8, Experts, 32, 32, 2, 1, 4, 4>(p, stream);
-        }
+    constexpr bool exact = X8 && std::is_same<T, F32>::value;
+    if (form == Form::small) return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
+    if constexpr (!Experts)
+        if (form == Form::few) return launchTiles<T, X8, false, 32, 32, 2, 1, 4, 4>(p, stream);
+    if constexpr (!exact) {
+        if (form == Form::middle) return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
+        launchWide<T, X8, Experts>(p, stream);
     }
-    const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 128) : over(p.rows, 128);
-    p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 128));
-    checkGrid("matmul micro", up * p.tilesN, 256);
-    hipLaunchKernelGGL((microTilesExact<Experts>), dim3(unsigned(up * p.tilesN)), dim3(256), 0, stream, p);
-    checkHip(hipGetLastError());
 }
 
 // Calls f with the element type's tag and whether rows are in 8 bits.
@@ -973,6 +875,11 @@ const char* matmulMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32
     return formName(formOf(rows, inner, outer, type, format));
 }
 
+const char* linearMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const char* product = matmulMicroForm(rows, inner, outer, type, format);
+    return fusedTokens(rows, inner, format) ? "microTokens" : product;
+}
+
 void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
                  std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, hipStream_t stream) {
     const char* where = "matmul micro";
@@ -1023,9 +930,8 @@ void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias
         Product p = productOf(w, bias, y, yStride, rows, inner, outer);
         p.dense = x.data, p.denseStride = x.stride, p.keep = keep.codes, p.keepExp = keep.exponents;
         withRows(x.type, format, [&](auto tag, auto x8) {
-            hipLaunchKernelGGL((microTokens<decltype(tag), decltype(x8)::value, 1, true, false>),
-                               dim3(unsigned(over(outer, 16))), dim3(kWave * kTokenWaves), fusedLds(rows, inner, format),
-                               stream, p);
+            hipLaunchKernelGGL((microTokens<decltype(tag), decltype(x8)::value>), dim3(unsigned(over(outer, 16))),
+                               dim3(kWave * kTokenWaves), fusedLds(rows, inner, format), stream, p);
         });
         return checkHip(hipGetLastError());
     }
@@ -1056,7 +962,7 @@ const char* matmulExpertsForm(ExpertPlan plan, std::uint32_t inner, std::uint32_
     checkType(where, type);
     checkFormat(where, format);
     if (!plan.experts || plan.experts > kMaxExperts) reject(where, "experts must be 1 to 1024");
-    return formName(expertFormOf(plan, outer, type, format));
+    return formName(expertFormOf(plan, inner, outer, type, format));
 }
 
 void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
@@ -1078,7 +984,7 @@ void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, vo
     p.offsets = plan.offsets, p.order = byToken ? plan.order : nullptr;
     p.experts = plan.experts, p.each = plan.each;
     withRows(type, x.format, [&](auto tag, auto x8) {
-        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, outer, type, x.format), p, stream);
+        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, inner, outer, type, x.format), p, stream);
     });
 }
 

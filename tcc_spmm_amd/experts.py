@@ -15,8 +15,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .blocks import _TYPES, E4M3, _away, _dense, _rows, _same_device, _stream, _stride, _workspace
-from .micro import MicroWeight, _code_pitch, _format
+from .blocks import _TYPES, E4M3, _away, _dense, _rows, _same_device, _stream, _stride
+from .micro import MicroWeight, _code_pitch, _format, _workspace
 
 MAX_EXPERTS = 1024
 MAX_EACH = 1024
@@ -107,9 +107,9 @@ def sort_experts(experts: torch.Tensor, count: int, stream=None) -> ExpertPlan:
     ids = experts.contiguous()
     choices = ids.numel()
     # One allocation: the lists of a plan live and end together.
-    lists = torch.empty(2 * choices + count + 1, dtype=torch.int32, device=device)
-    offsets, order, places = lists[:count + 1], lists[count + 1:count + 1 + choices], lists[count + 1 + choices:]
-    _space, at, size = _workspace(lib().tcc_sort_experts_workspace, (choices, count), device)
+    offsets, order, places = torch.empty(2 * choices + count + 1, dtype=torch.int32, device=device).split_with_sizes(
+        (count + 1, choices, choices))
+    _space, at, size = _workspace("tcc_sort_experts_workspace", (choices, count), device)
     check(lib().tcc_sort_experts(ids.data_ptr(), ids.element_size(), offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
                                  choices, count, at, size, _stream(device.index)))
     return _plan(offsets, order, places, tuple(ids.shape[:-1]), ids.shape[-1])
@@ -223,7 +223,7 @@ def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias:
     flat = _rows(x)
     dtype = _TYPES[x.dtype]
     y = torch.empty((plan.choices, outer), dtype=x.dtype, device=device)
-    _space, at, size = _workspace(lib().tcc_linear_experts_workspace,
+    _space, at, size = _workspace("tcc_linear_experts_workspace",
                                   (plan.choices, plan.each, by_token, inner, kind), device)
     check(lib().tcc_linear_experts(flat.data_ptr(), _stride(flat), dtype, kind, by_token, weight.codes.data_ptr(),
                                    weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, plan.offsets.data_ptr(),

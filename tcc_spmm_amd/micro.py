@@ -13,11 +13,14 @@ tcc_spmm_amd.blocks takes them.
 """
 from __future__ import annotations
 
+import ctypes as C
+import functools
+
 import torch
 
 from ._lib import check, lib
 from .blocks import (_TYPES, E4M3, BlockTensor, _away, _bias, _dense, _float_bias, _new_blocks, _rows, _same_device,
-                     _stream, _stride, _workspace, weight_grad_blocks)
+                     _stream, _stride, weight_grad_blocks)
 
 BLOCK = 32
 E2M1 = torch.float4_e2m1fn_x2
@@ -124,6 +127,22 @@ def _new_micro(shape, columns: int, device):
     """Codes and exponents of rows [*shape]."""
     return (torch.empty((*shape, _code_pitch(columns)), dtype=E2M1, device=device),
             torch.empty((*shape, _exponent_pitch(columns)), dtype=torch.uint8, device=device))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, *sizes) -> int:
+    """What the library's query says for these sizes, of which it is a function; asking costs 2 us."""
+    size = C.c_size_t()
+    check(getattr(lib(), query)(*sizes, C.byref(size)))
+    return size.value
+
+
+def _workspace(query: str, sizes, device):
+    size = _workspace_bytes(query, *sizes)
+    if not size:
+        return None, 0, 0
+    space = torch.empty(size, dtype=torch.uint8, device=device)
+    return space, space.data_ptr(), size
 
 
 def _format(codes) -> int:
@@ -246,7 +265,7 @@ def linear_micro(x: torch.Tensor, weight: MicroWeight, bias: torch.Tensor | None
     rows = flat.shape[0]
     y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
     kept = _new_blocks(rows, inner, E4M3, device) if keep else None
-    _space, at, size = _workspace(lib().tcc_linear_micro_workspace, (rows, inner, outer, dtype, kind, keep), device)
+    _space, at, size = _workspace("tcc_linear_micro_workspace", (rows, inner, outer, dtype, kind, keep), device)
     check(lib().tcc_linear_micro(flat.data_ptr(), _stride(flat), dtype, kind, weight.codes.data_ptr(),
                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer,
                                  kept.codes.data_ptr() if keep else 0, kept.exponents.data_ptr() if keep else 0,

@@ -33,7 +33,7 @@ def choices(tokens, each, experts, seed=0, away=0.0, dtype=torch.int64, kind="an
 
 
 PLANS = [(1, 1, 1), (1, 4, 8), (5, 3, 7), (24, 4, 32), (64, 8, 64), (1000, 4, 64), (1024, 4, 1024), (1025, 4, 1000), (4097, 1, 3),
-         (4096, 8, 128), (30001, 6, 130), (100, 1, 1023), (3, 1024, 9)]
+         (4096, 8, 128), (30001, 6, 130), (100, 1, 1023), (3, 1024, 9), (16385, 1, 6), (200003, 2, 70)]
 
 
 @pytest.mark.parametrize("tokens,each,experts", PLANS)

@@ -74,7 +74,7 @@ def test_product_refusals(form):
         rejected(linear(keep=P, keepe=P), b"E4M3")
     rejected(L.tcc_linear_micro_workspace(1000, 300, 64, 0, form, 0, None), b"null")
     name = ctypes.c_char_p()
-    assert L.tcc_matmul_micro_form(1, 128, 64, 1, form, ctypes.byref(name)) == 0 and name.value == b"microTokens"
+    assert L.tcc_linear_micro_form(1, 128, 64, 1, form, ctypes.byref(name)) == 0 and name.value == b"microTokens"
     rejected(L.tcc_matmul_micro_form(1, 128, 64, 1, 2, ctypes.byref(name)), b"row format")
     rejected(L.tcc_matmul_micro_form(1, 128, 64, 1, form, None), b"null")
 
@@ -83,7 +83,7 @@ def test_plan_refusals():
     from tcc_spmm_amd._lib import lib
     L = lib()
     size = ctypes.c_size_t()
-    assert L.tcc_sort_experts_workspace(4096, 64, ctypes.byref(size)) == 0 and size.value == 0
+    assert L.tcc_sort_experts_workspace(16384, 64, ctypes.byref(size)) == 0 and size.value == 0
     assert L.tcc_sort_experts_workspace(100000, 64, ctypes.byref(size)) == 0 and size.value
     call = lambda ids=P, wide=8, offsets=P, order=P, n=100000, experts=64, space=P, size=size.value: L.tcc_sort_experts(  # noqa: E731
         ids, wide, offsets, order, P, n, experts, space, size, None)
@@ -154,7 +154,7 @@ def test_expert_product_refusals():
     rejected(call(space=None), b"workspace too small")
     rejected(call(space=P + 8), b"16-byte")
     name = ctypes.c_char_p()
-    assert L.tcc_matmul_experts_form(80, 8, 128, 64, 1, 1, ctypes.byref(name)) == 0 and name.value == b"microTokens"
+    assert L.tcc_matmul_experts_form(80, 8, 128, 64, 1, 1, ctypes.byref(name)) == 0 and name.value == b"microTiles64"
     rejected(L.tcc_matmul_experts_form(80, 0, 128, 64, 1, 1, ctypes.byref(name)), b"1 to 1024")
 
 
