@@ -116,13 +116,17 @@ def _weight(codes, exponents, columns, codes_t, exponents_t) -> BlockWeight:
     return out
 
 
+# The current device; torch.cuda.current_device first asks whether CUDA is up, which a tensor on it has answered.
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _away(device, stream):
     """None if a call's outputs and launches belong where the caller already is, else the context to make it
     in: another stream than the current one, or another device."""
     if device.type != "cuda":
         raise ValueError("device entry points take CUDA (HIP) tensors")
     if stream is None:
-        return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        return None if device.index == _current() else torch.cuda.device(device)
     if stream.device != device:
         raise ValueError(f"stream on {stream.device}, tensors on {device}")
     return torch.cuda.stream(stream)

@@ -16,7 +16,7 @@ import torch
 
 from ._lib import check, lib
 from .blocks import _TYPES, E4M3, _away, _dense, _rows, _same_device, _stream, _stride
-from .micro import MicroWeight, _code_pitch, _format, _workspace
+from .micro import MicroWeight, _code_pitch, _format, _laid, _workspace
 
 MAX_EXPERTS = 1024
 MAX_EACH = 1024
@@ -27,7 +27,7 @@ class ExpertPlan:
     order // each), those of one expert in their own order and those for none of 0 .. experts - 1 last; `places` [choices] the
     row of each choice; expert e's rows are offsets[e] to offsets[e + 1]. `lead` is the tokens' shape."""
 
-    __slots__ = ("offsets", "order", "places", "lead", "each")
+    __slots__ = ("offsets", "order", "places", "lead", "each", "choices", "experts", "device")
 
     def __init__(self, offsets: torch.Tensor, order: torch.Tensor, places: torch.Tensor, lead, each: int):
         lead = tuple(lead)
@@ -44,40 +44,41 @@ class ExpertPlan:
             raise ValueError(f"choices of a token must be 1 to {MAX_EACH}")
         if order.numel() != tokens * each or places.numel() != tokens * each:
             raise ValueError(f"order and places must have {tokens * each} elements")
-        self.offsets, self.order, self.places, self.lead, self.each = offsets, order, places, lead, each
-
-    @property
-    def experts(self) -> int:
-        return self.offsets.numel() - 1
-
-    @property
-    def choices(self) -> int:
-        return self.order.numel()
+        _fill(self, offsets, order, places, lead, each)
 
     @property
     def tokens(self) -> int:
-        return self.order.numel() // self.each
+        return self.choices // self.each
+
+
+def _fill(plan, offsets, order, places, lead, each) -> ExpertPlan:
+    plan.offsets, plan.order, plan.places, plan.lead, plan.each = offsets, order, places, lead, each
+    plan.choices, plan.experts, plan.device = order.numel(), offsets.numel() - 1, offsets.device
+    return plan
 
 
 def _plan(offsets, order, places, lead, each) -> ExpertPlan:
     """An ExpertPlan of tensors that are laid out as its constructor would check."""
-    out = ExpertPlan.__new__(ExpertPlan)
-    out.offsets, out.order, out.places, out.lead, out.each = offsets, order, places, lead, each
-    return out
+    return _fill(ExpertPlan.__new__(ExpertPlan), offsets, order, places, lead, each)
+
+
+def _here(device, plan: ExpertPlan) -> None:
+    if device != plan.device:
+        raise ValueError(f"tensor on {device}, expected {plan.device}")
 
 
 def _sorted_rows(t: torch.Tensor, plan: ExpertPlan, name: str, columns: int | None = None) -> None:
     _dense(t, name, columns)
     if t.dim() != 2 or t.shape[0] != plan.choices:
         raise ValueError(f"{name} must be [{plan.choices}, columns], got {list(t.shape)}")
-    _same_device(t.device, plan.offsets)
+    _here(t.device, plan)
 
 
 def _token_rows(t: torch.Tensor, plan: ExpertPlan, name: str, columns: int | None = None) -> None:
     _dense(t, name, columns)
-    if tuple(t.shape[:-1]) != plan.lead:
+    if t.shape[:-1] != plan.lead:
         raise ValueError(f"{name} must be {[*plan.lead, 'columns']}, got {list(t.shape)}")
-    _same_device(t.device, plan.offsets)
+    _here(t.device, plan)
 
 
 def _weights(weights, plan: ExpertPlan) -> None:
@@ -85,9 +86,9 @@ def _weights(weights, plan: ExpertPlan) -> None:
         return
     if weights.dtype not in _TYPES:
         raise ValueError(f"weights must be float32, bfloat16 or float16, got {weights.dtype}")
-    if tuple(weights.shape) != (*plan.lead, plan.each):
+    if weights.shape != (*plan.lead, plan.each):
         raise ValueError(f"weights must be {[*plan.lead, plan.each]}, got {list(weights.shape)}")
-    _same_device(plan.offsets.device, weights)
+    _here(weights.device, plan)
 
 
 def sort_experts(experts: torch.Tensor, count: int, stream=None) -> ExpertPlan:
@@ -107,8 +108,8 @@ def sort_experts(experts: torch.Tensor, count: int, stream=None) -> ExpertPlan:
     ids = experts.contiguous()
     choices = ids.numel()
     # One allocation: the lists of a plan live and end together.
-    offsets, order, places = torch.empty(2 * choices + count + 1, dtype=torch.int32, device=device).split_with_sizes(
-        (count + 1, choices, choices))
+    lists = torch.empty(2 * choices + count + 1, dtype=torch.int32, device=device)
+    offsets, order, places = lists.split_with_sizes((count + 1, choices, choices))
     _space, at, size = _workspace("tcc_sort_experts_workspace", (choices, count), device)
     check(lib().tcc_sort_experts(ids.data_ptr(), ids.element_size(), offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
                                  choices, count, at, size, _stream(device.index)))
@@ -124,9 +125,9 @@ def gather_experts(x: torch.Tensor, plan: ExpertPlan, stream=None) -> torch.Tens
     if away:
         with away:
             return gather_experts(x, plan)
-    flat = _rows(x)
+    flat, _, _, stride = _laid(x)
     rows = torch.empty((plan.choices, width), dtype=x.dtype, device=device)
-    check(lib().tcc_gather_experts(flat.data_ptr(), _stride(flat), _TYPES[x.dtype], plan.offsets.data_ptr(),
+    check(lib().tcc_gather_experts(flat.data_ptr(), stride, _TYPES[x.dtype], plan.offsets.data_ptr(),
                                    plan.places.data_ptr(), plan.choices, plan.each, plan.experts, rows.data_ptr(), width,
                                    width, _stream(device.index)))
     return rows
@@ -143,10 +144,10 @@ def combine_experts(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor 
     if away:
         with away:
             return combine_experts(rows, plan, weights)
-    flat = _rows(rows)
+    flat, _, _, stride = _laid(rows)
     weights = None if weights is None else weights.contiguous()
     y = torch.empty((*plan.lead, width), dtype=rows.dtype, device=device)
-    check(lib().tcc_combine_experts(flat.data_ptr(), _stride(flat), _TYPES[rows.dtype], plan.offsets.data_ptr(),
+    check(lib().tcc_combine_experts(flat.data_ptr(), stride, _TYPES[rows.dtype], plan.offsets.data_ptr(),
                                     plan.places.data_ptr(), plan.choices, plan.each, plan.experts,
                                     0 if weights is None else weights.data_ptr(),
                                     0 if weights is None else _TYPES[weights.dtype], y.data_ptr(), width, width,
@@ -174,13 +175,13 @@ def combine_experts_backward(dy: torch.Tensor, rows: torch.Tensor | None, plan: 
     if away:
         with away:
             return combine_experts_backward(dy, rows, plan, weights, need=need)
-    flat = _rows(dy)
+    flat, _, _, stride = _laid(dy)
     rows = _rows(rows) if need[1] else None
     weights = None if weights is None else weights.contiguous()
     drows = torch.empty((plan.choices, width), dtype=dy.dtype, device=device) if need[0] else None
     dweights = torch.empty_like(weights) if need[1] else None
     check(lib().tcc_combine_experts_backward(
-        flat.data_ptr(), _stride(flat), rows.data_ptr() if need[1] else 0, _stride(rows) if need[1] else 0,
+        flat.data_ptr(), stride, rows.data_ptr() if need[1] else 0, _stride(rows) if need[1] else 0,
         _TYPES[dy.dtype], plan.offsets.data_ptr(), plan.places.data_ptr(), plan.choices, plan.each, plan.experts,
         0 if weights is None else weights.data_ptr(), 0 if weights is None else _TYPES[weights.dtype],
         drows.data_ptr() if need[0] else 0, width, dweights.data_ptr() if need[1] else 0, width, _stream(device.index)))
@@ -220,12 +221,12 @@ def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias:
     if by_token and plan.tokens * _code_pitch(inner) * (2 - kind) >= 1 << 31:
         # The kernels reach a token's codes by 32 bits.
         x, by_token = gather_experts(x, plan), False
-    flat = _rows(x)
+    flat, _, _, stride = _laid(x)
     dtype = _TYPES[x.dtype]
     y = torch.empty((plan.choices, outer), dtype=x.dtype, device=device)
     _space, at, size = _workspace("tcc_linear_experts_workspace",
                                   (plan.choices, plan.each, by_token, inner, kind), device)
-    check(lib().tcc_linear_experts(flat.data_ptr(), _stride(flat), dtype, kind, by_token, weight.codes.data_ptr(),
+    check(lib().tcc_linear_experts(flat.data_ptr(), stride, dtype, kind, by_token, weight.codes.data_ptr(),
                                    weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, plan.offsets.data_ptr(),
                                    plan.order.data_ptr(), plan.choices, plan.each, plan.experts, inner, outer, at, size,
                                    _stream(device.index)))

@@ -73,9 +73,10 @@ class MicroTensor:
 
 class MicroWeight:
     """A weight [outer, inner], or a stack of them [experts, outer, inner], in microscaled blocks along `inner`: codes and
-    exponents of its rows as a MicroTensor's, and for the input gradient the transposed weight's, if it is in tiles."""
+    exponents of its rows as a MicroTensor's, and for the input gradient the transposed weight's, if it is in tiles. `rows` is
+    outer, of one weight; `experts` the number of a stack, None for one weight."""
 
-    __slots__ = ("codes", "exponents", "columns", "codes_t", "exponents_t")
+    __slots__ = ("codes", "exponents", "columns", "codes_t", "exponents_t", "rows", "experts")
 
     def __init__(self, codes: torch.Tensor, exponents: torch.Tensor, columns: int,
                  codes_t: torch.Tensor | None = None, exponents_t: torch.Tensor | None = None):
@@ -91,18 +92,7 @@ class MicroWeight:
                                  f"got {list(codes_t.shape[:-1])}")
             if codes_t.device != codes.device:
                 raise ValueError(f"tensor on {codes_t.device}, expected {codes.device}")
-        self.codes, self.exponents, self.columns = codes, exponents, columns
-        self.codes_t, self.exponents_t = codes_t, exponents_t
-
-    @property
-    def rows(self) -> int:
-        """Of one weight: the layer's outputs."""
-        return self.codes.shape[-2]
-
-    @property
-    def experts(self) -> int | None:
-        """Weights of a stack; None for one weight."""
-        return self.codes.shape[0] if self.codes.dim() == 3 else None
+        _fill(self, codes, exponents, columns, codes_t, exponents_t)
 
     def transposed(self) -> "MicroWeight":
         """The transposed weight's view of the same codes."""
@@ -115,18 +105,31 @@ class MicroWeight:
         return dequantize_micro(rows, dtype, stream).reshape(*self.codes.shape[:-1], self.columns)
 
 
+def _fill(weight, codes, exponents, columns, codes_t, exponents_t) -> MicroWeight:
+    weight.codes, weight.exponents, weight.columns = codes, exponents, columns
+    weight.codes_t, weight.exponents_t = codes_t, exponents_t
+    weight.rows, weight.experts = codes.shape[-2], codes.shape[0] if codes.dim() == 3 else None
+    return weight
+
+
 def _weight(codes, exponents, columns, codes_t, exponents_t) -> MicroWeight:
     """A MicroWeight of tensors that are laid out as its constructor would check."""
-    out = MicroWeight.__new__(MicroWeight)
-    out.codes, out.exponents, out.columns = codes, exponents, columns
-    out.codes_t, out.exponents_t = codes_t, exponents_t
-    return out
+    return _fill(MicroWeight.__new__(MicroWeight), codes, exponents, columns, codes_t, exponents_t)
 
 
 def _new_micro(shape, columns: int, device):
     """Codes and exponents of rows [*shape]."""
     return (torch.empty((*shape, _code_pitch(columns)), dtype=E2M1, device=device),
             torch.empty((*shape, _exponent_pitch(columns)), dtype=torch.uint8, device=device))
+
+
+def _laid(t: torch.Tensor):
+    """t as rows (_rows), their number, their columns and their stride."""
+    if t.dim() == 2 and t.is_contiguous():
+        rows, columns = t.shape
+        return t, rows, columns, columns
+    t = _rows(t)
+    return t, t.shape[0], t.shape[1], _stride(t)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -164,12 +167,13 @@ def quantize_micro(x: torch.Tensor, stream=None) -> MicroTensor:
     if away:
         with away:
             return quantize_micro(x)
-    x = _rows(x)
+    x, rows, columns, stride = _laid(x)
     out = MicroTensor.__new__(MicroTensor)  # laid out as its constructor would check
-    out.codes, out.exponents = _new_micro((x.shape[0],), x.shape[1], device)
-    out.columns = x.shape[1]
-    check(lib().tcc_quantize_micro(x.data_ptr(), _stride(x), _TYPES[x.dtype], out.codes.data_ptr(),
-                                   out.exponents.data_ptr(), x.shape[0], x.shape[1], _stream(device.index)))
+    out.codes = codes = torch.empty((rows, -(-columns // 128) * 64), dtype=E2M1, device=device)
+    out.exponents = exponents = torch.empty((rows, -(-columns // 512) * 16), dtype=torch.uint8, device=device)
+    out.columns = columns
+    check(lib().tcc_quantize_micro(x.data_ptr(), stride, _TYPES[x.dtype], codes.data_ptr(), exponents.data_ptr(), rows, columns,
+                                   _stream(device.index)))
     return out
 
 
@@ -182,9 +186,10 @@ def dequantize_micro(x: MicroTensor, dtype=torch.float32, stream=None) -> torch.
     if away:
         with away:
             return dequantize_micro(x, dtype)
-    out = torch.empty((x.rows, x.columns), dtype=dtype, device=device)
-    check(lib().tcc_dequantize_micro(x.codes.data_ptr(), x.exponents.data_ptr(), out.data_ptr(), x.columns, _TYPES[dtype],
-                                     x.rows, x.columns, _stream(device.index)))
+    rows, columns = x.rows, x.columns
+    out = torch.empty((rows, columns), dtype=dtype, device=device)
+    check(lib().tcc_dequantize_micro(x.codes.data_ptr(), x.exponents.data_ptr(), out.data_ptr(), columns, _TYPES[dtype],
+                                     rows, columns, _stream(device.index)))
     return out
 
 
@@ -261,12 +266,11 @@ def linear_micro(x: torch.Tensor, weight: MicroWeight, bias: torch.Tensor | None
     if away:
         with away:
             return linear_micro(x, weight, bias, codes=codes, keep=keep)
-    flat = _rows(x)
-    rows = flat.shape[0]
-    y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
+    flat, rows, _, stride = _laid(x)
+    y = torch.empty((rows, outer) if x.dim() == 2 else (*x.shape[:-1], outer), dtype=x.dtype, device=device)
     kept = _new_blocks(rows, inner, E4M3, device) if keep else None
     _space, at, size = _workspace("tcc_linear_micro_workspace", (rows, inner, outer, dtype, kind, keep), device)
-    check(lib().tcc_linear_micro(flat.data_ptr(), _stride(flat), dtype, kind, weight.codes.data_ptr(),
+    check(lib().tcc_linear_micro(flat.data_ptr(), stride, dtype, kind, weight.codes.data_ptr(),
                                  weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer,
                                  kept.codes.data_ptr() if keep else 0, kept.exponents.data_ptr() if keep else 0,
                                  rows, inner, outer, at, size, _stream(device.index)))
