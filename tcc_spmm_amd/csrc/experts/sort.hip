@@ -88,17 +88,19 @@ template <typename Id, unsigned Turns, Counts C> __global__ __launch_bounds__(kT
     unsigned *counts = lds + wave * all, *starts = lds + kWaves * all;
     for (unsigned i = t; i < kWaves * all; i += kThreads) lds[i] = 0;
     __syncthreads();
-    // A wave's choices lie in a row.
-    const std::uint64_t first = std::uint64_t(run) * kRun + wave * (Turns * kWave) + lane;
+    // A wave's choices lie in a row; alone, the waves share what there is.
+    const unsigned turns = C == Counts::alone ? (a.choices + kThreads - 1) / kThreads : Turns;
+    const std::uint64_t first = std::uint64_t(run) * kRun + wave * turns * kWave + lane;
     unsigned expert[Turns], rank[Turns];
 #pragma unroll
     for (unsigned i = 0; i < Turns; ++i) {
         const std::uint64_t c = first + i * kWave;
-        expert[i] = c < a.choices ? expertOf<Id>(a, unsigned(c)) : ~0u;
+        expert[i] = i < turns && c < a.choices ? expertOf<Id>(a, unsigned(c)) : ~0u;
     }
     const unsigned bits = 32 - __builtin_clz(a.experts);
 #pragma unroll
     for (unsigned i = 0; i < Turns; ++i) {
+        if (i >= turns) break;
         const bool in = expert[i] != ~0u;
         std::uint64_t same = __ballot(in);
         for (unsigned b = 0; b < bits; ++b) {

@@ -401,50 +401,108 @@ __device__ __forceinline__ void multiplyInPlace(f32x4& acc, u32x4 w, u32x4 x0, u
 // for the last time a quarter or more before, and each has at least a step's time to arrive:
 //   quarter 0: pairs 2 and 3 of step k + 1;  1 and 2: x of step k + 2;  3: pairs 0 and 1 of step k + 2
 // with a barrier before quarters 1 and 3.
-template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wideTile(Product& a) {
+// The tiles that a workgroup goes through, one after the other, a grid apart: in the last pair of a tile's steps the loads are
+// those of the next tile's first, so that it begins as the sums of this one are stored. For experts the tiles and the rows'
+// sources are looked up in front of all, into LDS.
+constexpr unsigned kWideGroups = 256, kWideTiles = 16; // workgroups, one a CU; the most tiles of one, for experts
+
+struct WideTile {
+    unsigned expert, first, end, tn;
+};
+
+// What the loads of a tile go by.
+struct WideRows {
+    __amdgpu_buffer_rsrc_t x, w, xe, we;
+};
+
+template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wideTiles(const Product& a) {
     constexpr unsigned B = 256, Tiles = 8, Halves = X8 ? 1 : 2, WRow = Halves * 64, Stage = B * (128 + WRow);
     constexpr unsigned WL = B * WRow / 1024 / 4, WRows = 4096 / WRow; // a wave's loads of a step's weight; rows of all four's
     constexpr unsigned Exps = 2 * Tiles;                               // loads of exponents, for two steps
-    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages: 256 rows of x, 256 of w
+    extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages: 256 rows of x, 256 of w; experts: tiles, sources
     const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    Tile found;
-    if (!findTile<T, Experts, B, B>(a, lane, found)) return;
-    take<Experts>(a, found);
-    const unsigned tm = found.first, end = found.end, tn = found.tn;
-    const unsigned all = (a.count + Halves - 1) / Halves, pitch = xPitch<X8>(a), pitchW = wPitch(a);
+    const unsigned all = (a.count + Halves - 1) / Halves, pairs = (all + 1) / 2 * 2;
+    const unsigned pitch = xPitch<X8>(a), pitchW = wPitch(a), pitchXe = xExpPitch<X8>(a), pitchWe = wExpPitch(a);
     const bool byToken = Experts && a.order;
-    const unsigned xFirst = byToken ? 0 : tm, xRows = byToken ? a.rows / a.each : a.rows;
-    const auto xr = rowsAt(a.x, pitch, xFirst, xRows), wr = rowsAt(a.w, pitchW, tn, a.outer);
+    WideTile* const list = reinterpret_cast<WideTile*>(lds + 2 * Stage);
+    unsigned* const sources = reinterpret_cast<unsigned*>(lds + 2 * Stage + kWideTiles * sizeof(WideTile));
+    unsigned tiles = 0; // of this workgroup
+    if constexpr (Experts) {
+        for (; tiles < kWideTiles; ++tiles) {
+            Span s;
+            unsigned tn = 0;
+            const unsigned id0 = blockIdx.x + tiles * gridDim.x;
+            const bool some = spanOf(a, B, lane, [&](unsigned tilesM) {
+                const unsigned total = tilesM * a.tilesN;
+                const unsigned tile = id0 < total ? tileOf(id0, total, tilesM, a.tilesN) : 0;
+                tn = id0 < total ? tile / tilesM * B : 0;
+                return id0 < total ? tile % tilesM : tilesM;
+            }, s);
+            if (!some) break;
+            if (threadIdx.x == 0) list[tiles] = {s.expert, s.first, s.end, tn};
+            sources[tiles * B + threadIdx.x] = byToken ? sourceOf(a, s.first + threadIdx.x) : threadIdx.x;
+            if (s.expert >= a.experts) zeroTile<T>(a, s, B, tn, B);
+        }
+        tiles = __builtin_amdgcn_readfirstlane(tiles);
+        __syncthreads();
+    } else {
+        const unsigned total = a.tilesM * a.tilesN;
+        tiles = blockIdx.x < total ? (total - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    }
+    // Tile i of this workgroup; rows of no expert, which are zeros by now, as a tile of no rows.
+    auto tileAt = [&](unsigned i) {
+        if constexpr (Experts) {
+            const WideTile t = list[i];
+            return WideTile{unsigned(__builtin_amdgcn_readfirstlane(t.expert)), unsigned(__builtin_amdgcn_readfirstlane(t.first)),
+                            unsigned(__builtin_amdgcn_readfirstlane(t.end)), unsigned(__builtin_amdgcn_readfirstlane(t.tn))};
+        } else {
+            const unsigned tile = tileOf(blockIdx.x + i * gridDim.x, a.tilesM * a.tilesN, a.tilesM, a.tilesN);
+            return WideTile{0, tile % a.tilesM * B, a.rows, tile / a.tilesM * B};
+        }
+    };
+    // A tile's operands from its first rows on; by token all of x. `some` false: nothing, every load gives zeros.
+    auto rowsOf = [&](const WideTile& t, bool some) {
+        const std::uint64_t before = std::uint64_t(Experts ? min(t.expert, a.experts - 1) : 0) * a.outer;
+        const unsigned xFirst = byToken ? 0 : t.first, xRows = !some ? xFirst : byToken ? a.rows / a.each : a.rows;
+        const unsigned wRows = some ? a.outer : t.tn;
+        return WideRows{rowsAt(a.x, pitch, xFirst, xRows), rowsAt(a.w + before * pitchW, pitchW, t.tn, wRows),
+                        rowsAt(a.xe, pitchXe, xFirst, xRows), rowsAt(a.we + before * pitchWe, pitchWe, t.tn, wRows)};
+    };
+    if (!tiles) return;
     // Chunks and rows are dealt as in microTiles.
     auto keyX = [](unsigned r) { return r & 7; };
     auto keyW = [](unsigned r) { return X8 ? (r >> 1 & 1) | (r >> 2 & 2) : (r & 3) | (r >> 1 & 4); };
     const unsigned fill = wave * 8 + lane / 8, fillW = X8 ? wave * 16 + lane / 4 : fill;
     const unsigned chunk = (lane % 8) ^ keyX(fill), chunkW = X8 ? (lane % 4) ^ keyW(fillW) : (lane % 8) ^ keyW(fillW);
+    const unsigned wm = wave % 2 * 128, wn = wave / 2 * 128, l16 = lane % 16, g = lane / 16;
+    const unsigned wRow = l16 / 4 * 8 + l16 % 4, mine = stepsOfLane(a, g);
     // A wave's loads are 32 rows of x apart, with the same keys; a token's rows may lie anywhere.
-    unsigned xo[Experts ? 8 : 1];
+    unsigned xo[Experts ? 8 : 1], xeo[Experts ? Tiles : 1];
+    auto place = [&](unsigned i) {
 #pragma unroll
-    for (unsigned i = 0; i < (Experts ? 8 : 1); ++i)
-        xo[i] = (byToken ? sourceOf(a, tm + fill + i * 32) : fill + i * 32) * pitch + chunk * 16;
-    const unsigned wo = fillW * pitchW + chunkW * 16;
+        for (unsigned j = 0; j < (Experts ? 8 : 1); ++j) {
+            xo[j] = (Experts ? sources[i * B + fill + j * 32] : fill) * pitch + chunk * 16;
+            xeo[j] = (Experts ? sources[i * B + wm + j * 16 + l16] : wm + l16) * pitchXe + (X8 ? 0 : 4 * g);
+        }
+    };
+    const unsigned wo = fillW * pitchW + chunkW * 16, weo = (wn + wRow) * pitchWe + 4 * g;
     const unsigned woLast = a.count % Halves && chunkW >= 4 ? 0x7FFFFFFFu : wo; // the half of a step that is not there
     // Step k's rows of x or w into stage s; past the last zeros, from beyond the buffer.
-    auto loadX = [&](unsigned k, unsigned s, unsigned part) {
+    auto loadX = [&](const WideRows& r, unsigned k, unsigned s, unsigned part) {
         const unsigned from = k < all ? k * 128 : 0x7FFFFFFFu;
         std::uint8_t* to = lds + s * Stage + wave * 1024 + part * 4096;
         if constexpr (Experts)
-            loadToLds(xr, to, xo[part], from);
+            loadToLds(r.x, to, xo[part], from);
         else
-            loadToLds(xr, to, xo[0], from + part * 32 * pitch);
+            loadToLds(r.x, to, xo[0], from + part * 32 * pitch);
     };
-    auto loadW = [&](unsigned k, unsigned s, unsigned part) {
+    auto loadW = [&](const WideRows& r, unsigned k, unsigned s, unsigned part) {
         const unsigned from = k < all ? k * WRow : 0x7FFFFFFFu;
-        loadToLds(wr, lds + s * Stage + B * 128 + wave * 1024 + part * 4096, k + 1 == all ? woLast : wo,
+        loadToLds(r.w, lds + s * Stage + B * 128 + wave * 1024 + part * 4096, k + 1 == all ? woLast : wo,
                   from + part * WRows * pitchW);
     };
     // Load i of the first or the last two pairs of both halves of the waves.
     auto partW = [](unsigned last, unsigned i) { return X8 ? i * 2 + last : i / 2 + i % 2 * 4 + last * 2; };
-    const unsigned wm = wave % 2 * 128, wn = wave / 2 * 128, l16 = lane % 16, g = lane / 16;
-    const unsigned wRow = l16 / 4 * 8 + l16 % 4;
     // A lane's chunks of its row in either stage: bytes of LDS, which the loads' offsets reach a stage of.
     unsigned xRead[2][2], wRead[2][Halves];
 #pragma unroll
@@ -470,50 +528,44 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
             wf[n / 2 % 2][n % 2][c] = *reinterpret_cast<const u32x4*>(lds + (n / 2 * 32 + n % 2 * 4) * WRow + wRead[s][c]);
     };
     // Two steps' exponents at a time, of this lane's row of each operand: a byte for each MFMA.
-    const unsigned pitchXe = xExpPitch<X8>(a), pitchWe = wExpPitch(a), mine = stepsOfLane(a, g);
-    const auto xer = rowsAt(a.xe, pitchXe, xFirst, xRows), wer = rowsAt(a.we, pitchWe, tn, a.outer);
-    unsigned xeo[Experts ? Tiles : 1];
-#pragma unroll
-    for (unsigned m = 0; m < (Experts ? Tiles : 1); ++m) {
-        const unsigned r = wm + m * 16 + l16;
-        xeo[m] = (byToken ? sourceOf(a, tm + r) : r) * pitchXe + (X8 ? 0 : 4 * g);
-    }
-    const unsigned weo = (wn + wRow) * pitchWe + 4 * g;
     unsigned xs[Tiles], ws[Tiles], xsNext[Tiles], wsNext[Tiles];
-    auto loadExponents = [&](unsigned k) { // of steps k and k + 1, k even
-        k = min(k, (all - 1) / 2 * 2);
+    auto loadExponents = [&](const WideRows& r, unsigned k) { // of steps k and k + 1, k even
         const unsigned fromX = X8 ? k : k / 2 * 16, fromW = X8 ? k / 4 * 16 + k % 4 : k / 2 * 16;
 #pragma unroll
         for (unsigned m = 0; m < Tiles; ++m) {
             const unsigned at = Experts ? xeo[m] : xeo[0], from = fromX + (Experts ? 0 : m * 16 * pitchXe);
             const unsigned fromN = fromW + (m / 2 * 32 + m % 2 * 4) * pitchWe;
             if constexpr (X8) {
-                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(xer, at, from, 0);
-                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(wer, weo, fromN, 0);
+                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(r.xe, at, from, 0);
+                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b16(r.we, weo, fromN, 0);
             } else {
-                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(xer, at, from, 0);
-                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(wer, weo, fromN, 0);
+                xsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(r.xe, at, from, 0);
+                wsNext[m] = __builtin_amdgcn_raw_buffer_load_b32(r.we, weo, fromN, 0);
             }
         }
     };
-    f32x4 acc[Tiles][Tiles] = {};
-    loadExponents(0);
+    f32x4 acc[Tiles][Tiles];
+    WideTile tile = tileAt(0);
+    WideRows rows = rowsOf(tile, true), ahead = rows; // of this tile, and of the steps that are loaded now
+    place(0);
+    loadExponents(ahead, 0);
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i) loadX(0, 0, i);
+    for (unsigned i = 0; i < 8; ++i) loadX(ahead, 0, 0, i);
 #pragma unroll
-    for (unsigned i = 0; i < WL; ++i) loadW(0, 0, i);
+    for (unsigned i = 0; i < WL; ++i) loadW(ahead, 0, 0, i);
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i) loadX(1, 1, i);
+    for (unsigned i = 0; i < 8; ++i) loadX(ahead, 1, 1, i);
 #pragma unroll
-    for (unsigned i = 0; i < WL / 2; ++i) loadW(1, 1, partW(0, i));
+    for (unsigned i = 0; i < WL / 2; ++i) loadW(ahead, 1, 1, partW(0, i));
     waitBarrier<8 + WL / 2>();
 #pragma unroll
     for (unsigned i = 0; i < 2; ++i) readW(0, i);
 #pragma unroll
     for (unsigned i = 0; i < Tiles; ++i) readX(0, i, 0), readX(0, i, 1);
-    // Step S of the pair that the exponents are for. The fences keep the compiler from moving the reads and loads between
-    // the MFMAs down to where their results are needed, which is where they would be waited for.
-    auto blockStep = [&](unsigned k, auto block) {
+    // Step S of the pair that the exponents are for; the pair behind it begins at step f of `ahead`. The fences keep the
+    // compiler from moving the reads and loads between the MFMAs down to where their results are needed, which is where
+    // they would be waited for.
+    auto blockStep = [&](unsigned k, unsigned f, auto block) {
         constexpr unsigned S = decltype(block)::value;
 #pragma unroll
         for (unsigned q = 0; q < 4; ++q) {
@@ -534,10 +586,10 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
                     }
                     if (i % (turns / 4) == turns / 4 - 1) {
                         const unsigned j = i / (turns / 4);
-                        if (q == 0 && j < WL / 2) loadW(k + S + 1, 1 - S, partW(1, j));
-                        if (q == 1) loadX(k + S + 2, S, j);
-                        if (q == 2) loadX(k + S + 2, S, 4 + j);
-                        if (q == 3 && j < WL / 2) loadW(k + S + 2, S, partW(0, j));
+                        if (q == 0 && j < WL / 2) S == 0 ? loadW(rows, k + 1, 1, partW(1, j)) : loadW(ahead, f, 0, partW(1, j));
+                        if (q == 1) loadX(ahead, f + S, S, j);
+                        if (q == 2) loadX(ahead, f + S, S, 4 + j);
+                        if (q == 3 && j < WL / 2) loadW(ahead, f + S, S, partW(0, j));
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     auto multiply = [&](unsigned n, auto byte) {
@@ -558,57 +610,75 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
                     }
                 }
         }
-        // Where the loop ends the compiler copies the sums, without knowing that they come from an MFMA: the last
-        // ones, of up to 8 passes, have to be done by then.
+        // Where the loop ends the sums are read, by who does not know that they come from an MFMA: the last ones, of up to
+        // 8 passes, have to be done by then.
         if (S == 1)
             asm volatile("s_nop 15\n\ts_nop 3" : "+a"(acc[6][6]), "+a"(acc[7][6]), "+a"(acc[6][7]), "+a"(acc[7][7]));
     };
-    for (unsigned k = 0; k < all; k += 2) {
-        // Past the last block codes are zeros, and have to have finite exponents.
-        const unsigned keepW = finiteExponents(k * Halves, mine), keepX = X8 ? finiteExponents(k, a.count) : keepW;
+    for (unsigned i = 0; i < tiles; ++i) {
 #pragma unroll
-        for (unsigned m = 0; m < Tiles; ++m) {
-            xs[m] = (xsNext[m] & keepX) | (0x7F7F7F7Fu & ~keepX);
-            ws[m] = (wsNext[m] & keepW) | (0x7F7F7F7Fu & ~keepW);
+        for (unsigned n = 0; n < Tiles; ++n)
+#pragma unroll
+            for (unsigned m = 0; m < Tiles; ++m) acc[n][m] = f32x4{};
+        const bool more = i + 1 < tiles;
+        const WideTile next = more ? tileAt(i + 1) : tile;
+        for (unsigned k = 0; k < pairs; k += 2) {
+            // Past the last block codes are zeros, and have to have finite exponents.
+            const unsigned keepW = finiteExponents(k * Halves, mine), keepX = X8 ? finiteExponents(k, a.count) : keepW;
+#pragma unroll
+            for (unsigned m = 0; m < Tiles; ++m) {
+                xs[m] = (xsNext[m] & keepX) | (0x7F7F7F7Fu & ~keepX);
+                ws[m] = (wsNext[m] & keepW) | (0x7F7F7F7Fu & ~keepW);
+            }
+            const bool last = k + 2 >= pairs;
+            const unsigned f = last ? 0 : k + 2;
+            if (last) {
+                ahead = rowsOf(next, more);
+                if constexpr (Experts) place(i + more);
+            }
+            loadExponents(ahead, f);
+            blockStep(k, f, std::integral_constant<unsigned, 0>{});
+            blockStep(k, f, std::integral_constant<unsigned, 1>{});
         }
-        loadExponents(k + 2);
-        blockStep(k, std::integral_constant<unsigned, 0>{});
-        blockStep(k, std::integral_constant<unsigned, 1>{});
+        if (!Experts || tile.expert < a.experts) {
+            typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
+            const float* bias = a.bias ? a.bias + std::uint64_t(tile.expert) * a.outer : nullptr;
+            auto store = [&](auto whole) {
+                constexpr bool Whole = decltype(whole)::value;
+#pragma unroll
+                for (unsigned n = 0; n < Tiles; n += 2) {
+                    const unsigned column = tile.tn + wn + n * 16 + g * 8;
+                    float b[8];
+                    bias8<Whole>(bias, column, a.outer, b);
+#pragma unroll
+                    for (unsigned m = 0; m < Tiles; ++m) {
+                        const unsigned row = tile.first + wm + m * 16 + l16;
+                        float v[8];
+#pragma unroll
+                        for (unsigned j = 0; j < 8; ++j) // one by one: the compiler would move all sums at once, and spill
+                            asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[j]) : "a"(acc[n + j / 4][m][j % 4]));
+                        if (Whole || row < tile.end) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
+                    }
+                }
+            };
+            if (tile.first + B <= tile.end && tile.tn + B <= a.outer)
+                store(std::true_type{});
+            else
+                store(std::false_type{});
+        }
+        tile = next, rows = ahead;
     }
     // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    typename T::Raw* y = static_cast<typename T::Raw*>(a.y);
-    auto store = [&](auto whole) {
-        constexpr bool Whole = decltype(whole)::value;
-#pragma unroll
-        for (unsigned n = 0; n < Tiles; n += 2) {
-            const unsigned column = tn + wn + n * 16 + g * 8;
-            float b[8];
-            bias8<Whole>(a.bias, column, a.outer, b);
-#pragma unroll
-            for (unsigned m = 0; m < Tiles; ++m) {
-                const unsigned row = tm + wm + m * 16 + l16;
-                float v[8];
-#pragma unroll
-                for (unsigned j = 0; j < 8; ++j) // one by one: the compiler would move all sums at once, and spill
-                    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[j]) : "a"(acc[n + j / 4][m][j % 4]));
-                if (Whole || row < end) put8<T, Whole>(y + row * a.yStride, column, a.outer, v, b);
-            }
-        }
-    };
-    if (tm + B <= end && tn + B <= a.outer)
-        store(std::true_type{});
-    else
-        store(std::false_type{});
 }
 
 template <typename T, bool Experts>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void microWide8(Product a) {
-    wideTile<T, true, Experts>(a);
+    wideTiles<T, true, Experts>(a);
 }
 template <typename T, bool Experts>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void microWide4(Product a) {
-    wideTile<T, false, Experts>(a);
+    wideTiles<T, false, Experts>(a);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -790,12 +860,15 @@ void launchTiles(Product p, hipStream_t stream) {
 template <typename T, bool X8, bool Experts> void launchWide(Product p, hipStream_t stream) {
     const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 256) : over(p.rows, 256);
     p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 256));
-    checkGrid("matmul micro", up * p.tilesN, 256);
-    const dim3 grid(unsigned(up * p.tilesN)), threads(256);
+    const std::uint64_t tiles = up * p.tilesN, least = Experts ? over(tiles, 8 * kWideTiles) * 8 : 0;
+    checkGrid("matmul micro", tiles, 256);
+    // A multiple of the XCDs, so that a workgroup's tiles stay with one.
+    const dim3 grid(unsigned(std::min<std::uint64_t>(tiles, std::max<std::uint64_t>(kWideGroups, least)))), threads(256);
+    constexpr unsigned lds = 2 * 256 * (X8 ? 192 : 256) + (Experts ? kWideTiles * (sizeof(WideTile) + 256 * 4) : 0);
     if constexpr (X8)
-        hipLaunchKernelGGL((microWide8<T, Experts>), grid, threads, 2 * 256 * 192, stream, p);
+        hipLaunchKernelGGL((microWide8<T, Experts>), grid, threads, lds, stream, p);
     else
-        hipLaunchKernelGGL((microWide4<T, Experts>), grid, threads, 2 * 256 * 256, stream, p);
+        hipLaunchKernelGGL((microWide4<T, Experts>), grid, threads, lds, stream, p);
     checkHip(hipGetLastError());
 }
 
