@@ -59,7 +59,8 @@ void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, vo
                    ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, hipStream_t stream = nullptr);
 
 // The same on dense x, in `format`, with y's type that of x.
-std::size_t linearExpertsWorkspace(ExpertPlan plan, bool byToken, std::uint32_t inner, RowFormat format);
+std::size_t linearExpertsWorkspace(ExpertPlan plan, bool byToken, std::uint32_t inner, std::uint32_t outer, DenseType type,
+                                   RowFormat format);
 void linearExperts(DenseMatrix x, RowFormat format, bool byToken, MicroRows w, const float* bias, void* y,
                    std::uint64_t yStride, ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, void* workspace,
                    std::size_t workspaceBytes, hipStream_t stream = nullptr);

@@ -207,8 +207,8 @@ int tcc_matmul_experts(const uint8_t* xCodes, const uint8_t* xExponents, uint32_
                        const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t stride,
                        uint32_t type, const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each,
                        uint32_t experts, uint32_t inner, uint32_t outer, void* stream);
-int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, int byToken, uint32_t inner, uint32_t format,
-                                 size_t* bytes);
+int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, uint32_t experts, int byToken, uint32_t inner,
+                                 uint32_t outer, uint32_t type, uint32_t format, size_t* bytes);
 int tcc_linear_experts(const void* x, uint64_t stride, uint32_t type, uint32_t format, int byToken,
                        const uint8_t* wCodes, const uint8_t* wExponents, const float* bias, void* y, uint64_t yStride,
                        const int32_t* offsets, const int32_t* order, uint32_t choices, uint32_t each, uint32_t experts,

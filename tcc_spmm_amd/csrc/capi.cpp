@@ -496,12 +496,12 @@ int tcc_matmul_experts(const uint8_t* xCodes, const uint8_t* xExponents, uint32_
     });
 }
 
-int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, int byToken, uint32_t inner, uint32_t format,
-                                 size_t* bytes) {
+int tcc_linear_experts_workspace(uint32_t choices, uint32_t each, uint32_t experts, int byToken, uint32_t inner,
+                                 uint32_t outer, uint32_t type, uint32_t format, size_t* bytes) {
     return guarded([&] {
         need(bytes, "workspace size");
-        *bytes = linearExpertsWorkspace({nullptr, nullptr, nullptr, choices, each, 1}, byToken != 0, inner,
-                                        RowFormat(format));
+        *bytes = linearExpertsWorkspace({nullptr, nullptr, nullptr, choices, each, experts}, byToken != 0, inner, outer,
+                                        DenseType(type), RowFormat(format));
     });
 }
 

@@ -60,6 +60,10 @@ __device__ __forceinline__ unsigned exponentAt(unsigned step, unsigned i) { retu
 
 } // namespace micro
 
+// quantizeMicro, or with the exponents in the products' own order: 16 bytes of each row side by side, [fours of steps][rows].
+void quantizeMicroRowsTo(DenseMatrix x, MicroRows out, bool packed, std::uint32_t rows, std::uint32_t columns,
+                         hipStream_t stream);
+
 namespace micro {
 inline void checkMicro(const char* where, const MicroRows& r) {
     if (!r.codes || !r.exponents) reject(where, "null codes or exponents");

@@ -25,6 +25,7 @@ struct Product {
     void* y;
     std::uint64_t yStride;
     unsigned rows, inner, outer, count; // count: steps of a row
+    std::uint64_t xeRow, xeNext; // microWide: bytes from a row's exponents of x to the next row's, from four steps' to the next
     unsigned tilesM, tilesN;            // experts: tilesM is the most that their rows can make
     const void* dense;
     std::uint64_t denseStride;
@@ -102,13 +103,15 @@ __device__ __forceinline__ bool spanOf(const Product& a, unsigned tile, unsigned
     const unsigned id = idOf(total);
     if (id >= total) return false;
     unsigned base = 0;
-    while (id >= unsigned(__builtin_amdgcn_readlane(upTo, kWave - 1))) {
+    while (base <= a.experts && id >= unsigned(__builtin_amdgcn_readlane(upTo, kWave - 1))) {
         before = __builtin_amdgcn_readlane(upTo, kWave - 1), base += kWave;
         n = tilesOfLane(a, base + lane, tile, lo, hi), upTo = scanWave(n, lane) + before;
     }
-    const unsigned at = unsigned(__builtin_ctzll(__ballot(upTo > id)));
-    const unsigned start = __builtin_amdgcn_readlane(upTo - n, at);
-    s = {base + at, unsigned(__builtin_amdgcn_readlane(lo, at)) + (id - start) * tile, unsigned(__builtin_amdgcn_readlane(hi, at))};
+    const std::uint64_t past = __ballot(upTo > id);
+    if (!past) return false; // lists that are no plan, whose tiles are more than 32 bits hold
+    const unsigned at = unsigned(__builtin_ctzll(past)), start = __builtin_amdgcn_readlane(upTo - n, at);
+    const unsigned first = unsigned(__builtin_amdgcn_readlane(lo, at)) + (id - start) * tile;
+    s = {base + at, min(first, a.rows - 1), unsigned(__builtin_amdgcn_readlane(hi, at))};
     return true;
 }
 
@@ -410,6 +413,12 @@ struct WideTile {
     unsigned expert, first, end, tn;
 };
 
+// `bytes` from p on.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytesAt(const std::uint8_t* p, std::uint64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p), 0,
+                                             unsigned(min(bytes, std::uint64_t(0x7FFFFFFF))), 0x00020000);
+}
+
 // What the loads of a tile go by.
 struct WideRows {
     __amdgpu_buffer_rsrc_t x, w, xe, we;
@@ -422,7 +431,7 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
     extern __shared__ __align__(1024) std::uint8_t lds[]; // two stages: 256 rows of x, 256 of w; experts: tiles, sources
     const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const unsigned all = (a.count + Halves - 1) / Halves, pairs = (all + 1) / 2 * 2;
-    const unsigned pitch = xPitch<X8>(a), pitchW = wPitch(a), pitchXe = xExpPitch<X8>(a), pitchWe = wExpPitch(a);
+    const unsigned pitch = xPitch<X8>(a), pitchW = wPitch(a), pitchXe = unsigned(a.xeRow), pitchWe = wExpPitch(a);
     const bool byToken = Experts && a.order;
     WideTile* const list = reinterpret_cast<WideTile*>(lds + 2 * Stage);
     unsigned* const sources = reinterpret_cast<unsigned*>(lds + 2 * Stage + kWideTiles * sizeof(WideTile));
@@ -465,8 +474,11 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
         const std::uint64_t before = std::uint64_t(Experts ? min(t.expert, a.experts - 1) : 0) * a.outer;
         const unsigned xFirst = byToken ? 0 : t.first, xRows = !some ? xFirst : byToken ? a.rows / a.each : a.rows;
         const unsigned wRows = some ? a.outer : t.tn;
+        // Exponents behind the last row's may be any there are: no results of those rows are stored.
+        const std::uint64_t xBytes = std::uint64_t(byToken ? a.rows / a.each : a.rows) * xExpPitch<X8>(a);
         return WideRows{rowsAt(a.x, pitch, xFirst, xRows), rowsAt(a.w + before * pitchW, pitchW, t.tn, wRows),
-                        rowsAt(a.xe, pitchXe, xFirst, xRows), rowsAt(a.we + before * pitchWe, pitchWe, t.tn, wRows)};
+                        bytesAt(a.xe + xFirst * a.xeRow, xBytes - xFirst * a.xeRow),
+                        rowsAt(a.we + before * pitchWe, pitchWe, t.tn, wRows)};
     };
     if (!tiles) return;
     // Chunks and rows are dealt as in microTiles.
@@ -530,7 +542,8 @@ template <typename T, bool X8, bool Experts> __device__ __forceinline__ void wid
     // Two steps' exponents at a time, of this lane's row of each operand: a byte for each MFMA.
     unsigned xs[Tiles], ws[Tiles], xsNext[Tiles], wsNext[Tiles];
     auto loadExponents = [&](const WideRows& r, unsigned k) { // of steps k and k + 1, k even
-        const unsigned fromX = X8 ? k : k / 2 * 16, fromW = X8 ? k / 4 * 16 + k % 4 : k / 2 * 16;
+        const unsigned dword = X8 ? k / 4 : k / 2, in = X8 ? k % 4 : 0;
+        const unsigned fromX = dword * unsigned(a.xeNext) + in, fromW = dword * 16 + in;
 #pragma unroll
         for (unsigned m = 0; m < Tiles; ++m) {
             const unsigned at = Experts ? xeo[m] : xeo[0], from = fromX + (Experts ? 0 : m * 16 * pitchXe);
@@ -908,11 +921,50 @@ std::uint64_t exponentPitch(std::uint32_t inner, RowFormat f) {
 }
 std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
 
-void encode(DenseMatrix x, CodedRows out, std::uint32_t rows, std::uint32_t inner, hipStream_t stream) {
-    if (out.format == RowFormat::e4m3)
-        quantizeBlocks(x, {out.codes, out.exponents, BlockCodes::e4m3}, rows, inner, stream);
-    else
-        quantizeMicro(x, {out.codes, out.exponents}, rows, inner, stream);
+// x's exponents by fours of steps, all rows' side by side, as microWide is quickest to read them: what it wants of a row at a
+// time lies in a line of its own else. Rows in 4 bits are coded so, those in 8 bits have theirs copied into that order, 2 us.
+// For fewer than 2^31 bytes of them. (4096 x 4096 x 8192, 8-bit rows 136 us : 115, 4-bit 84 : 78; the weight's, 83.)
+__global__ __launch_bounds__(256) void packExponents(const unsigned* __restrict__ from, unsigned* __restrict__ to, unsigned rows,
+                                                     unsigned groups) {
+    const unsigned row = blockIdx.x * 256 + threadIdx.x;
+    if (row < rows) to[std::uint64_t(blockIdx.y) * rows + row] = from[std::uint64_t(row) * groups + blockIdx.y];
+}
+
+bool packs(Form form, std::uint64_t xRows, std::uint32_t inner, RowFormat format) {
+    return form == Form::wide && xRows * exponentPitch(inner, format) < std::uint64_t(1) << 31;
+}
+
+// Where microWide finds x's exponents.
+void setExponents(Product& p, RowFormat format, bool packed, std::uint64_t xRows) {
+    const std::uint64_t part = format == RowFormat::e4m3 ? 4 : 16;
+    p.xeRow = packed ? part : over(p.count, 4) * part, p.xeNext = packed ? xRows * part : part;
+}
+
+// Bytes of dense rows' codes and exponents, and of the packed copy of 8-bit ones'; `keep`: the first two are the caller's.
+std::size_t codedBytes(std::uint64_t rows, std::uint32_t inner, RowFormat format, bool packed, bool keep) {
+    const std::size_t exponents = rounded(rows * exponentPitch(inner, format));
+    return (keep ? 0 : rounded(rows * codePitch(inner, format)) + exponents) +
+           (packed && format == RowFormat::e4m3 ? exponents : 0);
+}
+
+// Codes dense rows into `space`, or what is kept of them, and lets p read them.
+void encode(Product& p, DenseMatrix x, RowFormat format, BlockRows keep, bool packed, std::uint32_t rows, std::uint32_t inner,
+            std::uint8_t* space, hipStream_t stream) {
+    CodedRows out = {keep.codes, keep.exponents, format};
+    if (!keep.codes) {
+        out.codes = space, out.exponents = space + rounded(rows * codePitch(inner, format));
+        space = out.exponents + rounded(rows * exponentPitch(inner, format));
+    }
+    p.x = out.codes, p.xe = out.exponents;
+    setExponents(p, format, packed, rows);
+    if (format == RowFormat::e2m1) return quantizeMicroRowsTo(x, {out.codes, out.exponents}, packed, rows, inner, stream);
+    quantizeBlocks(x, {out.codes, out.exponents, BlockCodes::e4m3}, rows, inner, stream);
+    if (!packed) return;
+    const unsigned groups = unsigned(over(p.count, 4));
+    hipLaunchKernelGGL(packExponents, dim3(unsigned(over(rows, 256)), groups), dim3(256), 0, stream,
+                       reinterpret_cast<const unsigned*>(out.exponents), reinterpret_cast<unsigned*>(space), rows, groups);
+    checkHip(hipGetLastError());
+    p.xe = space;
 }
 
 // LDS of x's codes and exponents in a fused product of few rows.
@@ -967,6 +1019,7 @@ void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType
     checkDense(where, y, stride, type, outer);
     Product p = productOf(w, bias, y, stride, rows, inner, outer);
     p.x = x.codes, p.xe = x.exponents;
+    setExponents(p, x.format, false, rows);
     withRows(type, x.format, [&](auto tag, auto x8) {
         launchForm<decltype(tag), decltype(x8)::value, false>(formOf(rows, inner, outer, type, x.format), p, stream);
     });
@@ -974,9 +1027,8 @@ void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType
 
 std::size_t linearMicroWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                  RowFormat format, bool keep) {
-    (void)outer, (void)type;
-    if (keep || fusedTokens(rows, inner, format)) return 0;
-    return rounded(rows * codePitch(inner, format)) + rounded(rows * exponentPitch(inner, format));
+    if (!rows || fusedTokens(rows, inner, format)) return 0;
+    return codedBytes(rows, inner, format, packs(formOf(rows, inner, outer, type, format), rows, inner, format), keep);
 }
 
 void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias, void* y, std::uint64_t yStride,
@@ -1008,11 +1060,12 @@ void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias
         });
         return checkHip(hipGetLastError());
     }
-    auto* spare = static_cast<std::uint8_t*>(workspace);
-    CodedRows coded = {keep.codes, keep.exponents, format};
-    if (!keep.codes) coded = {spare, spare + rounded(rows * codePitch(inner, format)), format};
-    encode(x, coded, rows, inner, stream);
-    matmulMicro(coded, w, bias, y, x.type, yStride, rows, inner, outer, stream);
+    const Form form = formOf(rows, inner, outer, x.type, format);
+    Product p = productOf(w, bias, y, yStride, rows, inner, outer);
+    encode(p, x, format, keep, packs(form, rows, inner, format), rows, inner, static_cast<std::uint8_t*>(workspace), stream);
+    withRows(x.type, format, [&](auto tag, auto x8) {
+        launchForm<decltype(tag), decltype(x8)::value, false>(form, p, stream);
+    });
 }
 
 namespace {
@@ -1038,6 +1091,29 @@ const char* matmulExpertsForm(ExpertPlan plan, std::uint32_t inner, std::uint32_
     return formName(expertFormOf(plan, inner, outer, type, format));
 }
 
+namespace {
+Product expertsProduct(bool byToken, MicroRows w, const float* bias, void* y, std::uint64_t stride, const ExpertPlan& plan,
+                       std::uint32_t inner, std::uint32_t outer) {
+    Product p = productOf(w, bias, y, stride, plan.choices, inner, outer);
+    p.offsets = plan.offsets, p.order = byToken ? plan.order : nullptr;
+    p.experts = plan.experts, p.each = plan.each;
+    return p;
+}
+
+std::uint32_t rowsOf(const ExpertPlan& plan, bool byToken) {
+    return byToken && plan.each ? plan.choices / plan.each : plan.choices;
+}
+bool packs(const ExpertPlan& plan, bool byToken, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    return packs(expertFormOf(plan, inner, outer, type, format), rowsOf(plan, byToken), inner, format);
+}
+
+// Codes of tokens are reached by 32 bits.
+void checkTokens(const char* where, const ExpertPlan& plan, bool byToken, std::uint32_t inner, RowFormat format) {
+    if (byToken && rowsOf(plan, true) * codePitch(inner, format) >> 31)
+        reject(where, "codes of tokens of 2^31 bytes or more: gather them");
+}
+} // namespace
+
 void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
                    ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, hipStream_t stream) {
     const char* where = "matmul experts";
@@ -1050,20 +1126,20 @@ void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, vo
     checkRowCodes(where, x);
     checkWeight(where, w, bias);
     checkDense(where, y, stride, type, outer);
-    if (byToken && plan.choices / plan.each * codePitch(inner, x.format) >> 31)
-        reject(where, "codes of tokens of 2^31 bytes or more: gather them");
-    Product p = productOf(w, bias, y, stride, plan.choices, inner, outer);
+    checkTokens(where, plan, byToken, inner, x.format);
+    Product p = expertsProduct(byToken, w, bias, y, stride, plan, inner, outer);
     p.x = x.codes, p.xe = x.exponents;
-    p.offsets = plan.offsets, p.order = byToken ? plan.order : nullptr;
-    p.experts = plan.experts, p.each = plan.each;
+    setExponents(p, x.format, false, plan.choices);
     withRows(type, x.format, [&](auto tag, auto x8) {
         launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, inner, outer, type, x.format), p, stream);
     });
 }
 
-std::size_t linearExpertsWorkspace(ExpertPlan plan, bool byToken, std::uint32_t inner, RowFormat format) {
-    const std::uint64_t rows = byToken && plan.each ? plan.choices / plan.each : plan.choices;
-    return rounded(rows * codePitch(inner, format)) + rounded(rows * exponentPitch(inner, format));
+std::size_t linearExpertsWorkspace(ExpertPlan plan, bool byToken, std::uint32_t inner, std::uint32_t outer, DenseType type,
+                                   RowFormat format) {
+    const std::uint64_t rows = rowsOf(plan, byToken);
+    if (!rows || !plan.experts) return 0;
+    return codedBytes(rows, inner, format, packs(plan, byToken, inner, outer, type, format), false);
 }
 
 void linearExperts(DenseMatrix x, RowFormat format, bool byToken, MicroRows w, const float* bias, void* y,
@@ -1076,16 +1152,18 @@ void linearExperts(DenseMatrix x, RowFormat format, bool byToken, MicroRows w, c
     checkFormat(where, format);
     checkExperts(where, plan);
     if (!plan.choices) return;
-    const std::uint32_t rows = byToken ? plan.choices / plan.each : plan.choices;
+    const std::uint32_t rows = rowsOf(plan, byToken);
     checkDense(where, x.data, x.stride, x.type, inner);
     checkDense(where, y, yStride, x.type, outer);
     checkWeight(where, w, bias);
-    const std::size_t need = linearExpertsWorkspace(plan, byToken, inner, format);
+    const std::size_t need = linearExpertsWorkspace(plan, byToken, inner, outer, x.type, format);
     if (need > workspaceBytes || !workspace) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
-    if (byToken && rows * codePitch(inner, format) >> 31) reject(where, "codes of tokens of 2^31 bytes or more: gather them");
-    auto* spare = static_cast<std::uint8_t*>(workspace);
-    const CodedRows coded = {spare, spare + rounded(rows * codePitch(inner, format)), format};
-    encode(x, coded, rows, inner, stream);
-    matmulExperts(coded, byToken, w, bias, y, x.type, yStride, plan, inner, outer, stream);
+    checkTokens(where, plan, byToken, inner, format);
+    Product p = expertsProduct(byToken, w, bias, y, yStride, plan, inner, outer);
+    encode(p, x, format, {}, packs(plan, byToken, inner, outer, x.type, format), rows, inner,
+           static_cast<std::uint8_t*>(workspace), stream);
+    withRows(x.type, format, [&](auto tag, auto x8) {
+        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, inner, outer, x.type, format), p, stream);
+    });
 }

@@ -17,8 +17,9 @@ template <typename T> constexpr bool kHalves = std::is_same<T, F32>::value;
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantizeMicroRows(const typename T::Raw* __restrict__ x, std::uint64_t stride,
-                                                               MicroRows out, unsigned items, unsigned columns,
-                                                               unsigned count, unsigned magic) {
+                                                               MicroRows out, std::uint64_t expRow, std::uint64_t expNext,
+                                                               unsigned items, unsigned columns, unsigned count,
+                                                               unsigned magic) {
     const unsigned lane = threadIdx.x % kBlockLanes;
     const unsigned item = flatGroup() * kGroups + threadIdx.x / kBlockLanes;
     if (item >= items) return;
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void quantizeMicroRows(const typename T::
     // Four lanes have each block's exponent: one writes it, the others, at the row's last step, fill the dword.
     const unsigned j = lane % 4;
     if (j == 0 || (step + 1 == count && step % 4 + j < 4))
-        out.exponents[std::uint64_t(row) * ((count + 3) / 4 * 16) + exponentAt(step, block) + j] = std::uint8_t(j ? 127u : e);
+        out.exponents[row * expRow + step / 4 * expNext + exponentAt(step % 4, block) + j] = std::uint8_t(j ? 127u : e);
 }
 
 template <typename T>
@@ -182,6 +183,11 @@ unsigned itemsOf(const char* where, std::uint32_t rows, unsigned count) {
 } // namespace
 
 void quantizeMicro(DenseMatrix x, MicroRows out, std::uint32_t rows, std::uint32_t columns, hipStream_t stream) {
+    quantizeMicroRowsTo(x, out, false, rows, columns, stream);
+}
+
+void quantizeMicroRowsTo(DenseMatrix x, MicroRows out, bool packed, std::uint32_t rows, std::uint32_t columns,
+                         hipStream_t stream) {
     const char* where = "quantize micro";
     checkColumns(where, columns);
     checkRows(where, rows);
@@ -193,8 +199,9 @@ void quantizeMicro(DenseMatrix x, MicroRows out, std::uint32_t rows, std::uint32
     withType(x.type, [&](auto tag) {
         typedef decltype(tag) T;
         hipLaunchKernelGGL((quantizeMicroRows<T>), grid, dim3(kThreads), 0, stream,
-                           static_cast<const typename T::Raw*>(x.data), x.stride, out, items, columns, count,
-                           rowMagic(count));
+                           static_cast<const typename T::Raw*>(x.data), x.stride, out,
+                           packed ? 16 : microExponentPitch(columns), packed ? std::uint64_t(rows) * 16 : 16, items, columns,
+                           count, rowMagic(count));
     });
     checkHip(hipGetLastError());
 }

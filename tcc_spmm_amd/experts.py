@@ -15,8 +15,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .blocks import _TYPES, E4M3, _away, _dense, _rows, _same_device, _stream, _stride
-from .micro import MicroWeight, _code_pitch, _format, _laid, _workspace
+from .blocks import _TYPES, E4M3, BlockTensor, _away, _dense, _rows, _same_device, _stream, _stride
+from .micro import _FORMATS, MicroTensor, MicroWeight, _code_pitch, _format, _laid, _workspace
 
 MAX_EXPERTS = 1024
 MAX_EACH = 1024
@@ -202,6 +202,36 @@ def _stack_bias(bias, experts: int, outer: int, device) -> int:
     return bias.data_ptr()
 
 
+def matmul_experts(x: BlockTensor | MicroTensor, weight: MicroWeight, plan: ExpertPlan,
+                   bias: torch.Tensor | None = None, *, by_token: bool = False, dtype=torch.bfloat16,
+                   stream=None) -> torch.Tensor:
+    """matmulExperts: the rows of linear_experts for x already in E4M3 blocks or in microscaled ones, a row for each sorted row
+    or, by_token, for each token. dtype is that of the result, with the sums of matmul_micro."""
+    if x.codes.dtype not in _FORMATS:
+        raise ValueError("x must have float8_e4m3fn or float4_e2m1fn_x2 codes")
+    if dtype not in _TYPES:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    _stack(weight, plan)
+    if x.columns != weight.columns:
+        raise ValueError(f"x has rows of {x.columns} elements, expected {weight.columns}")
+    if x.rows != (plan.tokens if by_token else plan.choices):
+        raise ValueError(f"x must have {plan.tokens if by_token else plan.choices} rows, got {x.rows}")
+    device, outer = x.codes.device, weight.rows
+    _here(device, plan)
+    _same_device(device, weight.codes)
+    at_bias = _stack_bias(bias, plan.experts, outer, device)
+    away = _away(device, stream)
+    if away:
+        with away:
+            return matmul_experts(x, weight, plan, bias, by_token=by_token, dtype=dtype)
+    y = torch.empty((plan.choices, outer), dtype=dtype, device=device)
+    check(lib().tcc_matmul_experts(x.codes.data_ptr(), x.exponents.data_ptr(), _FORMATS[x.codes.dtype], by_token,
+                                   weight.codes.data_ptr(), weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer,
+                                   _TYPES[dtype], plan.offsets.data_ptr(), plan.order.data_ptr(), plan.choices, plan.each,
+                                   plan.experts, x.columns, outer, _stream(device.index)))
+    return y
+
+
 def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias: torch.Tensor | None = None, *,
                    by_token: bool = False, codes=E4M3, stream=None) -> torch.Tensor:
     """linearExperts: rows [choices, outer] in x's type, each Q(x) times its expert's weight of the stack, plus that
@@ -225,7 +255,7 @@ def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias:
     dtype = _TYPES[x.dtype]
     y = torch.empty((plan.choices, outer), dtype=x.dtype, device=device)
     _space, at, size = _workspace("tcc_linear_experts_workspace",
-                                  (plan.choices, plan.each, by_token, inner, kind), device)
+                                  (plan.choices, plan.each, plan.experts, by_token, inner, outer, dtype, kind), device)
     check(lib().tcc_linear_experts(flat.data_ptr(), stride, dtype, kind, by_token, weight.codes.data_ptr(),
                                    weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer, plan.offsets.data_ptr(),
                                    plan.order.data_ptr(), plan.choices, plan.each, plan.experts, inner, outer, at, size,

@@ -137,7 +137,8 @@ PRODUCTS = [(1, 1, 1, 1, 1), (24, 4, 32, 512, 200), (3, 2, 5, 130, 33), (200, 4,
 @pytest.mark.parametrize("away,kind", [(0.0, "any"), (0.3, "few"), (0.0, "one")])
 def test_linear_experts(gpu, tokens, each, experts, inner, outer, dtype, codes, away, kind):
     from tcc_spmm_amd import experts as X
-    from tcc_spmm_amd.micro import quantize_weight_micro
+    from tcc_spmm_amd.blocks import quantize_blocks
+    from tcc_spmm_amd.micro import quantize_micro, quantize_weight_micro
     ids = choices(tokens, each, experts, 3, away, kind=kind)
     plan = X.sort_experts(ids, experts)
     offsets, order, _ = O.plan(ids.cpu().numpy(), experts)
@@ -164,6 +165,10 @@ def test_linear_experts(gpu, tokens, each, experts, inner, outer, dtype, codes, 
     near(X.linear_experts(x, weight, plan, by_token=True, codes=FORMATS[codes]), bare,
          (room + 4 * U * np.abs(bare)) * 1.01 + rounded(bare, dtype), "y without bias")
     assert not y[offsets[-1]:].any()
+    coded = (quantize_blocks if codes == "e4m3" else quantize_micro)(x)
+    assert torch.equal(X.matmul_experts(coded, weight, plan, bias, by_token=True, dtype=DTYPES[dtype]), y)
+    coded = (quantize_blocks if codes == "e4m3" else quantize_micro)(rows)
+    assert torch.equal(X.matmul_experts(coded, weight, plan, bias, dtype=DTYPES[dtype]), y)
 
 
 @pytest.mark.parametrize("tokens,each,experts,inner,outer", [(2100, 3, 5, 500, 600), (1100, 2, 2, 1153, 520), (900, 4, 7, 100, 3000)])
@@ -310,7 +315,7 @@ def test_calls_on_another_stream_and_captured(gpu):
 
 def test_refusals(gpu):
     from tcc_spmm_amd import experts as X
-    from tcc_spmm_amd.micro import quantize_weight_micro
+    from tcc_spmm_amd.micro import quantize_micro, quantize_weight_micro
     ids = choices(10, 2, 4)
     plan = X.sort_experts(ids, 4)
     x, w = random((10, 64), 1), random((10, 2), 2)
@@ -330,6 +335,9 @@ def test_refusals(gpu):
                  lambda: X.linear_experts(rows[:, :63], stack, plan),
                  lambda: X.linear_experts(rows, stack, plan, torch.zeros(32, device="cuda")),
                  lambda: X.linear_experts(rows, stack, plan, codes=torch.int8),
+                 lambda: X.matmul_experts(quantize_micro(x), stack, plan), lambda: X.matmul_experts(quantize_micro(rows), one, plan),
+                 lambda: X.matmul_experts(quantize_micro(rows), stack, plan, dtype=torch.float64),
+                 lambda: X.matmul_experts(quantize_micro(rows[:, :63]), stack, plan),
                  lambda: X.expert_linear(rows.clone().requires_grad_(), stack, plan),
                  lambda: X.expert_linear(rows, stack, plan, torch.zeros((4, 32), device="cuda", requires_grad=True)),
                  lambda: X.ExpertPlan(plan.offsets, plan.order[:-1], plan.places, (10,), 2),

@@ -146,7 +146,7 @@ def test_expert_product_refusals():
     rejected(matmul(by=1, n=1 << 26, k=1 << 8), b"gather them")
     assert matmul(n=0) == 0
     size = ctypes.c_size_t()
-    assert L.tcc_linear_experts_workspace(80, 2, 1, 300, 0, ctypes.byref(size)) == 0 and 40 * 388 <= size.value < 80 * 388
+    assert L.tcc_linear_experts_workspace(80, 2, 4, 1, 300, 64, 1, 0, ctypes.byref(size)) == 0 and 40 * 388 <= size.value < 80 * 388
     call = lambda x=P, space=P, size=size.value: L.tcc_linear_experts(  # noqa: E731
         x, 300, 1, 0, 1, P, P, None, P, 64, P, P, 80, 2, 4, 300, 64, space, size, None)
     rejected(call(x=None), b"null dense")
