@@ -7,7 +7,9 @@ counterpart in the original library, quantize_pack_features_int8 (both feature s
 and launch_spmm_int8_noalloc (no caller workspace).
 Dense layers on what the sparse product gives (module tcc_spmm_amd.blocks, no counterpart either): a linear
 layer in 8-bit blocks with its gradients, and activations that keep their input in 8 bits (BlockLinear,
-block_activation, linear_blocks and the rest). torch is imported lazily, only by these two modules.
+block_activation, linear_blocks and the rest). The same with weights in microscaled 4-bit blocks (module
+tcc_spmm_amd.micro), and layers of many experts on them (module tcc_spmm_amd.experts). torch is imported lazily, only by
+these four modules.
 """
 from .format import (NO_PARTIAL, SW32_BUCKET_ORDER, SW32_TASK_PANEL_LIMIT, CsrMatrix,
                      Sw32HostFormat, convert_csr_to_sw32, csr_from_arrays, load_matrix_market, make_canonical_csr,

