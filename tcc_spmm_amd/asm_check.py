@@ -69,7 +69,7 @@ def _parse(lines):
             asm_blocks.append((block, len(instrs)))
             block = None
         s = line.split(";")[0].strip()
-        m = re.match(r"^(\.LBB\S+):", s)
+        m = s.startswith(".LBB") and re.match(r"^(\.LBB\S+):", s)
         if m:
             labels[m.group(1)] = len(instrs)
             continue
@@ -97,6 +97,8 @@ def _info(ins: str):
 
 
 def _successors(instrs, labels, i):
+    if not instrs[i].startswith("s_"):
+        return [i + 1]
     op = instrs[i].split()[0]
     m = re.search(r"(\.LBB\S+)", instrs[i])
     if op.startswith("s_cbranch") and m:

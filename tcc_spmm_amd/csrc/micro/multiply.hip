@@ -321,18 +321,24 @@ __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
     };
     // Steps in runs of four, whose stages are constants, of one or two dwords of exponents.
     unsigned k = first;
-    auto four = [&](unsigned most) {
+    for (; k + 4 <= first + steps; k += 4) {
         nextExponents(k);
         step(k, std::integral_constant<unsigned, 0>{});
-        if (most > 1) step(k + 1, std::integral_constant<unsigned, 1>{});
-        if (most > 2) {
+        step(k + 1, std::integral_constant<unsigned, 1>{});
+        if constexpr (Dword == 2) nextExponents(k + 2);
+        step(k + 2, std::integral_constant<unsigned, 2>{});
+        step(k + 3, std::integral_constant<unsigned, 3>{});
+    }
+    // Of several groups each has whole dwords of steps.
+    if ((Groups == 1 || Dword == 2) && k < first + steps) {
+        nextExponents(k);
+        step(k, std::integral_constant<unsigned, 0>{});
+        if (k + 1 < first + steps) step(k + 1, std::integral_constant<unsigned, 1>{});
+        if (Groups == 1 && k + 2 < first + steps) {
             if constexpr (Dword == 2) nextExponents(k + 2);
             step(k + 2, std::integral_constant<unsigned, 2>{});
         }
-        if (most > 3) step(k + 3, std::integral_constant<unsigned, 3>{});
-    };
-    for (; k + 4 <= first + steps; k += 4) four(4);
-    if (k < first + steps) four(first + steps - k);
+    }
     // Loads to LDS past the last step have to land before the workgroup gives its LDS back.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (Groups > 1) {
