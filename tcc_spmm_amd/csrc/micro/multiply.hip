@@ -718,8 +718,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 // the MFMA's registers, each byte read once on the chip, four steps' loads at a time before the first is used; every
 // workgroup codes x for itself into LDS while its first weights are on their way. Measured: 1 x 4096 x 4096 bf16 4.9 us, 1.8 TB/s
 // of the weight, most of it the launch and two loads' ways, which the same layer in 8 bits takes 4.9 to 5.3 for as well: what 4
-// bits save here is memory. Already coded rows, and more of them, are quicker in microTiles (16 x 4096 x 4096 6.1 us, this way 6.6).
-constexpr unsigned kTokenWaves = 8, kFusedRows = 4;
+// bits save here is memory. A row more is 0.5 us, the coding in every workgroup.
+constexpr unsigned kTokenWaves = 8, kFusedRows = 16; // the rows of an MFMA
 
 template <typename T, bool X8> __global__ __launch_bounds__(kWave* kTokenWaves) void microTokens(Product a) {
     constexpr bool Exact = X8 && std::is_same<T, F32>::value;
@@ -992,8 +992,14 @@ std::size_t fusedLds(std::uint32_t rows, std::uint32_t inner, RowFormat f) {
     const std::size_t count = over(inner, kStep);
     return (rows * count * (f == RowFormat::e4m3 ? kStep + 1 : kStep / 2 + 4) + 15) / 16 * 16;
 }
-bool fusedTokens(std::uint32_t rows, std::uint32_t inner, RowFormat f) {
-    return rows <= kFusedRows && fusedLds(rows, inner, f) <= 48 * 1024;
+// Whether the layer takes microTokens: by its estimated time on the GPU against coding and product in launches of their own, of
+// which one more costs the caller 4 us and the GPU one of them. The constants fit these (rows x inner x outer, bf16, 8-bit
+// rows, this : two): 2 x 4096 x 4096 5.1 : 8.0, 8 x 4096 x 4096 8.1 : 8.1, 16 x 2048 x 4096 8.4 : 6.9, 16 x 512 x 4096 4.8 : 5.7,
+// 6 x 2048 x 8192 8.3 : 7.0, 8 x 4096 x 8192 11.5 : 8.0; the call's time 8 x 4096 x 4096 7.9 : 12.0, 16 x 2048 x 4096 8.2 : 11.9.
+bool fusedTokens(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, RowFormat f) {
+    const double count = double(over(inner, kStep)), more = double(over(outer, 4096)) - 1.0;
+    const double fused = 4.0 + more + 0.0165 * rows * count * (1.0 + 0.5 * more), two = 5.3 + 0.085 * count;
+    return rows <= kFusedRows && fusedLds(rows, inner, f) <= 48 * 1024 && fused <= two + 1.5;
 }
 
 Product productOf(MicroRows w, const float* bias, void* y, std::uint64_t stride, std::uint32_t rows, std::uint32_t inner,
@@ -1022,7 +1028,7 @@ const char* matmulMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32
 
 const char* linearMicroForm(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
     const char* product = matmulMicroForm(rows, inner, outer, type, format);
-    return fusedTokens(rows, inner, format) ? "microTokens" : product;
+    return fusedTokens(rows, inner, outer, format) ? "microTokens" : product;
 }
 
 void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
@@ -1047,7 +1053,7 @@ void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType
 
 std::size_t linearMicroWorkspace(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type,
                                  RowFormat format, bool keep) {
-    if (!rows || fusedTokens(rows, inner, format)) return 0;
+    if (!rows || fusedTokens(rows, inner, outer, format)) return 0;
     return codedBytes(rows, inner, format, packs(formOf(rows, inner, outer, type, format), rows, inner, format), keep);
 }
 
@@ -1071,7 +1077,7 @@ void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias
     const std::size_t need = linearMicroWorkspace(rows, inner, outer, x.type, format, keep.codes);
     if (need > workspaceBytes || (need && !workspace)) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
-    if (fusedTokens(rows, inner, format)) {
+    if (fusedTokens(rows, inner, outer, format)) {
         Product p = productOf(w, bias, y, yStride, rows, inner, outer);
         p.dense = x.data, p.denseStride = x.stride, p.keep = keep.codes, p.keepExp = keep.exponents;
         withRows(x.type, format, [&](auto tag, auto x8) {

@@ -33,8 +33,8 @@ PRODUCTS = [
     *(("microTiles128", *kind, 4091, 300, 4099) for kind in EIGHT + FOUR),
     *(("microTiles64", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((777, 1001, 1437), (1900, 1500, 500), (48, 4096, 8191))
       if (kind, size) != (EXACT[0], (48, 4096, 8191))),
-    *(("microTiles32", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((16, 4096, 1000), (32, 2900, 513))),
-    *(("microTokens", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((1, 4096, 130), (3, 100, 77), (4, 1001, 50))),
+    *(("microTiles32", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((16, 4096, 1000), (32, 2900, 513), (17, 1500, 40))),
+    *(("microTokens", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((1, 4096, 130), (3, 100, 77), (7, 4096, 300), (16, 1001, 50))),
 ]
 KERNELS = {"microWide", "microTiles128", "microTiles64", "microTiles32", "microTokens"}
 
