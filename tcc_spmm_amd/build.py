@@ -77,14 +77,14 @@ INLINE_MFMA = {CSRC / "blocks" / "product.hip": "multiplyWide", CSRC / "blocks" 
 # load, 4 or 8 a wait, after 28 in front of the loop, and nine loads of exponents a pair of blocks (25 - 16, 21 - 12).
 # multiplyTiles of four stages: two stages of 4 loads, after three in front of the loop. microWide4 and microWide8 as
 # multiplyWide, with 16 loads of exponents, and of rows in 8 bits half as many of the weight; microTiles as multiplyTiles,
-# a stage of 4 loads for rows in 4 bits and of 3 in 8; a name with a type stands for the kernel's other types too.
+# a stage of 4 loads for rows in 4 bits and of 3 in 8, in tiles of 64 x 32 of 6 and 5; a name with a type stands for the kernel's other types too.
 COUNTED_WAITS = {CSRC / "blocks" / "product.hip": {
     "multiplyWide": {25: (16, {4, 8}), 21: (12, {8}), 16: (16, {8}), 12: (12, {8, 28})},
     "multiplyTiles": {8: (8, {4, 12})},
 }, CSRC / "micro" / "multiply.hip": {
     "microWide4IN6blocks4BF16": {32: (16, {4, 8}), 28: (12, {8}), 16: (16, {8}), 12: (12, {8, 28})},
     "microWide8IN6blocks4BF16": {28: (12, {2, 4}), 26: (10, {8}), 12: (12, {4}), 10: (10, {8, 22})},
-    "microTilesIN6blocks4BF16": {8: (8, {4, 12}), 6: (6, {3, 9})},
+    "microTilesIN6blocks4BF16": {8: (8, {4, 12}), 6: (6, {3, 9}), 12: (12, {6, 18}), 10: (10, {5, 15})},
 }}
 
 

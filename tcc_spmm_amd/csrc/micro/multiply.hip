@@ -179,8 +179,8 @@ template <bool Experts> __device__ __forceinline__ void take(Product& a, Tile& t
 // An FP32 y of E4M3 rows takes the codes' values, exact in bf16, through the bf16 MFMA, whose sums are FP32's: a wave converts
 // the codes that it has read from LDS, four conversions for each MFMA of 16 cycles in tiles of 64.
 // What bounds them is the chain of a step, a barrier and the LDS reads behind it, and for few rows the weight's way from
-// memory. Measured, us: 48 x 4096 x 8191 f16 with 8-bit rows 11.9 in tiles of 64 (1.5 TB/s of the weight, 64 steps' chain);
-// 24 tokens to 4 of 32 experts, 2048 x 4096, 23 in tiles of 64, 6.1 TB/s of the weights; 6002 rows of 8 experts, 2048 x 1000, 30
+// memory. Measured, us: 48 x 4096 x 8191 with 8-bit rows 9.3 in tiles of 64 x 32 (11.5 in tiles of 64, twice the steps for half
+// the CUs); 17 x 4096 x 4096 6.6 in tiles of 32; 24 tokens to 4 of 32 experts, 2048 x 4096, 23 in tiles of 64, 6.1 TB/s of the weights; 6002 rows of 8 experts, 2048 x 1000, 30
 // in tiles of 128; FP32: 2001 x 1024 x 4097 32, 0.53 PFLOP/s, 2001 x 4097 x 1024 26, 0.64.
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
@@ -815,12 +815,13 @@ template <typename T, bool X8> __global__ __launch_bounds__(kWave* kTokenWaves) 
 // ------------------------------------------------------------------------------------------------
 // Host side
 
-enum class Form { wide, middle, small, few };
+enum class Form { wide, middle, small, half, few };
 const char* formName(Form f) {
     switch (f) {
     case Form::wide: return "microWide";
     case Form::middle: return "microTiles128";
     case Form::small: return "microTiles64";
+    case Form::half: return "microTiles64x32";
     default: return "microTiles32";
     }
 }
@@ -832,35 +833,52 @@ std::uint64_t mostTiles(std::uint64_t rows, std::uint64_t experts, unsigned tile
     return std::min(rows, rows / tile + experts + 1);
 }
 
-// The tile of a product: the least estimated time, in microseconds. A CU holds one workgroup of tiles of 256 or, with its
-// four groups of waves, 32, two of 128 and two or three of 64; while tiles of 128 or 64 are at most one a CU, each step is
-// quicker. tilesOf says how many row tiles of a size there are, launched how many workgroups a launch of it has. The constants
-// fit these times (rows x inner x outer: 256, 128, 64, 32; 8-bit rows in bf16, 4-bit rows, 8-bit rows in FP32):
-//   16 x 4096 x 4096   46 22 8.2 6.1, 28 20 7.4 5.8, - 41 14.8 7.0      48 x 4096 x 8192  47 24 9.6 11.6, 29 22 8.3 10.9, - 43 15.7 13.7
-//   200 x 1024 x 1024  21 8.7 4.3 4.8, 18 9.1 4.5 5.1, - 14 6.1 5.5     512 x 4096 x 4096 58 27 18 41, 35 24 16 38, - 47 26 48
-//   777 x 1001 x 1437  23 10.5 7.1 18, 20 11 7.4 20, - 15 9.3 21        2048 x 512 x 2048 14 7.4 8.2 52, 12 7.5 9.0 54, - 13 12 63
-//   1024 x 8192 x 2048 108 58 35 70, 63 49 28 61, - 96 49 78            4096 x 2048 x 4096 36 48 61 -, 27 46 61 -, - 105 92 -
-//   100000 x 256 x 256 25 21 26 -, 26 29 41 -, - 39 36 -                3000 x 2000 x 3000 34 37 38 120, 26 35 36 126, - 77 53 140
+// The tile of a product: the least estimated time, in microseconds. A CU holds one workgroup of tiles of 256, two of 128, two or
+// three of 64 and of those whose two groups of waves share the inner axis, 64 x 32 and 32; while tiles are at most one a CU, each
+// step is quicker. tilesOf says how many row tiles of a size there are, launched how many workgroups a launch of it has. The
+// constants fit these times (rows x inner x outer: 256, 128, 64, 64 x 32, 32; 8-bit rows in bf16, 4-bit rows, 8-bit rows in FP32):
+//   17 x 4096 x 4096   - 24 9.8 7.7 6.6, - 23 7.8 6.4 5.6, - - 16 11 8.3     48 x 4096 x 8191  47 26 12 9.3 10, 29 24 9.5 7.7 9.1, - - 16 12 12
+//   200 x 1024 x 1024  21 8.6 4.2 3.9 3.5, 18 9.1 4.4 3.9 3.4, - - 6.2 5.1 4.3   512 x 4096 x 1024 - 27 11 8.9 9.9, - 23 8.6 6.8 8.6, - - 16 11 12
+//   777 x 1001 x 1437  23 10 7.0 8.7 8.7, 20 11 7.3 9.5 9.0, - 15 9.3 10 10   2048 x 512 x 2048 14 7.4 8.2 - -, 12 7.5 9.0 - -, - 13 12 - -
+//   1024 x 8192 x 2048 108 58 35 - -, 63 49 28 - -, - 96 49 - -          4096 x 2048 x 4096 36 48 61 - -, 27 46 61 - -, - 105 92 - -
+//   100000 x 256 x 256 25 21 26 - -, 26 29 41 - -, - 39 36 - -           3000 x 2000 x 3000 34 37 38 - -, 26 35 36 - -, - 77 53 - -
 template <typename Tiles, typename Launched>
 Form leastOf(std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format, bool few, Tiles tilesOf, Launched launched) {
     const double k = double(over(inner, kStep));
     const bool x8 = format == RowFormat::e4m3, exact = x8 && type == DenseType::f32;
-    const auto tiles = [&](unsigned size) { return tilesOf(size) * double(over(outer, size)); };
+    const auto tiles = [&](unsigned up, unsigned across) { return tilesOf(up) * double(over(outer, across)); };
     const auto rounds = [](double n, unsigned slots) { return std::ceil(n / slots); };
-    const auto takes = [&](unsigned size, unsigned threads) { return launchTakes(launched(size) * over(outer, size), threads); };
-    const double never = 1e300, half = tiles(128), quarter = tiles(64);
-    double wide = rounds(tiles(256), 256) * (x8 ? 9.0 + 1.56 * k : 11.0 + 0.84 * k);
+    const auto takes = [&](unsigned up, unsigned across, unsigned threads) {
+        return launchTakes(launched(up) * over(outer, across), threads);
+    };
+    const auto by = [&](double n, double one, double oneStep, double some, double slots, double step) {
+        return n <= 256 ? one + oneStep * k : some + n / 512 * (slots + step * k);
+    };
+    constexpr double never = 1e300;
+    const double half = tiles(128, 128);
+    double wide = rounds(tiles(256, 256), 256) * (x8 ? 9.0 + 1.56 * k : 11.0 + 0.84 * k);
     double middle = half <= 256 ? (x8 ? 3.5 + 0.8 * k : 4.5 + 0.68 * k) : rounds(half, 512) * (x8 ? 2.7 + 1.32 * k : 5.2 + 1.1 * k);
-    double small = quarter <= 256 ? (exact ? 2.6 + 0.42 * k : x8 ? 2.3 + 0.235 * k : 2.8 + 0.18 * k)
-                                  : 2.2 + quarter / 512 * (exact ? 2.2 + 0.66 * k : x8 ? 1.1 + 0.44 * k : 2.2 + 0.38 * k);
-    double fewest = 0.7 + rounds(tiles(32), 256) * (exact ? 3.6 + 0.085 * k : 3.2 + 0.075 * k);
+    double small = exact ? by(tiles(64, 64), 2.6, 0.42, 2.2, 2.2, 0.66)
+                   : x8  ? by(tiles(64, 64), 2.2, 0.26, 2.2, 1.1, 0.44)
+                         : by(tiles(64, 64), 2.8, 0.18, 2.2, 2.2, 0.38);
+    double narrow = exact ? by(tiles(64, 32), 2.9, 0.255, 2.0, 3.5, 0.55)
+                    : x8  ? by(tiles(64, 32), 2.5, 0.195, 1.5, 3.0, 0.36)
+                          : by(tiles(64, 32), 3.0, 0.13, 2.0, 4.0, 0.35);
+    double fewest = exact ? by(tiles(32, 32), 2.8, 0.18, 1.5, 2.8, 0.25)
+                    : x8  ? by(tiles(32, 32), 2.4, 0.14, 1.5, 2.0, 0.21)
+                          : by(tiles(32, 32), 2.6, 0.1, 1.5, 2.6, 0.16);
     if (exact) wide = middle = never; // of no size the quickest: half the wave's conversions are of operands that others have too
-    if (!takes(128, 512)) middle = never;
-    if (!takes(64, 256)) small = never;
-    if (!few || !takes(32, 512)) fewest = never;
-    const double least = std::min(std::min(wide, middle), std::min(small, fewest));
+    if (!takes(128, 128, 512)) middle = never;
+    if (!takes(64, 64, 256)) small = never;
+    if (!few || !takes(64, 32, 256)) narrow = never;
+    if (!few || !takes(32, 32, 256)) fewest = never;
+    const double least = std::min({wide, middle, small, narrow, fewest});
     if (least == never) return exact ? Form::small : Form::wide; // more tiles than a launch takes: refused there
-    return least == small ? Form::small : least == fewest ? Form::few : least == middle ? Form::middle : Form::wide;
+    return least == small    ? Form::small
+           : least == narrow ? Form::half
+           : least == fewest ? Form::few
+           : least == middle ? Form::middle
+                             : Form::wide;
 }
 
 Form formOf(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
@@ -909,7 +927,9 @@ template <typename T, bool X8, bool Experts> void launchForm(Form form, Product 
     constexpr bool exact = X8 && std::is_same<T, F32>::value;
     if (form == Form::small) return launchTiles<T, X8, Experts, 64, 64, 2, 2, 4, 1>(p, stream);
     if constexpr (!Experts)
-        if (form == Form::few) return launchTiles<T, X8, false, 32, 32, 2, 1, 4, 4>(p, stream);
+        if (form == Form::few) return launchTiles<T, X8, false, 32, 32, 2, 1, 4, 2>(p, stream);
+    if constexpr (!Experts)
+        if (form == Form::half) return launchTiles<T, X8, false, 64, 32, 2, 1, 4, 2>(p, stream);
     if constexpr (!exact) {
         if (form == Form::middle) return launchTiles<T, X8, Experts, 128, 128, 4, 2, 2, 1>(p, stream);
         launchWide<T, X8, Experts>(p, stream);

@@ -31,12 +31,11 @@ PRODUCTS = [
     *(("microWide", *kind, *size) for kind in EIGHT for size in ((3900, 600, 4000), (3000, 2000, 3000), (4000, 900, 4090))),
     *(("microWide", *kind, *size) for kind in FOUR for size in ((3900, 600, 4000), (4097, 1153, 4000), (3000, 2000, 3000))),
     *(("microTiles128", *kind, 4091, 300, 4099) for kind in EIGHT + FOUR),
-    *(("microTiles64", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((777, 1001, 1437), (1900, 1500, 500), (48, 4096, 8191))
-      if (kind, size) != (EXACT[0], (48, 4096, 8191))),
-    *(("microTiles32", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((16, 4096, 1000), (32, 2900, 513), (17, 1500, 40))),
+    *(("microTiles64", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((777, 1001, 1437), (1900, 1500, 2300))),
+    *(("microTiles64x32", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((48, 4096, 8191), (500, 2900, 1001), (192, 4100, 2500))),
+    *(("microTiles32", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((16, 4096, 1000), (32, 2900, 513), (17, 130, 40))),
     *(("microTokens", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((1, 4096, 130), (3, 100, 77), (7, 4096, 300), (16, 1001, 50))),
 ]
-KERNELS = {"microWide", "microTiles128", "microTiles64", "microTiles32", "microTokens"}
 
 # tokens, each, experts, inner, outer
 EXPERTS = [
@@ -56,9 +55,9 @@ def test_the_sizes_below_take_every_kernel():
         assert expert_form(tokens * each, count, inner, outer, dtype, codes) == form, (dtype, codes, tokens, inner, outer)
     # each pair of types that a kernel is built for
     built = {("microWide", *k) for k in EIGHT + FOUR} | {("microTiles128", *k) for k in EIGHT + FOUR} | {
-        (name, *k) for name in ("microTiles64", "microTiles32", "microTokens") for k in EIGHT + FOUR + EXACT}
+        (name, *k) for name in ("microTiles64", "microTiles64x32", "microTiles32", "microTokens") for k in EIGHT + FOUR + EXACT}
     assert {p[:3] for p in PRODUCTS} == built
-    assert {p[:3] for p in EXPERTS} == {b for b in built if b[0] not in ("microTiles32", "microTokens")}
+    assert {p[:3] for p in EXPERTS} == {b for b in built if b[0] not in ("microTiles64x32", "microTiles32", "microTokens")}
 
 
 @pytest.mark.gpu
