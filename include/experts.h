@@ -11,8 +11,9 @@
 //
 // Every function is asynchronous on `stream` and allocates nothing. Without choices they return without a launch
 // (sortExperts still writes the offsets). Errors are thrown before any launch, as in blocks.h. Choices may be up to
-// 2^31 - 1, of up to 1024 each, and experts 1 to 1024. Kernels hold what they read of a plan to the sizes given, so that
-// a plan of other sizes gives wrong rows, never an access out of range.
+// 2^31 - 1, of up to 1024 each, and experts 1 to 1024; tokens of rows of more than 1024 elements fewer than 2^24 in a gather
+// or a combine, which is what a launch takes (of shorter rows a workgroup takes several). Kernels hold what they read of a
+// plan to the sizes given, so that a plan of other sizes gives wrong rows, never an access out of range.
 #pragma once
 
 #include "micro.h"

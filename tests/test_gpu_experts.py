@@ -313,6 +313,27 @@ def test_calls_on_another_stream_and_captured(gpu):
             assert all(torch.equal(a, b) for a, b in zip(out, layer(ids, x, w)))
 
 
+def test_two_calls_at_once(gpu):
+    """Two streams with one stack of weights, a plan of their own each, sizes that take the widest tile beside single tokens."""
+    from tcc_spmm_amd import experts as X
+    from tcc_spmm_amd.micro import E2M1, quantize_weight_micro
+    weight = quantize_weight_micro(random((8, 2048, 1024), 2, spread=0.03))
+    given = [(choices(n, 2, 8, n), random((n, 1024), n, "bf16"), random((n, 2), n + 1)) for n in (3001, 24, 2000)]
+
+    def calls(ids, x, w, stream=None):
+        plan = X.sort_experts(ids, 8, stream=stream)
+        rows = X.linear_experts(x, weight, plan, by_token=True, codes=E2M1, stream=stream)
+        return rows, X.combine_experts(rows, plan, w, stream=stream)
+
+    want = [calls(*g) for g in given]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in given]
+    for _ in range(5):
+        got = [calls(*g, stream) for g, stream in zip(given, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for one, two in zip(got, want) for a, b in zip(one, two))
+
+
 def test_refusals(gpu):
     from tcc_spmm_amd import experts as X
     from tcc_spmm_amd.micro import quantize_micro, quantize_weight_micro

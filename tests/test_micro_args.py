@@ -116,6 +116,7 @@ def test_rows_refusals():
     rejected(gather(experts=0), b"1 to 1024")
     rejected(gather(n=1 << 31), b"2^31")
     rejected(gather(width=0), b"zero elements")
+    rejected(L.tcc_gather_experts(P, 2048, 1, P, P, 1 << 25, 2, 4, P, 2048, 2048, None), b"than a launch takes")
     assert gather(n=0, offsets=None) == 0
     combine = lambda rows=P, w=P, wt=0, y=P: L.tcc_combine_experts(  # noqa: E731
         rows, 64, 1, P, P, 8, 2, 4, w, wt, y, 64, 64, None)
