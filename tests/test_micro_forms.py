@@ -40,7 +40,9 @@ PRODUCTS = [
 # tokens, each, experts, inner, outer
 EXPERTS = [
     *(("microWide", *kind, *size) for kind in EIGHT + FOUR for size in ((3001, 2, 8, 1000, 2048), (6000, 2, 4, 1200, 900))),
+    ("microWide", "bf16", "e2m1", 15000, 2, 70, 1000, 520),  # more experts than a wave has lanes, several tiles a workgroup
     *(("microTiles128", *kind, 3001, 2, 8, 2048, 1000) for kind in EIGHT + FOUR),
+    ("microTiles128", "f16", "e4m3", 15000, 2, 70, 1000, 520),
     *(("microTiles64", *kind, *size) for kind in EIGHT + FOUR + EXACT for size in ((24, 4, 32, 2048, 400), (400, 2, 8, 300, 129),
                                                                                  (90, 3, 200, 130, 70))),
 ]
