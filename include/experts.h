@@ -39,15 +39,15 @@ void sortExperts(const void* ids, std::uint32_t idBytes, ExpertPlan plan, void* 
 void gatherExperts(DenseMatrix x, ExpertPlan plan, void* rows, std::uint64_t stride, std::uint32_t width,
                    hipStream_t stream = nullptr);
 
-// y[t] = the sum over t's choices c of weights[c] * rows[places[c]], in FP32 and in the choices' order, rounded once to the
-// rows' type; null weights are ones, and choices for no expert here add nothing. Without weights it is the gradient
+// y[t] = the sum over t's choices c of weights[c] * rows[places[c]], in FP32 and in the choices' order, rounded once to
+// the rows' type; null weights are ones, and choices for no expert here add nothing. Without weights it is the gradient
 // of gatherExperts.
 void combineExperts(DenseMatrix rows, ExpertPlan plan, const void* weights, DenseType weightType, void* y,
                     std::uint64_t stride, std::uint32_t width, hipStream_t stream = nullptr);
 
-// The gradients of combineExperts from dy [tokens][width]: drows[places[c]] = weights[c] * dy[t], of dy's type, zeros for rows
-// of no expert, and dweights[c] = dy[t] . rows[places[c]], summed in FP32, of weightType, zero for choices of no expert here.
-// Either may be null; without dweights rows are not read. rows has dy's type.
+// The gradients of combineExperts from dy [tokens][width]: drows[places[c]] = weights[c] * dy[t], of dy's type, zeros for
+// rows of no expert, and dweights[c] = dy[t] . rows[places[c]], summed in FP32, of weightType, zero for choices of no
+// expert here. Either may be null; without dweights rows are not read. rows has dy's type.
 void combineExpertsBackward(DenseMatrix dy, DenseMatrix rows, ExpertPlan plan, const void* weights, DenseType weightType,
                             void* drows, std::uint64_t stride, void* dweights, std::uint32_t width,
                             hipStream_t stream = nullptr);
