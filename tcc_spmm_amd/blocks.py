@@ -140,10 +140,11 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
 def _dense(t: torch.Tensor, name: str, columns: int | None = None) -> None:
     if t.dtype not in _TYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() < 1 or t.shape[-1] < 1:
+    shape = t.shape
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name} needs a last dimension of at least one element")
-    if columns is not None and t.shape[-1] != columns:
-        raise ValueError(f"{name} has rows of {t.shape[-1]} elements, expected {columns}")
+    if columns is not None and shape[-1] != columns:
+        raise ValueError(f"{name} has rows of {shape[-1]} elements, expected {columns}")
 
 
 def _same_device(device, *tensors) -> None:

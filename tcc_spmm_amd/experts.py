@@ -248,7 +248,7 @@ def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias:
     if away:
         with away:
             return linear_experts(x, weight, plan, bias, by_token=by_token, codes=codes)
-    if by_token and plan.tokens * _code_pitch(inner) * (2 - kind) >= 1 << 31:
+    if by_token and plan.choices // plan.each * _code_pitch(inner) * (2 - kind) >= 1 << 31:
         # The kernels reach a token's codes by 32 bits.
         x, by_token = gather_experts(x, plan), False
     flat, _, _, stride = _laid(x)

@@ -41,6 +41,27 @@ def test_product_past_32_bits(room, codes):  # noqa: F811
         assert (y[part] != want).float().mean() < 0.01
 
 
+def test_product_of_more_rows_than_small_tiles_have_threads_for(room):  # noqa: F811
+    """2^30 + 300 rows are too many tiles of 64 rows for a launch. Most rows are zeros; the others are those of a product
+    of them alone."""
+    from tcc_spmm_amd import micro as M
+    room(140)
+    rows, outer = (1 << 30) + 300, 8
+    codes = torch.zeros((rows, 64), device="cuda", dtype=torch.uint8)
+    exponents = torch.full((rows, 16), 127, device="cuda", dtype=torch.uint8)
+    weight = M.quantize_weight_micro(random((outer, 128), 1))
+    parts = [slice(at, at + 300) for at in (0, (1 << 29) - 100, rows - 300)]
+    for i, p in enumerate(parts):
+        some = M.quantize_micro(random((300, 128), 2 + i))
+        codes[p], exponents[p] = some.codes.view(torch.uint8), some.exponents
+    y = M.matmul_micro(M.MicroTensor(codes.view(M.E2M1), exponents, 128), weight)
+    for p in parts:
+        want = M.matmul_micro(M.MicroTensor(codes[p].view(M.E2M1), exponents[p], 128), weight)
+        # products of 4-bit codes are added exactly as far as FP32 goes, in whatever tile
+        assert (y[p].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+    assert not y[1000:2000].any()
+
+
 def test_weight_stack_past_32_bits(room):  # noqa: F811
     """Experts whose stacked codes pass 2^32 bytes, in tiles, with the transposed copies: the last expert's rows are those of
     that expert alone."""
