@@ -826,6 +826,20 @@ const char* formName(Form f) {
     }
 }
 
+// Rows and columns of a form's tile, and the threads that take one.
+struct TileSize {
+    unsigned up, across, threads;
+};
+constexpr TileSize tileSize(Form f) {
+    switch (f) {
+    case Form::wide: return {256, 256, 256};
+    case Form::middle: return {128, 128, 512};
+    case Form::small: return {64, 64, 256};
+    case Form::half: return {64, 32, 256};
+    default: return {32, 32, 256};
+    }
+}
+
 std::uint64_t over(std::uint64_t n, std::uint64_t size) { return (n + size - 1) / size; }
 
 // The most row tiles that `rows` sorted rows of `experts` experts and of none can make.
@@ -848,8 +862,8 @@ Form leastOf(std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat
     const bool x8 = format == RowFormat::e4m3, exact = x8 && type == DenseType::f32;
     const auto tiles = [&](unsigned up, unsigned across) { return tilesOf(up) * double(over(outer, across)); };
     const auto rounds = [](double n, unsigned slots) { return std::ceil(n / slots); };
-    const auto takes = [&](unsigned up, unsigned across, unsigned threads) {
-        return launchTakes(launched(up) * over(outer, across), threads);
+    const auto takes = [&](Form f) {
+        return launchTakes(launched(tileSize(f).up) * over(outer, tileSize(f).across), tileSize(f).threads);
     };
     const auto by = [&](double n, double one, double oneStep, double some, double slots, double step) {
         return n <= 256 ? one + oneStep * k : some + n / 512 * (slots + step * k);
@@ -868,12 +882,12 @@ Form leastOf(std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat
                     : x8  ? by(tiles(32, 32), 2.4, 0.14, 1.5, 2.0, 0.21)
                           : by(tiles(32, 32), 2.6, 0.1, 1.5, 2.6, 0.16);
     if (exact) wide = middle = never; // of no size the quickest: half the wave's conversions are of operands that others have too
-    if (!takes(128, 128, 512)) middle = never;
-    if (!takes(64, 64, 256)) small = never;
-    if (!few || !takes(64, 32, 256)) narrow = never;
-    if (!few || !takes(32, 32, 256)) fewest = never;
+    if (!takes(Form::middle)) middle = never;
+    if (!takes(Form::small)) small = never;
+    if (!few || !takes(Form::half)) narrow = never;
+    if (!few || !takes(Form::few)) fewest = never;
     const double least = std::min({wide, middle, small, narrow, fewest});
-    if (least == never) return exact ? Form::small : Form::wide; // more tiles than a launch takes: refused there
+    if (least == never) return Form::small; // more tiles than a launch takes, which checkTiles refuses
     return least == small    ? Form::small
            : least == narrow ? Form::half
            : least == fewest ? Form::few
@@ -896,13 +910,28 @@ Form expertFormOf(const ExpertPlan& plan, std::uint32_t inner, std::uint32_t out
                    [&](unsigned size) { return mostTiles(plan.choices, plan.experts, size); });
 }
 
+// A form's tiles, for calls to refuse before they launch anything, the coding of x among it.
+void checkTiles(const char* where, Form form, std::uint64_t up, std::uint32_t outer) {
+    checkGrid(where, up * over(outer, tileSize(form).across), tileSize(form).threads);
+}
+Form checkedForm(const char* where, std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, DenseType type, RowFormat format) {
+    const Form form = formOf(rows, inner, outer, type, format);
+    checkTiles(where, form, over(rows, tileSize(form).up), outer);
+    return form;
+}
+Form checkedForm(const char* where, const ExpertPlan& plan, std::uint32_t inner, std::uint32_t outer, DenseType type,
+                 RowFormat format) {
+    const Form form = expertFormOf(plan, inner, outer, type, format);
+    checkTiles(where, form, mostTiles(plan.choices, plan.experts, tileSize(form).up), outer);
+    return form;
+}
+
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 void launchTiles(Product p, hipStream_t stream) {
     const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, BM) : over(p.rows, BM);
     p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, BN));
     const std::uint64_t tiles = up * p.tilesN;
     constexpr unsigned lds = Groups * Stages * (BM * 128 + BN * (X8 ? 64 : 128));
-    checkGrid("matmul micro", tiles, 64 * WM * WN * Groups);
     hipLaunchKernelGGL((microTiles<T, X8, Experts, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
                        dim3(64 * WM * WN * Groups), lds, stream, p);
     checkHip(hipGetLastError());
@@ -912,7 +941,6 @@ template <typename T, bool X8, bool Experts> void launchWide(Product p, hipStrea
     const std::uint64_t up = Experts ? mostTiles(p.rows, p.experts, 256) : over(p.rows, 256);
     p.tilesM = unsigned(up), p.tilesN = unsigned(over(p.outer, 256));
     const std::uint64_t tiles = up * p.tilesN, least = Experts ? over(tiles, 8 * kWideTiles) * 8 : 0;
-    checkGrid("matmul micro", tiles, 256);
     // A multiple of the XCDs, so that a workgroup's tiles stay with one.
     const dim3 grid(unsigned(std::min<std::uint64_t>(tiles, std::max<std::uint64_t>(kWideGroups, least)))), threads(256);
     constexpr unsigned lds = 2 * 256 * (X8 ? 192 : 256) + (Experts ? kWideTiles * (sizeof(WideTile) + 256 * 4) : 0);
@@ -1066,8 +1094,9 @@ void matmulMicro(CodedRows x, MicroRows w, const float* bias, void* y, DenseType
     Product p = productOf(w, bias, y, stride, rows, inner, outer);
     p.x = x.codes, p.xe = x.exponents;
     setExponents(p, x.format, false, rows);
+    const Form form = checkedForm(where, rows, inner, outer, type, x.format);
     withRows(type, x.format, [&](auto tag, auto x8) {
-        launchForm<decltype(tag), decltype(x8)::value, false>(formOf(rows, inner, outer, type, x.format), p, stream);
+        launchForm<decltype(tag), decltype(x8)::value, false>(form, p, stream);
     });
 }
 
@@ -1106,7 +1135,7 @@ void linearMicro(DenseMatrix x, RowFormat format, MicroRows w, const float* bias
         });
         return checkHip(hipGetLastError());
     }
-    const Form form = formOf(rows, inner, outer, x.type, format);
+    const Form form = checkedForm(where, rows, inner, outer, x.type, format);
     Product p = productOf(w, bias, y, yStride, rows, inner, outer);
     encode(p, x, format, keep, packs(form, rows, inner, format), rows, inner, static_cast<std::uint8_t*>(workspace), stream);
     withRows(x.type, format, [&](auto tag, auto x8) {
@@ -1176,8 +1205,9 @@ void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, vo
     Product p = expertsProduct(byToken, w, bias, y, stride, plan, inner, outer);
     p.x = x.codes, p.xe = x.exponents;
     setExponents(p, x.format, false, plan.choices);
+    const Form form = checkedForm(where, plan, inner, outer, type, x.format);
     withRows(type, x.format, [&](auto tag, auto x8) {
-        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, inner, outer, type, x.format), p, stream);
+        launchForm<decltype(tag), decltype(x8)::value, true>(form, p, stream);
     });
 }
 
@@ -1206,10 +1236,11 @@ void linearExperts(DenseMatrix x, RowFormat format, bool byToken, MicroRows w, c
     if (need > workspaceBytes || !workspace) reject(where, "workspace too small");
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16) reject(where, "workspace must be 16-byte aligned");
     checkTokens(where, plan, byToken, inner, format);
+    const Form form = checkedForm(where, plan, inner, outer, x.type, format);
     Product p = expertsProduct(byToken, w, bias, y, yStride, plan, inner, outer);
     encode(p, x, format, {}, packs(plan, byToken, inner, outer, x.type, format), rows, inner,
            static_cast<std::uint8_t*>(workspace), stream);
     withRows(x.type, format, [&](auto tag, auto x8) {
-        launchForm<decltype(tag), decltype(x8)::value, true>(expertFormOf(plan, inner, outer, x.type, format), p, stream);
+        launchForm<decltype(tag), decltype(x8)::value, true>(form, p, stream);
     });
 }
