@@ -826,12 +826,29 @@ Form formOf(std::uint32_t rows, std::uint32_t outer, unsigned count) {
     return least == wide ? Form::wide : least == middle ? Form::middle : least == small ? Form::small : Form::few;
 }
 
+// The launch of a product, for calls to refuse before they launch anything, the coding of x among it. multiplyTokens is taken
+// for no more rows than a launch takes.
+void checkTiles(const char* where, std::uint32_t rows, std::uint32_t outer, unsigned count, DenseType type) {
+    const auto check = [&](unsigned size, unsigned threads) {
+        checkGrid(where, std::uint64_t((rows + size - 1) / size) * ((outer + size - 1) / size), threads);
+    };
+    if (type == DenseType::f32) {
+        if (!exactTokens(rows, outer, count)) check(128, 256);
+        return;
+    }
+    switch (formOf(rows, outer, count)) {
+    case Form::wide: return check(256, 256);
+    case Form::middle: return check(128, 512);
+    case Form::small: return check(64, 256);
+    case Form::few: return check(32, 512);
+    }
+}
+
 template <typename T, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 void launchTiles(Product p, hipStream_t stream) {
     p.tilesM = (p.rows + BM - 1) / BM, p.tilesN = (p.outer + BN - 1) / BN;
     const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
     const std::size_t lds = Groups * Stages * (BM + BN) * kBlock;
-    checkGrid("matmul blocks", tiles, 64 * WM * WN * Groups);
     hipLaunchKernelGGL((multiplyTiles<T, BM, BN, WM, WN, Stages, Groups>), dim3(unsigned(tiles)),
                        dim3(64 * WM * WN * Groups), lds, stream, p);
     checkHip(hipGetLastError());
@@ -840,7 +857,6 @@ void launchTiles(Product p, hipStream_t stream) {
 template <typename T> void launchWide(Product p, hipStream_t stream) {
     p.tilesM = (p.rows + 255) / 256, p.tilesN = (p.outer + 255) / 256;
     const std::uint64_t tiles = std::uint64_t(p.tilesM) * p.tilesN;
-    checkGrid("matmul blocks", tiles, 256);
     hipLaunchKernelGGL((multiplyWide<T>), dim3(unsigned(tiles)), dim3(256), 2 * 2 * 256 * kBlock, stream, p);
     checkHip(hipGetLastError());
 }
@@ -850,7 +866,6 @@ template <typename T> void launchProduct(Product p, hipStream_t stream) {
         if (exactTokens(p.rows, p.outer, p.count)) return launchTokens(p, stream);
         p.tilesM = (p.rows + 127) / 128;
         const std::uint64_t tiles = std::uint64_t(p.tilesM) * ((p.outer + 127) / 128);
-        checkGrid("matmul blocks", tiles, 256);
         hipLaunchKernelGGL(multiplyTilesExact, dim3(unsigned(tiles)), dim3(256), 0, stream, p);
         checkHip(hipGetLastError());
     } else {
@@ -887,6 +902,7 @@ void matmulBlocks(BlockRows x, BlockWeightView w, const float* bias, void* y, De
     p.y = y, p.yStride = stride, p.rows = rows, p.outer = outer, p.inner = inner;
     p.count = (inner + kBlock - 1) / kBlock;
     p.expPitch = unsigned(blockExponentPitch(inner));
+    checkTiles(where, rows, outer, p.count, type);
     withType(type, [&](auto tag) { launchProduct<decltype(tag)>(p, stream); });
 }
 
@@ -979,6 +995,7 @@ void linearBlocks(DenseMatrix x, BlockWeightView w, const float* bias, void* y, 
         });
         return;
     }
+    checkTiles(where, rows, outer, (inner + kBlock - 1) / kBlock, x.type);
     auto* spare = static_cast<std::uint8_t*>(workspace);
     if (!keep.codes) keep = {spare, spare + rounded(rows * blockCodePitch(inner)), BlockCodes::e4m3};
     quantizeBlocks(x, keep, rows, inner, stream);

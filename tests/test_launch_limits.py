@@ -39,3 +39,13 @@ def test_linear_experts(t, form, choices, each, inner, outer):
         # tokens' codes are reached by 32 bits: of one too many rows for that the call says so
         rejected(call, b"gather them" if by_token and choices // each * (64 if form else 128) >> 31 else
                  b"linear experts: more tiles than a launch takes")
+
+
+@pytest.mark.parametrize("t,rows,inner,outer", [(0, MOST, 600, 512), (1, MOST, 600, 512), (2, 1 << 24, 600, 1 << 18)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_linear_blocks(t, rows, inner, outer, keep):
+    from tcc_spmm_amd._lib import lib
+    size = workspace("tcc_linear_blocks_workspace", rows, inner, outer, t, keep)
+    keep = P if keep else None
+    rejected(lib().tcc_linear_blocks(P, inner, t, P, P, None, P, outer, keep, keep, rows, inner, outer, P, size, None),
+             b"linear blocks: more tiles than a launch takes")
