@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -410,6 +411,13 @@ def activation_blocks_backward(dy: torch.Tensor, kept: BlockTensor, kind: str = 
 # Under autograd
 
 
+def _recorded() -> bool:
+    """Whether a differentiable call goes through its Function: with gradients on, and where forward mode or a trace has to
+    see it, which no_grad does not switch off: past the Function a tangent would be lost, and a trace would hold the empty
+    output without the kernel."""
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0 or torch.jit.is_tracing()
+
+
 def _float_bias(bias):
     """A bias of any type and layout as the products take it."""
     return None if bias is None else bias.float().contiguous()
@@ -467,7 +475,7 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     added at their own precision."""
     if x.is_cuda and x.dtype in _TYPES and torch.is_autocast_enabled("cuda"):
         x = x.to(torch.get_autocast_dtype("cuda"))
-    if not torch.is_grad_enabled():
+    if not _recorded():
         # Inside a Function the mode is off and its arguments still say that they require a gradient.
         weight = quantize_weight_blocks(w, transposed=False)
         return linear_blocks(x, weight, _float_bias(bias))
@@ -477,9 +485,9 @@ def block_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
 def block_activation(x: torch.Tensor, kind: str = "silu", *, gated: bool = False, codes=INT8) -> torch.Tensor:
     """activation_blocks, differentiable: what autograd keeps of x is its blocks, so codes=None is for inputs that
     need no gradient."""
-    if not torch.is_grad_enabled():
+    if not _recorded():
         return activation_blocks(x, kind, gated=gated, codes=None)[0]
-    if codes is None and x.requires_grad:
+    if codes is None and x.requires_grad and torch.is_grad_enabled():
         raise ValueError("x requires a gradient, which codes=None keeps nothing for")
     return _Activation.apply(x, kind, gated, codes)
 

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .blocks import _TYPES, E4M3, BlockTensor, _away, _dense, _rows, _same_device, _stream, _stride
+from .blocks import _TYPES, E4M3, BlockTensor, _away, _dense, _recorded, _rows, _same_device, _stream, _stride
 from .micro import _FORMATS, MicroTensor, MicroWeight, _code_pitch, _format, _laid, _workspace
 
 MAX_EXPERTS = 1024
@@ -312,12 +312,12 @@ class _Linear(torch.autograd.Function):
 
 def expert_gather(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """gather_experts, differentiable."""
-    return _Gather.apply(x, plan) if torch.is_grad_enabled() else gather_experts(x, plan)
+    return _Gather.apply(x, plan) if _recorded() else gather_experts(x, plan)
 
 
 def expert_combine(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | None = None) -> torch.Tensor:
     """combine_experts, differentiable in the rows and the weights."""
-    return _Combine.apply(rows, plan, weights) if torch.is_grad_enabled() else combine_experts(rows, plan, weights)
+    return _Combine.apply(rows, plan, weights) if _recorded() else combine_experts(rows, plan, weights)
 
 
 def expert_linear(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias: torch.Tensor | None = None, *,
@@ -327,10 +327,10 @@ def expert_linear(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias: 
     cast to its type first."""
     if x.is_cuda and x.dtype in _TYPES and torch.is_autocast_enabled("cuda"):
         x = x.to(torch.get_autocast_dtype("cuda"))
-    if not torch.is_grad_enabled():
+    if not _recorded():
         return linear_experts(x, weight, plan, bias, by_token=by_token, codes=codes)
-    if bias is not None and bias.requires_grad:
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("the experts are frozen: their bias has no gradient")
-    if x.requires_grad and weight.codes_t is None:
+    if x.requires_grad and weight.codes_t is None and torch.is_grad_enabled():
         raise ValueError("x requires a gradient, which needs the weight's transposed copy")
     return _Linear.apply(x, weight, plan, bias, by_token, codes)

@@ -19,8 +19,8 @@ import functools
 import torch
 
 from ._lib import check, lib
-from .blocks import (_TYPES, E4M3, BlockTensor, _away, _bias, _dense, _float_bias, _new_blocks, _rows, _same_device,
-                     _stream, _stride, weight_grad_blocks)
+from .blocks import (_TYPES, E4M3, BlockTensor, _away, _bias, _dense, _float_bias, _new_blocks, _recorded, _rows,
+                     _same_device, _stream, _stride, weight_grad_blocks)
 
 BLOCK = 32
 E2M1 = torch.float4_e2m1fn_x2
@@ -329,7 +329,7 @@ def micro_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         x = x.to(torch.get_autocast_dtype("cuda"))
     if w.dim() != 2:
         raise ValueError("w must be [outer, inner]")
-    if not torch.is_grad_enabled():
+    if not _recorded():
         # Inside a Function the mode is off and its arguments still say that they require a gradient.
         return linear_micro(x, quantize_weight_micro(w, tiles=True), _float_bias(bias))
     return _Linear.apply(x, w, bias)
