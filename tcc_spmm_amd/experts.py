@@ -267,22 +267,43 @@ def linear_experts(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias:
 # Under autograd
 
 
+# Plans and frozen weights are not saved as autograd saves tensors, whose hooks may move or copy what they are given: a
+# Function holds them, and their versions, itself.
+
+
+def _hold(ctx, plan: ExpertPlan, *weights: torch.Tensor) -> None:
+    ctx.plan = _plan(plan.offsets, plan.order, plan.places, plan.lead, plan.each)
+    ctx.versions = _versions(ctx.plan, weights)
+
+
+def _versions(plan: ExpertPlan, weights):
+    """Inference tensors, which have no versions, count as unchanged."""
+    return [None if t.is_inference() else t._version for t in (plan.offsets, plan.order, plan.places, *weights)]
+
+
+def _held(ctx, *weights: torch.Tensor) -> ExpertPlan:
+    if _versions(ctx.plan, weights) != ctx.versions:
+        raise RuntimeError("the experts' plan or weight has been modified by an inplace operation since the forward pass, "
+                           "whose gradient needs it as it was")
+    return ctx.plan
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan = plan
+        _hold(ctx, plan)
         return gather_experts(x, plan)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        return combine_experts(drows, ctx.plan), None
+        return combine_experts(drows, _held(ctx)), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, plan, weights):
-        ctx.plan = plan
+        _hold(ctx, plan)
         # rows are what the weights' gradient needs, weights what both do.
         ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, weights)
         return combine_experts(rows, plan, weights)
@@ -292,21 +313,26 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, dy):
         rows, weights = ctx.saved_tensors
         need = (ctx.needs_input_grad[0], ctx.needs_input_grad[2])
-        drows, dweights = combine_experts_backward(dy, rows, ctx.plan, weights, need=need)
+        drows, dweights = combine_experts_backward(dy, rows, _held(ctx), weights, need=need)
         return drows, None, dweights
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, plan, bias, by_token, codes):
-        ctx.call = (weight, plan, by_token, codes)
+        # Without a gradient of x there is no backward pass.
+        back = weight.transposed() if ctx.needs_input_grad[0] and weight.codes_t is not None else None
+        if back is not None:
+            _hold(ctx, plan, back.codes, back.exponents)
+        ctx.call = (back, by_token, codes)
         return linear_experts(x, weight, plan, bias, by_token=by_token, codes=codes)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        weight, plan, by_token, codes = ctx.call
-        dx = linear_experts(dy, weight.transposed(), plan, codes=codes)
+        back, by_token, codes = ctx.call
+        plan = _held(ctx, back.codes, back.exponents)
+        dx = linear_experts(dy, back, plan, codes=codes)
         return (combine_experts(dx, plan) if by_token else dx), None, None, None, None, None
 
 
