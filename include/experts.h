@@ -54,7 +54,8 @@ void combineExpertsBackward(DenseMatrix dy, DenseMatrix rows, ExpertPlan plan, c
 
 // y[r] = x[row] w[e]^T + bias[e] for each sorted row r of expert e, with the sums of matmulMicro; zeros for rows of no
 // expert. x has a row for each sorted row, or, byToken, for each token, and row r takes that of its token; codes of
-// tokens are then at most 2^31 - 1 bytes. w is a stack of [experts][outer] rows of `inner` elements; bias null or FP32
+// tokens are then at most 2^31 - 1 bytes (of more: gatherExperts moves codes and exponents as 16-bit matrices of half as many
+// columns as they are). w is a stack of [experts][outer] rows of `inner` elements; bias null or FP32
 // [experts][outer]. With the transposed stack it gives the rows' input gradient.
 void matmulExperts(CodedRows x, bool byToken, MicroRows w, const float* bias, void* y, DenseType type, std::uint64_t stride,
                    ExpertPlan plan, std::uint32_t inner, std::uint32_t outer, hipStream_t stream = nullptr);

@@ -193,6 +193,18 @@ def _stack(weight: MicroWeight, plan: ExpertPlan) -> None:
         raise ValueError(f"weight must be a stack of {plan.experts} experts' weights")
 
 
+def _gather_codes(x: BlockTensor | MicroTensor, plan: ExpertPlan) -> BlockTensor | MicroTensor:
+    """Tokens' codes and exponents as rows in the experts' order: both are whole numbers of pairs of bytes, which a gather
+    moves as they are."""
+    moved = type(x).__new__(type(x))  # laid out as x is
+    moved.columns = x.columns
+    for name in ("codes", "exponents"):
+        t = getattr(x, name)
+        pairs = t.view(torch.uint8).view(torch.bfloat16).reshape(*plan.lead, -1)
+        setattr(moved, name, gather_experts(pairs, plan).view(torch.uint8).view(t.dtype))
+    return moved
+
+
 def _stack_bias(bias, experts: int, outer: int, device) -> int:
     if bias is None:
         return 0
@@ -224,6 +236,9 @@ def matmul_experts(x: BlockTensor | MicroTensor, weight: MicroWeight, plan: Expe
     if away:
         with away:
             return matmul_experts(x, weight, plan, bias, by_token=by_token, dtype=dtype)
+    if by_token and x.codes.numel() >= 1 << 31:
+        # The kernels reach a token's codes by 32 bits.
+        x, by_token = _gather_codes(x, plan), False
     y = torch.empty((plan.choices, outer), dtype=dtype, device=device)
     check(lib().tcc_matmul_experts(x.codes.data_ptr(), x.exponents.data_ptr(), _FORMATS[x.codes.dtype], by_token,
                                    weight.codes.data_ptr(), weight.exponents.data_ptr(), at_bias, y.data_ptr(), outer,
