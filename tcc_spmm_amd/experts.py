@@ -15,7 +15,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .blocks import _TYPES, E4M3, BlockTensor, _away, _dense, _recorded, _rows, _same_device, _stream, _stride
+from .blocks import (_TYPES, E4M3, BlockTensor, _away, _dense, _float_bias, _recorded, _rows, _same_device, _stream,
+                     _stride)
 from .micro import _FORMATS, MicroTensor, MicroWeight, _code_pitch, _format, _laid, _workspace
 
 MAX_EXPERTS = 1024
@@ -363,15 +364,15 @@ def expert_combine(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor |
 
 def expert_linear(x: torch.Tensor, weight: MicroWeight, plan: ExpertPlan, bias: torch.Tensor | None = None, *,
                   by_token: bool = False, codes=E4M3) -> torch.Tensor:
-    """linear_experts, differentiable in x; the experts are frozen. The gradient goes through the output gradient's codes and
-    the weight's transposed copy; by_token each row's is rounded to x's type before a token's are added. Under autocast x is
-    cast to its type first."""
+    """linear_experts, differentiable in x; the experts are frozen, their bias is of any type and layout. The gradient goes
+    through the output gradient's codes and the weight's transposed copy; by_token each row's is rounded to x's type before a
+    token's are added. Under autocast x is cast to its type first."""
     if x.is_cuda and x.dtype in _TYPES and torch.is_autocast_enabled("cuda"):
         x = x.to(torch.get_autocast_dtype("cuda"))
     if not _recorded():
-        return linear_experts(x, weight, plan, bias, by_token=by_token, codes=codes)
+        return linear_experts(x, weight, plan, _float_bias(bias), by_token=by_token, codes=codes)
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("the experts are frozen: their bias has no gradient")
     if x.requires_grad and weight.codes_t is None and torch.is_grad_enabled():
         raise ValueError("x requires a gradient, which needs the weight's transposed copy")
-    return _Linear.apply(x, weight, plan, bias, by_token, codes)
+    return _Linear.apply(x, weight, plan, _float_bias(bias), by_token, codes)
