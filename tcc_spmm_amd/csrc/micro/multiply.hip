@@ -54,7 +54,8 @@ __device__ __forceinline__ f32x4 multiply(u32x4 w, u32x4 x0, u32x4 x1, f32x4 acc
                                                             X8 ? 0 : 4, S, int(ws), S, int(xs));
 }
 
-// The values of 8 E2M1 codes as bf16, exact at every finite scale.
+// The values of 8 E2M1 codes as bf16. Exact but for the upper end: values of 2^128 and more, which exponents above 252 can
+// give and quantizing does not, are infinite.
 __device__ __forceinline__ bf16x8 microValues8(unsigned q, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0);
     const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1);
