@@ -199,7 +199,7 @@ template <bool Experts> __device__ __forceinline__ void take(Product& a, Tile& t
 // the codes that it has read from LDS, four conversions for each MFMA of 16 cycles in tiles of 64.
 // What bounds them is the chain of a step, a barrier and the LDS reads behind it, and for few rows the weight's way from
 // memory. Measured, us: 48 x 4096 x 8191 with 8-bit rows 9.3 in tiles of 64 x 32 (11.5 in tiles of 64, twice the steps for half
-// the CUs); 17 x 4096 x 4096 6.6 in tiles of 32; 24 tokens to 4 of 32 experts, 2048 x 4096, 23 in tiles of 64, 6.1 TB/s of the weights; 6002 rows of 8 experts, 2048 x 1000, 30
+// the CUs); 17 x 4096 x 4096 6.6 in tiles of 32; 24 tokens to 4 of 32 experts, 2048 x 4096, 25 in tiles of 64, 5.8 TB/s of the weights; 6002 rows of 8 experts, 2048 x 1000, 30
 // in tiles of 128; FP32: 2001 x 1024 x 4097 32, 0.53 PFLOP/s, 2001 x 4097 x 1024 26, 0.64.
 template <typename T, bool X8, bool Experts, unsigned BM, unsigned BN, unsigned WM, unsigned WN, unsigned Stages, unsigned Groups>
 __global__ __launch_bounds__(64 * WM * WN * Groups) void microTiles(Product a) {
@@ -435,11 +435,11 @@ __device__ __forceinline__ void multiplyInPlace(f32x4& acc, u32x4 w, u32x4 x0, u
 // for the last time a quarter or more before, and each has at least a step's time to arrive:
 //   quarter 0: pairs 2 and 3 of step k + 1;  1 and 2: x of step k + 2;  3: pairs 0 and 1 of step k + 2
 // with a barrier before quarters 1 and 3.
-// Measured: 4096 x 4096 x 8192 with 8-bit rows, bf16, 111 us, 2.5 PFLOP/s; 8192 x 4096 x 8192 in 4 bits 144, 3.8 PFLOP/s; 8192
-// tokens to 4 of 32 experts, 2048 x 4096 in 4 bits, 266, 2.1. A step in 4 bits is 1.6 us on all CUs at once, 5.1 PFLOP/s, where
-// this card's power lets registers alone multiply random codes at 5.8 (zeros 6.7); in 8 bits 1.5 of 4.1. What remains is a
-// tile's beginning and end, 8 us: all CUs store at once (5 us at HBM's rate), and its first loads. MFMAs are busy 41% of all
-// cycles, 59% with 8-bit rows, and no LDS access conflicts.
+// Measured: 4096 x 4096 x 8192 with 8-bit rows, bf16, 116 us, 2.4 PFLOP/s; 8192 x 4096 x 8192 in 4 bits 148, 3.7 PFLOP/s; 8192
+// tokens to 4 of 32 experts, 2048 x 4096 in 4 bits, 271, 2.0. A step in 4 bits, 256 elements, is 1.8 us on all CUs at once, 4.7
+// PFLOP/s, where this card's power lets registers alone multiply random codes at 5.8 (zeros 6.7); one in 8 bits, 128 elements,
+// 1.5 us, 2.9 PFLOP/s of 4.1. What remains is a tile's beginning and end, 8 us: all CUs store at once (5 us at HBM's rate), and
+// its first loads. MFMAs are busy 43% of all cycles, 58% with 8-bit rows, and no LDS access conflicts.
 // The tiles that a workgroup goes through, one after the other, a grid apart: in the last pair of a tile's steps the loads are
 // those of the next tile's first, so that it begins as the sums of this one are stored (8192 x 512 x 8192 52 us : 45, 8 even
 // rounds of experts 238 : 232, nine uneven ones 297 : 271). For experts the tiles and the rows' sources are looked up in front
@@ -1007,7 +1007,8 @@ std::uint64_t exponentPitch(std::uint32_t inner, RowFormat f) {
 std::size_t rounded(std::uint64_t bytes) { return std::size_t((bytes + 255) / 256 * 256); }
 
 // x's exponents by fours of steps, all rows' side by side, as microWide is quickest to read them: what it wants of a row at a
-// time lies in a line of its own else. Rows in 4 bits are coded so, those in 8 bits have theirs copied into that order, 2 us.
+// time lies in a line of its own else. Rows in 4 bits are coded so, those in 8 bits have theirs copied into that order (of
+// 4096 x 4096 4.8 us, of 6002 x 1000 2.3).
 // For fewer than 2^31 bytes of them. (4096 x 4096 x 8192, 8-bit rows 136 us : 115, 4-bit 84 : 78; the weight's, 83.)
 __global__ __launch_bounds__(256) void packExponents(const unsigned* __restrict__ from, unsigned* __restrict__ to, unsigned rows,
                                                      unsigned groups) {
@@ -1061,6 +1062,7 @@ std::size_t fusedLds(std::uint32_t rows, std::uint32_t inner, RowFormat f) {
 // which one more costs the caller 4 us and the GPU one of them. The constants fit these (rows x inner x outer, bf16, 8-bit
 // rows, this : two): 2 x 4096 x 4096 5.1 : 8.0, 8 x 4096 x 4096 8.1 : 8.1, 16 x 2048 x 4096 8.4 : 6.9, 16 x 512 x 4096 4.8 : 5.7,
 // 6 x 2048 x 8192 8.3 : 7.0, 8 x 4096 x 8192 11.5 : 8.0; the call's time 8 x 4096 x 4096 7.9 : 12.0, 16 x 2048 x 4096 8.2 : 11.9.
+// Beyond 4096 x 8192 neither side has been measured, and the estimates have no term for a weight that comes from HBM.
 bool fusedTokens(std::uint32_t rows, std::uint32_t inner, std::uint32_t outer, RowFormat f) {
     const double count = double(over(inner, kStep)), more = double(over(outer, 4096)) - 1.0;
     const double fused = 4.0 + more + 0.0165 * rows * count * (1.0 + 0.5 * more), two = 5.3 + 0.085 * count;
