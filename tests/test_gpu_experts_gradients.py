@@ -1,11 +1,9 @@
 """The experts' input gradient against its formula in 64 bits and against differences."""
 import numpy as np
 import pytest
-import torch
 
-import blocks_oracle as B8
 import micro_oracle as O
-from blocks_oracle import DTYPES, ROUNDING, f64
+from blocks_oracle import ROUNDING, f64
 from test_gpu_blocks import U, near, random, rounded
 from test_gpu_experts import choices
 from test_gpu_micro import FORMATS, product_room, row_values
